@@ -760,6 +760,76 @@ SNAG_API int snag_gat_layer_bwd(const float* x, int64_t N, int f, int H, const f
 SNAG_API int snag_spmm_csr(const int32_t* rowptr, const int32_t* col, const float* val, const float* x, int64_t N, int f,
                            const float* bias, float* out, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * A cross-attention block and the optimiser of its matrices.  The Mformer reads at most six tokens of a fixed number
+ * (model/SNAG_tools.py:158-209); these entries read any number of an encoder's states per sequence (the patches or words of an
+ * entity), in fp32, bf16 or fp16.
+ */
+#define SNAG_F32 0
+#define SNAG_BF16 1
+#define SNAG_F16 2
+
+/* Attention of queries over states of another length.  Per batch entry b and head h, hk = h / (H / Hkv):
+ *   out[b,l,h] = sum_s p(l,s) v[b,s,hk],   p(l,.) = softmax over the seen keys of scale * q[b,l,h] . k[b,s,hk]
+ * q [B, Lq, H, d], k and v [B, Lk, Hkv, d]: strides_host (HOST memory) holds the element strides of batch, position and head of q, k and v
+ * (nine values); the d elements of a head are adjacent, d <= SNAG_CROSS_MAX_HEAD_DIM.  All three and out are of type dtype.
+ * Key s is seen when s < kv_lens[b] (int32 / int64 by lens_bytes, clamped to 0..Lk; NULL = Lk) and key_mask[b * mask_ld + s] != 0 (NULL = all).
+ * What memory holds at an unseen key, NaN included, does not reach any result.  A query that sees no key gets out = 0 and lse = -inf.
+ * out [B, Lq, H, d] dense; lse [B, H, Lq] = log2 of the sum of exp2(scale * log2(e) * q . k), kept for the backward.
+ * Scores, running maximum, sums and outputs are accumulated in fp32; for 16-bit types the probabilities (and d scores) are rounded to dtype
+ * for the product with v (k, q).
+ * The backward OVERWRITES d_q (as out), d_k and d_v [B, Lk, Hkv, d] dense (zero at unseen keys); heads that share a key/value head add up
+ * in a fixed order: no atomics, bit-reproducible.  out, lse: the forward's; d_out [B, Lq, H, d] dense.
+ * work: snag_cross_work_floats(..., backward) floats (may be 0), uninitialised; launches sharing it must be stream-ordered. */
+#define SNAG_CROSS_MAX_HEAD_DIM 128
+SNAG_API int64_t snag_cross_work_floats(int dtype, int B, int Lq, int Lk, int H, int Hkv, int d, int backward);
+SNAG_API int snag_cross_fwd(const void* q, const void* k, const void* v, int dtype, int B, int Lq, int Lk, int H, int Hkv, int d,
+                            const int64_t* strides_host, const void* kv_lens, int lens_bytes, const uint8_t* key_mask, int64_t mask_ld, float scale,
+                            void* out, float* lse, float* work, int64_t work_floats, void* stream);
+SNAG_API int snag_cross_bwd(const void* q, const void* k, const void* v, int dtype, int B, int Lq, int Lk, int H, int Hkv, int d,
+                            const int64_t* strides_host, const void* kv_lens, int lens_bytes, const uint8_t* key_mask, int64_t mask_ld, float scale,
+                            const void* out, const float* lse, const void* d_out, void* d_q, void* d_k, void* d_v,
+                            float* work, int64_t work_floats, void* stream);
+
+/* The norms after and before a block with its gate and the residual, in one pass (the Mformer's own form, model/SNAG_tools.py:218-222,
+ * is a LayerNorm of the sum):   h = res_scale x + gate (post_w N(y) + post_b),   z = pre_w N(h) + pre_b
+ * x: the residual stream, y: the block's output, [rows, dim] dense; z is the next block's input.  N: kind SNAG_NORM_RMS v / sqrt(mean v^2 + eps),
+ * SNAG_NORM_LAYER (v - mean) / sqrt(var + eps) with the biased variance.  y and z are of type y_dtype, x and h of x_dtype (the same or fp32),
+ * post_w, post_b, pre_w, pre_b [dim] of w_dtype and gate of gate_dtype (each the same as y_dtype or fp32); any of the five may be NULL (1 / 0 / 1 / 0 / 1).
+ * gate [rows / rows_per_gate, dim]: rows_per_gate neighbouring rows share a gate row (rows: one gate per channel; 1: one per row).
+ * dim <= SNAG_SANDWICH_MAX_DIM.  Everything is computed in fp32 and rounded once; z comes from the unrounded h.
+ * stats [rows, 4] fp32 (16-byte aligned; may be NULL when no backward follows): mean and 1 / deviation of y and of h.
+ * The backward takes d_h and d_z (either may be NULL: zero) and OVERWRITES d_x, d_y and the parameter gradients that are not NULL (types of
+ * what they belong to), summed in a fixed order (with no rows, d_gate is left as it was).  work: snag_sandwich_work_floats(...) floats (rows_per_gate = rows without a gate). */
+#define SNAG_NORM_RMS 0
+#define SNAG_NORM_LAYER 1
+#define SNAG_SANDWICH_MAX_DIM 8192
+SNAG_API int snag_sandwich_fwd(const void* x, int x_dtype, const void* y, int y_dtype, int64_t rows, int dim, const void* post_w, const void* post_b,
+                               const void* pre_w, const void* pre_b, int w_dtype, const void* gate, int gate_dtype, int64_t rows_per_gate,
+                               float res_scale, int kind, float eps, void* h, void* z, float* stats, void* stream);
+SNAG_API int64_t snag_sandwich_work_floats(int64_t rows, int64_t rows_per_gate, int dim);
+SNAG_API int snag_sandwich_bwd(const void* x, int x_dtype, const void* y, int y_dtype, int64_t rows, int dim, const void* post_w, const void* post_b,
+                               const void* pre_w, int w_dtype, const void* gate, int gate_dtype, int64_t rows_per_gate, float res_scale, int kind,
+                               const float* stats, const void* d_h, const void* d_z, void* d_x, void* d_y, void* d_post_w, void* d_post_b,
+                               void* d_pre_w, void* d_pre_b, void* d_gate, float* work, int64_t work_floats, void* stream);
+
+/* Newton-Schulz orthogonalisation of a list of matrices, and the Muon update built on it (beside snag_adamw_step_groups: the optimiser for
+ * matrix-shaped parameters).  g_host, out_host, w_host, momentum_host: HOST arrays of `count` device pointers; matrix i is [rows_host[i], cols_host[i]] dense,
+ * sides 1..SNAG_MUON_MAX_SIDE.  dtype is that of g, out and w; momentum is fp32.
+ *   orthogonalize:  X = g / (|g|_F + eps);  `steps` times X <- a X + (b A + c A^2) X, A = X X^T (X^T X from the right for tall matrices),
+ *                   (a, b, c) = (3.4445, -4.7750, 2.0315);  out = X.   out[i] may be g[i].
+ *   muon step:      M <- mu M + (1 - mu) g;  U = nesterov ? (1 - mu) g + mu M : M;  X = orthogonalize(U);
+ *                   w <- (1 - lr decay) w - lr s X,  s = sqrt(max(1, rows / cols)), or 0.2 sqrt(max(rows, cols)) with match_rms.
+ * Products accumulate in fp32; fp32 matrices carry 22 bits through them, 16-bit matrices 11 (csrc/muon.hip states the error of each).
+ * work: snag_muon_work_bytes(...) bytes, 256-byte aligned, uninitialised; launches sharing it must be stream-ordered. */
+#define SNAG_MUON_MAX_SIDE 16384
+SNAG_API int64_t snag_muon_work_bytes(const int32_t* rows_host, const int32_t* cols_host, int count);
+SNAG_API int snag_orthogonalize(const void* const* g_host, void* const* out_host, const int32_t* rows_host, const int32_t* cols_host, int count, int dtype,
+                                int steps, float eps, void* work, int64_t work_bytes, void* stream);
+SNAG_API int snag_muon_step(void* const* w_host, const void* const* g_host, float* const* momentum_host, const int32_t* rows_host, const int32_t* cols_host,
+                            int count, int dtype, float lr, float momentum, int nesterov, float weight_decay, int match_rms, int steps, float eps,
+                            void* work, int64_t work_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

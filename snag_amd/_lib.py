@@ -164,13 +164,20 @@ SIGNATURES = {
     "snag_rank_summary_pair": [_P, _P, _I, _P, _I, _P, _P],
     "snag_argmin_rows_cols": [_P, _L, _I, _I, _P, _P, _P, _P],
     "snag_entity_token_fwd": [_P, _L, _I, _P, _P, _F, _P, _L, _P],
+    "snag_cross_fwd": [_P, _P, _P] + [_I] * 7 + [_P, _P, _I, _P, _L, _F, _P, _P, _P, _L, _P],
+    "snag_cross_bwd": [_P, _P, _P] + [_I] * 7 + [_P, _P, _I, _P, _L, _F] + [_P] * 7 + [_L, _P],
+    "snag_sandwich_fwd": [_P, _I, _P, _I, _L, _I, _P, _P, _P, _P, _I, _P, _I, _L, _F, _I, _F, _P, _P, _P, _P],
+    "snag_sandwich_bwd": [_P, _I, _P, _I, _L, _I, _P, _P, _P, _I, _P, _I, _L, _F, _I] + [_P] * 11 + [_L, _P],
+    "snag_orthogonalize": [_P, _P, _P, _P, _I, _I, _I, _F, _P, _L, _P],
+    "snag_muon_step": [_P, _P, _P, _P, _P, _I, _I, _F, _F, _I, _F, _I, _I, _F, _P, _L, _P],
 }
 _SPECIAL = {"snag_version": ([], _I), "snag_last_error": ([], _c.c_char_p),
             "snag_gemm_workspace_floats": ([_I, _I, _I], _L),
             "snag_fusion_save_floats": ([_I] * 7, _L), "snag_fusion_work_floats": ([_I] * 7, _L),
             "snag_colstats_work_floats": ([_I], _L), "snag_atten_weight_work_floats": ([_I], _L), "snag_eval_work_floats": ([_I, _I], _L),
             "snag_gat_work_floats": ([_L, _I, _I], _L), "snag_score_seg_work_bytes": ([_L, _L, _L, _I, _I], _L),
-            "snag_score_touched_work_bytes": ([_L, _L, _L, _I, _I], _L)}
+            "snag_score_touched_work_bytes": ([_L, _L, _L, _I, _I], _L), "snag_cross_work_floats": ([_I] * 8, _L),
+            "snag_sandwich_work_floats": ([_L, _L, _I], _L), "snag_muon_work_bytes": ([_P, _P, _I], _L)}
 
 _lib = None
 

@@ -1,0 +1,155 @@
+"""A cross-attention block: tokens read an encoder's states of another length.
+
+The reference fuses one vector per modality (model/SNAG_tools.py:23-51: at most six tokens an entity, attended by themselves).  Here an
+entity's tokens read ANY number of states per modality -- image patches, words, attribute values -- with the block's norms, gate and
+residual fused around it.  All arithmetic is in the HIP library, forward and backward; fp32, bf16 and fp16; there is no CPU path.
+
+  cross_attention(q, k, v, ...)   attention of queries over keys and values of another length
+  sandwich_norm(x, y, ...)        the norm after a block, its gate, the residual and the next block's norm, in one pass
+  CrossModalLayer                 the two with fp32 projections and a feed-forward block: one layer of a deeper fusion
+"""
+import math
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import _lib, ops
+from .projection import Linear, ProjectionHead
+
+LN2 = math.log(2.0)
+
+
+def _note_leaves(*ts):
+    """A leaf's gradient node belongs to the stream of the first live graph that reaches it.  A backward captured on another stream would pull
+    that stream into the capture, and torch then ends the process: refuse such a capture while an earlier graph made here is alive.
+    -> the nodes, to be held until the new graph holds them."""
+    st, nodes = None, []
+    for t in ts:
+        if t is not None and t.requires_grad and t.is_leaf:
+            st = _lib.stream() if st is None else st
+            nodes.append(torch.autograd.graph.get_gradient_edge(t).node)
+            if nodes[-1].metadata.setdefault("snag_stream", st) != st and torch.cuda.is_current_stream_capturing():
+                raise _lib.SnagHipError("a backward cannot be captured while an eager graph of the same leaves lives on another stream: drop that graph's outputs first")
+    return nodes
+
+
+class _CrossAttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, kv_lens, key_mask, scale):
+        out, lse = ops.cross_attention_fwd(q, k, v, kv_lens, key_mask, scale)
+        ctx.save_for_backward(q, k, v, kv_lens, key_mask, out, lse)
+        ctx.scale = scale
+        ctx.mark_non_differentiable(lse)
+        return out, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_out, _):
+        q, k, v, kv_lens, key_mask, out, lse = ctx.saved_tensors
+        dq, dk, dv = ops.cross_attention_bwd(q, k, v, out, lse, d_out.contiguous(), kv_lens, key_mask, ctx.scale)
+        need = ctx.needs_input_grad
+        return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None
+
+
+def cross_attention(q, k, v, kv_lens=None, key_mask=None, scale=None, return_lse=False):
+    """Attention of q [B, Lq, H, d] over k, v [B, Lk, Hkv, d] -> [B, Lq, H, d], differentiable in q, k and v.
+
+    H is a multiple of Hkv (heads h (H / Hkv) .. share a key/value head), d <= 128.  Any strides whose last one is 1; fp32, bf16 or fp16.
+    ``kv_lens`` [B] (int32 / int64, on the device): keys at and behind it are not seen; ``key_mask`` [B, Lk] (bool): nor are those that are
+    False.  Unseen keys may hold anything.  A query that sees no key gets zeros, and gives none of its gradient on.  ``scale`` defaults to d ** -0.5.
+    ``return_lse`` adds the natural log-sum-exp of every row's scores [B, H, Lq] (-inf where no key is seen), not differentiable."""
+    _lib.require_gpu()
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        nodes = _note_leaves(q, k, v)
+        out, lse = _CrossAttentionFn.apply(q, k, v, kv_lens, key_mask, scale)
+    else:
+        out, lse = ops.cross_attention_fwd(q, k, v, kv_lens, key_mask, scale)
+    return (out, lse * LN2) if return_lse else out
+
+
+class _SandwichNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, y, post_weight, pre_weight, post_bias, pre_bias, gate, res_scale, kind, eps):
+        h, z, stats = ops.sandwich_norm_fwd(x, y, post_weight, pre_weight, post_bias, pre_bias, gate, res_scale, kind, eps)
+        ctx.save_for_backward(x, y, stats, post_weight, pre_weight, post_bias, pre_bias, gate)
+        ctx.cfg = (res_scale, kind)
+        ctx.set_materialize_grads(False)
+        return h, z
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_h, d_z):
+        x, y, stats, post_weight, pre_weight, post_bias, pre_bias, gate = ctx.saved_tensors
+        grads = ops.sandwich_norm_bwd(x, y, stats, None if d_h is None else d_h.contiguous(), None if d_z is None else d_z.contiguous(),
+                                      post_weight, pre_weight, post_bias, pre_bias, gate, *ctx.cfg)
+        return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None, None)
+
+
+def sandwich_norm(x, y, post_weight=None, pre_weight=None, post_bias=None, pre_bias=None, gate=None, res_scale=1.0, kind="rms", eps=1e-6):
+    """The norms around a block: h = res_scale x + gate (post_weight N(y) + post_bias), z = pre_weight N(h) + pre_bias -> (h, z).
+
+    x: the residual stream, y: the block's output, [..., dim] (dim <= 8192); h continues the stream, z enters the next block.  ``kind`` "rms"
+    (v / sqrt(mean v^2 + eps)) or "layer" (around the mean, biased variance).  ``gate`` [dim], or [G, dim] whose rows serve rows / G
+    neighbouring rows each (one gate per sequence, or per row).  x may stay fp32 while y is 16-bit; h has x's type, z y's.  Weights and biases
+    share one type, fp32 or y's; so does the gate.  Differentiable in every tensor."""
+    _lib.require_gpu()
+    x, y = x.contiguous(), y.contiguous()
+    params = (post_weight, pre_weight, post_bias, pre_bias, gate)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, y, *params)):
+        nodes = _note_leaves(x, y, *params)
+        return _SandwichNormFn.apply(x, y, *params, res_scale, kind, eps)
+    h, z, _ = ops.sandwich_norm_fwd(x, y, *params, res_scale, kind, eps, want_stats=False)
+    return h, z
+
+
+class _SandwichNorm(nn.Module):
+    """Parameters of one sandwich_norm: both norms' weights and the gate (one per channel, small at the start: the layer begins near the identity)."""
+
+    def __init__(self, dim, gate, res_scale, kind, eps):
+        super().__init__()
+        self.post_weight = nn.Parameter(torch.ones(dim))
+        self.pre_weight = nn.Parameter(torch.ones(dim))
+        self.gate = nn.Parameter(torch.full((dim,), float(gate)))
+        self.res_scale, self.kind, self.eps = float(res_scale), kind, float(eps)
+
+    def forward(self, x, y):
+        return sandwich_norm(x, y, self.post_weight, self.pre_weight, gate=self.gate, res_scale=self.res_scale, kind=self.kind, eps=self.eps)
+
+
+class CrossModalLayer(nn.Module):
+    """One layer in which the tokens of an entity read a modality's states: cross attention, then a feed-forward block, each inside a
+    sandwich norm.  fp32, like the modules beside it (``MformerFusion`` reads the M vectors this layer puts out).
+
+    ``layer(x, states, kv_lens, key_mask) -> (h, z)``: x [N, M, D] tokens, states [N, L, state_dim]; h is the residual stream, z its norm,
+    which the next layer takes as ``z`` (the first layer's tokens are taken as they are)."""
+
+    def __init__(self, dim, num_heads, state_dim=None, kv_heads=None, intermediate_size=None, gate=0.1, res_scale=1.0, kind="rms", eps=1e-6):
+        super().__init__()
+        kv_heads = num_heads if kv_heads is None else kv_heads
+        if dim % num_heads or num_heads % kv_heads:
+            raise ValueError(f"hidden size {dim} is not a multiple of {num_heads} heads, or those not of {kv_heads} key/value heads")
+        state_dim, head = dim if state_dim is None else state_dim, dim // num_heads
+        if head > ops.CROSS_MAX_HEAD_DIM:
+            raise ValueError(f"head dimension {head} > {ops.CROSS_MAX_HEAD_DIM}")
+        self.num_heads, self.kv_heads, self.head = num_heads, kv_heads, head
+        self.query = Linear(dim, dim)
+        self.key = Linear(state_dim, kv_heads * head)
+        self.value = Linear(state_dim, kv_heads * head)
+        self.output = Linear(dim, dim)
+        self.attention_norm = _SandwichNorm(dim, gate, res_scale, kind, eps)
+        self.feed_forward = ProjectionHead(dim, 4 * dim if intermediate_size is None else intermediate_size, dim, 0.0)
+        self.feed_forward_norm = _SandwichNorm(dim, gate, res_scale, kind, eps)
+
+    def forward(self, x, states, kv_lens=None, key_mask=None, z=None):
+        N, M, D = x.shape
+        L = states.shape[1]
+        z = x if z is None else z
+        flat = lambda t: t.reshape(-1, t.shape[-1])
+        q = self.query(flat(z)).view(N, M, self.num_heads, self.head)
+        k = self.key(flat(states)).view(N, L, self.kv_heads, self.head)
+        v = self.value(flat(states)).view(N, L, self.kv_heads, self.head)
+        a = cross_attention(q, k, v, kv_lens, key_mask)
+        x, z = self.attention_norm(x, self.output(a.reshape(N * M, D)).view(N, M, D))
+        f = self.feed_forward(flat(z))
+        return self.feed_forward_norm(x, f.view(N, M, D))

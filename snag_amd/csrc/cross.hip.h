@@ -1,0 +1,79 @@
+// Cross attention: what its kernels share (csrc/cross.hip: tiles on the matrix pipe; csrc/cross_rows.hip: a few rows per key/value head).
+//
+// The rows of one problem (b, hk) are the Lq * G queries of the G = H / Hkv heads that share key/value head hk, row = l * G + g: a key/value
+// tile is read once for all of them, and d K, d V of a shared head are sums inside one workgroup (no atomics).
+#pragma once
+#include <hip/hip_bf16.h>
+#include "common.hip.h"
+
+namespace snag {
+
+using bf16_t = __bf16;
+using f16_t = _Float16;
+using f32x4 = __attribute__((ext_vector_type(4))) float;
+
+struct CrossArgs {
+    const void *q, *k, *v;
+    int64_t qsb, qsl, qsh, ksb, ksl, ksh, vsb, vsl, vsh;      // element strides of batch / position / head; the head's own elements are adjacent
+    int B, Lq, Lk, H, Hkv, G, d;
+    int rows;                    // Lq * G
+    const void* lens;            // [B] int32 / int64 or NULL: keys at and behind lens[b] are not seen
+    int lens_bytes;
+    const uint8_t* mask;         // [B, Lk] (row pitch mask_ld) or NULL: 0 = key not seen
+    int64_t mask_ld;
+    float scale, c2;             // c2 = scale * log2(e)
+    int vec_q, vec_k, vec_v;     // 16-byte loads legal for this operand
+    void* out;                   // [B, Lq, H, d] dense
+    float* lse;                  // [B, H, Lq]: log2 of the row's sum of exp2(c2 q.k); -inf for a row that sees no key
+    int splits;                  // key ranges (forward, d q) or row ranges (d k, d v) worked on by different workgroups
+    int per_split;               // tiles per range
+    float* part;                 // splits > 1: partial results, see the kernels
+    // backward
+    const void *o, *dout;        // [B, Lq, H, d] dense
+    const float* delta;          // [B, H, Lq]: sum_d dout * o
+    void *dq, *dk, *dv;          // dense, shapes of q, k, v
+    int vec_o;                   // 16-byte access legal for the dense tensors (d a multiple of the chunk, aligned bases)
+};
+
+__device__ __forceinline__ int cross_len(const CrossArgs& a, int b) {
+    if (a.lens == nullptr) return a.Lk;
+    const int64_t n = a.lens_bytes == 4 ? (int64_t)((const int32_t*)a.lens)[b] : ((const int64_t*)a.lens)[b];
+    return (int)(n < 0 ? 0 : (n > a.Lk ? a.Lk : n));
+}
+
+// Workgroup ids are dealt round-robin over the 8 XCDs: give neighbours in the logical order (the workgroups that read the same keys) one XCD's L2.
+__device__ __forceinline__ int64_t xcd_order(int64_t id, int64_t n) {
+    const int64_t per = n >> 3;
+    return id < per * 8 ? (id & 7) * per + (id >> 3) : id;
+}
+
+template <class T> struct Chunk;                    // the 16 bytes a lane moves at once
+template <> struct Chunk<float> { static constexpr int n = 4; using vec = __attribute__((ext_vector_type(4))) float; };
+template <> struct Chunk<bf16_t> { static constexpr int n = 8; using vec = __attribute__((ext_vector_type(8))) __bf16; };
+template <> struct Chunk<f16_t> { static constexpr int n = 8; using vec = __attribute__((ext_vector_type(8))) _Float16; };
+
+// elements col .. col + n of a row of d elements; zero where the row is not valid or ends
+template <class T>
+__device__ __forceinline__ typename Chunk<T>::vec load_chunk(const T* __restrict__ row, int col, int d, bool valid, int vec) {
+    typename Chunk<T>::vec r;
+#pragma unroll
+    for (int j = 0; j < Chunk<T>::n; ++j) r[j] = (T)0.f;
+    if (valid && col < d) {
+        if (vec) {
+            r = *(const typename Chunk<T>::vec*)(row + col);
+        } else {
+#pragma unroll
+            for (int j = 0; j < Chunk<T>::n; ++j)
+                if (col + j < d) r[j] = row[col + j];
+        }
+    }
+    return r;
+}
+
+static inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+int cross_rows_fwd(const CrossArgs& a, int dtype, hipStream_t st);
+int cross_rows_bwd(const CrossArgs& a, int dtype, hipStream_t st);
+int cross_rows_splits(int B, int Hkv, int Lk, int d, int dtype);
+
+}  // namespace snag

@@ -1,0 +1,371 @@
+// Cross attention for at most four rows per key/value head: a single new token, an entity's few modality tokens.
+//
+// A 32 x 32 matrix product would multiply mostly padding, and the keys and values are read once whatever is done with them: the work is
+// the stream of K and V from memory, so it runs on the vector pipe.  DP / (16 bytes) lanes hold one key (16 bytes a lane), 64 / that
+// many keys are worked on side by side, the R rows stay in registers; every lane group keeps a running maximum, sum and output of its
+// own (fp32) and they are joined once at the end: over the groups by lane exchanges, over the waves of a problem through LDS, over the
+// workgroups of a long problem by cross_combine_kernel.  The backward is one pass too: with all rows of a key/value head in one wave, d K
+// and d V of a key are complete when its scores are, and only d Q is joined.
+#include "cross.hip.h"
+
+namespace snag {
+
+// all-reduce over each aligned group of N lanes (N = 4 .. 32), every lane ends with the same value
+template <int N>
+__device__ __forceinline__ float group_sum(float v) {
+    v += dpp_f32<0xB1>(v);                        // quad_perm: lane ^ 1
+    v += dpp_f32<0x4E>(v);                        // quad_perm: lane ^ 2
+    if constexpr (N >= 8) v += dpp_f32<0x141>(v); // row_half_mirror: the other quad of the eight
+    if constexpr (N >= 16) v += dpp_f32<0x140>(v);// row_mirror: the other eight of the sixteen
+    if constexpr (N >= 32) v += __shfl_xor(v, 16);
+    return v;
+}
+
+struct RowsItem { int b, hk, split, wave; bool live; };
+// waves-per-problem W divides the workgroup's waves; ids of one problem's workgroups are neighbours
+__device__ __forceinline__ RowsItem rows_item(const CrossArgs& a, int W) {
+    const int wave = wave_id_uniform(), per_block = (int)(blockDim.x >> 6) / W;
+    const int64_t item = (int64_t)blockIdx.x * per_block + wave / W, n = (int64_t)a.B * a.Hkv * a.splits;
+    RowsItem r;
+    r.live = item < n;
+    const int64_t i = r.live ? item : 0;
+    r.split = (int)(i % a.splits);
+    const int64_t bh = i / a.splits;
+    r.hk = (int)(bh % a.Hkv);
+    r.b = (int)(bh / a.Hkv);
+    r.wave = wave % W;
+    return r;
+}
+
+__device__ __forceinline__ bool rows_key_seen(const CrossArgs& a, int b, int key, int len) {
+    return key < len && (a.mask == nullptr || a.mask[(int64_t)b * a.mask_ld + key] != 0);
+}
+
+template <class T, int DP, int R>
+__global__ __launch_bounds__(512) void cross_rows_fwd_kernel(CrossArgs a, int W) {
+    constexpr int C = Chunk<T>::n, LPK = DP / C, NK = 64 / LPK, U = 4;
+    extern __shared__ float join[];               // [waves][R][DP + 2]
+    const int lane = threadIdx.x & 63, slot = lane / LPK, col = (lane % LPK) * C;
+    const RowsItem it = rows_item(a, W);
+    const int len = it.live ? cross_len(a, it.b) : 0;
+    float q[R][C], acc[R][C], m[R], sum[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int l = r < a.rows ? r / a.G : 0, head = it.hk * a.G + (r < a.rows ? r % a.G : 0);
+        const auto c = load_chunk<T>((const T*)a.q + it.b * a.qsb + l * a.qsl + head * a.qsh, col, a.d, r < a.rows && it.live, a.vec_q);
+#pragma unroll
+        for (int j = 0; j < C; ++j) q[r][j] = (float)c[j], acc[r][j] = 0.f;
+        m[r] = -INFINITY;
+        sum[r] = 0.f;
+    }
+    const T* kb = (const T*)a.k + it.b * a.ksb + it.hk * a.ksh;
+    const T* vb = (const T*)a.v + it.b * a.vsb + it.hk * a.vsh;
+    const int k0 = it.split * a.per_split, k1 = min(len, k0 + a.per_split);
+    for (int base = k0 + it.wave * NK * U; base < k1; base += W * NK * U) {
+        typename Chunk<T>::vec kc[U], vc[U];
+        bool seen[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int key = base + u * NK + slot;
+            seen[u] = key < k1 && rows_key_seen(a, it.b, key, len);
+            kc[u] = load_chunk<T>(kb + (int64_t)key * a.ksl, col, a.d, seen[u], a.vec_k);
+            vc[u] = load_chunk<T>(vb + (int64_t)key * a.vsl, col, a.d, seen[u], a.vec_v);
+        }
+        float s[U][R];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float t = 0.f;
+#pragma unroll
+                for (int j = 0; j < C; ++j) t = fmaf(q[r][j], (float)kc[u][j], t);
+                s[u][r] = seen[u] ? group_sum<LPK>(t) * a.c2 : -INFINITY;
+            }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float mn = m[r];
+#pragma unroll
+            for (int u = 0; u < U; ++u) mn = fmaxf(mn, s[u][r]);
+            const float ref = mn == -INFINITY ? 0.f : mn, alpha = __builtin_amdgcn_exp2f(m[r] - ref);
+            m[r] = mn;
+            sum[r] *= alpha;
+#pragma unroll
+            for (int j = 0; j < C; ++j) acc[r][j] *= alpha;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float p = __builtin_amdgcn_exp2f(s[u][r] - ref);
+                sum[r] += p;
+#pragma unroll
+                for (int j = 0; j < C; ++j) acc[r][j] = fmaf(p, (float)vc[u][j], acc[r][j]);
+            }
+        }
+    }
+    // the lane groups of the wave
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        float mn = m[r];
+#pragma unroll
+        for (int x = LPK; x < 64; x <<= 1) mn = fmaxf(mn, __shfl_xor(mn, x));
+        const float w = __builtin_amdgcn_exp2f(m[r] - (mn == -INFINITY ? 0.f : mn));
+        m[r] = mn;
+        sum[r] *= w;
+#pragma unroll
+        for (int x = LPK; x < 64; x <<= 1) sum[r] += __shfl_xor(sum[r], x);
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            acc[r][j] *= w;
+#pragma unroll
+            for (int x = LPK; x < 64; x <<= 1) acc[r][j] += __shfl_xor(acc[r][j], x);
+        }
+    }
+    // the waves of the problem
+    if (W > 1) {
+        constexpr int P = DP + 2;
+        float* mine = join + wave_id_uniform() * R * P;
+        if (slot == 0) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+#pragma unroll
+                for (int j = 0; j < C; ++j) mine[r * P + col + j] = acc[r][j];
+                if (col == 0) mine[r * P + DP] = m[r], mine[r * P + DP + 1] = sum[r];
+            }
+        }
+        __syncthreads();
+        if (it.wave != 0) return;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float mn = -INFINITY;
+            for (int w = 0; w < W; ++w) mn = fmaxf(mn, mine[(w * R + r) * P + DP]);
+            const float ref = mn == -INFINITY ? 0.f : mn;
+            m[r] = mn;
+            sum[r] = 0.f;
+#pragma unroll
+            for (int j = 0; j < C; ++j) acc[r][j] = 0.f;
+            for (int w = 0; w < W; ++w) {
+                const float f = __builtin_amdgcn_exp2f(mine[(w * R + r) * P + DP] - ref);
+                sum[r] = fmaf(f, mine[(w * R + r) * P + DP + 1], sum[r]);
+#pragma unroll
+                for (int j = 0; j < C; ++j) acc[r][j] = fmaf(f, mine[(w * R + r) * P + col + j], acc[r][j]);
+            }
+        }
+    }
+    if (!it.live || slot != 0) return;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        if (r >= a.rows) break;
+        const int l = r / a.G, head = it.hk * a.G + r % a.G;
+        const int64_t at = ((int64_t)it.b * a.H + head) * a.Lq + l, n = (int64_t)a.B * a.H * a.Lq;
+        if (a.splits > 1) {
+            float* o = a.part + (it.split * n + at) * a.d;
+#pragma unroll
+            for (int j = 0; j < C; ++j)
+                if (col + j < a.d) o[col + j] = acc[r][j];
+            if (col == 0) {
+                float* ml = a.part + (int64_t)a.splits * n * a.d + (it.split * n + at) * 2;
+                ml[0] = m[r];
+                ml[1] = sum[r];
+            }
+            continue;
+        }
+        const float inv = sum[r] > 0.f ? 1.f / sum[r] : (sum[r] == 0.f ? 0.f : sum[r]);
+        T* o = (T*)a.out + (((int64_t)it.b * a.Lq + l) * a.H + head) * a.d;
+        typename Chunk<T>::vec c;
+#pragma unroll
+        for (int j = 0; j < C; ++j) c[j] = (T)(acc[r][j] * inv);
+        if (a.vec_o && col < a.d) {
+            *(typename Chunk<T>::vec*)(o + col) = c;
+        } else {
+#pragma unroll
+            for (int j = 0; j < C; ++j)
+                if (col + j < a.d) o[col + j] = c[j];
+        }
+        if (col == 0) a.lse[at] = sum[r] == 0.f ? -INFINITY : m[r] + __builtin_amdgcn_logf(sum[r]);
+    }
+}
+
+template <class T>
+__device__ __forceinline__ void store_chunk(T* row, int col, int d, int vec, typename Chunk<T>::vec c) {
+    if (vec && col < d) {
+        *(typename Chunk<T>::vec*)(row + col) = c;
+    } else {
+#pragma unroll
+        for (int j = 0; j < Chunk<T>::n; ++j)
+            if (col + j < d) row[col + j] = c[j];
+    }
+}
+
+template <class T, int DP, int R>
+__global__ __launch_bounds__(512) void cross_rows_bwd_kernel(CrossArgs a, int W) {
+    constexpr int C = Chunk<T>::n, LPK = DP / C, NK = 64 / LPK, U = 2;
+    extern __shared__ float join[];               // [waves][R][DP]
+    const int lane = threadIdx.x & 63, slot = lane / LPK, col = (lane % LPK) * C;
+    const RowsItem it = rows_item(a, W);
+    const int len = it.live ? cross_len(a, it.b) : 0;
+    float q[R][C], g[R][C], dq[R][C], lse[R], delta[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const bool ok = r < a.rows && it.live;
+        const int l = r < a.rows ? r / a.G : 0, head = it.hk * a.G + (r < a.rows ? r % a.G : 0);
+        const int64_t dense = (((int64_t)it.b * a.Lq + l) * a.H + head) * a.d;
+        const auto c = load_chunk<T>((const T*)a.q + it.b * a.qsb + l * a.qsl + head * a.qsh, col, a.d, ok, a.vec_q);
+        const auto e = load_chunk<T>((const T*)a.dout + dense, col, a.d, ok, a.vec_o);
+        const auto f = load_chunk<T>((const T*)a.o + dense, col, a.d, ok, a.vec_o);
+        float t = 0.f;
+#pragma unroll
+        for (int j = 0; j < C; ++j) q[r][j] = (float)c[j], g[r][j] = (float)e[j], t = fmaf((float)e[j], (float)f[j], t), dq[r][j] = 0.f;
+        delta[r] = group_sum<LPK>(t);
+        const float s = ok ? a.lse[((int64_t)it.b * a.H + head) * a.Lq + l] : INFINITY;
+        lse[r] = s == -INFINITY ? INFINITY : s;   // a row that sees no key: every p is 0
+    }
+    const T* kb = (const T*)a.k + it.b * a.ksb + it.hk * a.ksh;
+    const T* vb = (const T*)a.v + it.b * a.vsb + it.hk * a.vsh;
+    const int k0 = it.split * a.per_split, k1 = it.live ? min(a.Lk, k0 + a.per_split) : 0;
+    for (int base = k0 + it.wave * NK * U; base < k1; base += W * NK * U) {
+        typename Chunk<T>::vec kc[U], vc[U];
+        bool seen[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int key = base + u * NK + slot;
+            seen[u] = key < k1 && rows_key_seen(a, it.b, key, len);
+            kc[u] = load_chunk<T>(kb + (int64_t)key * a.ksl, col, a.d, seen[u], a.vec_k);
+            vc[u] = load_chunk<T>(vb + (int64_t)key * a.vsl, col, a.d, seen[u], a.vec_v);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int key = base + u * NK + slot;
+            float dk[C], dv[C];
+#pragma unroll
+            for (int j = 0; j < C; ++j) dk[j] = dv[j] = 0.f;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float s = 0.f, dp = 0.f;
+#pragma unroll
+                for (int j = 0; j < C; ++j) s = fmaf(q[r][j], (float)kc[u][j], s), dp = fmaf(g[r][j], (float)vc[u][j], dp);
+                s = group_sum<LPK>(s);
+                dp = group_sum<LPK>(dp);
+                const float p = seen[u] ? __builtin_amdgcn_exp2f(fmaf(s, a.c2, -lse[r])) : 0.f;
+                const float ds = seen[u] ? p * (dp - delta[r]) * a.scale : 0.f;
+#pragma unroll
+                for (int j = 0; j < C; ++j) {
+                    dv[j] = fmaf(p, g[r][j], dv[j]);
+                    dk[j] = fmaf(ds, q[r][j], dk[j]);
+                    dq[r][j] = fmaf(ds, (float)kc[u][j], dq[r][j]);
+                }
+            }
+            if (key < k1) {
+                typename Chunk<T>::vec ck, cv;
+#pragma unroll
+                for (int j = 0; j < C; ++j) ck[j] = (T)(seen[u] ? dk[j] : 0.f), cv[j] = (T)(seen[u] ? dv[j] : 0.f);
+                const int64_t dense = (((int64_t)it.b * a.Lk + key) * a.Hkv + it.hk) * a.d;
+                store_chunk<T>((T*)a.dk + dense, col, a.d, a.vec_o, ck);
+                store_chunk<T>((T*)a.dv + dense, col, a.d, a.vec_o, cv);
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int j = 0; j < C; ++j)
+#pragma unroll
+            for (int x = LPK; x < 64; x <<= 1) dq[r][j] += __shfl_xor(dq[r][j], x);
+    if (W > 1) {
+        float* mine = join + wave_id_uniform() * R * DP;
+        if (slot == 0) {
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int j = 0; j < C; ++j) mine[r * DP + col + j] = dq[r][j];
+        }
+        __syncthreads();
+        if (it.wave != 0) return;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int j = 0; j < C; ++j) {
+                dq[r][j] = 0.f;
+                for (int w = 0; w < W; ++w) dq[r][j] += mine[(w * R + r) * DP + col + j];
+            }
+    }
+    if (!it.live || slot != 0) return;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        if (r >= a.rows) break;
+        const int l = r / a.G, head = it.hk * a.G + r % a.G;
+        const int64_t dense = (((int64_t)it.b * a.Lq + l) * a.H + head) * a.d;
+        if (a.splits > 1) {
+            float* o = a.part + (int64_t)it.split * a.B * a.Lq * a.H * a.d + dense;
+#pragma unroll
+            for (int j = 0; j < C; ++j)
+                if (col + j < a.d) o[col + j] = dq[r][j];
+        } else {
+            typename Chunk<T>::vec c;
+#pragma unroll
+            for (int j = 0; j < C; ++j) c[j] = (T)dq[r][j];
+            store_chunk<T>((T*)a.dq + dense, col, a.d, a.vec_o, c);
+        }
+    }
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------
+static int keys_per_step(int d, int dtype) {           // NK * U of the forward
+    const int c = dtype == SNAG_F32 ? 4 : 8, dp = d <= 32 ? 32 : d <= 64 ? 64 : 128;
+    return 64 / (dp / c) * 4;
+}
+
+// Waves a problem is given inside one workgroup: enough problems fill the chip with one wave each (4096 waves = 4 per SIMD); fewer are cut
+// over the waves of a workgroup as long as each still has a step of keys.
+static int rows_waves(int64_t problems, int Lk, int step) {
+    if (problems >= 4096 || Lk <= step) return 1;
+    if (problems >= 1024 || Lk <= 8 * step) return 4;
+    return 8;
+}
+
+// Key ranges on different workgroups (joined by a second launch): only where a problem's eight waves would walk more than 8 steps each while
+// most of the chip idles.
+int cross_rows_splits(int B, int Hkv, int Lk, int d, int dtype) {
+    const int64_t problems = (int64_t)B * Hkv;
+    const int step = keys_per_step(d, dtype);
+    if (problems == 0 || problems >= 256 || Lk <= 8 * 8 * step) return 1;
+    const int64_t want = (512 + problems - 1) / problems, most = Lk / (8 * 2 * step);
+    return (int)(want < most ? want : most);
+}
+
+template <class T, int DP>
+static void rows_launch(const CrossArgs& a, int W, bool bwd, hipStream_t st) {
+    const int threads = W == 8 ? 512 : 256, per_block = threads / 64 / W;
+    const int64_t items = (int64_t)a.B * a.Hkv * a.splits;
+    const dim3 grid((unsigned)((items + per_block - 1) / per_block));
+    const int R = a.rows;
+#define GO(RR)                                                                                                            \
+    do {                                                                                                                  \
+        const size_t lds = W > 1 ? sizeof(float) * (threads / 64) * RR * (bwd ? DP : DP + 2) : 0;                         \
+        if (bwd) cross_rows_bwd_kernel<T, DP, RR><<<grid, threads, lds, st>>>(a, W);                                      \
+        else cross_rows_fwd_kernel<T, DP, RR><<<grid, threads, lds, st>>>(a, W);                                          \
+    } while (0)
+    switch (R) {
+        case 1: GO(1); break;
+        case 2: GO(2); break;
+        case 3: GO(3); break;
+        default: GO(4); break;
+    }
+#undef GO
+}
+
+static int rows_go(CrossArgs a, int dtype, bool bwd, hipStream_t st) {
+    const int step = keys_per_step(a.d, dtype);
+    const int64_t problems = (int64_t)a.B * a.Hkv;
+    const int W = rows_waves(problems * a.splits, a.Lk, step);
+    SNAG_REQUIRE(problems * a.splits < (int64_t)1 << 31, SNAG_ERR_UNSUPPORTED, "cross attention: %lld problems", (long long)problems);
+    a.per_split = (a.Lk + a.splits - 1) / a.splits;
+#define GO(T) a.d <= 32 ? rows_launch<T, 32>(a, W, bwd, st) : a.d <= 64 ? rows_launch<T, 64>(a, W, bwd, st) : rows_launch<T, 128>(a, W, bwd, st)
+    if (dtype == SNAG_F32) GO(float);
+    else if (dtype == SNAG_BF16) GO(bf16_t);
+    else GO(f16_t);
+#undef GO
+    return check_launch(bwd ? "cross_rows_bwd" : "cross_rows_fwd");
+}
+
+int cross_rows_fwd(const CrossArgs& a, int dtype, hipStream_t st) { return rows_go(a, dtype, false, st); }
+int cross_rows_bwd(const CrossArgs& a, int dtype, hipStream_t st) { return rows_go(a, dtype, true, st); }
+
+}  // namespace snag

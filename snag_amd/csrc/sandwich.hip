@@ -1,0 +1,471 @@
+// The two norms around a block with its gate and its residual in one pass over the rows:
+//
+//   h = res_scale x + gate * (post_w N(y) + post_b),   z = pre_w N(h) + pre_b,     N = RMS or layer norm
+//
+// and its backward with every parameter gradient.  Bound by memory: a row of x and y is read and a row of h and z written, once; the
+// backward reads x, y, dh, dz and writes dx, dy.  It recomputes h from x and y (the same bytes as a stored h, and exact: a 16-bit h would
+// put its rounding into d pre_w), from the four statistics per row the forward saved.  All arithmetic and all sums are fp32, each output is
+// rounded once; the variance is taken around the mean (two passes over registers).
+//
+// TPR threads work on one row (32, 64: lane groups, no LDS; 256: a workgroup) with NU x 4 elements per thread in registers.  In the backward
+// a worker walks a run of rows and keeps the parameter gradients of its columns in registers; its run lies inside one gate row or covers
+// whole gate rows, the partial sums go to a slab [worker][gradient][dim] and are added up in the workers' order (no atomics).
+#include <type_traits>
+#include "cross.hip.h"
+
+namespace snag {
+
+struct SandwichArgs {
+    const void *x, *y, *post_w, *post_b, *pre_w, *pre_b, *gate;
+    int w32, g32;                  // parameters / gate in fp32 (else y's type)
+    int64_t rows, rows_per_gate;
+    int dim, layer;
+    float res_scale, eps;
+    void *h, *z;
+    float* stats;                  // [rows][4]: mean y, 1 / deviation y, mean h, 1 / deviation h (means 0 for RMS)
+    // backward
+    const void *dh, *dz;           // NULL: zero
+    void *dx, *dy, *dgate;
+    int dgate_direct;              // every gate row lies inside one worker's run: written by it
+    int64_t workers, run, chunks;  // rows per worker; workers per gate row (dgate_direct: 1)
+    float* slab;                   // [workers][kGrads][dim]
+};
+enum { kPostW, kPostB, kPreW, kPreB, kGate, kGrads };
+
+template <class T> struct Four { using vec = __attribute__((ext_vector_type(4))) T; };
+
+// thread t's four elements of step u: neighbours (VEC) or a stride of TPR apart (any dim, any alignment)
+template <int TPR, bool VEC> __device__ __forceinline__ int column(int u, int j, int t) { return VEC ? (u * TPR + t) * 4 + j : (u * 4 + j) * TPR + t; }
+
+template <class T, int TPR, int NU, bool VEC>
+__device__ __forceinline__ void load_row(float (&r)[NU][4], const T* p, int D, int t) {
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+        if constexpr (VEC) {
+            const int c = column<TPR, VEC>(u, 0, t);
+            typename Four<T>::vec v{};
+            if (c < D) v = *(const typename Four<T>::vec*)(p + c);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[u][j] = (float)v[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int c = column<TPR, VEC>(u, j, t);
+                r[u][j] = c < D ? (float)p[c] : 0.f;
+            }
+        }
+    }
+}
+template <class T, int TPR, int NU, bool VEC>
+__device__ __forceinline__ void store_row(T* p, const float (&r)[NU][4], int D, int t) {
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+        if constexpr (VEC) {
+            const int c = column<TPR, VEC>(u, 0, t);
+            typename Four<T>::vec v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = (T)r[u][j];
+            if (c < D) *(typename Four<T>::vec*)(p + c) = v;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int c = column<TPR, VEC>(u, j, t);
+                if (c < D) p[c] = (T)r[u][j];
+            }
+        }
+    }
+}
+// a parameter row (fp32 or T), `none` where there is none
+template <class T, int TPR, int NU, bool VEC>
+__device__ __forceinline__ void load_param(float (&r)[NU][4], const void* p, int is32, int64_t row, float none, int D, int t) {
+    if (p == nullptr) {
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[u][j] = none;
+    } else if (is32) {
+        load_row<float, TPR, NU, VEC>(r, (const float*)p + row * D, D, t);
+    } else {
+        load_row<T, TPR, NU, VEC>(r, (const T*)p + row * D, D, t);
+    }
+}
+
+// sums over the TPR threads of a row; every thread gets them
+template <int TPR, int N>
+__device__ __forceinline__ void row_sums(float (&s)[N], float (*red)[4][2], int& turn) {
+    if constexpr (TPR == 32) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] = sum16(s[i]), s[i] += __shfl_xor(s[i], 16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] = sum64(s[i]);
+        if constexpr (TPR == 256) {
+            // two sets of slots in turn: one barrier per sum
+            float (*slot)[2] = red[turn];
+            turn ^= 1;
+            const int wave = threadIdx.x >> 6;
+            if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) slot[wave][i] = s[i];
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < N; ++i) s[i] = slot[0][i] + slot[1][i] + slot[2][i] + slot[3][i];
+        }
+    }
+}
+
+template <int TPR, int NU, bool VEC>
+__device__ __forceinline__ void row_stats(const float (&v)[NU][4], int D, int layer, float eps, int t, float (*red)[4][2], int& turn, float& mean, float& rstd) {
+    mean = 0.f;
+    if (layer) {
+        float s[1] = {0.f};
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[0] += v[u][j];
+        row_sums<TPR, 1>(s, red, turn);
+        mean = s[0] / (float)D;
+    }
+    float s[1] = {0.f};
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float e = column<TPR, VEC>(u, j, t) < D ? v[u][j] - mean : 0.f;
+            s[0] = fmaf(e, e, s[0]);
+        }
+    row_sums<TPR, 1>(s, red, turn);
+    rstd = 1.0f / sqrtf(s[0] / (float)D + eps);
+}
+
+template <class TX, class TY, int TPR, int NU, bool VEC>
+__global__ __launch_bounds__(256) void sandwich_fwd_kernel(SandwichArgs a) {
+    __shared__ float red[2][4][2];
+    int turn = 0;
+    const int t = threadIdx.x % TPR;
+    const int64_t row = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+    if (TPR < 256 && row >= a.rows) return;       // TPR == 256: one row per workgroup
+    const int D = a.dim;
+    float y[NU][4], x[NU][4], p[NU][4], b[NU][4], g[NU][4];
+    load_row<TY, TPR, NU, VEC>(y, (const TY*)a.y + row * D, D, t);
+    load_row<TX, TPR, NU, VEC>(x, (const TX*)a.x + row * D, D, t);
+    load_param<TY, TPR, NU, VEC>(p, a.post_w, a.w32, 0, 1.f, D, t);
+    load_param<TY, TPR, NU, VEC>(b, a.post_b, a.w32, 0, 0.f, D, t);
+    load_param<TY, TPR, NU, VEC>(g, a.gate, a.g32, row / a.rows_per_gate, 1.f, D, t);
+    float my, ry, mh, rh;
+    row_stats<TPR, NU, VEC>(y, D, a.layer, a.eps, t, red, turn, my, ry);
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float post = fmaf((y[u][j] - my) * ry, p[u][j], b[u][j]);
+            x[u][j] = column<TPR, VEC>(u, j, t) < D ? fmaf(g[u][j], post, a.res_scale * x[u][j]) : 0.f;
+        }
+    store_row<TX, TPR, NU, VEC>((TX*)a.h + row * D, x, D, t);
+    load_param<TY, TPR, NU, VEC>(p, a.pre_w, a.w32, 0, 1.f, D, t);
+    load_param<TY, TPR, NU, VEC>(b, a.pre_b, a.w32, 0, 0.f, D, t);
+    row_stats<TPR, NU, VEC>(x, D, a.layer, a.eps, t, red, turn, mh, rh);
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[u][j] = fmaf((x[u][j] - mh) * rh, p[u][j], b[u][j]);
+    store_row<TY, TPR, NU, VEC>((TY*)a.z + row * D, x, D, t);
+    if (t == 0 && a.stats != nullptr) *(f32x4*)(a.stats + row * 4) = f32x4{my, ry, mh, rh};
+}
+
+template <class TX, class TY, int TPR, int NU, bool VEC>
+__global__ __launch_bounds__(256) void sandwich_bwd_kernel(SandwichArgs a) {
+    __shared__ float red[2][4][2];
+    int turn = 0;
+    const int t = threadIdx.x % TPR;
+    const int64_t worker = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+    if (TPR < 256 && worker >= a.workers) return;
+    const int D = a.dim;
+    // rows of this worker: run `worker % chunks` of gate row `worker / chunks`, or `run` rows anywhere (whole gate rows)
+    int64_t r0, r1;
+    if (a.dgate_direct) {
+        r0 = worker * a.run;
+        r1 = min(a.rows, r0 + a.run);
+    } else {
+        const int64_t group = worker / a.chunks;
+        r0 = group * a.rows_per_gate + worker % a.chunks * a.run;
+        r1 = min((group + 1) * a.rows_per_gate, r0 + a.run);
+    }
+    float sum[kGrads][NU][4];
+#pragma unroll
+    for (int k = 0; k < kGrads; ++k)
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum[k][u][j] = 0.f;
+    const float inv_d = 1.0f / (float)D;
+    for (int64_t row = r0; row < r1; ++row) {
+        const int64_t grow = row / a.rows_per_gate;
+        float y[NU][4], x[NU][4], d[NU][4], e[NU][4], p[NU][4], b[NU][4], g[NU][4], w[NU][4];
+        load_row<TY, TPR, NU, VEC>(y, (const TY*)a.y + row * D, D, t);
+        load_row<TX, TPR, NU, VEC>(x, (const TX*)a.x + row * D, D, t);
+        if (a.dh != nullptr) {
+            load_row<TX, TPR, NU, VEC>(d, (const TX*)a.dh + row * D, D, t);
+        } else {
+#pragma unroll
+            for (int u = 0; u < NU; ++u)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) d[u][j] = 0.f;
+        }
+        const f32x4 st = *(const f32x4*)(a.stats + row * 4);
+        load_param<TY, TPR, NU, VEC>(p, a.post_w, a.w32, 0, 1.f, D, t);
+        load_param<TY, TPR, NU, VEC>(b, a.post_b, a.w32, 0, 0.f, D, t);
+        load_param<TY, TPR, NU, VEC>(g, a.gate, a.g32, grow, 1.f, D, t);
+        const float my = st[0], ry = st[1], mh = st[2], rh = st[3];
+        // y <- N(y), x <- N(h), b <- post
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                y[u][j] = (y[u][j] - my) * ry;
+                b[u][j] = fmaf(y[u][j], p[u][j], b[u][j]);
+                x[u][j] = (fmaf(g[u][j], b[u][j], a.res_scale * x[u][j]) - mh) * rh;
+            }
+        if (a.dz != nullptr) {
+            load_row<TY, TPR, NU, VEC>(e, (const TY*)a.dz + row * D, D, t);
+            load_param<TY, TPR, NU, VEC>(w, a.pre_w, a.w32, 0, 1.f, D, t);
+            float s[2] = {0.f, 0.f};
+#pragma unroll
+            for (int u = 0; u < NU; ++u)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    sum[kPreW][u][j] = fmaf(e[u][j], x[u][j], sum[kPreW][u][j]);
+                    sum[kPreB][u][j] += e[u][j];
+                    e[u][j] *= w[u][j];                       // 0 behind the row's end, as dz is
+                    s[0] = fmaf(e[u][j], x[u][j], s[0]);
+                    s[1] += e[u][j];
+                }
+            row_sums<TPR, 2>(s, red, turn);
+            const float m1 = s[0] * inv_d, m2 = a.layer ? s[1] * inv_d : 0.f;
+#pragma unroll
+            for (int u = 0; u < NU; ++u)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) d[u][j] = fmaf(rh, e[u][j] - fmaf(x[u][j], m1, m2), d[u][j]);
+        }
+        float s[2] = {0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bool in = column<TPR, VEC>(u, j, t) < D;
+                x[u][j] = a.res_scale * d[u][j];
+                b[u][j] = in ? d[u][j] * b[u][j] : 0.f;       // d gate
+                const float dp = in ? d[u][j] * g[u][j] : 0.f;
+                sum[kPostW][u][j] = fmaf(dp, y[u][j], sum[kPostW][u][j]);
+                sum[kPostB][u][j] += dp;
+                sum[kGate][u][j] += b[u][j];
+                e[u][j] = dp * p[u][j];
+                s[0] = fmaf(e[u][j], y[u][j], s[0]);
+                s[1] += e[u][j];
+            }
+        store_row<TX, TPR, NU, VEC>((TX*)a.dx + row * D, x, D, t);
+        row_sums<TPR, 2>(s, red, turn);
+        const float m1 = s[0] * inv_d, m2 = a.layer ? s[1] * inv_d : 0.f;
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) e[u][j] = ry * (e[u][j] - fmaf(y[u][j], m1, m2));
+        store_row<TY, TPR, NU, VEC>((TY*)a.dy + row * D, e, D, t);
+        if (a.dgate_direct && a.dgate != nullptr && (row + 1) % a.rows_per_gate == 0) {
+            if (a.g32) store_row<float, TPR, NU, VEC>((float*)a.dgate + grow * D, sum[kGate], D, t);
+            else store_row<TY, TPR, NU, VEC>((TY*)a.dgate + grow * D, sum[kGate], D, t);
+#pragma unroll
+            for (int u = 0; u < NU; ++u)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum[kGate][u][j] = 0.f;
+        }
+    }
+    float* out = a.slab + worker * kGrads * D;
+#pragma unroll
+    for (int k = 0; k < kGrads; ++k)
+        if (k != kGate || !a.dgate_direct) store_row<float, TPR, NU, VEC>(out + k * D, sum[k], D, t);
+}
+
+// Column sums of the slab: y = gradient (0..3: all workers; from 4 on: gate row y - 4, its own workers), 64 columns x 16 runs of workers a workgroup.
+struct SandwichSums {
+    const float* slab;
+    int64_t workers, chunks;
+    int dim;
+    void* out[4];
+    int w32;
+    void* dgate;
+    int g32;
+};
+template <class TY>
+__global__ __launch_bounds__(1024) void sandwich_sums_kernel(SandwichSums a) {
+    __shared__ float part[16][64];
+    const int lane = threadIdx.x & 63, run = threadIdx.x >> 6, c = blockIdx.x * 64 + lane, k = min((int)blockIdx.y, (int)kGate);
+    const int64_t group = (int64_t)blockIdx.y - kGate;
+    void* out = k < kGate ? a.out[k] : a.dgate;
+    if (out == nullptr) return;                   // the whole workgroup
+    const int64_t w0 = k < kGate ? 0 : group * a.chunks, n = k < kGate ? a.workers : a.chunks, per = (n + 15) / 16;
+    const int64_t b0 = w0 + run * per, b1 = min(w0 + n, b0 + per);
+    float s = 0.f;
+    if (c < a.dim) {
+        const float* p = a.slab + (b0 * kGrads + k) * a.dim + c;
+        const int64_t step = (int64_t)kGrads * a.dim;
+        int64_t i = b0;
+        for (; i + 8 <= b1; i += 8, p += 8 * step) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = p[u * step];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s += v[u];
+        }
+        for (; i < b1; ++i, p += step) s += *p;
+    }
+    part[run][lane] = s;
+    __syncthreads();
+    if (run != 0 || c >= a.dim) return;
+#pragma unroll
+    for (int r = 1; r < 16; ++r) s += part[r][lane];
+    if (k < kGate ? a.w32 : a.g32) ((float*)out)[(k < kGate ? 0 : group * a.dim) + c] = s;
+    else ((TY*)out)[(k < kGate ? 0 : group * a.dim) + c] = (TY)s;
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------
+static int threads_per_row(int dim) { return dim <= 128 ? 32 : dim <= 1024 ? 64 : 256; }
+
+struct SandwichPlan { int direct; int64_t workers, run, chunks; };
+// Workers: enough to fill the chip (8 lane-group workers a workgroup: 4096; workgroup-wide ones: 1024), no more than rows.
+static SandwichPlan sandwich_plan(int64_t rows, int64_t rows_per_gate, int dim) {
+    const int64_t want = threads_per_row(dim) == 256 ? 1024 : 4096;
+    SandwichPlan p{};
+    const int64_t share = (rows + want - 1) / want;
+    if (rows_per_gate <= share) {
+        p.direct = 1, p.chunks = 1;
+        p.run = (share + rows_per_gate - 1) / rows_per_gate * rows_per_gate;
+        p.workers = (rows + p.run - 1) / p.run;
+    } else {
+        const int64_t gates = rows / rows_per_gate;
+        p.chunks = (rows_per_gate + share - 1) / share;
+        p.run = (rows_per_gate + p.chunks - 1) / p.chunks;
+        p.chunks = (rows_per_gate + p.run - 1) / p.run;
+        p.workers = gates * p.chunks;
+    }
+    return p;
+}
+
+template <class TX, class TY>
+static void sandwich_launch(const SandwichArgs& a, bool vec, bool bwd, hipStream_t st) {
+    const int tpr = threads_per_row(a.dim);
+    const int64_t items = bwd ? a.workers : a.rows;
+    const dim3 grid((unsigned)((items + 256 / tpr - 1) / (256 / tpr)));
+#define GO(TPR, NU)                                                                       \
+    do {                                                                                  \
+        if (bwd) {                                                                        \
+            if (vec) sandwich_bwd_kernel<TX, TY, TPR, NU, true><<<grid, 256, 0, st>>>(a); \
+            else sandwich_bwd_kernel<TX, TY, TPR, NU, false><<<grid, 256, 0, st>>>(a);    \
+        } else {                                                                          \
+            if (vec) sandwich_fwd_kernel<TX, TY, TPR, NU, true><<<grid, 256, 0, st>>>(a); \
+            else sandwich_fwd_kernel<TX, TY, TPR, NU, false><<<grid, 256, 0, st>>>(a);    \
+        }                                                                                 \
+    } while (0)
+    const int D = a.dim;
+    if (D <= 128) GO(32, 1);
+    else if (D <= 256) GO(64, 1);
+    else if (D <= 512) GO(64, 2);
+    else if (D <= 1024) GO(64, 4);
+    else if (D <= 2048) GO(256, 2);
+    else if (D <= 4096) GO(256, 4);
+    else GO(256, 8);
+#undef GO
+}
+
+static int sandwich_check(const void* x, int x_dtype, const void* y, int y_dtype, int64_t rows, int dim, int w_dtype, const void* gate, int gate_dtype, int64_t rows_per_gate, int kind) {
+    SNAG_REQUIRE(y_dtype == SNAG_F32 || y_dtype == SNAG_BF16 || y_dtype == SNAG_F16, SNAG_ERR_ARG, "sandwich norm: dtype %d", y_dtype);
+    SNAG_REQUIRE(x_dtype == y_dtype || x_dtype == SNAG_F32, SNAG_ERR_UNSUPPORTED, "sandwich norm: the residual stream is fp32 or of the block output's type");
+    SNAG_REQUIRE(w_dtype == y_dtype || w_dtype == SNAG_F32, SNAG_ERR_UNSUPPORTED, "sandwich norm: weights and biases are fp32 or of the block output's type");
+    SNAG_REQUIRE(gate == nullptr || gate_dtype == y_dtype || gate_dtype == SNAG_F32, SNAG_ERR_UNSUPPORTED, "sandwich norm: the gate is fp32 or of the block output's type");
+    SNAG_REQUIRE(rows >= 0 && dim >= 1, SNAG_ERR_ARG, "sandwich norm: %lld rows of %d", (long long)rows, dim);
+    SNAG_REQUIRE(dim <= SNAG_SANDWICH_MAX_DIM, SNAG_ERR_UNSUPPORTED, "sandwich norm: row width %d > %d", dim, SNAG_SANDWICH_MAX_DIM);
+    SNAG_REQUIRE(rows < (int64_t)1 << 31, SNAG_ERR_UNSUPPORTED, "sandwich norm: %lld rows", (long long)rows);
+    SNAG_REQUIRE(kind == SNAG_NORM_RMS || kind == SNAG_NORM_LAYER, SNAG_ERR_ARG, "sandwich norm: kind %d", kind);
+    SNAG_REQUIRE(gate == nullptr || (rows_per_gate >= 1 && rows % rows_per_gate == 0), SNAG_ERR_ARG, "sandwich norm: %lld rows are not a multiple of %lld rows per gate", (long long)rows,
+                 (long long)rows_per_gate);
+    SNAG_REQUIRE(rows == 0 || (x != nullptr && y != nullptr), SNAG_ERR_ARG, "sandwich norm: null x / y");
+    return SNAG_OK;
+}
+static size_t bytes_of(int dtype) { return dtype == SNAG_F32 ? 4 : 2; }
+static bool aligned4(const void* p, int dtype) { return ((uintptr_t)p & (4 * bytes_of(dtype) - 1)) == 0; }
+
+static void sandwich_go(const SandwichArgs& a, int x_dtype, int y_dtype, bool vec, bool bwd, hipStream_t st) {
+    if (y_dtype == SNAG_F32) sandwich_launch<float, float>(a, vec, bwd, st);
+    else if (y_dtype == SNAG_BF16) x_dtype == SNAG_F32 ? sandwich_launch<float, bf16_t>(a, vec, bwd, st) : sandwich_launch<bf16_t, bf16_t>(a, vec, bwd, st);
+    else x_dtype == SNAG_F32 ? sandwich_launch<float, f16_t>(a, vec, bwd, st) : sandwich_launch<f16_t, f16_t>(a, vec, bwd, st);
+}
+
+}  // namespace snag
+
+using namespace snag;
+
+extern "C" SNAG_API int snag_sandwich_fwd(const void* x, int x_dtype, const void* y, int y_dtype, int64_t rows, int dim, const void* post_w, const void* post_b,
+                                          const void* pre_w, const void* pre_b, int w_dtype, const void* gate, int gate_dtype, int64_t rows_per_gate,
+                                          float res_scale, int kind, float eps, void* h, void* z, float* stats, void* stream) {
+    if (int rc = sandwich_check(x, x_dtype, y, y_dtype, rows, dim, w_dtype, gate, gate_dtype, rows_per_gate, kind)) return rc;
+    if (rows == 0) return SNAG_OK;
+    SNAG_REQUIRE(h != nullptr && z != nullptr, SNAG_ERR_ARG, "sandwich norm: null h / z");
+    SNAG_REQUIRE(stats == nullptr || ((uintptr_t)stats & 15) == 0, SNAG_ERR_ARG, "sandwich norm: stats are not 16-byte aligned");
+    SandwichArgs a{};
+    a.x = x, a.y = y, a.post_w = post_w, a.post_b = post_b, a.pre_w = pre_w, a.pre_b = pre_b, a.gate = gate;
+    a.w32 = w_dtype == SNAG_F32, a.g32 = gate_dtype == SNAG_F32;
+    a.rows = rows, a.rows_per_gate = gate != nullptr ? rows_per_gate : rows, a.dim = dim, a.layer = kind == SNAG_NORM_LAYER, a.res_scale = res_scale, a.eps = eps;
+    a.h = h, a.z = z, a.stats = stats;
+    const bool vec = dim % 4 == 0 && aligned4(x, x_dtype) && aligned4(y, y_dtype) && aligned4(h, x_dtype) && aligned4(z, y_dtype) && aligned4(post_w, w_dtype) &&
+                     aligned4(post_b, w_dtype) && aligned4(pre_w, w_dtype) && aligned4(pre_b, w_dtype) && aligned4(gate, gate_dtype);
+    sandwich_go(a, x_dtype, y_dtype, vec, false, (hipStream_t)stream);
+    return check_launch("sandwich_fwd");
+}
+
+extern "C" SNAG_API int64_t snag_sandwich_work_floats(int64_t rows, int64_t rows_per_gate, int dim) {
+    if (rows <= 0 || rows_per_gate < 1 || dim < 1) return 0;
+    return sandwich_plan(rows, rows_per_gate, dim).workers * kGrads * dim;
+}
+
+extern "C" SNAG_API int snag_sandwich_bwd(const void* x, int x_dtype, const void* y, int y_dtype, int64_t rows, int dim, const void* post_w, const void* post_b,
+                                          const void* pre_w, int w_dtype, const void* gate, int gate_dtype, int64_t rows_per_gate, float res_scale, int kind,
+                                          const float* stats, const void* d_h, const void* d_z, void* d_x, void* d_y, void* d_post_w, void* d_post_b,
+                                          void* d_pre_w, void* d_pre_b, void* d_gate, float* work, int64_t work_floats, void* stream) {
+    if (int rc = sandwich_check(x, x_dtype, y, y_dtype, rows, dim, w_dtype, gate, gate_dtype, rows_per_gate, kind)) return rc;
+    SNAG_REQUIRE(gate != nullptr || d_gate == nullptr, SNAG_ERR_ARG, "sandwich norm backward: d_gate without a gate");
+    SandwichArgs a{};
+    const int64_t rpg = gate != nullptr ? rows_per_gate : (rows > 0 ? rows : 1);
+    SNAG_REQUIRE(rows == 0 || (stats != nullptr && d_x != nullptr && d_y != nullptr), SNAG_ERR_ARG, "sandwich norm backward: null stats / d_x / d_y");
+    SNAG_REQUIRE(((uintptr_t)stats & 15) == 0, SNAG_ERR_ARG, "sandwich norm backward: stats are not 16-byte aligned");
+    SandwichPlan p{};
+    if (rows > 0) p = sandwich_plan(rows, rpg, dim);
+    SNAG_REQUIRE(rows == 0 || (work != nullptr && work_floats >= p.workers * kGrads * dim), SNAG_ERR_ARG, "sandwich norm backward: workspace of %lld floats, %lld needed",
+                 (long long)work_floats, (long long)(p.workers * kGrads * dim));
+    hipStream_t st = (hipStream_t)stream;
+    if (rows > 0) {
+        a.x = x, a.y = y, a.post_w = post_w, a.post_b = post_b, a.pre_w = pre_w, a.gate = gate;
+        a.w32 = w_dtype == SNAG_F32, a.g32 = gate_dtype == SNAG_F32;
+        a.rows = rows, a.rows_per_gate = rpg, a.dim = dim, a.layer = kind == SNAG_NORM_LAYER, a.res_scale = res_scale;
+        a.stats = (float*)stats, a.dh = d_h, a.dz = d_z, a.dx = d_x, a.dy = d_y, a.dgate = d_gate;
+        a.dgate_direct = p.direct, a.workers = p.workers, a.run = p.run, a.chunks = p.chunks, a.slab = work;
+        const bool vec = dim % 4 == 0 && aligned4(x, x_dtype) && aligned4(y, y_dtype) && aligned4(post_w, w_dtype) && aligned4(post_b, w_dtype) &&
+                         aligned4(pre_w, w_dtype) && aligned4(gate, gate_dtype) && aligned4(d_h, x_dtype) && aligned4(d_z, y_dtype) && aligned4(d_x, x_dtype) &&
+                         aligned4(d_y, y_dtype) && aligned4(d_gate, gate_dtype) && aligned16(work);
+        sandwich_go(a, x_dtype, y_dtype, vec, true, st);
+        if (int rc = check_launch("sandwich_bwd")) return rc;
+    }
+    if (d_post_w == nullptr && d_post_b == nullptr && d_pre_w == nullptr && d_pre_b == nullptr && d_gate == nullptr) return SNAG_OK;
+    SandwichSums s{};
+    s.slab = work, s.workers = p.workers, s.chunks = p.chunks, s.dim = dim;
+    s.out[kPostW] = d_post_w, s.out[kPostB] = d_post_b, s.out[kPreW] = d_pre_w, s.out[kPreB] = d_pre_b;
+    s.w32 = w_dtype == SNAG_F32, s.g32 = gate_dtype == SNAG_F32;
+    const int64_t gates = d_gate != nullptr && rows > 0 && !p.direct ? rows / rpg : 0;
+    s.dgate = gates > 0 ? d_gate : nullptr;
+    SNAG_REQUIRE(gates + kGate <= 65535, SNAG_ERR_UNSUPPORTED, "sandwich norm backward: %lld gate rows", (long long)gates);
+    const dim3 grid((unsigned)((dim + 63) / 64), (unsigned)(kGate + gates));
+    if (y_dtype == SNAG_F32) sandwich_sums_kernel<float><<<grid, 1024, 0, st>>>(s);
+    else if (y_dtype == SNAG_BF16) sandwich_sums_kernel<bf16_t><<<grid, 1024, 0, st>>>(s);
+    else sandwich_sums_kernel<f16_t><<<grid, 1024, 0, st>>>(s);
+    return check_launch("sandwich_sums");
+}

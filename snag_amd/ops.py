@@ -3,6 +3,8 @@
 Shape/dtype/contiguity errors are raised in Python before the call, mirroring the reference's
 assert/exception convention (SURVEY.md par. 8b "Errors").
 """
+import ctypes
+
 import torch
 
 from . import _lib
@@ -535,3 +537,259 @@ def sample_negatives(h, r, t, n_neg, n_ent, n_rel, seed, known_sorted=None, head
     call("snag_sample_negatives", int(seed), ptr(tick), ptr(h), ptr(r), ptr(t), B, int(n_neg), int(n_ent), int(n_rel), int(head_or_tail),
          ptr(known_sorted), known_sorted.numel() if known_sorted is not None else 0, ptr(neg_h), ptr(neg_t), stream())
     return (neg_h, neg_t) if head_or_tail else neg_t
+
+
+# --- cross attention, the norms around a block, Muon -----------------------------------------------------------------
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # SNAG_F32, SNAG_BF16, SNAG_F16
+CROSS_MAX_HEAD_DIM = 128       # SNAG_CROSS_MAX_HEAD_DIM
+SANDWICH_MAX_DIM = 8192        # SNAG_SANDWICH_MAX_DIM
+MUON_MAX_SIDE = 16384          # SNAG_MUON_MAX_SIDE
+NORMS = {"rms": 0, "layer": 1}
+
+
+def _any(t, name, ndim=None):
+    """A CUDA tensor of one of the three types these operators take; any strides."""
+    if not torch.is_tensor(t):
+        raise TypeError(f"{name}: expected a torch.Tensor, got {type(t).__name__}")
+    if t.dtype not in DTYPES:
+        raise TypeError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
+    if not t.is_cuda:
+        raise _lib.SnagHipError(f"{name}: tensor is on {t.device}; snag_amd kernels run on the GPU only (no CPU fallback)")
+    if ndim is not None and t.dim() != ndim:
+        raise ValueError(f"{name}: expected {ndim} dims, got shape {tuple(t.shape)}")
+    return t
+
+
+def _call_on(device, name, *args):
+    """The entry on the current stream of the operands' device (which need not be the current one)."""
+    if device.index == torch.cuda.current_device():
+        call(name, *args, stream())
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, stream())
+
+
+def _one_device(device, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, the first operand on {device}")
+
+
+def _cross_args(q, k, v, kv_lens, key_mask, scale):
+    _any(q, "q", 4), _any(k, "k", 4), _any(v, "v", 4)
+    B, Lq, H, d = q.shape
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"q, k and v must share one type, got {q.dtype}, {k.dtype}, {v.dtype}")
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != d:
+        raise ValueError(f"k and v must be [{B}, Lk, Hkv, {d}], got {tuple(k.shape)} and {tuple(v.shape)}")
+    Lk, Hkv = k.shape[1], k.shape[2]
+    if H == 0 or Hkv == 0 or H % Hkv:
+        raise ValueError(f"{H} heads are not a multiple of {Hkv} key/value heads")
+    if not 1 <= d <= CROSS_MAX_HEAD_DIM:
+        raise ValueError(f"head dimension {d} is not in 1..{CROSS_MAX_HEAD_DIM}")
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        if t.numel() and t.stride(3) != 1 and d > 1:
+            raise ValueError(f"{name}: the elements of a head must be adjacent (strides {tuple(t.stride())})")
+    lens_bytes = 4
+    if kv_lens is not None:
+        _idx(kv_lens, "kv_lens", 1)
+        if kv_lens.shape[0] != B:
+            raise ValueError(f"kv_lens must be [{B}], got {tuple(kv_lens.shape)}")
+        lens_bytes = kv_lens.element_size()
+    mask_ld = 0
+    if key_mask is not None:
+        if not torch.is_tensor(key_mask) or key_mask.dtype not in (torch.bool, torch.uint8):
+            raise TypeError("key_mask: expected a bool (or uint8) tensor, true where a key is seen")
+        if tuple(key_mask.shape) != (B, Lk):
+            raise ValueError(f"key_mask must be [{B}, {Lk}], got {tuple(key_mask.shape)}")
+        if not key_mask.is_cuda:
+            raise _lib.SnagHipError(f"key_mask: tensor is on {key_mask.device}; snag_amd kernels run on the GPU only (no CPU fallback)")
+        if Lk > 1 and key_mask.stride(1) != 1:
+            raise ValueError("key_mask: a row's elements must be adjacent")
+        mask_ld = key_mask.stride(0) if B > 1 else Lk
+    _one_device(q.device, k=k, v=v, kv_lens=kv_lens, key_mask=key_mask)
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    strides = (ctypes.c_int64 * 9)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
+    shape = (DTYPES[q.dtype], B, Lq, Lk, H, Hkv, d)
+    return shape, (ptr(q), ptr(k), ptr(v), *shape, ctypes.addressof(strides), ptr(kv_lens), lens_bytes, ptr(key_mask), mask_ld, scale), strides
+
+
+def _cross_work(shape, backward, device):
+    n = _lib.load().snag_cross_work_floats(*shape, int(backward))
+    return (torch.empty(n, device=device, dtype=f32) if n else None), n
+
+
+def cross_attention_fwd(q, k, v, kv_lens=None, key_mask=None, scale=None):
+    """q [B, Lq, H, d], k / v [B, Lk, Hkv, d] (any strides with adjacent head elements) -> out [B, Lq, H, d], lse [B, H, Lq] (log2).
+    C ABI: snag_cross_fwd."""
+    shape, args, hold = _cross_args(q, k, v, kv_lens, key_mask, scale)
+    out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], device=q.device, dtype=f32)
+    work, n = _cross_work(shape, False, q.device)
+    _call_on(q.device, "snag_cross_fwd", *args, ptr(out), ptr(lse), ptr(work), n)
+    return out, lse
+
+
+def cross_attention_bwd(q, k, v, out, lse, d_out, kv_lens=None, key_mask=None, scale=None):
+    """-> d_q, d_k, d_v (dense).  C ABI: snag_cross_bwd."""
+    shape, args, hold = _cross_args(q, k, v, kv_lens, key_mask, scale)
+    for t, name in ((out, "out"), (d_out, "d_out")):
+        _chk(t, name, dtype=q.dtype, ndim=4)
+        if t.shape != q.shape:
+            raise ValueError(f"{name} must be {tuple(q.shape)}, got {tuple(t.shape)}")
+    _chk(lse, "lse", ndim=3)
+    if tuple(lse.shape) != (q.shape[0], q.shape[2], q.shape[1]):
+        raise ValueError(f"lse must be [B, H, Lq], got {tuple(lse.shape)}")
+    _one_device(q.device, out=out, lse=lse, d_out=d_out)
+    dq, dk, dv = (torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k, v))
+    work, n = _cross_work(shape, True, q.device)
+    _call_on(q.device, "snag_cross_bwd", *args, ptr(out), ptr(lse), ptr(d_out), ptr(dq), ptr(dk), ptr(dv), ptr(work), n)
+    return dq, dk, dv
+
+
+def _sandwich_args(x, y, post_weight, post_bias, pre_weight, pre_bias, gate, kind):
+    """-> rows, dim, (weights' dtype code), (gate dtype code), rows per gate row."""
+    _any(x, "x"), _any(y, "y")
+    if x.shape != y.shape or x.dim() < 1:
+        raise ValueError(f"x and y must have one shape [..., dim], got {tuple(x.shape)} and {tuple(y.shape)}")
+    for t, name in ((x, "x"), (y, "y")):
+        if not t.is_contiguous():
+            raise ValueError(f"{name}: tensor must be contiguous")
+    if x.dtype not in (y.dtype, f32):
+        raise TypeError(f"x (the residual stream) must be float32 or of y's type {y.dtype}, got {x.dtype}")
+    if kind not in NORMS:
+        raise ValueError(f"kind must be one of {sorted(NORMS)}, got {kind!r}")
+    dim = x.shape[-1]
+    if not 1 <= dim <= SANDWICH_MAX_DIM:
+        raise ValueError(f"row width {dim} is not in 1..{SANDWICH_MAX_DIM}")
+    rows = x.numel() // dim
+    wt = None
+    for t, name in ((post_weight, "post_weight"), (post_bias, "post_bias"), (pre_weight, "pre_weight"), (pre_bias, "pre_bias")):
+        if t is None:
+            continue
+        _any(t, name, 1)
+        if t.shape[0] != dim or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous [{dim}], got {tuple(t.shape)}")
+        if t.dtype not in (y.dtype, f32) or wt not in (None, t.dtype):
+            raise TypeError(f"weights and biases must share one type, float32 or y's {y.dtype}; {name} is {t.dtype}")
+        wt = t.dtype
+    per_gate, gt = max(rows, 1), y.dtype
+    if gate is not None:
+        _any(gate, "gate")
+        if gate.dim() not in (1, 2) or gate.shape[-1] != dim or not gate.is_contiguous():
+            raise ValueError(f"gate must be a contiguous [{dim}] or [G, {dim}], got {tuple(gate.shape)}")
+        if gate.dtype not in (y.dtype, f32):
+            raise TypeError(f"gate must be float32 or of y's type {y.dtype}, got {gate.dtype}")
+        G = gate.shape[0] if gate.dim() == 2 else 1
+        if rows and (G == 0 or rows % G):
+            raise ValueError(f"{rows} rows do not divide among {G} gate rows")
+        per_gate, gt = (max(rows // G, 1) if G else 1), gate.dtype
+    _one_device(x.device, y=y, post_weight=post_weight, post_bias=post_bias, pre_weight=pre_weight, pre_bias=pre_bias, gate=gate)
+    return rows, dim, DTYPES[wt if wt is not None else y.dtype], DTYPES[gt], per_gate
+
+
+def sandwich_norm_fwd(x, y, post_weight=None, pre_weight=None, post_bias=None, pre_bias=None, gate=None, res_scale=1.0, kind="rms", eps=1e-6, want_stats=True):
+    """h = res_scale x + gate (post_weight N(y) + post_bias), z = pre_weight N(h) + pre_bias -> h, z, stats [rows, 4] (or None).
+    C ABI: snag_sandwich_fwd."""
+    rows, dim, wt, gt, per_gate = _sandwich_args(x, y, post_weight, post_bias, pre_weight, pre_bias, gate, kind)
+    h, z = torch.empty_like(x), torch.empty_like(y)
+    stats = torch.empty(rows, 4, device=x.device, dtype=f32) if want_stats else None
+    _call_on(x.device, "snag_sandwich_fwd", ptr(x), DTYPES[x.dtype], ptr(y), DTYPES[y.dtype], rows, dim, ptr(post_weight), ptr(post_bias), ptr(pre_weight),
+             ptr(pre_bias), wt, ptr(gate), gt, per_gate, float(res_scale), NORMS[kind], float(eps), ptr(h), ptr(z), ptr(stats))
+    return h, z, stats
+
+
+def sandwich_norm_bwd(x, y, stats, d_h, d_z, post_weight=None, pre_weight=None, post_bias=None, pre_bias=None, gate=None, res_scale=1.0, kind="rms"):
+    """-> d_x, d_y, d_post_weight, d_pre_weight, d_post_bias, d_pre_bias, d_gate (None for a parameter that is None).  d_h or d_z may be None (zero).
+    C ABI: snag_sandwich_bwd."""
+    rows, dim, wt, gt, per_gate = _sandwich_args(x, y, post_weight, post_bias, pre_weight, pre_bias, gate, kind)
+    for t, like, name in ((d_h, x, "d_h"), (d_z, y, "d_z")):
+        if t is not None:
+            _chk(t, name, dtype=like.dtype)
+            if t.shape != like.shape:
+                raise ValueError(f"{name} must be {tuple(like.shape)}, got {tuple(t.shape)}")
+    _chk(stats, "stats", ndim=2)
+    if tuple(stats.shape) != (rows, 4):
+        raise ValueError(f"stats must be [{rows}, 4], got {tuple(stats.shape)}")
+    _one_device(x.device, stats=stats, d_h=d_h, d_z=d_z)
+    new = lambda t: None if t is None else torch.empty_like(t) if rows else torch.zeros_like(t)
+    dx, dy, dpw, dqw, dpb, dqb, dg = (new(t) for t in (x, y, post_weight, pre_weight, post_bias, pre_bias, gate))
+    n = _lib.load().snag_sandwich_work_floats(rows, per_gate, dim)
+    work = torch.empty(n, device=x.device, dtype=f32)
+    _call_on(x.device, "snag_sandwich_bwd", ptr(x), DTYPES[x.dtype], ptr(y), DTYPES[y.dtype], rows, dim, ptr(post_weight), ptr(post_bias), ptr(pre_weight), wt,
+             ptr(gate), gt, per_gate, float(res_scale), NORMS[kind], ptr(stats), ptr(d_h), ptr(d_z), ptr(dx), ptr(dy), ptr(dpw), ptr(dpb), ptr(dqw), ptr(dqb),
+             ptr(dg), ptr(work), n)
+    return dx, dy, dpw, dqw, dpb, dqb, dg
+
+
+def _matrices(ts, name, dtype=None, shapes=None):
+    """A list of contiguous 2-D CUDA tensors of one type on one device."""
+    ts = list(ts)
+    for i, t in enumerate(ts):
+        _any(t, f"{name}[{i}]", 2)
+        if t.dtype != (dtype or ts[0].dtype):
+            raise TypeError(f"{name}[{i}]: expected {dtype or ts[0].dtype}, got {t.dtype}")
+        if not t.is_contiguous():
+            raise ValueError(f"{name}[{i}]: tensor must be contiguous")
+        if shapes is not None and tuple(t.shape) != tuple(shapes[i]):
+            raise ValueError(f"{name}[{i}] must be {tuple(shapes[i])}, got {tuple(t.shape)}")
+        if not (1 <= t.shape[0] <= MUON_MAX_SIDE and 1 <= t.shape[1] <= MUON_MAX_SIDE):
+            raise ValueError(f"{name}[{i}]: sides must be in 1..{MUON_MAX_SIDE}, got {tuple(t.shape)}")
+        _one_device(ts[0].device, **{f"{name}[{i}]": t})
+    return ts
+
+
+def _muon_lists(*lists):
+    return [(ctypes.c_void_p * len(ts))(*[t.data_ptr() for t in ts]) for ts in lists]
+
+
+def _muon_shapes(ts):
+    n = len(ts)
+    rows, cols = (ctypes.c_int32 * n)(*[t.shape[0] for t in ts]), (ctypes.c_int32 * n)(*[t.shape[1] for t in ts])
+    nbytes = _lib.load().snag_muon_work_bytes(ctypes.addressof(rows), ctypes.addressof(cols), n)
+    return rows, cols, torch.empty(nbytes, device=ts[0].device, dtype=torch.uint8), nbytes
+
+
+def orthogonalize(gs, outs=None, steps=5, eps=1e-7):
+    """Newton-Schulz orthogonalisation of a list of matrices of one type -> list (or into ``outs``; outs[i] may be gs[i]).
+    C ABI: snag_orthogonalize."""
+    gs = _matrices(gs, "gs")
+    if not 1 <= int(steps) <= 100:
+        raise ValueError(f"steps must be in 1..100, got {steps}")
+    outs = [torch.empty_like(g) for g in gs] if outs is None else _matrices(outs, "outs", gs[0].dtype if gs else None, [g.shape for g in gs])
+    if len(outs) != len(gs):
+        raise ValueError(f"{len(gs)} matrices, {len(outs)} outputs")
+    if not gs:
+        return outs
+    _one_device(gs[0].device, outs=outs[0])
+    rows, cols, work, n = _muon_shapes(gs)
+    pg, po = _muon_lists(gs, outs)
+    _call_on(gs[0].device, "snag_orthogonalize", ctypes.addressof(pg), ctypes.addressof(po), ctypes.addressof(rows), ctypes.addressof(cols), len(gs),
+             DTYPES[gs[0].dtype], int(steps), float(eps), ptr(work), n)
+    return outs
+
+
+def muon_step(weights, grads, momenta, lr, momentum=0.95, nesterov=True, weight_decay=0.0, match_rms=False, steps=5, eps=1e-7):
+    """One Muon update, in place on ``weights`` (one type) and ``momenta`` (fp32); ``grads`` have the weights' type.  C ABI: snag_muon_step."""
+    weights = _matrices(weights, "weights")
+    shapes = [w.shape for w in weights]
+    grads, momenta = list(grads), list(momenta)
+    if len(grads) != len(weights) or len(momenta) != len(weights):
+        raise ValueError(f"{len(weights)} weights, {len(grads)} gradients, {len(momenta)} momenta")
+    if not 1 <= int(steps) <= 100:
+        raise ValueError(f"steps must be in 1..100, got {steps}")
+    if not 0.0 <= momentum < 1.0:
+        raise ValueError(f"momentum must be in [0, 1), got {momentum}")
+    if not weights:
+        return
+    _matrices(grads, "grads", weights[0].dtype, shapes), _matrices(momenta, "momenta", f32, shapes)
+    _one_device(weights[0].device, grads=grads[0], momenta=momenta[0])
+    if len({t.data_ptr() for t in weights}) != len(weights) or len({t.data_ptr() for t in momenta}) != len(momenta):
+        raise ValueError("a matrix is listed twice")
+    rows, cols, work, n = _muon_shapes(weights)
+    pw, pg, pm = _muon_lists(weights, grads, momenta)
+    _call_on(weights[0].device, "snag_muon_step", ctypes.addressof(pw), ctypes.addressof(pg), ctypes.addressof(pm), ctypes.addressof(rows), ctypes.addressof(cols),
+             len(weights), DTYPES[weights[0].dtype], float(lr), float(momentum), int(nesterov), float(weight_decay), int(match_rms), int(steps), float(eps),
+             ptr(work), n)

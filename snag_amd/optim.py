@@ -2,9 +2,88 @@
 called from main.py:92): parameter groups by NAME -- for ``model_name == "SNAG"`` anything containing ``weight_raw`` / ``bias`` /
 ``multi_loss_layer`` is not decayed and ``multi_loss_layer`` runs at 5x the learning rate -- AdamW or Adam, and the fixed / linear /
 cosine schedules with warm-up.  Plain host code on torch.optim: the drop-in ``snag_amd.mmea.SNAG`` keeps the reference's parameter
-names, so the groups come out identical (golden G14)."""
+names, so the groups come out identical (golden G14).
+
+Not in the reference: ``orthogonalize`` / ``muon_step`` (HIP, csrc/muon.hip) and the ``Muon`` optimiser, which ``set_optim`` builds for
+``opt.optim == "muon"`` -- each group above is then cut into its matrices (Muon, at ``opt.muon_lr`` if given) and the rest (AdamW)."""
 import torch
 from torch import optim
+from torch.optim.adamw import adamw
+
+from . import ops
+
+
+def orthogonalize(matrices, steps=5, eps=1e-7):
+    """Newton-Schulz orthogonalisation on the matrix pipe: X = G / (|G|_F + eps), then ``steps`` times X <- a X + (b A + c A^2) X with
+    A = X X^T and (a, b, c) = (3.4445, -4.7750, 2.0315), which takes every singular value that is not tiny into about 0.7 .. 1.2.
+    One matrix or a list of matrices of one type (fp32, bf16, fp16) -> the same, new tensors.  All matrices of a list share the launches."""
+    if torch.is_tensor(matrices):
+        return ops.orthogonalize([matrices.detach()], steps=steps, eps=eps)[0]
+    return ops.orthogonalize([m.detach() for m in matrices], steps=steps, eps=eps)
+
+
+def muon_step(weights, grads, momenta, lr, momentum=0.95, nesterov=True, weight_decay=0.0, match_rms=False, steps=5, eps=1e-7):
+    """One Muon update of a list of matrices, in place: M <- mu M + (1 - mu) G; U = (1 - mu) G + mu M (``nesterov``) or M;
+    W <- (1 - lr weight_decay) W - lr s orthogonalize(U), s = sqrt(max(1, rows / cols)) or, with ``match_rms``, 0.2 sqrt(max(rows, cols)).
+    ``momenta`` are fp32, ``grads`` of the weights' type."""
+    ops.muon_step([w.detach() for w in weights], [g.detach() for g in grads], momenta, lr, momentum, nesterov, weight_decay, match_rms, steps, eps)
+
+
+class Muon(optim.Optimizer):
+    """Muon for matrices (``muon=True`` groups, the default: every parameter is 2-D) and AdamW for what is none (``muon=False`` groups), as one
+    torch optimiser.  State: fp32 ``momentum_buffer`` per matrix."""
+
+    def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, match_rms=False, steps=5, eps=1e-7, betas=(0.9, 0.999), adam_eps=1e-8):
+        if lr < 0 or weight_decay < 0 or not 0 <= momentum < 1:
+            raise ValueError(f"Muon: lr {lr}, momentum {momentum}, weight_decay {weight_decay}")
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, match_rms=match_rms, steps=steps, eps=eps,
+                                      betas=betas, adam_eps=adam_eps, muon=True))
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        group = self.param_groups[-1]
+        if group["muon"] and any(p.dim() != 2 for p in group["params"]):
+            self.param_groups.pop()
+            raise ValueError("Muon: a parameter that is not a matrix (put it into a group with muon=False)")
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            ps = [p for p in group["params"] if p.grad is not None]
+            if group["muon"]:
+                self._muon(group, ps)
+            elif ps:
+                self._adamw(group, ps)
+        return loss
+
+    def _muon(self, group, ps):
+        for p in ps:
+            if not self.state[p]:
+                self.state[p]["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
+        lists = {}                                       # one call per type and device
+        for p in ps:
+            lists.setdefault((p.dtype, p.device), []).append(p)
+        for same in lists.values():
+            muon_step(same, [p.grad.contiguous() for p in same], [self.state[p]["momentum_buffer"] for p in same], group["lr"], group["momentum"],
+                      group["nesterov"], group["weight_decay"], group["match_rms"], group["steps"], group["eps"])
+
+    def _adamw(self, group, ps):
+        for p in ps:
+            st = self.state[p]
+            if not st:
+                st["step"], st["exp_avg"], st["exp_avg_sq"] = torch.zeros(()), torch.zeros_like(p), torch.zeros_like(p)
+        st = [self.state[p] for p in ps]
+        adamw(ps, [p.grad for p in ps], [s["exp_avg"] for s in st], [s["exp_avg_sq"] for s in st], [], [s["step"] for s in st], amsgrad=False,
+              beta1=group["betas"][0], beta2=group["betas"][1], lr=group["lr"], weight_decay=group["weight_decay"], eps=group["adam_eps"], maximize=False)
+
+
+def _is_matrix(name, p):
+    """What Muon updates: matrices that are multiplied by; tables that rows are looked up in and weights of other ranks stay with AdamW."""
+    return p.dim() == 2 and min(p.shape) > 1 and "emb" not in name
 
 
 def set_optim(opt, model_list, freeze_part=(), no_freeze_part=(), accumulation_step=None):
@@ -33,6 +112,15 @@ def set_optim(opt, model_list, freeze_part=(), no_freeze_part=(), accumulation_s
         optimizer = optim.AdamW(groups, lr=opt.lr, eps=opt.adam_epsilon)
     elif opt.optim == "adam":
         optimizer = optim.Adam(groups, lr=opt.lr)
+    elif opt.optim == "muon":
+        names = {p: n for n, p in named}
+        cut = []
+        for g in groups:
+            for muon in (True, False):
+                ps = [p for p in g["params"] if _is_matrix(names[p], p) == muon]
+                if ps:
+                    cut.append({**g, "params": ps, "muon": muon, "lr": getattr(opt, "muon_lr", g["lr"]) if muon else g["lr"]})
+        optimizer = Muon(cut, lr=opt.lr, adam_eps=opt.adam_epsilon)
     else:
         raise ValueError(f"unknown optimiser {opt.optim!r}")
     if accumulation_step is None:
