@@ -20,18 +20,13 @@ from .projection import Linear, ProjectionHead
 LN2 = math.log(2.0)
 
 
-def _note_leaves(*ts):
-    """A leaf's gradient node belongs to the stream of the first live graph that reaches it.  A backward captured on another stream would pull
-    that stream into the capture, and torch then ends the process: refuse such a capture while an earlier graph made here is alive.
-    -> the nodes, to be held until the new graph holds them."""
-    st, nodes = None, []
-    for t in ts:
-        if t is not None and t.requires_grad and t.is_leaf:
-            st = _lib.stream() if st is None else st
-            nodes.append(torch.autograd.graph.get_gradient_edge(t).node)
-            if nodes[-1].metadata.setdefault("snag_stream", st) != st and torch.cuda.is_current_stream_capturing():
-                raise _lib.SnagHipError("a backward cannot be captured while an eager graph of the same leaves lives on another stream: drop that graph's outputs first")
-    return nodes
+def _note_stream(out):
+    """A gradient node belongs to the stream it was made on, a leaf's to that of the first live graph that reaches it.  A backward captured on
+    another stream would pull that stream into the capture, and torch then ends the process: refuse the capture while such a graph is alive."""
+    st = ops._raw_stream(out.device.index)
+    for node, _ in out.grad_fn.next_functions:
+        if node is not None and node.metadata.setdefault("snag_stream", st) != st and torch.cuda.is_current_stream_capturing():
+            raise _lib.SnagHipError("a backward cannot be captured while an eager graph of the same leaves lives on another stream: drop that graph's outputs first")
 
 
 class _CrossAttentionFn(torch.autograd.Function):
@@ -59,10 +54,9 @@ def cross_attention(q, k, v, kv_lens=None, key_mask=None, scale=None, return_lse
     ``kv_lens`` [B] (int32 / int64, on the device): keys at and behind it are not seen; ``key_mask`` [B, Lk] (bool): nor are those that are
     False.  Unseen keys may hold anything.  A query that sees no key gets zeros, and gives none of its gradient on.  ``scale`` defaults to d ** -0.5.
     ``return_lse`` adds the natural log-sum-exp of every row's scores [B, H, Lq] (-inf where no key is seen), not differentiable."""
-    _lib.require_gpu()
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        nodes = _note_leaves(q, k, v)
         out, lse = _CrossAttentionFn.apply(q, k, v, kv_lens, key_mask, scale)
+        _note_stream(out)
     else:
         out, lse = ops.cross_attention_fwd(q, k, v, kv_lens, key_mask, scale)
     return (out, lse * LN2) if return_lse else out
@@ -93,12 +87,12 @@ def sandwich_norm(x, y, post_weight=None, pre_weight=None, post_bias=None, pre_b
     (v / sqrt(mean v^2 + eps)) or "layer" (around the mean, biased variance).  ``gate`` [dim], or [G, dim] whose rows serve rows / G
     neighbouring rows each (one gate per sequence, or per row).  x may stay fp32 while y is 16-bit; h has x's type, z y's.  Weights and biases
     share one type, fp32 or y's; so does the gate.  Differentiable in every tensor."""
-    _lib.require_gpu()
     x, y = x.contiguous(), y.contiguous()
     params = (post_weight, pre_weight, post_bias, pre_bias, gate)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, y, *params)):
-        nodes = _note_leaves(x, y, *params)
-        return _SandwichNormFn.apply(x, y, *params, res_scale, kind, eps)
+        h, z = _SandwichNormFn.apply(x, y, *params, res_scale, kind, eps)
+        _note_stream(h)
+        return h, z
     h, z, _ = ops.sandwich_norm_fwd(x, y, *params, res_scale, kind, eps, want_stats=False)
     return h, z
 

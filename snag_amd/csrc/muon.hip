@@ -34,8 +34,7 @@ using s16x4 = __attribute__((ext_vector_type(4))) short;
 
 constexpr float kNsA = 3.4445f, kNsB = -4.7750f, kNsC = 2.0315f;
 constexpr float kScaleX = 16384.f, kScaleA = 8192.f;
-constexpr int kTile = 128, kDepth = 64;        // output tile, contraction per LDS stage
-constexpr int kMaxList = 24;                   // matrices per launch (they travel as kernel arguments)
+constexpr int kMaxList = 24;                   // matrices per launch (they travel as kernel arguments of the first one)
 constexpr int kNormParts = 256;                // partial sums of |U|^2 per matrix
 
 struct MuonMatrix {
@@ -45,35 +44,35 @@ struct MuonMatrix {
     char* work;              // this matrix's workspace
     int r, c, m, n, mp, np;  // shape; m <= n; both rounded up to whole tiles
     int tall, splits;        // A is summed from `splits` ranges of n
-    int first[3];            // first workgroup of this matrix in a product launch (A, B, X)
     float update;            // lr * s
+    int pad;
 };
-struct MuonList {
-    MuonMatrix a[kMaxList];
+// What every launch needs, in device memory: kernel arguments lie in host memory, and a launch of a few workgroups spent most of its time on
+// the chain of reads that finds its matrix (15 us for one tile).  The first launch of an update writes it.
+struct MuonTable {
+    int first[3][kMaxList];  // first workgroup of a matrix in a product launch (A, B, X)
     int count, dtype, step, nesterov;
     float mu, keep, eps;     // keep = 1 - lr * decay
+    int pad;
+    MuonMatrix a[kMaxList];
 };
+static_assert(sizeof(MuonTable) <= 4096 && sizeof(MuonTable) % 16 == 0 && sizeof(MuonMatrix) % 8 == 0, "travels as kernel arguments");
+constexpr int kTableBytes = 4096;
 
 // workspace of one matrix
-struct Planes { _Float16 *xh[2], *xl[2], *rh, *rl, *bh, *bl; float *da, *db, *slab; double* norm; };
-__host__ __device__ inline Planes planes_of(const MuonMatrix& a) {
-    Planes p;
-    const int64_t x = (int64_t)a.mp * a.np, s = (int64_t)a.mp * a.mp;
-    _Float16* h = (_Float16*)a.work;
-    p.xh[0] = h, p.xl[0] = h + x, p.xh[1] = h + 2 * x, p.xl[1] = h + 3 * x;
-    h += 4 * x;
-    p.rh = h, p.rl = h + s, p.bh = h + 2 * s, p.bl = h + 3 * s;
-    h += 4 * s;
-    p.norm = (double*)h;
-    float* f = (float*)(p.norm + kNormParts);
-    p.da = f, p.db = f + a.mp, p.slab = f + 2 * a.mp;
-    return p;
-}
+__host__ __device__ inline int64_t plane_x(const MuonMatrix& a) { return (int64_t)a.mp * a.np; }
+__host__ __device__ inline int64_t plane_s(const MuonMatrix& a) { return (int64_t)a.mp * a.mp; }
+// X in copy `k` (the iterations alternate), plane 0 = hi, 1 = lo
+__device__ __forceinline__ _Float16* x_plane(const MuonMatrix& a, int k, int plane) { return (_Float16*)a.work + (2 * k + plane) * plane_x(a); }
+// plane 0, 1: off-diagonal part of A; 2, 3: of B
+__device__ __forceinline__ _Float16* s_plane(const MuonMatrix& a, int plane) { return (_Float16*)a.work + 4 * plane_x(a) + plane * plane_s(a); }
+__device__ __forceinline__ double* norm_of(const MuonMatrix& a) { return (double*)((_Float16*)a.work + 4 * plane_x(a) + 4 * plane_s(a)); }
+// diagonals of A (0) and B (1)
+__device__ __forceinline__ float* diagonal(const MuonMatrix& a, int which) { return (float*)(norm_of(a) + kNormParts) + which * a.mp; }
+__device__ __forceinline__ float* slab_of(const MuonMatrix& a) { return (float*)(norm_of(a) + kNormParts) + 2 * a.mp; }
 
+template <int DT> using TypeOf = std::conditional_t<DT == SNAG_F32, float, std::conditional_t<DT == SNAG_BF16, bf16_t, f16_t>>;
 template <class T> __device__ __forceinline__ float value(const void* p, int64_t i) { return (float)((const T*)p)[i]; }
-__device__ __forceinline__ float value_of(const void* p, int dtype, int64_t i) {
-    return dtype == SNAG_F32 ? value<float>(p, i) : dtype == SNAG_BF16 ? value<bf16_t>(p, i) : value<f16_t>(p, i);
-}
 
 __device__ __forceinline__ void split16(float v, _Float16& hi, _Float16& lo) {
     hi = (_Float16)v;
@@ -81,89 +80,96 @@ __device__ __forceinline__ void split16(float v, _Float16& hi, _Float16& lo) {
 }
 
 // ---- momentum and norm: grid (kNormParts, matrices) ----------------------------------------------------------------------
-__device__ __forceinline__ float update_of(const MuonList& L, float g, float m) { return L.nesterov ? fmaf(1.f - L.mu, g, L.mu * m) : m; }
+__device__ __forceinline__ float update_of(int nesterov, float mu, float g, float m) { return nesterov ? fmaf(1.f - mu, g, mu * m) : m; }
 
-template <int DT>
-__global__ __launch_bounds__(256) void muon_norm_kernel(MuonList L) {
-    const MuonMatrix& a = L.a[blockIdx.y];
-    using T = std::conditional_t<DT == SNAG_F32, float, std::conditional_t<DT == SNAG_BF16, bf16_t, f16_t>>;
+template <int DT, bool VEC>
+__global__ __launch_bounds__(256) void muon_norm_kernel(MuonTable L, MuonTable* __restrict__ table) {
+    const MuonMatrix a = L.a[blockIdx.y];
+    using T = TypeOf<DT>;
+    if (blockIdx.x == 0 && blockIdx.y == 0) {
+        const int* src = (const int*)&L;
+        for (int i = threadIdx.x; i < (int)(sizeof(MuonTable) / 4); i += 256) ((int*)table)[i] = src[i];
+    }
     const int64_t n = (int64_t)a.r * a.c;
     double s = 0.0;                                // the norm of gradients of any size: fp32 squares would end at 1e19
-    auto one = [&](int64_t i) {
-        float u = value<T>(a.g, i);
-        if (L.step) {
-            const float m = fmaf(L.mu, a.mom[i], (1.f - L.mu) * u);
-            a.mom[i] = m;
-            u = update_of(L, u, m);
-        }
-        return u;
-    };
-    // four neighbours a turn: their squares are summed in double as well
     const int64_t step = (int64_t)gridDim.x * 256 * 4;
     for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += step) {
+        float u[4];
+        if (VEC) {
+            using V = __attribute__((ext_vector_type(4))) T;
+            const V v = *(const V*)((const T*)a.g + i);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (i + j < n) {
-                const double u = (double)one(i + j);
-                s += u * u;
+            for (int j = 0; j < 4; ++j) u[j] = (float)v[j];
+            if (L.step) {
+                f32x4 m = *(const f32x4*)(a.mom + i);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) m[j] = fmaf(L.mu, m[j], (1.f - L.mu) * u[j]), u[j] = update_of(L.nesterov, L.mu, u[j], m[j]);
+                *(f32x4*)(a.mom + i) = m;
             }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                u[j] = 0.f;
+                if (i + j >= n) continue;
+                u[j] = value<T>(a.g, i + j);
+                if (L.step) {
+                    const float m = fmaf(L.mu, a.mom[i + j], (1.f - L.mu) * u[j]);
+                    a.mom[i + j] = m;
+                    u[j] = update_of(L.nesterov, L.mu, u[j], m);
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s += (double)u[j] * (double)u[j];
     }
     __shared__ double red[4];
 #pragma unroll
     for (int x = 32; x > 0; x >>= 1) s += __shfl_xor(s, x);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
-    if (threadIdx.x == 0) planes_of(a).norm[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+    if (threadIdx.x == 0) norm_of(a)[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
 }
 
 // ---- X = U / (|U| + eps) as (hi, lo), padded with zeros: 64 x 64 blocks of X ----------------------------------------------
 template <int DT>
-__global__ __launch_bounds__(256) void muon_start_kernel(MuonList L) {
+__global__ __launch_bounds__(256) void muon_start_kernel(const MuonTable* __restrict__ L) {
     __shared__ float tile[64][65];
     __shared__ double red[4];
-    const MuonMatrix& a = L.a[blockIdx.y];
-    using T = std::conditional_t<DT == SNAG_F32, float, std::conditional_t<DT == SNAG_BF16, bf16_t, f16_t>>;
-    const Planes p = planes_of(a);
+    const MuonMatrix a = L->a[blockIdx.y];
+    using T = TypeOf<DT>;
+    const int step = L->step, nesterov = L->nesterov;
+    const float mu = L->mu;
     const int cols = a.np / 64, blocks = (a.mp / 64) * cols;
     if ((int)blockIdx.x >= blocks) return;         // the whole workgroup
-    double s = p.norm[threadIdx.x];
+    double s = norm_of(a)[threadIdx.x];
 #pragma unroll
     for (int x = 32; x > 0; x >>= 1) s += __shfl_xor(s, x);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
-    const double norm = sqrt(red[0] + red[1] + red[2] + red[3]) + (double)L.eps;
-    const float inv = (float)((double)kScaleX / norm);
+    const double norm = sqrt(red[0] + red[1] + red[2] + red[3]) + (double)L->eps;
+    const double inv = (double)kScaleX / norm;     // beyond fp32's range for tiny gradients
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    _Float16 *xh = x_plane(a, 0, 0), *xl = x_plane(a, 0, 1);
+    auto u_at = [&](int r, int c) {
+        if (r >= a.r || c >= a.c) return 0.f;
+        const int64_t at = (int64_t)r * a.c + c;
+        float v = value<T>(a.g, at);
+        if (step) v = update_of(nesterov, mu, v, a.mom[at]);
+        return (float)((double)v * inv);
+    };
     for (int blk = blockIdx.x; blk < blocks; blk += gridDim.x) {
         const int i0 = blk / cols * 64, j0 = blk % cols * 64;       // rows and columns of X
         if (a.tall) {
             __syncthreads();
-            for (int u = wave; u < 64; u += 4) {                    // row j0 + u of U, column i0 + lane
-                const int r = j0 + u, c = i0 + lane;
-                float v = 0.f;
-                if (r < a.r && c < a.c) {
-                    const int64_t at = (int64_t)r * a.c + c;
-                    v = value<T>(a.g, at);
-                    if (L.step) v = update_of(L, v, a.mom[at]);
-                }
-                tile[u][lane] = v;
-            }
+            for (int u = wave; u < 64; u += 4) tile[u][lane] = u_at(j0 + u, i0 + lane);
             __syncthreads();
         }
         for (int u = wave; u < 64; u += 4) {
-            const int r = i0 + u, c = j0 + lane;
-            float v = 0.f;
-            if (a.tall) {
-                v = tile[lane][u];
-            } else if (r < a.r && c < a.c) {
-                const int64_t at = (int64_t)r * a.c + c;
-                v = value<T>(a.g, at);
-                if (L.step) v = update_of(L, v, a.mom[at]);
-            }
+            const int64_t at = (int64_t)(i0 + u) * a.np + j0 + lane;
             _Float16 hi, lo;
-            split16(v * inv, hi, lo);
-            p.xh[0][(int64_t)r * a.np + c] = hi;
-            p.xl[0][(int64_t)r * a.np + c] = lo;
+            split16(a.tall ? tile[lane][u] : u_at(i0 + u, j0 + lane), hi, lo);
+            xh[at] = hi;
+            xl[at] = lo;
         }
     }
 }
@@ -171,27 +177,55 @@ __global__ __launch_bounds__(256) void muon_start_kernel(MuonList L) {
 // ---- products -------------------------------------------------------------------------------------------------------------
 enum { kGram, kPoly, kApply };
 
-struct TileAt { int matrix, i, j, split; };
-template <int MODE>
-__device__ __forceinline__ TileAt tile_at(const MuonList& L) {
-    TileAt t;
-    const int id = (int)xcd_order(blockIdx.x, gridDim.x);
-    t.matrix = 0;
-    while (t.matrix + 1 < L.count && id >= L.a[t.matrix + 1].first[MODE]) ++t.matrix;
-    const MuonMatrix& a = L.a[t.matrix];
-    int k = id - a.first[MODE];
-    t.split = 0;
-    if (MODE == kApply) {
-        t.i = k % (a.mp / kTile);                  // the tiles of one column block read the same X
-        t.j = k / (a.mp / kTile);
-    } else {
-        if (MODE == kGram) t.split = k % a.splits, k /= a.splits;
-        t.i = (int)((sqrtf(8.f * k + 1.f) - 1.f) * 0.5f);
-        while ((t.i + 1) * (t.i + 2) / 2 <= k) ++t.i;
-        while (t.i * (t.i + 1) / 2 > k) --t.i;
-        t.j = k - t.i * (t.i + 1) / 2;
+// Two workgroup shapes: 4 waves on a 128 x 128 tile (64 x 64 a wave), 8 waves on a 256 x 256 tile (128 x 64 a wave); 64 / PLANES of the contraction
+// per LDS stage, NST stages.
+template <int TILE, int PLANES, int NST> struct Shape {
+    static constexpr int kWaves = TILE == 128 ? 4 : 8, kThreads = kWaves * 64;
+    static constexpr int kWm = TILE / 2, kWn = 64;                     // a wave's part
+    static constexpr int kDepth = 64 / PLANES, kChunks = kDepth / 8;   // 16-byte chunks per row of a stage
+    static constexpr int kOperand = TILE * kDepth, kStage = 2 * PLANES * kOperand;     // fp16 values
+    static constexpr int kLoads = kStage / 8 / kThreads;               // 16-byte loads of a thread per stage
+    static constexpr size_t kLds = NST * kStage * sizeof(_Float16);
+};
+
+// Tile order: squares of 8 x 8 tiles one after another, so that the tiles that one XCD works on at a time share their operands in its L2.
+constexpr int kSquare = 8;
+__device__ __forceinline__ void tri_at(int k, int t, int& i, int& j) {     // tile k of those on and below the diagonal of t x t
+    int I = 0, rows = min(kSquare, t);
+    for (;;) {
+        const int n = I * kSquare * rows + rows * (rows + 1) / 2;
+        if (k < n) break;
+        k -= n;
+        ++I;
+        rows = min(kSquare, t - I * kSquare);
     }
-    return t;
+    const int J = k / (kSquare * rows);
+    if (J < I) {
+        k -= J * kSquare * rows;
+        i = I * kSquare + k % rows;
+        j = J * kSquare + k / rows;
+    } else {
+        k -= I * kSquare * rows;
+        int q = 0;
+        while ((q + 1) * (q + 2) / 2 <= k) ++q;
+        i = I * kSquare + q;
+        j = I * kSquare + k - q * (q + 1) / 2;
+    }
+}
+__device__ __forceinline__ void rect_at(int k, int t, int u, int& i, int& j) {      // tile k of t x u
+    const int J = k / (kSquare * t), cols = min(kSquare, u - J * kSquare);
+    k -= J * kSquare * t;
+    const int I = k / (kSquare * cols), rows = min(kSquare, t - I * kSquare);
+    k -= I * kSquare * cols;
+    i = I * kSquare + k % rows;
+    j = J * kSquare + k / rows;
+}
+
+// the matrix a workgroup belongs to: one parallel look at the table's first[] and a vote
+__device__ __forceinline__ int matrix_of(const int* __restrict__ first, int count, int id) {
+    const int lane = threadIdx.x & 63;
+    const bool before = lane < count && first[lane < kMaxList ? lane : 0] <= id;
+    return __builtin_amdgcn_readfirstlane((int)__popcll(__ballot(before)) - 1);
 }
 
 // one 16-byte chunk per lane straight from global memory into LDS: the wave's 64 chunks land at lds, in lane order
@@ -201,280 +235,610 @@ __device__ __forceinline__ void to_lds(const void* src, void* lds) {
 #endif
 }
 
-// LDS stage of a K-contiguous operand: [128 rows][64] fp16, chunk c (8 values) of row r at place c ^ (r & 7): the 32 rows a fragment reads
-// at once then spread over all banks.
+// LDS stage of a K-contiguous operand: [TILE rows][kDepth] fp16 with the chunks of a row permuted by the row.  LDS delivers 256 bytes a cycle, so
+// the 16 rows that a fragment read touches at a time have to lie in different banks: rows of 128 bytes: chunk ^ row / 2 % 8, of 64 bytes:
+// chunk ^ row / 4 % 4.
+template <class S> __device__ __forceinline__ int place(int row, int chunk) { return S::kChunks == 8 ? chunk ^ ((row >> 1) & 7) : chunk ^ ((row >> 2) & 3); }
+template <class S, int TILE>
 __device__ __forceinline__ void stage_rows(const _Float16* src, int ld, int row0, int k0, _Float16* lds, int wave, int lane) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-        const int r = (u * 4 + wave) * 8 + (lane >> 3), c = (lane & 7) ^ (r & 7);
-        to_lds(src + (int64_t)(row0 + r) * ld + k0 + c * 8, lds + (u * 4 + wave) * 512);
+    for (int u = 0; u < TILE * S::kChunks / S::kThreads; ++u) {
+        const int e = (u * S::kWaves + wave) * 64 + lane, r = e / S::kChunks, c = place<S>(r, e % S::kChunks);
+        to_lds(src + (int64_t)(row0 + r) * ld + k0 + c * 8, lds + (u * S::kWaves + wave) * 512);
     }
 }
+template <class S>
 __device__ __forceinline__ f16x8 frag_rows(const _Float16* lds, int row, int kb, int lane) {
     const int r = row + (lane & 31);
-    return *(const f16x8*)(lds + r * 64 + (((kb * 2 + (lane >> 5)) ^ (r & 7)) * 8));
+    return *(const f16x8*)(lds + r * S::kDepth + place<S>(lane & 31, kb * 2 + (lane >> 5)) * 8);       // row is a multiple of 32
 }
-// LDS stage of X as the right operand: [64 rows of the contraction][128 columns], chunk c of row r at place c ^ 4 (r & 3): the four rows a
+// LDS stage of X as the right operand: [kDepth rows of the contraction][TILE columns], chunk c of row r at place c ^ 4 (r & 3): the four rows a
 // transposing read takes from a 16-lane group lie in different banks.
+template <class S, int TILE>
 __device__ __forceinline__ void stage_cols(const _Float16* src, int ld, int k0, int col0, _Float16* lds, int wave, int lane) {
+    constexpr int kRow = TILE / 8;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-        const int r = (u * 4 + wave) * 4 + (lane >> 4), c = (lane & 15) ^ ((r & 3) << 2);
-        to_lds(src + (int64_t)(k0 + r) * ld + col0 + c * 8, lds + (u * 4 + wave) * 512);
+    for (int u = 0; u < TILE * S::kChunks / S::kThreads; ++u) {
+        const int e = (u * S::kWaves + wave) * 64 + lane, r = e / kRow, c = (e % kRow) ^ ((r & 3) << 2);
+        to_lds(src + (int64_t)(k0 + r) * ld + col0 + c * 8, lds + (u * S::kWaves + wave) * 512);
     }
 }
+template <int TILE>
 __device__ __forceinline__ f16x8 frag_cols(const _Float16* lds, int col, int kb, int lane) {
     union { f16x8 f; s16x4 h[2]; } v;
-    const int r = kb * 16 + (lane >> 5) * 8 + ((lane & 15) >> 2), n = col + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-        const int row = r + 4 * w;
-        const _Float16* p = lds + row * 128 + (((n >> 3) ^ ((row & 3) << 2)) * 8) + (n & 7);
+    const int r = (lane >> 5) * 8 + ((lane & 15) >> 2), n = ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+    const int at = r * TILE + ((((col + n) >> 3) ^ ((r & 3) << 2)) * 8) + (n & 7) + kb * 16 * TILE;      // col is a multiple of 32
 #if defined(__HIP_DEVICE_COMPILE__)
-        v.h[w] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SNAG_LDS s16x4*)p);
+#pragma unroll
+    for (int w = 0; w < 2; ++w) v.h[w] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SNAG_LDS s16x4*)(lds + at + 4 * w * TILE));
 #endif
-    }
     return v.f;
 }
 
-// What a 32 x 32 block of the product becomes.  acc: register i of lane (h, l) = element (row0 + 8 (i / 4) + 4 h + i % 4, col0 + l).
+// 16 neighbouring fp16 pairs; as fp32 sums, and back
+struct Pairs { f16x8 hi[2], lo[2]; };
+__device__ __forceinline__ Pairs load_pairs(const _Float16* hi, const _Float16* lo) { return Pairs{{*(const f16x8*)hi, *(const f16x8*)(hi + 8)}, {*(const f16x8*)lo, *(const f16x8*)(lo + 8)}}; }
+__device__ __forceinline__ float sum_of(const Pairs& p, int j) { return (float)p.hi[j >> 3][j & 7] + (float)p.lo[j >> 3][j & 7]; }
+__device__ __forceinline__ Pairs pairs_of(const float (&v)[16]) {
+    Pairs p;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        _Float16 x, y;
+        split16(v[j], x, y);
+        p.hi[j >> 3][j & 7] = x;
+        p.lo[j >> 3][j & 7] = y;
+    }
+    return p;
+}
+__device__ __forceinline__ void store_pairs(_Float16* hi, _Float16* lo, const Pairs& p) {
+    *(f16x8*)hi = p.hi[0], *(f16x8*)(hi + 8) = p.hi[1];
+    *(f16x8*)lo = p.lo[0], *(f16x8*)(lo + 8) = p.lo[1];
+}
+
+// What a 32 x 32 block of the product becomes.  acc: register i of lane (h, l) = element (row0 + 8 (i / 4) + 4 h + i % 4, col0 + l).  The block goes
+// through this wave's own piece of LDS (32 rows of kPitch floats), so that a lane holds 16 neighbours of one row and everything moves 16 bytes at
+// a time; a tall result and the mirror image take 16 neighbours of one column instead.
+constexpr int kPitch = 33;
+// LDS keeps a wave's accesses in order; this keeps the compiler from moving one lane's reads in front of another's writes
+__device__ __forceinline__ void lds_turn() { asm volatile("" ::: "memory"); }
+// what a block needs of memory: X (APPLY) or the off-diagonal part of A (POLY) where it lies
 template <int MODE>
-__device__ __forceinline__ void finish(const MuonList& L, const MuonMatrix& a, const Planes& p, const f32x16& acc, int row0, int col0, bool mirror, int from, bool last, int lane) {
-    const int h = lane >> 5, col = col0 + (lane & 31);
-    if constexpr (MODE == kApply) {
-        const _Float16 *xh = p.xh[from], *xl = p.xl[from];
+__device__ __forceinline__ Pairs block_pairs(const MuonMatrix& a, int row0, int col0, int from, int lane) {
+    const int row = row0 + (lane >> 1), col = col0 + (lane & 1) * 16;
+    if (MODE == kApply) return load_pairs(x_plane(a, from, 0) + (int64_t)row * a.np + col, x_plane(a, from, 1) + (int64_t)row * a.np + col);
+    if (MODE == kPoly) return load_pairs(s_plane(a, 0) + (int64_t)row * a.mp + col, s_plane(a, 1) + (int64_t)row * a.mp + col);
+    return Pairs{};
+}
+// values of 16 neighbours of a row become 16 neighbours of a column: lane (r, c) gets rows c .. c + 15 of column r
+__device__ __forceinline__ void turn(float* block, float (&v)[16], int r, int c) {
+    lds_turn();
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int row = row0 + 8 * g + 4 * h;
-            float y[4];
+    for (int j = 0; j < 16; ++j) block[r * kPitch + c + j] = v[j];
+    lds_turn();
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int64_t at = (int64_t)(row + j) * a.np + col;
-                const float x = (float)xh[at] + (float)xl[at];                         // times 2^14
-                y[j] = fmaf(kNsA + p.db[row + j], x, acc[4 * g + j] * (1.f / kScaleA));
+    for (int j = 0; j < 16; ++j) v[j] = block[(c + j) * kPitch + r];
+}
+// the last iteration's 16 values of X (row, col ..; times 2^14) into the user's matrix
+template <class T>
+__device__ __forceinline__ void store_result(const MuonTable* __restrict__ L, const MuonMatrix& a, float (&v)[16], int row0, int col0, float* block, int lane) {
+    const int r = lane >> 1, c = (lane & 1) * 16;
+    int i0 = row0 + r, j0 = col0 + c;                      // where they go: row i0, columns j0 ..
+    if (a.tall) {
+        turn(block, v, r, c);
+        i0 = col0 + r;
+        j0 = row0 + c;
+    }
+    if (i0 >= a.r || j0 >= a.c) return;
+    T* out = (T*)a.w + (int64_t)i0 * a.c + j0;
+    using V = typename Chunk<T>::vec;
+    constexpr int C = Chunk<T>::n;
+    const int step = L->step;
+    const float keep = L->keep;
+    if (j0 + 16 <= a.c && a.c % C == 0 && ((uintptr_t)a.w & 15) == 0) {
+#pragma unroll
+        for (int q = 0; q < 16 / C; ++q) {
+            V o;
+            if (step) o = *(const V*)(out + q * C);
+#pragma unroll
+            for (int j = 0; j < C; ++j) {
+                const float x = v[q * C + j] * (1.f / kScaleX);
+                o[j] = (T)(step ? fmaf(-a.update, x, keep * (float)o[j]) : x);
             }
-            if (!last) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int64_t at = (int64_t)(row + j) * a.np + col;
-                    _Float16 hi, lo;
-                    split16(y[j], hi, lo);
-                    p.xh[from ^ 1][at] = hi;
-                    p.xl[from ^ 1][at] = lo;
-                }
-                continue;
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (row + j >= a.m || col >= a.n) continue;
-                const int64_t at = a.tall ? (int64_t)col * a.c + row + j : (int64_t)(row + j) * a.c + col;
-                float v = y[j] * (1.f / kScaleX);
-                if (L.step) v = fmaf(-a.update, v, L.keep * value_of(a.w, L.dtype, at));
-                if (L.dtype == SNAG_F32) ((float*)a.w)[at] = v;
-                else if (L.dtype == SNAG_BF16) ((bf16_t*)a.w)[at] = (bf16_t)v;
-                else ((f16_t*)a.w)[at] = (f16_t)v;
-            }
+            *(V*)(out + q * C) = o;
         }
     } else {
-        _Float16 *oh = MODE == kGram ? p.rh : p.bh, *ol = MODE == kGram ? p.rl : p.bl;
-        float* diag = MODE == kGram ? p.da : p.db;
-        const float dj = MODE == kPoly ? p.da[col] : 0.f;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int row = row0 + 8 * g + 4 * h;
-            f16x4 hi, lo;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int64_t at = (int64_t)(row + j) * a.mp + col;
-                const bool on = row + j == col;
-                float v;
-                if constexpr (MODE == kGram) {
-                    v = acc[4 * g + j] * (1.f / (kScaleX * kScaleX));
-                    if (on) diag[col] = v;
-                    v *= kScaleA;
-                } else {
-                    const float sq = acc[4 * g + j] * (1.f / kScaleA), r = (float)p.rh[at] + (float)p.rl[at], di = p.da[row + j];      // both times 2^13
-                    if (on) diag[col] = fmaf(kNsB, di, kNsC * fmaf(di, di, sq * (1.f / kScaleA)));
-                    v = fmaf(fmaf(kNsC, di + dj, kNsB), r, kNsC * sq);
-                }
-                _Float16 vh, vl;
-                split16(on ? 0.f : v, vh, vl);
-                hi[j] = vh, lo[j] = vl;
-                oh[at] = vh;
-                ol[at] = vl;
-            }
-            if (mirror) {
-                *(f16x4*)(oh + (int64_t)col * a.mp + row) = hi;
-                *(f16x4*)(ol + (int64_t)col * a.mp + row) = lo;
-            }
+        for (int j = 0; j < 16; ++j) {
+            if (j0 + j >= a.c) continue;
+            const float x = v[j] * (1.f / kScaleX);
+            out[j] = (T)(step ? fmaf(-a.update, x, keep * (float)out[j]) : x);
         }
     }
 }
 
-// 128 x 128 tile, four waves of 64 x 64; PLANES 1: hi hi, 2: hi hi + hi lo + lo hi.  Two LDS stages filled straight from memory, one ahead.
-template <int MODE, int PLANES>
-__global__ __launch_bounds__(256) void muon_product_kernel(MuonList L, int from, int last) {
+template <int MODE, int DT>
+__device__ __forceinline__ void finish(const MuonTable* __restrict__ L, const MuonMatrix& a, const f32x16& acc, const Pairs& p, int row0, int col0, bool mirror, int from, bool last, float* block, int lane) {
+    const int h = lane >> 5, r = lane >> 1, c = (lane & 1) * 16;           // row r, columns c .. c + 15 of the block
+    lds_turn();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) block[(8 * (i >> 2) + 4 * h + (i & 3)) * kPitch + (lane & 31)] = acc[i];
+    lds_turn();
+    float v[16];
+    const int row = row0 + r, col = col0 + c;
+    if constexpr (MODE == kApply) {
+        const float d = kNsA + diagonal(a, 1)[row];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = fmaf(d, sum_of(p, j), block[r * kPitch + c + j] * (1.f / kScaleA));            // times 2^14
+        if (last) store_result<TypeOf<DT>>(L, a, v, row0, col0, block, lane);
+        else store_pairs(x_plane(a, from ^ 1, 0) + (int64_t)row * a.np + col, x_plane(a, from ^ 1, 1) + (int64_t)row * a.np + col, pairs_of(v));
+    } else {
+        _Float16 *oh = s_plane(a, MODE == kGram ? 0 : 2), *ol = s_plane(a, MODE == kGram ? 1 : 3);
+        float* diag = diagonal(a, MODE == kGram ? 0 : 1);
+        if constexpr (MODE == kGram) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                v[j] = block[r * kPitch + c + j] * (1.f / (kScaleX * kScaleX));
+                if (row == col + j) diag[row] = v[j], v[j] = 0.f;
+                v[j] *= kScaleA;
+            }
+        } else {
+            const float* da = diagonal(a, 0);
+            const float di = da[row];
+            float dj[16];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) *(f32x4*)(dj + 4 * q) = *(const f32x4*)(da + col + 4 * q);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const float sq = block[r * kPitch + c + j] * (1.f / kScaleA);                                              // times 2^13
+                v[j] = fmaf(fmaf(kNsC, di + dj[j], kNsB), sum_of(p, j), kNsC * sq);
+                if (row == col + j) diag[row] = fmaf(kNsB, di, kNsC * fmaf(di, di, sq * (1.f / kScaleA))), v[j] = 0.f;
+            }
+        }
+        store_pairs(oh + (int64_t)row * a.mp + col, ol + (int64_t)row * a.mp + col, pairs_of(v));
+        if (mirror) {
+            turn(block, v, r, c);
+            const int64_t at = (int64_t)(col0 + r) * a.mp + row0 + c;
+            store_pairs(oh + at, ol + at, pairs_of(v));
+        }
+    }
+}
+
+// PLANES 1: hi hi, 2: hi hi + hi lo + lo hi.  The LDS stages are filled straight from memory, NST - 1 ahead; the fragments of the next 16 of the
+// contraction are read while the present ones are multiplied, across the stages too: the barrier that opens a stage stands in front of the
+// last products of the stage before it.
+template <int MODE, int DT, int TILE, int NST>
+__global__ __launch_bounds__(TILE == 128 ? 256 : 512, NST == 2 ? 2 : 1) void muon_product_kernel(const MuonTable* __restrict__ L, int from, int last) {
+    constexpr int PLANES = DT == SNAG_F32 ? 2 : 1;
+    using S = Shape<TILE, PLANES, NST>;
+    constexpr int NI = S::kWm / 32, NJ = S::kWn / 32, KB = S::kDepth / 16;
+    static_assert(KB % 2 == 0, "fragment sets alternate");
     extern __shared__ __attribute__((aligned(16))) char smem[];
     _Float16* lds = (_Float16*)smem;
-    constexpr int kOperand = kTile * kDepth, kStage = 2 * PLANES * kOperand;     // in fp16 values
     const int lane = threadIdx.x & 63, wave = wave_id_uniform();
-    const TileAt t = tile_at<MODE>(L);
-    const MuonMatrix& a = L.a[t.matrix];
-    const Planes p = planes_of(a);
-    const _Float16 *ah[2], *bh[2];
-    if (MODE == kGram) ah[0] = bh[0] = p.xh[from], ah[1] = bh[1] = p.xl[from];
-    else if (MODE == kPoly) ah[0] = bh[0] = p.rh, ah[1] = bh[1] = p.rl;
-    else ah[0] = p.bh, ah[1] = p.bl, bh[0] = p.xh[from], bh[1] = p.xl[from];
+    const int id = (int)xcd_order(blockIdx.x, gridDim.x);
+    const int which = matrix_of(L->first[MODE], L->count, id);
+    const MuonMatrix a = L->a[which];
+    int k = id - L->first[MODE][which], split = 0, ti, tj;
+    if (MODE == kApply) {
+        rect_at(k, a.mp / TILE, a.np / TILE, ti, tj);
+    } else {
+        const int t = a.mp / TILE;
+        if (MODE == kGram) {
+            const int tiles = t * (t + 1) / 2;
+            split = k / tiles;
+            k -= split * tiles;
+        }
+        tri_at(k, t, ti, tj);
+    }
     const int lda = MODE == kGram ? a.np : a.mp;
-    int k0 = 0, k1 = MODE == kGram ? a.np : a.mp;
+    int k0 = 0, k1 = lda;
     if (MODE == kGram && a.splits > 1) {
-        const int per = (a.np / kDepth + a.splits - 1) / a.splits * kDepth;
-        k0 = t.split * per;
+        const int per = (a.np / 64 + a.splits - 1) / a.splits * 64;
+        k0 = split * per;
         k1 = min(a.np, k0 + per);
     }
-    auto stage = [&](int k, int s) {
+    const int n = k1 > k0 ? (k1 - k0) / S::kDepth : 0;                 // stages
+    const _Float16* left = MODE == kGram ? x_plane(a, from, 0) : s_plane(a, MODE == kPoly ? 0 : 2);
+    const _Float16* right = MODE == kPoly ? left : x_plane(a, from, 0);
+    const int64_t left_lo = MODE == kGram ? plane_x(a) : plane_s(a), right_lo = MODE == kPoly ? plane_s(a) : plane_x(a);
+    auto stage = [&](int t) {
+        const int kk = k0 + t * S::kDepth;
 #pragma unroll
         for (int q = 0; q < PLANES; ++q) {
-            _Float16* base = lds + s * kStage + q * 2 * kOperand;
-            stage_rows(ah[q], lda, t.i * kTile, k, base, wave, lane);
-            if (MODE == kApply) stage_cols(bh[q], a.np, k, t.j * kTile, base + kOperand, wave, lane);
-            else stage_rows(bh[q], lda, t.j * kTile, k, base + kOperand, wave, lane);
+            _Float16* base = lds + t % NST * S::kStage + q * 2 * S::kOperand;
+            stage_rows<S, TILE>(left + q * left_lo, lda, ti * TILE, kk, base, wave, lane);
+            if (MODE == kApply) stage_cols<S, TILE>(right + q * right_lo, a.np, kk, tj * TILE, base + S::kOperand, wave, lane);
+            else stage_rows<S, TILE>(right + q * right_lo, lda, tj * TILE, kk, base + S::kOperand, wave, lane);
         }
     };
-    f32x16 acc[2][2];
+    f32x16 acc[NI][NJ];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = f32x16{};
-    const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-    if (k0 < k1) stage(k0, 0);
-    int s = 0;
-    for (int k = k0; k < k1; k += kDepth, s ^= 1) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // this wave's part of stage s has landed ...
-        __syncthreads();                                        // ... and everybody's; everybody is done with the other stage
-        if (k + kDepth < k1) stage(k + kDepth, s ^ 1);
-        const _Float16* base = lds + s * kStage;
+        for (int j = 0; j < NJ; ++j) acc[i][j] = f32x16{};
+    constexpr int kWavesN = TILE / S::kWn;
+    const int wm = (wave / kWavesN) * S::kWm, wn = (wave % kWavesN) * S::kWn;
+    // A launch of one workgroup per CU takes its blocks' own values along with the first stages; otherwise they are fetched one block ahead.
+    Pairs own[NI * NJ];
+    const int i0 = ti * TILE + wm, j0 = tj * TILE + wn;
+    auto fetch = [&](int q) { own[q] = block_pairs<MODE>(a, i0 + q / NJ * 32, j0 + q % NJ * 32, from, lane); };
+    if (NST > 2) {
 #pragma unroll
-        for (int kb = 0; kb < kDepth / 16; ++kb) {
-            f16x8 fa[PLANES][2], fb[PLANES][2];
+        for (int q = 0; q < NI * NJ; ++q) fetch(q);
+    }
+    f16x8 fa[2][PLANES][NI], fb[2][PLANES][NJ];
+    auto read = [&](int set, int t, int kb) {
 #pragma unroll
-            for (int q = 0; q < PLANES; ++q)
+        for (int q = 0; q < PLANES; ++q) {
+            const _Float16* o = lds + t % NST * S::kStage + q * 2 * S::kOperand;
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const _Float16* o = base + q * 2 * kOperand;
-                    fa[q][i] = frag_rows(o, wm + i * 32, kb, lane);
-                    fb[q][i] = MODE == kApply ? frag_cols(o + kOperand, wn + i * 32, kb, lane) : frag_rows(o + kOperand, wn + i * 32, kb, lane);
-                }
+            for (int i = 0; i < NI; ++i) fa[set][q][i] = frag_rows<S>(o, wm + i * 32, kb, lane);
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) fb[set][q][j] = MODE == kApply ? frag_cols<TILE>(o + S::kOperand, wn + j * 32, kb, lane) : frag_rows<S>(o + S::kOperand, wn + j * 32, kb, lane);
+        }
+    };
+    // stage t has landed, everybody's part of it, and everybody is done reading the one before it.  Loads in flight: of stages t .. t + NST - 2
+    auto open = [&](int t) {
+        if (NST > 2 && t + NST - 2 < n) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NST - 2) * S::kLoads) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    if (n > 0) {
+#pragma unroll
+        for (int t = 0; t < NST - 1; ++t)
+            if (t < n) stage(t);
+        open(0);
+        if (NST - 1 < n) stage(NST - 1);
+        read(0, 0, 0);
+    }
+    for (int t = 0; t < n; ++t) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            if (kb + 1 < KB) {
+                read((kb + 1) & 1, t, kb + 1);
+            } else if (t + 1 < n) {
+                open(t + 1);
+                if (t + NST < n) stage(t + NST);
+                read(0, t + 1, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            const int set = kb & 1;
 #if defined(__HIP_DEVICE_COMPILE__)
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < NI; ++i)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][i], fb[0][j], acc[i][j], 0, 0, 0);
+                for (int j = 0; j < NJ; ++j) {
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[set][0][i], fb[set][0][j], acc[i][j], 0, 0, 0);
                     if constexpr (PLANES == 2) {
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][i], fb[1][j], acc[i][j], 0, 0, 0);
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[1][i], fb[0][j], acc[i][j], 0, 0, 0);
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[set][0][i], fb[set][1][j], acc[i][j], 0, 0, 0);
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[set][1][i], fb[set][0][j], acc[i][j], 0, 0, 0);
                     }
                 }
 #endif
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
-    const int i0 = t.i * kTile + wm, j0 = t.j * kTile + wn;
     if (MODE == kGram && a.splits > 1) {
         // the range's partial tile, in register order: muon_gram_sum_kernel adds the ranges up
-        const int tiles = (a.mp / kTile) * (a.mp / kTile + 1) / 2, id = t.i * (t.i + 1) / 2 + t.j;
-        float* out = p.slab + ((int64_t)(t.split * tiles + id) * 16 + wave * 4) * 1024 + lane * 16;
+        const int t = a.mp / TILE, tiles = t * (t + 1) / 2;
+        float* out = slab_of(a) + ((int64_t)(split * tiles + k) * S::kWaves + wave) * NI * NJ * 1024 + lane * 16;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < NI; ++i)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) *(f32x16*)(out + (i * 2 + j) * 1024) = acc[i][j];
+            for (int j = 0; j < NJ; ++j) *(f32x16*)(out + (i * NJ + j) * 1024) = acc[i][j];
         return;
     }
+    __syncthreads();                                           // the stages become the waves' blocks
+    float* block = (float*)smem + wave * 32 * kPitch;
+    if (NST == 2) fetch(0);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) finish<MODE>(L, a, p, acc[i][j], i0 + i * 32, j0 + j * 32, t.i != t.j, from, last != 0, lane);
+    for (int q = 0; q < NI * NJ; ++q) {
+        if (NST == 2 && q + 1 < NI * NJ) fetch(q + 1);
+        finish<MODE, DT>(L, a, acc[q / NJ][q % NJ], own[q], i0 + q / NJ * 32, j0 + q % NJ * 32, ti != tj, from, last != 0, block, lane);
+    }
 }
 
-// A from its ranges, one wave per 32 x 32 block: grid (16 x the largest number of tiles, matrices)
-__global__ __launch_bounds__(64) void muon_gram_sum_kernel(MuonList L) {
-    const MuonMatrix& a = L.a[blockIdx.y];
-    const int tiles = (a.mp / kTile) * (a.mp / kTile + 1) / 2, id = blockIdx.x >> 4, sub = blockIdx.x & 15, lane = threadIdx.x;
-    if (a.splits == 1 || id >= tiles) return;
-    const Planes p = planes_of(a);
+// A from its ranges: a workgroup per 32 x 32 block of the 128 x 128 tiles, each of its four waves adds up a quarter of the ranges, in order; the
+// quarters are joined through LDS.  Grid (16 x the largest number of tiles, matrices)
+__global__ __launch_bounds__(256) void muon_gram_sum_kernel(const MuonTable* __restrict__ L) {
+    __shared__ float block[32 * kPitch];
+    __shared__ __attribute__((aligned(16))) f32x16 part[3][64];
+    const MuonMatrix a = L->a[blockIdx.y];
+    const int t = a.mp / 128, tiles = t * (t + 1) / 2, id = blockIdx.x >> 4, sub = blockIdx.x & 15, lane = threadIdx.x & 63, quarter = wave_id_uniform();
+    if (a.splits == 1 || id >= tiles) return;     // the whole workgroup
+    const int per = (a.splits + 3) / 4, s1 = min(a.splits, (quarter + 1) * per);
+    int s = quarter * per;
     f32x16 acc{};
-    for (int s = 0; s < a.splits; ++s) acc += *(const f32x16*)(p.slab + ((int64_t)(s * tiles + id) * 16 + sub) * 1024 + lane * 16);
-    int i = 0;
-    while ((i + 1) * (i + 2) / 2 <= id) ++i;
-    const int j = id - i * (i + 1) / 2, wave = sub >> 2, q = sub & 3;
-    finish<kGram>(L, a, p, acc, i * kTile + (wave >> 1) * 64 + (q >> 1) * 32, j * kTile + (wave & 1) * 64 + (q & 1) * 32, i != j, 0, false, lane);
+    const int64_t step = (int64_t)tiles * 16 * 1024;
+    const float* p = slab_of(a) + ((int64_t)id * 16 + sub) * 1024 + lane * 16 + s * step;
+    for (; s + 8 <= s1; s += 8, p += 8 * step) {
+        f32x16 v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = *(const f32x16*)(p + u * step);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) acc += v[u];
+    }
+    for (; s < s1; ++s, p += step) acc += *(const f32x16*)p;
+    if (quarter > 0) part[quarter - 1][lane] = acc;
+    __syncthreads();
+    if (quarter > 0) return;
+#pragma unroll
+    for (int u = 0; u < 3; ++u) acc += part[u][lane];
+    int i, j;
+    tri_at(id, t, i, j);
+    const int wave = sub >> 2, q = sub & 3;
+    finish<kGram, SNAG_F32>(L, a, acc, Pairs{}, i * 128 + (wave >> 1) * 64 + (q >> 1) * 32, j * 128 + (wave & 1) * 64 + (q & 1) * 32, i != j, 0, false, block, lane);
+}
+
+// ---- one side of at most 128 ------------------------------------------------------------------------------------------------
+// A is one 128 x 128 tile: every workgroup of a 128-column block of X computes B for itself, in LDS, and goes on to its block of the new X and
+// that block's share of the next A.  An iteration is two launches (this one and muon_gram_sum_kernel, which adds the shares up) in place of
+// four, and these matrices are all launch latency: 128 x 128 .. 128 x 4096, 22 launches of 6-14 us before, 13 now.
+// LDS images are [128 rows][128] fp16, chunk c (16 bytes) of row r at place c ^ (4 (r % 4) + r / 4 % 4): without bank conflicts both for
+// fragments along the rows and for transposing reads across them.
+constexpr int kImage = 128 * 128;
+__device__ __forceinline__ int image_at(int row, int col) { return row * 128 + (((col >> 3) ^ (((row & 3) << 2) | ((row >> 2) & 3))) << 3) + (col & 7); }
+__device__ __forceinline__ void image_load(const _Float16* src, int ld, _Float16* lds, int wave, int lane) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+        const int e = (u * 4 + wave) * 64 + lane, r = e >> 4, c = (e & 15) ^ (((r & 3) << 2) | ((r >> 2) & 3));
+        to_lds(src + (int64_t)r * ld + c * 8, lds + (u * 4 + wave) * 512);
+    }
+}
+__device__ __forceinline__ f16x8 image_rows(const _Float16* lds, int row, int kb, int lane) { return *(const f16x8*)(lds + image_at(row + (lane & 31), kb * 16 + (lane >> 5) * 8)); }
+__device__ __forceinline__ f16x8 image_cols(const _Float16* lds, int col, int kb, int lane) {
+    union { f16x8 f; s16x4 h[2]; } v;
+    const int r = kb * 16 + (lane >> 5) * 8 + ((lane & 15) >> 2), n = col + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+#if defined(__HIP_DEVICE_COMPILE__)
+#pragma unroll
+    for (int w = 0; w < 2; ++w) v.h[w] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SNAG_LDS s16x4*)(lds + image_at(r + 4 * w, n)));
+#endif
+    return v.f;
+}
+// 64 x 64 part (wm, wn) of a product of two images; RIGHT_COLS: the right operand's contraction runs down its rows
+template <int PLANES, bool RIGHT_COLS>
+__device__ __forceinline__ void image_product(f32x16 (&acc)[4], const _Float16* left, const _Float16* right, int wm, int wn, int lane) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) acc[q] = f32x16{};
+#pragma unroll
+    for (int kb = 0; kb < 8; ++kb) {
+        f16x8 fa[PLANES][2], fb[PLANES][2];
+#pragma unroll
+        for (int p = 0; p < PLANES; ++p)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                fa[p][i] = image_rows(left + p * kImage, wm + i * 32, kb, lane);
+                fb[p][i] = RIGHT_COLS ? image_cols(right + p * kImage, wn + i * 32, kb, lane) : image_rows(right + p * kImage, wn + i * 32, kb, lane);
+            }
+#if defined(__HIP_DEVICE_COMPILE__)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            acc[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][q >> 1], fb[0][q & 1], acc[q], 0, 0, 0);
+            if constexpr (PLANES == 2) {
+                acc[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][q >> 1], fb[1][q & 1], acc[q], 0, 0, 0);
+                acc[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[1][q >> 1], fb[0][q & 1], acc[q], 0, 0, 0);
+            }
+        }
+#endif
+    }
+}
+__device__ __forceinline__ Pairs image_pairs(const _Float16* hi, const _Float16* lo, int row, int col) {
+    return Pairs{{*(const f16x8*)(hi + image_at(row, col)), *(const f16x8*)(hi + image_at(row, col + 8))},
+                 {*(const f16x8*)(lo + image_at(row, col)), *(const f16x8*)(lo + image_at(row, col + 8))}};
+}
+__device__ __forceinline__ void image_store(_Float16* hi, _Float16* lo, int row, int col, const Pairs& p) {
+    *(f16x8*)(hi + image_at(row, col)) = p.hi[0], *(f16x8*)(hi + image_at(row, col + 8)) = p.hi[1];
+    *(f16x8*)(lo + image_at(row, col)) = p.lo[0], *(f16x8*)(lo + image_at(row, col + 8)) = p.lo[1];
+}
+
+// start: only the first A's shares of X copy 0.  One workgroup per 128-column block; slab[block][wave][4][1024] as the product kernel's ranges.
+template <int DT>
+__global__ __launch_bounds__(256) void muon_narrow_kernel(const MuonTable* __restrict__ L, int from, int start, int last) {
+    constexpr int PLANES = DT == SNAG_F32 ? 2 : 1;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    _Float16 *X = (_Float16*)smem, *S = X + 2 * kImage;                // hi, lo of X's block; hi, lo of A, later of B
+    float* block = (float*)(S + 2 * kImage);                           // 4 x 32 x kPitch
+    const int lane = threadIdx.x & 63, wave = wave_id_uniform();
+    const int which = matrix_of(L->first[kApply], L->count, blockIdx.x);
+    const MuonMatrix a = L->a[which];
+    const int col0 = ((int)blockIdx.x - L->first[kApply][which]) * 128;
+    const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
+    block += wave * 32 * kPitch;
+    image_load(x_plane(a, from, 0) + col0, a.np, X, wave, lane);
+    image_load(x_plane(a, from, 1) + col0, a.np, X + kImage, wave, lane);
+    f32x16 acc[4];
+    const int r = lane >> 1, c = (lane & 1) * 16, h = lane >> 5;
+    auto to_block = [&](const f32x16& v) {
+        lds_turn();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) block[(8 * (i >> 2) + 4 * h + (i & 3)) * kPitch + (lane & 31)] = v[i];
+        lds_turn();
+    };
+    if (!start) {
+        image_load(s_plane(a, 0), 128, S, wave, lane);
+        image_load(s_plane(a, 1), 128, S + kImage, wave, lane);
+        const float* da = diagonal(a, 0);
+        float di[2], dj[2][16];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            di[i] = da[wm + i * 32 + r];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) *(f32x4*)(dj[i] + 4 * q) = *(const f32x4*)(da + wn + i * 32 + c + 4 * q);
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        image_product<PLANES, false>(acc, S, S, wm, wn, lane);
+        // B in the place of A; its diagonal stays with the lanes that hold it and goes through LDS below
+        Pairs b[4];
+        float db[2] = {0.f, 0.f};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int row = wm + (q >> 1) * 32 + r, col = wn + (q & 1) * 32 + c;
+            const Pairs p = image_pairs(S, S + kImage, row, col);
+            to_block(acc[q]);
+            float v[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const float sq = block[r * kPitch + c + j] * (1.f / kScaleA);
+                v[j] = fmaf(fmaf(kNsC, di[q >> 1] + dj[q & 1][j], kNsB), sum_of(p, j), kNsC * sq);
+                if (row == col + j) db[q >> 1] = fmaf(kNsB, di[q >> 1], kNsC * fmaf(di[q >> 1], di[q >> 1], sq * (1.f / kScaleA))), v[j] = 0.f;
+            }
+            b[q] = pairs_of(v);
+        }
+        __syncthreads();
+        float* diag = (float*)(S + 2 * kImage) + 4 * 32 * kPitch;      // [128]
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int row = wm + (q >> 1) * 32 + r, col = wn + (q & 1) * 32 + c;
+            image_store(S, S + kImage, row, col, b[q]);
+            if (row >= col && row < col + 16) diag[row] = db[q >> 1];
+        }
+        __syncthreads();
+        image_product<PLANES, true>(acc, S, X, wm, wn, lane);
+        Pairs y[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int row = wm + (q >> 1) * 32 + r, col = wn + (q & 1) * 32 + c;
+            const Pairs p = image_pairs(X, X + kImage, row, col);
+            to_block(acc[q]);
+            const float d = kNsA + diag[row];
+            float v[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = fmaf(d, sum_of(p, j), block[r * kPitch + c + j] * (1.f / kScaleA));
+            if (last) {
+                store_result<TypeOf<DT>>(L, a, v, wm + (q >> 1) * 32, col0 + wn + (q & 1) * 32, block, lane);
+                continue;
+            }
+            y[q] = pairs_of(v);
+            const int64_t at = (int64_t)row * a.np + col0 + col;
+            store_pairs(x_plane(a, from ^ 1, 0) + at, x_plane(a, from ^ 1, 1) + at, y[q]);
+        }
+        if (last) return;
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < 4; ++q) image_store(X, X + kImage, wm + (q >> 1) * 32 + r, wn + (q & 1) * 32 + c, y[q]);
+    } else {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    __syncthreads();
+    image_product<PLANES, false>(acc, X, X, wm, wn, lane);
+    if (a.splits == 1) {                                               // the only block: A is complete
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            finish<kGram, DT>(L, a, acc[q], Pairs{}, wm + (q >> 1) * 32, wn + (q & 1) * 32, false, 0, false, block, lane);
+        return;
+    }
+    float* out = slab_of(a) + ((int64_t)(col0 / 128) * 4 + wave) * 4096 + lane * 16;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) *(f32x16*)(out + q * 1024) = acc[q];
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
-static int pad_tile(int n) { return (n + kTile - 1) / kTile * kTile; }
+static int pad_to(int n, int tile) { return (n + tile - 1) / tile * tile; }
+constexpr int kCus = 256;
 
-// A has few tiles when m is small, and its contraction is the long side: cut it until the launch has about one workgroup per CU, never below
-// four LDS stages a range.
-static int gram_splits(int mp, int np) {
-    const int tiles = (mp / kTile) * (mp / kTile + 1) / 2, stages = np / kDepth;
-    int s = 256 / tiles;
-    if (s > stages / 4) s = stages / 4;
-    return s < 1 ? 1 : s;
-}
-
-static int64_t matrix_bytes(int r, int c) {
-    const int mp = pad_tile(r < c ? r : c), np = pad_tile(r < c ? c : r), s = gram_splits(mp, np);
-    const int64_t x = (int64_t)mp * np, q = (int64_t)mp * mp, tiles = (int64_t)(mp / kTile) * (mp / kTile + 1) / 2;
-    const int64_t n = 8 * x + 8 * q + 8 * kNormParts + 8 * (int64_t)mp + (s > 1 ? 4 * s * tiles * kTile * kTile : 0);
-    return (n + 255) / 256 * 256;
-}
-
-template <int MODE>
-static int product(const MuonList& L, int from, int last, hipStream_t st) {
-    const MuonMatrix& e = L.a[L.count - 1];
-    const int t = e.mp / kTile;
-    const int n = e.first[MODE] + (MODE == kApply ? t * (e.np / kTile) : t * (t + 1) / 2 * (MODE == kGram ? e.splits : 1));
-    const int planes = L.dtype == SNAG_F32 ? 2 : 1;
-    const size_t lds = (size_t)2 * 2 * planes * kTile * kDepth * sizeof(_Float16);
-    if (planes == 2) {
-        static const hipError_t grown = hipFuncSetAttribute((const void*)muon_product_kernel<MODE, 2>, hipFuncAttributeMaxDynamicSharedMemorySize, 2 * 2 * 2 * kTile * kDepth * 2);
-        SNAG_REQUIRE(grown == hipSuccess, SNAG_ERR_LAUNCH, "muon: %s", hipGetErrorString(grown));
-        muon_product_kernel<MODE, 2><<<dim3(n), 256, lds, st>>>(L, from, last);
-    } else {
-        muon_product_kernel<MODE, 1><<<dim3(n), 256, lds, st>>>(L, from, last);
+// How one list of matrices is worked on.  narrow: every m <= 128 (muon_narrow_kernel).  Otherwise 256 x 256 tiles for the product with X when the
+// list has enough of them to occupy most CUs (they read half as much per multiplication; 128 x 128 ones fill the chip earlier).  The symmetric
+// products, half as many tiles, always run on 128 x 128 ones.
+struct MuonPlan { bool narrow; int tile, stages; };
+static MuonPlan plan_of(const int32_t* rows, const int32_t* cols, const int* at, int count) {
+    MuonPlan p{true, 128, 4};
+    int64_t big = 0, total = 0;
+    for (int k = 0; k < count; ++k) {
+        const int r = rows[at[k]], c = cols[at[k]], m = r < c ? r : c, n = r < c ? c : r;
+        p.narrow = p.narrow && m <= 128;
+        big += (int64_t)(pad_to(m, 256) / 256) * (pad_to(n, 256) / 256);
+        const int64_t t = pad_to(m, 128) / 128;
+        total += t * (t + 1) / 2 * (pad_to(n, 128) / 64);
     }
+    if (!p.narrow && big >= kCus * 3 / 8) p.tile = 256;
+    // LDS stages in a range of A's contraction: the list's stages over all CUs, at least four
+    const int64_t per = (total + kCus - 1) / kCus;
+    p.stages = (int)(per < 4 ? 4 : per);
+    return p;
+}
+static int splits_of(const MuonPlan& p, int np) { return p.narrow ? np / 128 : (np / 64 + p.stages - 1) / p.stages; }
+
+static int64_t matrix_bytes(const MuonPlan& p, int r, int c) {
+    const int m = r < c ? r : c, n = r < c ? c : r, mp = pad_to(m, p.tile), np = pad_to(n, p.tile), s = splits_of(p, np);
+    const int64_t x = (int64_t)mp * np, q = (int64_t)mp * mp, t = mp / 128;
+    const int64_t bytes = 8 * x + 8 * q + 8 * kNormParts + 8 * (int64_t)mp + (s > 1 ? 4 * s * (t * (t + 1) / 2) * 128 * 128 : 0);
+    return (bytes + 255) / 256 * 256;
+}
+
+// A call's matrices in the order they are worked on: the narrow ones first, kMaxList at a time.
+struct MuonLists {
+    const int32_t *rows, *cols;
+    int count, pass = 0, i = 0, n = 0, at[kMaxList];
+    MuonLists(const int32_t* r, const int32_t* c, int k) : rows(r), cols(c), count(k) {}
+    bool next() {                                              // the next list in at[0 .. n)
+        for (n = 0; pass < 2; ++pass, i = 0) {
+            for (; i < count && n < kMaxList; ++i)
+                if (((rows[i] < cols[i] ? rows[i] : cols[i]) <= 128) == (pass == 0)) at[n++] = i;
+            if (n > 0) return true;
+        }
+        return false;
+    }
+};
+
+struct MuonRun { MuonTable L; MuonTable* table; MuonPlan plan; int blocks_of[3], gram_tiles, blocks; bool vec; };
+
+template <class K>
+static int grow_lds(K kernel, size_t bytes) {
+    const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    return e == hipSuccess ? SNAG_OK : fail(SNAG_ERR_LAUNCH, "muon: %s", hipGetErrorString(e));
+}
+template <int MODE, int DT, int TILE, int NST>
+static int product_of(const MuonRun& R, int from, int last, hipStream_t st) {
+    using S = Shape<TILE, DT == SNAG_F32 ? 2 : 1, NST>;
+    static const int grown = grow_lds(muon_product_kernel<MODE, DT, TILE, NST>, S::kLds);
+    if (grown != SNAG_OK) return grown;
+    muon_product_kernel<MODE, DT, TILE, NST><<<dim3(R.blocks_of[MODE]), S::kThreads, S::kLds, st>>>(R.table, from, last);
     return check_launch("muon_product");
 }
+// A 128 x 128 workgroup takes 64 KB of LDS with two stages, so that two fit a CU and hide each other's waits; a launch with at most one per CU
+// takes 128 KB and loads three stages ahead instead.
+template <int MODE, int DT>
+static int product(const MuonRun& R, int from, int last, hipStream_t st) {
+    if constexpr (MODE == kApply) {
+        if (R.plan.tile == 256) return product_of<MODE, DT, 256, 2>(R, from, last, st);
+    }
+    if (R.blocks_of[MODE] <= kCus) return product_of<MODE, DT, 128, 4>(R, from, last, st);
+    return product_of<MODE, DT, 128, 2>(R, from, last, st);
+}
 
-// one list of at most kMaxList matrices
-static int muon_go(MuonList& L, int steps, hipStream_t st) {
-    int first[3] = {0, 0, 0}, blocks = 0, gram_tiles = 0;
-    for (int i = 0; i < L.count; ++i) {
-        MuonMatrix& a = L.a[i];
-        const int t = a.mp / kTile, tri = t * (t + 1) / 2;
-        for (int k = 0; k < 3; ++k) a.first[k] = first[k];
-        first[kGram] += tri * a.splits;
-        first[kPoly] += tri;
-        first[kApply] += t * (a.np / kTile);
-        const int b = (a.mp / 64) * (a.np / 64);
-        blocks = b > blocks ? b : blocks;
-        if (a.splits > 1 && tri > gram_tiles) gram_tiles = tri;
-    }
-    const dim3 gn(kNormParts, L.count), gs(blocks < 2048 ? blocks : 2048, L.count);
-    switch (L.dtype) {
-        case SNAG_F32: muon_norm_kernel<SNAG_F32><<<gn, 256, 0, st>>>(L); muon_start_kernel<SNAG_F32><<<gs, 256, 0, st>>>(L); break;
-        case SNAG_BF16: muon_norm_kernel<SNAG_BF16><<<gn, 256, 0, st>>>(L); muon_start_kernel<SNAG_BF16><<<gs, 256, 0, st>>>(L); break;
-        default: muon_norm_kernel<SNAG_F16><<<gn, 256, 0, st>>>(L); muon_start_kernel<SNAG_F16><<<gs, 256, 0, st>>>(L); break;
-    }
+static int gram_sum(const MuonRun& R, hipStream_t st) {
+    if (R.gram_tiles == 0) return SNAG_OK;
+    muon_gram_sum_kernel<<<dim3(16 * R.gram_tiles, R.L.count), 256, 0, st>>>(R.table);
+    return check_launch("muon_gram_sum");
+}
+
+template <int DT>
+static int muon_go(const MuonRun& R, int steps, hipStream_t st) {
+    const dim3 gn(kNormParts, R.L.count), gs(R.blocks < 2048 ? R.blocks : 2048, R.L.count);
+    if (R.vec) muon_norm_kernel<DT, true><<<gn, 256, 0, st>>>(R.L, R.table);
+    else muon_norm_kernel<DT, false><<<gn, 256, 0, st>>>(R.L, R.table);
+    if (int rc = check_launch("muon_norm")) return rc;
+    muon_start_kernel<DT><<<gs, 256, 0, st>>>(R.table);
     if (int rc = check_launch("muon_start")) return rc;
-    for (int k = 0; k < steps; ++k) {
-        if (int rc = product<kGram>(L, k & 1, 0, st)) return rc;
-        if (gram_tiles > 0) {
-            muon_gram_sum_kernel<<<dim3(16 * gram_tiles, L.count), 64, 0, st>>>(L);
-            if (int rc = check_launch("muon_gram_sum")) return rc;
+    if (R.plan.narrow) {
+        constexpr size_t lds = 4 * kImage * sizeof(_Float16) + (4 * 32 * kPitch + 128) * sizeof(float);
+        static const int grown = grow_lds(muon_narrow_kernel<DT>, lds);
+        if (grown != SNAG_OK) return grown;
+        for (int k = -1; k < steps; ++k) {
+            if (k >= 0)
+                if (int rc = gram_sum(R, st)) return rc;
+            muon_narrow_kernel<DT><<<dim3(R.blocks_of[kApply]), 256, lds, st>>>(R.table, k < 0 ? 0 : k & 1, k < 0, k + 1 == steps);
+            if (int rc = check_launch("muon_narrow")) return rc;
         }
-        if (int rc = product<kPoly>(L, k & 1, 0, st)) return rc;
-        if (int rc = product<kApply>(L, k & 1, k + 1 == steps, st)) return rc;
+        return SNAG_OK;
+    }
+    for (int k = 0; k < steps; ++k) {
+        if (int rc = product<kGram, DT>(R, k & 1, 0, st)) return rc;
+        if (int rc = gram_sum(R, st)) return rc;
+        if (int rc = product<kPoly, DT>(R, k & 1, 0, st)) return rc;
+        if (int rc = product<kApply, DT>(R, k & 1, k + 1 == steps, st)) return rc;
     }
     return SNAG_OK;
 }
@@ -490,7 +854,18 @@ static int muon_check(const char* what, const int32_t* rows, const int32_t* cols
     return SNAG_OK;
 }
 
-// All matrices of a call, kMaxList a launch; every list of launches starts at the workspace's beginning (they follow each other on the stream).
+static int64_t work_bytes_of(const int32_t* rows, const int32_t* cols, int count) {
+    int64_t most = 0;
+    for (MuonLists o(rows, cols, count); o.next();) {
+        const MuonPlan p = plan_of(rows, cols, o.at, o.n);
+        int64_t bytes = kTableBytes;
+        for (int i = 0; i < o.n; ++i) bytes += matrix_bytes(p, rows[o.at[i]], cols[o.at[i]]);
+        most = bytes > most ? bytes : most;
+    }
+    return most;
+}
+
+// All matrices of a call; every list of launches starts at the workspace's beginning (they follow each other on the stream).
 static int muon_run(const char* what, void* const* w, const void* const* g, float* const* mom, const int32_t* rows, const int32_t* cols, int count, int dtype, float lr, float mu, int nesterov,
                     float decay, int match_rms, int steps, float eps, void* work, int64_t work_bytes, void* stream) {
     if (int rc = muon_check(what, rows, cols, count, dtype)) return rc;
@@ -499,25 +874,40 @@ static int muon_run(const char* what, void* const* w, const void* const* g, floa
     if (count == 0) return SNAG_OK;
     SNAG_REQUIRE(w != nullptr && g != nullptr, SNAG_ERR_ARG, "%s: null pointer lists", what);
     for (int i = 0; i < count; ++i) SNAG_REQUIRE(w[i] != nullptr && g[i] != nullptr && (mom == nullptr || mom[i] != nullptr), SNAG_ERR_ARG, "%s: null matrix %d", what, i);
-    const int64_t need = snag_muon_work_bytes(rows, cols, count);
+    const int64_t need = work_bytes_of(rows, cols, count);
     SNAG_REQUIRE(work != nullptr && ((uintptr_t)work & 255) == 0 && work_bytes >= need, SNAG_ERR_ARG, "%s: workspace of %lld bytes (256-byte aligned), %lld needed", what, (long long)work_bytes,
                  (long long)need);
-    for (int i0 = 0; i0 < count; i0 += kMaxList) {
-        MuonList L{};
-        L.count = count - i0 < kMaxList ? count - i0 : kMaxList;
+    for (MuonLists o(rows, cols, count); o.next();) {
+        const int *at = o.at, n = o.n;
+        MuonRun R{};
+        R.plan = plan_of(rows, cols, at, n);
+        const int tile = R.plan.tile;
+        MuonTable& L = R.L;
+        L.count = n;
         L.dtype = dtype, L.step = mom != nullptr, L.nesterov = nesterov, L.mu = mu, L.keep = 1.f - lr * decay, L.eps = eps;
-        char* at = (char*)work;
-        for (int i = 0; i < L.count; ++i) {
+        R.table = (MuonTable*)work, R.vec = true;
+        char* space = (char*)work + kTableBytes;
+        for (int i = 0; i < n; ++i) {
             MuonMatrix& a = L.a[i];
-            const int r = rows[i0 + i], c = cols[i0 + i];
-            a.g = g[i0 + i], a.w = w[i0 + i], a.mom = mom != nullptr ? mom[i0 + i] : nullptr, a.work = at;
-            a.r = r, a.c = c, a.tall = r > c, a.m = r < c ? r : c, a.n = r < c ? c : r, a.mp = pad_tile(a.m), a.np = pad_tile(a.n);
-            a.splits = gram_splits(a.mp, a.np);
+            const int r = rows[at[i]], c = cols[at[i]];
+            a.g = g[at[i]], a.w = w[at[i]], a.mom = mom != nullptr ? mom[at[i]] : nullptr, a.work = space;
+            a.r = r, a.c = c, a.tall = r > c, a.m = r < c ? r : c, a.n = r < c ? c : r;
+            a.mp = pad_to(a.m, tile), a.np = pad_to(a.n, tile);
+            a.splits = splits_of(R.plan, a.np);
             const double s = match_rms ? 0.2 * sqrt((double)a.n) : sqrt(r > c ? (double)r / c : 1.0);
             a.update = (float)(lr * s);
-            at += matrix_bytes(r, c);
+            space += matrix_bytes(R.plan, r, c);
+            const int t = a.mp / 128, tri = t * (t + 1) / 2, b = (a.mp / 64) * (a.np / 64);
+            for (int q = 0; q < 3; ++q) L.first[q][i] = R.blocks_of[q];
+            R.blocks_of[kGram] += tri * a.splits;
+            R.blocks_of[kPoly] += tri;
+            R.blocks_of[kApply] += (a.mp / tile) * (a.np / tile);
+            R.blocks = b > R.blocks ? b : R.blocks;
+            if (a.splits > 1 && tri > R.gram_tiles) R.gram_tiles = tri;
+            R.vec = R.vec && (int64_t)r * c % 4 == 0 && aligned16(a.g) && aligned16(a.mom);
         }
-        if (int rc = muon_go(L, steps, (hipStream_t)stream)) return rc;
+        hipStream_t st = (hipStream_t)stream;
+        if (int rc = dtype == SNAG_F32 ? muon_go<SNAG_F32>(R, steps, st) : dtype == SNAG_BF16 ? muon_go<SNAG_BF16>(R, steps, st) : muon_go<SNAG_F16>(R, steps, st)) return rc;
     }
     return SNAG_OK;
 }
@@ -527,14 +917,10 @@ static int muon_run(const char* what, void* const* w, const void* const* g, floa
 using namespace snag;
 
 extern "C" SNAG_API int64_t snag_muon_work_bytes(const int32_t* rows_host, const int32_t* cols_host, int count) {
-    int64_t most = 0;
-    for (int i0 = 0; i0 < count && rows_host != nullptr && cols_host != nullptr; i0 += kMaxList) {
-        int64_t n = 0;
-        for (int i = i0; i < count && i < i0 + kMaxList; ++i)
-            if (rows_host[i] >= 1 && cols_host[i] >= 1) n += matrix_bytes(rows_host[i], cols_host[i]);
-        most = n > most ? n : most;
-    }
-    return most;
+    if (rows_host == nullptr || cols_host == nullptr) return 0;
+    for (int i = 0; i < count; ++i)
+        if (rows_host[i] < 1 || cols_host[i] < 1) return 0;
+    return work_bytes_of(rows_host, cols_host, count);
 }
 
 extern "C" SNAG_API int snag_orthogonalize(const void* const* g_host, void* const* out_host, const int32_t* rows_host, const int32_t* cols_host, int count, int dtype,

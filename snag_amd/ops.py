@@ -4,6 +4,7 @@ Shape/dtype/contiguity errors are raised in Python before the call, mirroring th
 assert/exception convention (SURVEY.md par. 8b "Errors").
 """
 import ctypes
+import functools
 
 import torch
 
@@ -545,11 +546,12 @@ CROSS_MAX_HEAD_DIM = 128       # SNAG_CROSS_MAX_HEAD_DIM
 SANDWICH_MAX_DIM = 8192        # SNAG_SANDWICH_MAX_DIM
 MUON_MAX_SIDE = 16384          # SNAG_MUON_MAX_SIDE
 NORMS = {"rms": 0, "layer": 1}
+_Strides = ctypes.c_int64 * 9
 
 
 def _any(t, name, ndim=None):
     """A CUDA tensor of one of the three types these operators take; any strides."""
-    if not torch.is_tensor(t):
+    if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a torch.Tensor, got {type(t).__name__}")
     if t.dtype not in DTYPES:
         raise TypeError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
@@ -560,13 +562,18 @@ def _any(t, name, ndim=None):
     return t
 
 
+# the current stream / device as plain numbers: building torch's Stream object costs more than the launch
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+
 def _call_on(device, name, *args):
     """The entry on the current stream of the operands' device (which need not be the current one)."""
-    if device.index == torch.cuda.current_device():
-        call(name, *args, stream())
+    index = device.index
+    if index == _current_device():
+        call(name, *args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            call(name, *args, stream())
+            call(name, *args, _raw_stream(index))
 
 
 def _one_device(device, **tensors):
@@ -575,30 +582,35 @@ def _one_device(device, **tensors):
             raise ValueError(f"{name} is on {t.device}, the first operand on {device}")
 
 
+@functools.lru_cache(maxsize=4096)
+def _cross_work_floats(shape, backward):
+    return _lib.load().snag_cross_work_floats(*shape, backward)
+
+
 def _cross_args(q, k, v, kv_lens, key_mask, scale):
     _any(q, "q", 4), _any(k, "k", 4), _any(v, "v", 4)
-    B, Lq, H, d = q.shape
+    (B, Lq, H, d), ks = q.shape, k.shape
     if k.dtype != q.dtype or v.dtype != q.dtype:
         raise TypeError(f"q, k and v must share one type, got {q.dtype}, {k.dtype}, {v.dtype}")
-    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != d:
+    if ks != v.shape or ks[0] != B or ks[3] != d:
         raise ValueError(f"k and v must be [{B}, Lk, Hkv, {d}], got {tuple(k.shape)} and {tuple(v.shape)}")
-    Lk, Hkv = k.shape[1], k.shape[2]
+    Lk, Hkv = ks[1], ks[2]
     if H == 0 or Hkv == 0 or H % Hkv:
         raise ValueError(f"{H} heads are not a multiple of {Hkv} key/value heads")
     if not 1 <= d <= CROSS_MAX_HEAD_DIM:
         raise ValueError(f"head dimension {d} is not in 1..{CROSS_MAX_HEAD_DIM}")
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        if t.numel() and t.stride(3) != 1 and d > 1:
-            raise ValueError(f"{name}: the elements of a head must be adjacent (strides {tuple(t.stride())})")
-    lens_bytes = 4
+    qs, kt, vt = q.stride(), k.stride(), v.stride()
+    for t, st, name in ((q, qs, "q"), (k, kt, "k"), (v, vt, "v")):
+        if st[3] != 1 and d > 1 and t.numel():
+            raise ValueError(f"{name}: the elements of a head must be adjacent (strides {st})")
+    lens_bytes = mask_ld = 0
     if kv_lens is not None:
         _idx(kv_lens, "kv_lens", 1)
         if kv_lens.shape[0] != B:
             raise ValueError(f"kv_lens must be [{B}], got {tuple(kv_lens.shape)}")
         lens_bytes = kv_lens.element_size()
-    mask_ld = 0
     if key_mask is not None:
-        if not torch.is_tensor(key_mask) or key_mask.dtype not in (torch.bool, torch.uint8):
+        if not isinstance(key_mask, torch.Tensor) or key_mask.dtype not in (torch.bool, torch.uint8):
             raise TypeError("key_mask: expected a bool (or uint8) tensor, true where a key is seen")
         if tuple(key_mask.shape) != (B, Lk):
             raise ValueError(f"key_mask must be [{B}, {Lk}], got {tuple(key_mask.shape)}")
@@ -611,13 +623,13 @@ def _cross_args(q, k, v, kv_lens, key_mask, scale):
     scale = d ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < float("inf"):
         raise ValueError(f"scale must be positive and finite, got {scale}")
-    strides = (ctypes.c_int64 * 9)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
+    strides = _Strides(*qs[:3], *kt[:3], *vt[:3])
     shape = (DTYPES[q.dtype], B, Lq, Lk, H, Hkv, d)
     return shape, (ptr(q), ptr(k), ptr(v), *shape, ctypes.addressof(strides), ptr(kv_lens), lens_bytes, ptr(key_mask), mask_ld, scale), strides
 
 
 def _cross_work(shape, backward, device):
-    n = _lib.load().snag_cross_work_floats(*shape, int(backward))
+    n = _cross_work_floats(shape, int(backward))
     return (torch.empty(n, device=device, dtype=f32) if n else None), n
 
 
@@ -649,6 +661,11 @@ def cross_attention_bwd(q, k, v, out, lse, d_out, kv_lens=None, key_mask=None, s
     return dq, dk, dv
 
 
+@functools.lru_cache(maxsize=4096)
+def _sandwich_work_floats(rows, per_gate, dim):
+    return _lib.load().snag_sandwich_work_floats(rows, per_gate, dim)
+
+
 def _sandwich_args(x, y, post_weight, post_bias, pre_weight, pre_bias, gate, kind):
     """-> rows, dim, (weights' dtype code), (gate dtype code), rows per gate row."""
     _any(x, "x"), _any(y, "y")
@@ -665,7 +682,9 @@ def _sandwich_args(x, y, post_weight, post_bias, pre_weight, pre_bias, gate, kin
     if not 1 <= dim <= SANDWICH_MAX_DIM:
         raise ValueError(f"row width {dim} is not in 1..{SANDWICH_MAX_DIM}")
     rows = x.numel() // dim
-    wt = None
+    wt, dev = None, x.device
+    if y.device != dev:
+        raise ValueError(f"y is on {y.device}, x on {dev}")
     for t, name in ((post_weight, "post_weight"), (post_bias, "post_bias"), (pre_weight, "pre_weight"), (pre_bias, "pre_bias")):
         if t is None:
             continue
@@ -674,6 +693,8 @@ def _sandwich_args(x, y, post_weight, post_bias, pre_weight, pre_bias, gate, kin
             raise ValueError(f"{name} must be a contiguous [{dim}], got {tuple(t.shape)}")
         if t.dtype not in (y.dtype, f32) or wt not in (None, t.dtype):
             raise TypeError(f"weights and biases must share one type, float32 or y's {y.dtype}; {name} is {t.dtype}")
+        if t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, x on {dev}")
         wt = t.dtype
     per_gate, gt = max(rows, 1), y.dtype
     if gate is not None:
@@ -685,8 +706,9 @@ def _sandwich_args(x, y, post_weight, post_bias, pre_weight, pre_bias, gate, kin
         G = gate.shape[0] if gate.dim() == 2 else 1
         if rows and (G == 0 or rows % G):
             raise ValueError(f"{rows} rows do not divide among {G} gate rows")
+        if gate.device != dev:
+            raise ValueError(f"gate is on {gate.device}, x on {dev}")
         per_gate, gt = (max(rows // G, 1) if G else 1), gate.dtype
-    _one_device(x.device, y=y, post_weight=post_weight, post_bias=post_bias, pre_weight=pre_weight, pre_bias=pre_bias, gate=gate)
     return rows, dim, DTYPES[wt if wt is not None else y.dtype], DTYPES[gt], per_gate
 
 
@@ -716,7 +738,7 @@ def sandwich_norm_bwd(x, y, stats, d_h, d_z, post_weight=None, pre_weight=None, 
     _one_device(x.device, stats=stats, d_h=d_h, d_z=d_z)
     new = lambda t: None if t is None else torch.empty_like(t) if rows else torch.zeros_like(t)
     dx, dy, dpw, dqw, dpb, dqb, dg = (new(t) for t in (x, y, post_weight, pre_weight, post_bias, pre_bias, gate))
-    n = _lib.load().snag_sandwich_work_floats(rows, per_gate, dim)
+    n = _sandwich_work_floats(rows, per_gate, dim)
     work = torch.empty(n, device=x.device, dtype=f32)
     _call_on(x.device, "snag_sandwich_bwd", ptr(x), DTYPES[x.dtype], ptr(y), DTYPES[y.dtype], rows, dim, ptr(post_weight), ptr(post_bias), ptr(pre_weight), wt,
              ptr(gate), gt, per_gate, float(res_scale), NORMS[kind], ptr(stats), ptr(d_h), ptr(d_z), ptr(dx), ptr(dy), ptr(dpw), ptr(dpb), ptr(dqw), ptr(dqb),
@@ -724,47 +746,64 @@ def sandwich_norm_bwd(x, y, stats, d_h, d_z, post_weight=None, pre_weight=None, 
     return dx, dy, dpw, dqw, dpb, dqb, dg
 
 
-def _matrices(ts, name, dtype=None, shapes=None):
-    """A list of contiguous 2-D CUDA tensors of one type on one device."""
+def _matrices(ts, name, dtype=None, shapes=None, device=None):
+    """A list of contiguous 2-D CUDA tensors of one type on one device -> (list, shapes)."""
     ts = list(ts)
+    if ts:
+        dtype, device = dtype or _any(ts[0], f"{name}[0]").dtype, device or ts[0].device
+    got = []
     for i, t in enumerate(ts):
-        _any(t, f"{name}[{i}]", 2)
-        if t.dtype != (dtype or ts[0].dtype):
-            raise TypeError(f"{name}[{i}]: expected {dtype or ts[0].dtype}, got {t.dtype}")
+        _any(t, name, 2)
+        s = t.shape
+        if t.dtype != dtype:
+            raise TypeError(f"{name}[{i}]: expected {dtype}, got {t.dtype}")
         if not t.is_contiguous():
             raise ValueError(f"{name}[{i}]: tensor must be contiguous")
-        if shapes is not None and tuple(t.shape) != tuple(shapes[i]):
-            raise ValueError(f"{name}[{i}] must be {tuple(shapes[i])}, got {tuple(t.shape)}")
-        if not (1 <= t.shape[0] <= MUON_MAX_SIDE and 1 <= t.shape[1] <= MUON_MAX_SIDE):
-            raise ValueError(f"{name}[{i}]: sides must be in 1..{MUON_MAX_SIDE}, got {tuple(t.shape)}")
-        _one_device(ts[0].device, **{f"{name}[{i}]": t})
-    return ts
+        if shapes is not None and s != shapes[i]:
+            raise ValueError(f"{name}[{i}] must be {tuple(shapes[i])}, got {tuple(s)}")
+        if not (1 <= s[0] <= MUON_MAX_SIDE and 1 <= s[1] <= MUON_MAX_SIDE):
+            raise ValueError(f"{name}[{i}]: sides must be in 1..{MUON_MAX_SIDE}, got {tuple(s)}")
+        if t.device != device:
+            raise ValueError(f"{name}[{i}] is on {t.device}, the first matrix on {device}")
+        got.append(s)
+    return ts, got
 
 
 def _muon_lists(*lists):
     return [(ctypes.c_void_p * len(ts))(*[t.data_ptr() for t in ts]) for ts in lists]
 
 
-def _muon_shapes(ts):
-    n = len(ts)
-    rows, cols = (ctypes.c_int32 * n)(*[t.shape[0] for t in ts]), (ctypes.c_int32 * n)(*[t.shape[1] for t in ts])
-    nbytes = _lib.load().snag_muon_work_bytes(ctypes.addressof(rows), ctypes.addressof(cols), n)
-    return rows, cols, torch.empty(nbytes, device=ts[0].device, dtype=torch.uint8), nbytes
+@functools.lru_cache(maxsize=256)
+def _muon_shapes(shapes):
+    """Host arrays of the shapes and the workspace they need (by shape alone)."""
+    n = len(shapes)
+    rows, cols = (ctypes.c_int32 * n)(*[s[0] for s in shapes]), (ctypes.c_int32 * n)(*[s[1] for s in shapes])
+    return rows, cols, _lib.load().snag_muon_work_bytes(ctypes.addressof(rows), ctypes.addressof(cols), n)
 
 
 def orthogonalize(gs, outs=None, steps=5, eps=1e-7):
     """Newton-Schulz orthogonalisation of a list of matrices of one type -> list (or into ``outs``; outs[i] may be gs[i]).
     C ABI: snag_orthogonalize."""
-    gs = _matrices(gs, "gs")
+    gs, shapes = _matrices(gs, "gs")
     if not 1 <= int(steps) <= 100:
         raise ValueError(f"steps must be in 1..100, got {steps}")
-    outs = [torch.empty_like(g) for g in gs] if outs is None else _matrices(outs, "outs", gs[0].dtype if gs else None, [g.shape for g in gs])
-    if len(outs) != len(gs):
-        raise ValueError(f"{len(gs)} matrices, {len(outs)} outputs")
+    if outs is None:
+        outs = [torch.empty_like(g) for g in gs]
+    else:
+        outs = list(outs)
+        if len(outs) != len(gs):
+            raise ValueError(f"{len(gs)} matrices, {len(outs)} outputs")
+        if gs:
+            _matrices(outs, "outs", gs[0].dtype, shapes, gs[0].device)
+            if len({t.data_ptr() for t in outs}) != len(outs):
+                raise ValueError("a matrix is listed twice")
+            at = {g.data_ptr(): i for i, g in enumerate(gs)}
+            if any(at.get(t.data_ptr(), i) != i for i, t in enumerate(outs)):
+                raise ValueError("an output may be its own input, not another one's")
     if not gs:
         return outs
-    _one_device(gs[0].device, outs=outs[0])
-    rows, cols, work, n = _muon_shapes(gs)
+    rows, cols, n = _muon_shapes(tuple(shapes))
+    work = torch.empty(n, device=gs[0].device, dtype=torch.uint8)
     pg, po = _muon_lists(gs, outs)
     _call_on(gs[0].device, "snag_orthogonalize", ctypes.addressof(pg), ctypes.addressof(po), ctypes.addressof(rows), ctypes.addressof(cols), len(gs),
              DTYPES[gs[0].dtype], int(steps), float(eps), ptr(work), n)
@@ -773,8 +812,7 @@ def orthogonalize(gs, outs=None, steps=5, eps=1e-7):
 
 def muon_step(weights, grads, momenta, lr, momentum=0.95, nesterov=True, weight_decay=0.0, match_rms=False, steps=5, eps=1e-7):
     """One Muon update, in place on ``weights`` (one type) and ``momenta`` (fp32); ``grads`` have the weights' type.  C ABI: snag_muon_step."""
-    weights = _matrices(weights, "weights")
-    shapes = [w.shape for w in weights]
+    weights, shapes = _matrices(weights, "weights")
     grads, momenta = list(grads), list(momenta)
     if len(grads) != len(weights) or len(momenta) != len(weights):
         raise ValueError(f"{len(weights)} weights, {len(grads)} gradients, {len(momenta)} momenta")
@@ -784,11 +822,12 @@ def muon_step(weights, grads, momenta, lr, momentum=0.95, nesterov=True, weight_
         raise ValueError(f"momentum must be in [0, 1), got {momentum}")
     if not weights:
         return
-    _matrices(grads, "grads", weights[0].dtype, shapes), _matrices(momenta, "momenta", f32, shapes)
-    _one_device(weights[0].device, grads=grads[0], momenta=momenta[0])
+    dev = weights[0].device
+    _matrices(grads, "grads", weights[0].dtype, shapes, dev), _matrices(momenta, "momenta", f32, shapes, dev)
     if len({t.data_ptr() for t in weights}) != len(weights) or len({t.data_ptr() for t in momenta}) != len(momenta):
         raise ValueError("a matrix is listed twice")
-    rows, cols, work, n = _muon_shapes(weights)
+    rows, cols, n = _muon_shapes(tuple(shapes))
+    work = torch.empty(n, device=dev, dtype=torch.uint8)
     pw, pg, pm = _muon_lists(weights, grads, momenta)
     _call_on(weights[0].device, "snag_muon_step", ctypes.addressof(pw), ctypes.addressof(pg), ctypes.addressof(pm), ctypes.addressof(rows), ctypes.addressof(cols),
              len(weights), DTYPES[weights[0].dtype], float(lr), float(momentum), int(nesterov), float(weight_decay), int(match_rms), int(steps), float(eps),
