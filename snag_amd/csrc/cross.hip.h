@@ -17,6 +17,7 @@ struct CrossArgs {
     int64_t qsb, qsl, qsh, ksb, ksl, ksh, vsb, vsl, vsh;      // element strides of batch / position / head; the head's own elements are adjacent
     int B, Lq, Lk, H, Hkv, G, d;
     int rows;                    // Lq * G
+    uint32_t g_magic;            // high word of row * g_magic = row / G for every row; 0: divide
     const void* lens;            // [B] int32 / int64 or NULL: keys at and behind lens[b] are not seen
     int lens_bytes;
     const uint8_t* mask;         // [B, Lk] (row pitch mask_ld) or NULL: 0 = key not seen
@@ -26,7 +27,7 @@ struct CrossArgs {
     void* out;                   // [B, Lq, H, d] dense
     float* lse;                  // [B, H, Lq]: log2 of the row's sum of exp2(c2 q.k); -inf for a row that sees no key
     int splits;                  // key ranges (forward, d q) or row ranges (d k, d v) worked on by different workgroups
-    int per_split;               // tiles per range
+    int per_split;               // keys / rows per range, a multiple of 64
     float* part;                 // splits > 1: partial results, see the kernels
     // backward
     const void *o, *dout;        // [B, Lq, H, d] dense
@@ -88,6 +89,26 @@ __device__ __forceinline__ typename Chunk<T>::vec load_chunk(const T* __restrict
 
 static inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
+// How a call is worked on (csrc/cross.hip chooses)
+struct CrossPlan {
+    int rows_path;               // a few rows per key/value head: csrc/cross_rows.hip
+    int nw_q, nw_k;              // waves of a workgroup that owns rows / keys
+    int dp;                      // d rounded up to what the kernels are built for
+    int s_fwd, s_dq, s_dkv;      // ranges
+};
+#define SNAG_CROSS_DP(CALL)                  \
+    switch (p.dp) {                          \
+        case 32: CALL(32); break;            \
+        case 64: CALL(64); break;            \
+        default: CALL(128); break;           \
+    }
+
+static inline int range_of(int n, int ranges) { return ((n + 63) / 64 + ranges - 1) / ranges * 64; }      // of n keys or rows
+
+int cross_tiles_fwd(const CrossArgs& a, const CrossPlan& p, int dtype, hipStream_t st);
+int cross_tiles_bwd(const CrossArgs& a, const CrossPlan& p, float* delta, int dtype, hipStream_t st);
+int cross_combine(const CrossArgs& a, int dtype, hipStream_t st);
+int cross_sum(const float* part, int64_t n, int ranges, void* out, int dtype, hipStream_t st);
 int cross_rows_fwd(const CrossArgs& a, int dtype, hipStream_t st);
 int cross_rows_bwd(const CrossArgs& a, int dtype, hipStream_t st);
 int cross_rows_splits(int B, int Hkv, int Lk, int d, int dtype);

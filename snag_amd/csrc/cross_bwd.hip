@@ -1,0 +1,304 @@
+// Cross attention, tiled backward (csrc/cross_tiles.hip.h has the scheme): d q, d k / d v, and the joins of split ranges.
+//
+// Two passes, each recomputing the scores: d q with 32 rows per wave (three products per key tile), d k / d v with 32 keys per wave (four).  One
+// pass that did both would save two of the seven products and need atomics for one of the sides.  Bound by the matrix pipe.
+#include "cross_tiles.hip.h"
+
+namespace snag {
+
+// delta[b, head, l] = sum_d dout o, one 16-lane group per row
+template <class T>
+__global__ __launch_bounds__(256) void cross_delta_kernel(CrossArgs a, float* __restrict__ delta) {
+    constexpr int C = Chunk<T>::n;
+    const int64_t n = (int64_t)a.B * a.Lq * a.H, at = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    const int t = threadIdx.x & 15;
+    float s = 0.f;
+    if (at < n)
+        for (int col = t * C; col < a.d; col += 16 * C) {
+            const auto x = load_chunk<T>((const T*)a.o + at * a.d, col, a.d, true, a.vec_o);
+            const auto y = load_chunk<T>((const T*)a.dout + at * a.d, col, a.d, true, a.vec_o);
+#pragma unroll
+            for (int j = 0; j < C; ++j) s = fmaf((float)x[j], (float)y[j], s);
+        }
+    s = sum16(s);
+    if (at < n && t == 0) {
+        const int64_t head = at % a.H, bl = at / a.H, l = bl % a.Lq, b = bl / a.Lq;
+        delta[(b * a.H + head) * a.Lq + l] = s;
+    }
+}
+
+// d q: as the forward, 32 rows per wave; splits > 1: part[split][B, Lq, H, d], joined by cross_sum_kernel
+template <class T, int DP, int NW, int KT, bool DIRECT>
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 128 ? 1 : 2) void cross_dq_kernel(CrossArgs a) {
+    using M = Mma<T>;
+    constexpr int NT = NW * 64;
+    __shared__ __attribute__((aligned(16))) T lk[2][KT * DP];
+    __shared__ __attribute__((aligned(16))) T lv[2][KT * DP];
+    __shared__ __attribute__((aligned(16))) float bias[2][DIRECT ? 4 : KT];
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_id_uniform(), h = lane >> 5;
+    const int64_t tiles = (a.rows + NW * 32 - 1) / (NW * 32);
+    const Problem pr = problem_of(a, tiles);
+    const int b = pr.b, hk = pr.hk;
+    const int len = cross_len(a, b);
+    const int row = (int)pr.tile * NW * 32 + wave * 32 + (lane & 31);
+    const bool own = row < a.rows;
+    const int l = own ? row_l(a, row) : 0, head = hk * a.G + (own ? row - l * a.G : 0);
+    const T* kb = (const T*)a.k + b * a.ksb + hk * a.ksh;
+    const T* vb = (const T*)a.v + b * a.vsb + hk * a.vsh;
+    const int64_t at = ((int64_t)b * a.H + head) * a.Lq + l, dense = (((int64_t)b * a.Lq + l) * a.H + head) * a.d;
+
+    const int t0 = pr.split * a.per_split / KT, t1 = min((len + KT - 1) / KT, t0 + a.per_split / KT);
+    TileFetch<T, DP, KT, NT, DIRECT> fk, fv;
+    float fb = 0.f;
+    auto fetch = [&](int t) {
+        const int key0 = t * KT;
+        auto row_at = [&](const T* base, int64_t step, int i, bool& ok) {
+            const int key = DIRECT ? min(key0 + i, len - 1) : key0 + i;
+            ok = DIRECT || key_seen(a, b, key, len);
+            return base + key * step;
+        };
+        fk.fetch([&](int i, bool& ok) { return row_at(kb, a.ksl, i, ok); }, lk[t & 1], a.d, a.vec_k, tid);
+        fv.fetch([&](int i, bool& ok) { return row_at(vb, a.vsl, i, ok); }, lv[t & 1], a.d, a.vec_v, tid);
+        if (!DIRECT && tid < KT) fb = key_seen(a, b, key0 + tid, len) ? 0.f : -INFINITY;
+    };
+    auto store = [&](int t) {
+        fk.store(lk[t & 1], tid);
+        fv.store(lv[t & 1], tid);
+        if (!DIRECT && tid < KT) bias[t & 1][tid] = fb;
+    };
+    if (t0 < t1) fetch(t0);
+    typename M::Frag q[DP / 16], dout[DP / 16];
+    own_row<T, DP>(q, (const T*)a.q + b * a.qsb + l * a.qsl + head * a.qsh, a.d, own, a.vec_q, lane);
+    own_row<T, DP>(dout, (const T*)a.dout + dense, a.d, own, a.vec_o, lane);
+    const float lse = own ? usable_lse(a.lse[at]) : INFINITY, delta = own ? a.delta[at] : 0.f;
+    if (t0 < t1) store(t0);
+    f32x16 acc[DP / 32];
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) acc[i] = f32x16{};
+    for (int t = t0; t < t1; ++t) {
+        tile_ready();
+        if (t + 1 < t1) fetch(t + 1);
+        const T *ck = lk[t & 1], *cv = lv[t & 1];
+        const bool biased = DIRECT ? (t + 1) * KT > len : a.mask != nullptr || (t + 1) * KT > len;
+#pragma unroll
+        for (int kt = 0; kt < KT / 32; ++kt) {
+            f32x16 s{}, dp{};
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) {
+                s = M::mma(M::template rows<DP>(ck, kt * 32, c * 16, lane), q[c], s);
+                dp = M::mma(M::template rows<DP>(cv, kt * 32, c * 16, lane), dout[c], dp);
+            }
+            if (biased) {
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int i = kt * 32 + g * 8 + h * 4;
+                    if constexpr (DIRECT) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) s[4 * g + j] = t * KT + i + j < len ? s[4 * g + j] : -INFINITY;
+                    } else {
+                        const f32x4 bb = *(const f32x4*)(bias[t & 1] + i);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) s[4 * g + j] += bb[j];
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.c2, -lse)) * (dp[i] - delta);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const typename M::Frag ds = pack<T>(s, u);
+#pragma unroll
+                for (int db = 0; db < DP / 32; ++db) acc[db] = M::mma(M::template cols<DP>(ck, kt * 32 + u * 16, db * 32, lane), ds, acc[db]);
+            }
+        }
+        if (t + 1 < t1) store(t + 1);
+    }
+    if (!own) return;
+    if (a.splits > 1) store_row<float, DP>(a.part + (int64_t)pr.split * a.B * a.Lq * a.H * a.d + dense, acc, a.scale, a.d, lane);
+    else store_row<T, DP>((T*)a.dq + dense, acc, a.scale, a.d, lane);
+}
+
+// d k, d v: 32 keys per wave, row tiles of RT through LDS; splits > 1: part[2][split][B, Lk, Hkv, d] (d k, then d v)
+template <class T, int DP, int NW, int RT, bool DIRECT>
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void cross_dkv_kernel(CrossArgs a) {
+    using M = Mma<T>;
+    constexpr int NT = NW * 64, KEYS = NW * 32;
+    // 16-bit rows of 128: d k and d v take 128 registers, k another 32; v, the fourth operand, is read from LDS so that two waves fit a SIMD
+    constexpr bool VLDS = sizeof(T) == 2 && DP == 128 && NW == 4;
+    __shared__ __attribute__((aligned(16))) T lvv[VLDS ? KEYS * DP : 16];
+    __shared__ __attribute__((aligned(16))) T lq[2][RT * DP];
+    __shared__ __attribute__((aligned(16))) T lo[2][RT * DP];
+    __shared__ __attribute__((aligned(16))) float stat[2][2][RT];
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_id_uniform(), h = lane >> 5;
+    const int64_t tiles = (a.Lk + NW * 32 - 1) / (NW * 32);
+    const Problem pr = problem_of(a, tiles);
+    const int b = pr.b, hk = pr.hk;
+    const int len = cross_len(a, b);
+    const int key0 = (int)pr.tile * NW * 32, key = key0 + wave * 32 + (lane & 31);
+    const bool own = key < a.Lk, seen = own && key_seen(a, b, key, len);
+
+    f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) dk[i] = dv[i] = f32x16{};
+    const int t0 = pr.split * a.per_split / RT, t1 = key0 < len ? min((a.rows + RT - 1) / RT, t0 + a.per_split / RT) : t0;
+    if (t0 < t1) {
+        TileFetch<T, DP, RT, NT, DIRECT> fq, fo;
+        float fs0 = 0.f, fs1 = 0.f;
+        // DIRECT: rows behind the last one are read as the last one, their p is 0
+        auto fetch = [&](int t) {
+            const int r0 = t * RT;
+            fq.fetch([&](int i, bool& ok) {
+                const int r = min(r0 + i, a.rows - 1), l = row_l(a, r);
+                ok = r0 + i < a.rows;
+                return (const T*)a.q + b * a.qsb + l * a.qsl + (hk * a.G + r - l * a.G) * a.qsh;
+            }, lq[t & 1], a.d, a.vec_q, tid);
+            fo.fetch([&](int i, bool& ok) {
+                const int r = min(r0 + i, a.rows - 1), l = row_l(a, r);
+                ok = r0 + i < a.rows;
+                return (const T*)a.dout + (((int64_t)b * a.Lq + l) * a.H + hk * a.G + r - l * a.G) * a.d;
+            }, lo[t & 1], a.d, a.vec_o, tid);
+            if (tid < RT) {
+                const int r = min(r0 + tid, a.rows - 1), l = row_l(a, r);
+                const int64_t at = ((int64_t)b * a.H + hk * a.G + r - l * a.G) * a.Lq + l;
+                fs0 = r0 + tid < a.rows ? usable_lse(a.lse[at]) : INFINITY;
+                fs1 = r0 + tid < a.rows ? a.delta[at] : 0.f;
+            }
+        };
+        auto store = [&](int t) {
+            fq.store(lq[t & 1], tid);
+            fo.store(lo[t & 1], tid);
+            if (tid < RT) stat[t & 1][0][tid] = fs0, stat[t & 1][1][tid] = fs1;
+        };
+        fetch(t0);
+        if constexpr (VLDS) {
+            TileFetch<T, DP, KEYS, NT, DIRECT> fv;
+            fv.fetch([&](int i, bool& ok) {
+                const int at = DIRECT ? min(key0 + i, len - 1) : key0 + i;
+                ok = DIRECT || key_seen(a, b, at, len);
+                return (const T*)a.v + b * a.vsb + hk * a.vsh + at * a.vsl;
+            }, lvv, a.d, a.vec_v, tid);
+            fv.store(lvv, tid);
+        }
+        typename M::Frag k[DP / 16], v[VLDS ? 1 : DP / 16];
+        own_row<T, DP>(k, (const T*)a.k + b * a.ksb + hk * a.ksh + key * a.ksl, a.d, seen, a.vec_k, lane);
+        if constexpr (!VLDS) own_row<T, DP>(v, (const T*)a.v + b * a.vsb + hk * a.vsh + key * a.vsl, a.d, seen, a.vec_v, lane);
+        store(t0);
+        for (int t = t0; t < t1; ++t) {
+            tile_ready();
+            if (t + 1 < t1) fetch(t + 1);
+            const T *cq = lq[t & 1], *co = lo[t & 1];
+#pragma unroll
+            for (int rt = 0; rt < RT / 32; ++rt) {
+                f32x16 s{}, dp{};
+#pragma unroll
+                for (int c = 0; c < DP / 16; ++c) {
+                    s = M::mma(M::template rows<DP>(cq, rt * 32, c * 16, lane), k[c], s);
+                    if constexpr (VLDS) dp = M::mma(M::template rows<DP>(co, rt * 32, c * 16, lane), M::template rows<DP>(lvv, wave * 32, c * 16, lane), dp);
+                    else dp = M::mma(M::template rows<DP>(co, rt * 32, c * 16, lane), v[c], dp);
+                }
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int i0 = rt * 32 + g * 8 + h * 4;
+                    const f32x4 ls = *(const f32x4*)(stat[t & 1][0] + i0), de = *(const f32x4*)(stat[t & 1][1] + i0);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int i = 4 * g + j;
+                        s[i] = seen ? __builtin_amdgcn_exp2f(fmaf(s[i], a.c2, -ls[j])) : 0.f;
+                        dp[i] = seen ? s[i] * (dp[i] - de[j]) : 0.f;
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const typename M::Frag p = pack<T>(s, u), ds = pack<T>(dp, u);
+#pragma unroll
+                    for (int db = 0; db < DP / 32; ++db) {
+                        dv[db] = M::mma(M::template cols<DP>(co, rt * 32 + u * 16, db * 32, lane), p, dv[db]);
+                        dk[db] = M::mma(M::template cols<DP>(cq, rt * 32 + u * 16, db * 32, lane), ds, dk[db]);
+                    }
+                }
+            }
+            if (t + 1 < t1) store(t + 1);
+        }
+    }
+    if (!own) return;
+    const int64_t dense = (((int64_t)b * a.Lk + key) * a.Hkv + hk) * a.d, n = (int64_t)a.B * a.Lk * a.Hkv * a.d;
+    if (a.splits > 1) {
+        store_row<float, DP>(a.part + pr.split * n + dense, dk, a.scale, a.d, lane);
+        store_row<float, DP>(a.part + (a.splits + pr.split) * n + dense, dv, 1.f, a.d, lane);
+    } else {
+        store_row<T, DP>((T*)a.dk + dense, dk, a.scale, a.d, lane);
+        store_row<T, DP>((T*)a.dv + dense, dv, 1.f, a.d, lane);
+    }
+}
+
+// out[i] = sum over ranges of part[range][i], in order
+template <class T>
+__global__ __launch_bounds__(256) void cross_sum_kernel(const float* __restrict__ part, int64_t n, int ranges, T* __restrict__ out) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    float s = 0.f;
+    for (int r = 0; r < ranges; ++r) s += part[r * n + i];
+    out[i] = (T)s;
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------
+template <class T>
+static int sum_ranges(const float* part, int64_t n, int ranges, void* out, hipStream_t st) {
+    if (n == 0) return SNAG_OK;
+    cross_sum_kernel<T><<<dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st>>>(part, n, ranges, (T*)out);
+    return check_launch("cross_sum");
+}
+int cross_sum(const float* part, int64_t n, int ranges, void* out, int dtype, hipStream_t st) {
+    return dtype == SNAG_F32 ? sum_ranges<float>(part, n, ranges, out, st) : dtype == SNAG_BF16 ? sum_ranges<bf16_t>(part, n, ranges, out, st) : sum_ranges<f16_t>(part, n, ranges, out, st);
+}
+
+template <class T, int T4>
+static int bwd(CrossArgs a, const CrossPlan& p, float* delta, int dtype, hipStream_t st) {
+    const int64_t nq = (int64_t)a.B * a.Lq * a.H, nk = (int64_t)a.B * a.Lk * a.Hkv;
+    const bool whole = a.d == p.dp && a.vec_q && a.vec_k && a.vec_v && a.vec_o;
+    a.delta = delta;
+    if (nq > 0) {
+        cross_delta_kernel<T><<<dim3((unsigned)((nq + 15) / 16)), 256, 0, st>>>(a, delta);
+        if (int rc = check_launch("cross_delta")) return rc;
+        a.splits = p.s_dq;
+        a.per_split = range_of(a.Lk, a.splits);
+        const int64_t tiles = (a.rows + p.nw_q * 32 - 1) / (p.nw_q * 32), n = (int64_t)a.B * a.Hkv * tiles * a.splits;
+        SNAG_REQUIRE(n < (int64_t)1 << 31, SNAG_ERR_UNSUPPORTED, "cross attention: %lld workgroups", (long long)n);
+        const dim3 grid((unsigned)n);
+        const bool direct = p.nw_q == 4 && whole && a.mask == nullptr;
+#define CALL(DP)                                                                                  \
+    if (direct) cross_dq_kernel<T, DP, 4, T4, true><<<grid, 256, 0, st>>>(a);                     \
+    else if (p.nw_q == 4) cross_dq_kernel<T, DP, 4, DP == 128 ? 32 : T4, false><<<grid, 256, 0, st>>>(a); \
+    else if constexpr (sizeof(T) == 2 || DP < 128) cross_dq_kernel<T, DP, 1, 32, false><<<grid, 64, 0, st>>>(a)
+        SNAG_CROSS_DP(CALL)
+#undef CALL
+        if (int rc = check_launch("cross_dq")) return rc;
+        if (a.splits > 1)
+            if (int rc = sum_ranges<T>(a.part, nq * a.d, a.splits, a.dq, st)) return rc;
+    }
+    if (nk > 0) {
+        a.splits = p.s_dkv;
+        a.per_split = range_of(a.rows, a.splits);
+        const int64_t tiles = (a.Lk + p.nw_k * 32 - 1) / (p.nw_k * 32), n = (int64_t)a.B * a.Hkv * tiles * a.splits;
+        SNAG_REQUIRE(n < (int64_t)1 << 31, SNAG_ERR_UNSUPPORTED, "cross attention: %lld workgroups", (long long)n);
+        const dim3 grid((unsigned)n);
+        const bool direct = p.nw_k == 4 && whole && a.rows > 0;
+#define CALL(DP)                                                                                  \
+    if (direct) cross_dkv_kernel<T, DP, 4, DP == 128 ? 32 : T4, true><<<grid, 256, 0, st>>>(a);           \
+    else if (p.nw_k == 4) cross_dkv_kernel<T, DP, 4, DP == 128 ? 32 : T4, false><<<grid, 256, 0, st>>>(a);\
+    else if constexpr (sizeof(T) == 2 || DP < 128) cross_dkv_kernel<T, DP, 1, 32, false><<<grid, 64, 0, st>>>(a)
+        SNAG_CROSS_DP(CALL)
+#undef CALL
+        if (int rc = check_launch("cross_dkv")) return rc;
+        if (a.splits > 1) {
+            if (int rc = sum_ranges<T>(a.part, nk * a.d, a.splits, a.dk, st)) return rc;
+            if (int rc = sum_ranges<T>(a.part + a.splits * nk * a.d, nk * a.d, a.splits, a.dv, st)) return rc;
+        }
+    }
+    return SNAG_OK;
+}
+int cross_tiles_bwd(const CrossArgs& a, const CrossPlan& p, float* delta, int dtype, hipStream_t st) {
+    return dtype == SNAG_F32 ? bwd<float, 32>(a, p, delta, dtype, st) : dtype == SNAG_BF16 ? bwd<bf16_t, 64>(a, p, delta, dtype, st) : bwd<f16_t, 64>(a, p, delta, dtype, st);
+}
+
+}  // namespace snag

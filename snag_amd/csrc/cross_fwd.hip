@@ -1,0 +1,202 @@
+// Cross attention, tiled forward (csrc/cross_tiles.hip.h has the scheme) and the join of key ranges.
+//
+// Bound by the matrix pipe and, nearly as much, by the vector pipe's exponentials: 64 keys x 32 rows of 128 elements are 1024 cycles of products and
+// about 900 of softmax per wave, which two waves per SIMD overlap (hence at most 256 registers).  The running maximum is only moved -- and the
+// 64 accumulators rescaled -- when a score passes it by more than 8 (in log2): until then p stays below 2^8, which costs nothing in fp32 sums or
+// in the 8 / 11 significant bits of the rounded p.
+#include "cross_tiles.hip.h"
+
+namespace snag {
+
+constexpr float kSlack = 8.f;
+
+// Workgroup: NW waves x 32 rows; key tiles of KT.  splits > 1: per range part[split][B H Lq][d] = sum exp2(S - m) v (not normalised) and, behind
+// all of those, [split][B H Lq][2] = (m, sum); cross_combine_kernel joins them.
+template <class T, int DP, int NW, int KT, bool DIRECT>
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 128 ? 1 : 2) void cross_fwd_kernel(CrossArgs a) {
+    using M = Mma<T>;
+    constexpr int NT = NW * 64;
+    __shared__ __attribute__((aligned(16))) T lk[2][KT * DP];
+    __shared__ __attribute__((aligned(16))) T lv[2][KT * DP];
+    __shared__ __attribute__((aligned(16))) float bias[2][DIRECT ? 4 : KT];
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_id_uniform(), h = lane >> 5;
+    const int64_t tiles = (a.rows + NW * 32 - 1) / (NW * 32);
+    const Problem pr = problem_of(a, tiles);
+    const int b = pr.b, hk = pr.hk;
+    const int len = cross_len(a, b);
+    const int row = (int)pr.tile * NW * 32 + wave * 32 + (lane & 31);
+    const bool own = row < a.rows;
+    const int l = own ? row_l(a, row) : 0, head = hk * a.G + (own ? row - l * a.G : 0);
+    const T* kb = (const T*)a.k + b * a.ksb + hk * a.ksh;
+    const T* vb = (const T*)a.v + b * a.vsb + hk * a.vsh;
+
+    const int t0 = pr.split * a.per_split / KT, t1 = min((len + KT - 1) / KT, t0 + a.per_split / KT);
+    TileFetch<T, DP, KT, NT, DIRECT> fk, fv;
+    float fb = 0.f;
+    // DIRECT: rows behind the last key are read as the last key, their scores become -inf below
+    auto fetch = [&](int t) {
+        const int key0 = t * KT;
+        auto at = [&](const T* base, int64_t step, int i, bool& ok) {
+            const int key = DIRECT ? min(key0 + i, len - 1) : key0 + i;
+            ok = DIRECT || key_seen(a, b, key, len);
+            return base + key * step;
+        };
+        fk.fetch([&](int i, bool& ok) { return at(kb, a.ksl, i, ok); }, lk[t & 1], a.d, a.vec_k, tid);
+        fv.fetch([&](int i, bool& ok) { return at(vb, a.vsl, i, ok); }, lv[t & 1], a.d, a.vec_v, tid);
+        if (!DIRECT && tid < KT) fb = key_seen(a, b, key0 + tid, len) ? 0.f : -INFINITY;
+    };
+    auto store = [&](int t) {
+        fk.store(lk[t & 1], tid);
+        fv.store(lv[t & 1], tid);
+        if (!DIRECT && tid < KT) bias[t & 1][tid] = fb;
+    };
+    if (t0 < t1) fetch(t0);
+    typename M::Frag q[DP / 16];
+    own_row<T, DP>(q, (const T*)a.q + b * a.qsb + l * a.qsl + head * a.qsh, a.d, own, a.vec_q, lane);
+    if (t0 < t1) store(t0);
+    f32x16 acc[DP / 32];
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) acc[i] = f32x16{};
+    float m = -INFINITY, sum = 0.f;                        // m: what the exponentials are relative to, within kSlack of the maximum
+    for (int t = t0; t < t1; ++t) {
+        tile_ready();
+        if (t + 1 < t1) fetch(t + 1);
+        const T *ck = lk[t & 1], *cv = lv[t & 1];
+        f32x16 s[KT / 32];
+#pragma unroll
+        for (int kt = 0; kt < KT / 32; ++kt) {
+            s[kt] = f32x16{};
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) s[kt] = M::mma(M::template rows<DP>(ck, kt * 32, c * 16, lane), q[c], s[kt]);
+        }
+        if (DIRECT ? (t + 1) * KT > len : a.mask != nullptr || (t + 1) * KT > len) {
+#pragma unroll
+            for (int kt = 0; kt < KT / 32; ++kt)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int i = kt * 32 + g * 8 + h * 4;
+                    if constexpr (DIRECT) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) s[kt][4 * g + j] = t * KT + i + j < len ? s[kt][4 * g + j] : -INFINITY;
+                    } else {
+                        const f32x4 bb = *(const f32x4*)(bias[t & 1] + i);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) s[kt][4 * g + j] += bb[j];
+                    }
+                }
+        }
+        float top = -INFINITY, lo, hi;
+#pragma unroll
+        for (int kt = 0; kt < KT / 32; ++kt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kt][i]);
+        halves(top, lo, hi);
+        top = fmaxf(lo, hi) * a.c2;
+        if (__any(top > m + kSlack)) {                     // also the first score a row sees: m is -inf until then
+            const float mn = fmaxf(m, top), alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            sum *= alpha;
+#pragma unroll
+            for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[db][i] *= alpha;
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kt = 0; kt < KT / 32; ++kt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[kt][i] = __builtin_amdgcn_exp2f(fmaf(s[kt][i], a.c2, -ref));
+                part[i & 3] += s[kt][i];
+            }
+        sum += (part[0] + part[1]) + (part[2] + part[3]);
+#pragma unroll
+        for (int kt = 0; kt < KT / 32; ++kt)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const typename M::Frag p = pack<T>(s[kt], u);
+#pragma unroll
+                for (int db = 0; db < DP / 32; ++db) acc[db] = M::mma(M::template cols<DP>(cv, kt * 32 + u * 16, db * 32, lane), p, acc[db]);
+            }
+        if (t + 1 < t1) store(t + 1);
+    }
+    float lo, hi;
+    halves(sum, lo, hi);
+    sum = lo + hi;
+    if (!own) return;
+    const int64_t at = ((int64_t)b * a.H + head) * a.Lq + l, n = (int64_t)a.B * a.H * a.Lq;
+    if (a.splits > 1) {
+        store_row<float, DP>(a.part + ((int64_t)pr.split * n + at) * a.d, acc, 1.f, a.d, lane);
+        if (h == 0) {
+            float* ml = a.part + (int64_t)a.splits * n * a.d + ((int64_t)pr.split * n + at) * 2;
+            ml[0] = m;
+            ml[1] = sum;
+        }
+        return;
+    }
+    store_row<T, DP>((T*)a.out + (((int64_t)b * a.Lq + l) * a.H + head) * a.d, acc, sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum), a.d, lane);
+    if (h == 0) a.lse[at] = sum == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(sum);
+}
+
+// Joins the key ranges of the forward: one wave per row (b, head, l).
+template <class T>
+__global__ __launch_bounds__(256) void cross_combine_kernel(CrossArgs a) {
+    const int64_t n = (int64_t)a.B * a.H * a.Lq, at = (int64_t)blockIdx.x * 4 + wave_id_uniform();
+    const int lane = threadIdx.x & 63;
+    if (at >= n) return;
+    const float* ml = a.part + (int64_t)a.splits * n * a.d;
+    float m = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ml[(s * n + at) * 2]);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float sum = 0.f, o[2] = {0.f, 0.f};
+    for (int s = 0; s < a.splits; ++s) {
+        const float w = __builtin_amdgcn_exp2f(ml[(s * n + at) * 2] - ref), t = ml[(s * n + at) * 2 + 1];
+        if (t == 0.f) continue;                       // a range none of whose keys is seen
+        sum += w * t;
+        const float* p = a.part + (s * n + at) * a.d;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            if (lane + 64 * u < a.d) o[u] = fmaf(w, p[lane + 64 * u], o[u]);
+    }
+    const int64_t l = at % a.Lq, bh = at / a.Lq, head = bh % a.H, b = bh / a.H;
+    T* out = (T*)a.out + ((b * a.Lq + l) * a.H + head) * a.d;
+    const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+        if (lane + 64 * u < a.d) out[lane + 64 * u] = (T)(o[u] * inv);
+    if (lane == 0) a.lse[at] = sum == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(sum);
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------
+template <class T, int KT4>
+static void go(const CrossArgs& a, const CrossPlan& p, dim3 grid, hipStream_t st) {
+    const bool direct = p.nw_q == 4 && a.mask == nullptr && a.d == p.dp && a.vec_k && a.vec_v;
+#define CALL(DP)                                                                                   \
+    if (direct) cross_fwd_kernel<T, DP, 4, KT4, true><<<grid, 256, 0, st>>>(a);                    \
+    else if (p.nw_q == 4) cross_fwd_kernel<T, DP, 4, KT4, false><<<grid, 256, 0, st>>>(a);         \
+    else if constexpr (sizeof(T) == 2 || DP < 128) cross_fwd_kernel<T, DP, 1, 32, false><<<grid, 64, 0, st>>>(a)
+    SNAG_CROSS_DP(CALL)
+#undef CALL
+}
+
+int cross_tiles_fwd(const CrossArgs& a, const CrossPlan& p, int dtype, hipStream_t st) {
+    const int64_t tiles = (a.rows + p.nw_q * 32 - 1) / (p.nw_q * 32), n = (int64_t)a.B * a.Hkv * tiles * a.splits;
+    SNAG_REQUIRE(n < (int64_t)1 << 31, SNAG_ERR_UNSUPPORTED, "cross attention: %lld workgroups", (long long)n);
+    const dim3 grid((unsigned)n);
+    if (dtype == SNAG_F32) go<float, 32>(a, p, grid, st);
+    else if (dtype == SNAG_BF16) go<bf16_t, 64>(a, p, grid, st);
+    else go<f16_t, 64>(a, p, grid, st);
+    return check_launch("cross_fwd");
+}
+
+int cross_combine(const CrossArgs& a, int dtype, hipStream_t st) {
+    const int64_t n = (int64_t)a.B * a.H * a.Lq;
+    const dim3 grid((unsigned)((n + 3) / 4));
+    if (dtype == SNAG_F32) cross_combine_kernel<float><<<grid, 256, 0, st>>>(a);
+    else if (dtype == SNAG_BF16) cross_combine_kernel<bf16_t><<<grid, 256, 0, st>>>(a);
+    else cross_combine_kernel<f16_t><<<grid, 256, 0, st>>>(a);
+    return check_launch("cross_combine");
+}
+
+}  // namespace snag
