@@ -772,7 +772,7 @@ SNAG_API int snag_spmm_csr(const int32_t* rowptr, const int32_t* col, const floa
 /* Attention of queries over states of another length.  Per batch entry b and head h, hk = h / (H / Hkv):
  *   out[b,l,h] = sum_s p(l,s) v[b,s,hk],   p(l,.) = softmax over the seen keys of scale * q[b,l,h] . k[b,s,hk]
  * q [B, Lq, H, d], k and v [B, Lk, Hkv, d]: strides_host (HOST memory) holds the element strides of batch, position and head of q, k and v
- * (nine values); the d elements of a head are adjacent, d <= SNAG_CROSS_MAX_HEAD_DIM.  All three and out are of type dtype.
+ * (nine values); the d elements of a head are adjacent, d <= SNAG_CROSS_MAX_HEAD_DIM; Lq (H / Hkv) <= 2^30, Lq (H / Hkv)^2 < 2^32.  All three and out are of type dtype.
  * Key s is seen when s < kv_lens[b] (int32 / int64 by lens_bytes, clamped to 0..Lk; NULL = Lk) and key_mask[b * mask_ld + s] != 0 (NULL = all).
  * What memory holds at an unseen key, NaN included, does not reach any result.  A query that sees no key gets out = 0 and lse = -inf.
  * out [B, Lq, H, d] dense; lse [B, H, Lq] = log2 of the sum of exp2(scale * log2(e) * q . k), kept for the backward.

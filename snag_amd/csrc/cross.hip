@@ -33,6 +33,7 @@ static CrossPlan cross_plan(int dtype, int B, int Lq, int Lk, int H, int Hkv, in
     return p;
 }
 
+static int64_t stat_floats(const CrossPlan& p, int B, int Lq, int H, int Hkv) { return p.rows_path ? 0 : 2 * (int64_t)B * Hkv * padded_rows(Lq * (H / Hkv)); }
 static int64_t fwd_part_floats(const CrossPlan& p, int64_t n, int d) { return p.s_fwd > 1 ? p.s_fwd * n * (d + 2) : 0; }
 static int64_t bwd_part_floats(const CrossPlan& p, int64_t nq, int64_t nk, int d) {
     const int64_t dq = p.s_dq > 1 ? p.s_dq * nq * d : 0, dkv = p.s_dkv > 1 ? 2 * p.s_dkv * nk * d : 0;
@@ -44,7 +45,9 @@ static int cross_shapes(int dtype, int B, int Lq, int Lk, int H, int Hkv, int d)
     SNAG_REQUIRE(B >= 0 && Lq >= 0 && Lk >= 0 && H >= 1 && Hkv >= 1, SNAG_ERR_ARG, "cross attention: negative or empty size (B %d, Lq %d, Lk %d, H %d, Hkv %d)", B, Lq, Lk, H, Hkv);
     SNAG_REQUIRE(H % Hkv == 0, SNAG_ERR_ARG, "cross attention: %d heads are not a multiple of %d key/value heads", H, Hkv);
     SNAG_REQUIRE(d >= 1 && d <= SNAG_CROSS_MAX_HEAD_DIM, SNAG_ERR_UNSUPPORTED, "cross attention: head dimension %d is not in 1..%d", d, SNAG_CROSS_MAX_HEAD_DIM);
-    SNAG_REQUIRE((int64_t)Lq * (H / Hkv) <= (1 << 30) && (int64_t)Lk <= (1 << 30), SNAG_ERR_UNSUPPORTED, "cross attention: more than 2^30 rows or keys in one problem");
+    const int64_t G = H / Hkv;
+    SNAG_REQUIRE(G <= 65535 && (int64_t)Lq * G <= (1 << 30) && Lk <= (1 << 30), SNAG_ERR_UNSUPPORTED, "cross attention: more than 2^30 rows or keys in one problem");
+    SNAG_REQUIRE((int64_t)Lq * G * G < (int64_t)1 << 32, SNAG_ERR_UNSUPPORTED, "cross attention: Lq (H / Hkv)^2 = %lld is not below 2^32", (long long)((int64_t)Lq * G * G));
     return SNAG_OK;
 }
 
@@ -63,9 +66,9 @@ static int cross_args(CrossArgs& a, const void* q, const void* k, const void* v,
     a.qsb = s[0], a.qsl = s[1], a.qsh = s[2], a.ksb = s[3], a.ksl = s[4], a.ksh = s[5], a.vsb = s[6], a.vsl = s[7], a.vsh = s[8];
     a.B = B, a.Lq = Lq, a.Lk = Lk, a.H = H, a.Hkv = Hkv, a.G = H / Hkv, a.d = d, a.rows = Lq * a.G;
     a.lens = lens, a.lens_bytes = lens_bytes, a.mask = mask, a.mask_ld = mask_ld;
-    // ceil(2^32 / G) as a multiplier is exact below 2^32 / (its excess): checked against the largest row
-    const uint64_t magic = a.G > 1 ? (((uint64_t)1 << 32) + a.G - 1) / a.G : 0;
-    a.g_magic = a.G > 1 && (uint64_t)a.rows * (magic * a.G - ((uint64_t)1 << 32)) < (uint64_t)1 << 32 ? (uint32_t)magic : 0;
+    // ceil(2^32 / G) as a multiplier is exact for rows below 2^32 / (its excess over 2^32 / G, times G), and that is below G
+    a.g_magic = a.G > 1 ? (uint32_t)((((uint64_t)1 << 32) + a.G - 1) / a.G) : 0;
+    a.g_one = a.G > 1 ? 0 : ~0u;
     a.scale = scale, a.c2 = scale * 1.44269504088896340736f;
     const int c = 16 / elem_size(dtype);
     auto vec = [&](const void* p, const int64_t* t) { return d % c == 0 && aligned16(p) && t[0] % c == 0 && t[1] % c == 0 && t[2] % c == 0; };
@@ -81,7 +84,7 @@ extern "C" SNAG_API int64_t snag_cross_work_floats(int dtype, int B, int Lq, int
     if (cross_shapes(dtype, B, Lq, Lk, H, Hkv, d) != SNAG_OK || B == 0) return 0;
     const CrossPlan p = cross_plan(dtype, B, Lq, Lk, H, Hkv, d);
     const int64_t nq = (int64_t)B * Lq * H, nk = (int64_t)B * Lk * Hkv;
-    return backward ? (nq + 3) / 4 * 4 + bwd_part_floats(p, nq, nk, d) : fwd_part_floats(p, nq, d);
+    return backward ? stat_floats(p, B, Lq, H, Hkv) + bwd_part_floats(p, nq, nk, d) : fwd_part_floats(p, nq, d);
 }
 
 extern "C" SNAG_API int snag_cross_fwd(const void* q, const void* k, const void* v, int dtype, int B, int Lq, int Lk, int H, int Hkv, int d,
@@ -117,7 +120,7 @@ extern "C" SNAG_API int snag_cross_bwd(const void* q, const void* k, const void*
     hipStream_t st = (hipStream_t)stream;
     a.o = out, a.lse = (float*)lse, a.dout = d_out, a.dq = d_q, a.dk = d_k, a.dv = d_v;
     a.vec_o = d % (16 / elem_size(dtype)) == 0 && aligned16(out) && aligned16(d_out) && aligned16(d_q) && aligned16(d_k) && aligned16(d_v);
-    a.part = work + ((int64_t)B * Lq * H + 3) / 4 * 4;
+    a.part = work + stat_floats(p, B, Lq, H, Hkv);
     if (p.rows_path && Lq > 0) {
         a.splits = p.s_dq;
         if (int rc = cross_rows_bwd(a, dtype, st)) return rc;

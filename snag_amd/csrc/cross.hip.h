@@ -17,7 +17,7 @@ struct CrossArgs {
     int64_t qsb, qsl, qsh, ksb, ksl, ksh, vsb, vsl, vsh;      // element strides of batch / position / head; the head's own elements are adjacent
     int B, Lq, Lk, H, Hkv, G, d;
     int rows;                    // Lq * G
-    uint32_t g_magic;            // high word of row * g_magic = row / G for every row; 0: divide
+    uint32_t g_magic, g_one;     // row / G = high word of row * g_magic; G == 1: g_magic = 0, g_one = all ones
     const void* lens;            // [B] int32 / int64 or NULL: keys at and behind lens[b] are not seen
     int lens_bytes;
     const uint8_t* mask;         // [B, Lk] (row pitch mask_ld) or NULL: 0 = key not seen
@@ -31,7 +31,7 @@ struct CrossArgs {
     float* part;                 // splits > 1: partial results, see the kernels
     // backward
     const void *o, *dout;        // [B, Lq, H, d] dense
-    const float* delta;          // [B, H, Lq]: sum_d dout * o
+    const float* stat;           // [B, Hkv, padded_rows(rows)][2] = lse (+inf: no key seen), sum_d dout * o
     void *dq, *dk, *dv;          // dense, shapes of q, k, v
     int vec_o;                   // 16-byte access legal for the dense tensors (d a multiple of the chunk, aligned bases)
 };
@@ -103,10 +103,11 @@ struct CrossPlan {
         default: CALL(128); break;           \
     }
 
+__host__ __device__ static inline int64_t padded_rows(int rows) { return ((int64_t)rows + 63) / 64 * 64; }
 static inline int range_of(int n, int ranges) { return ((n + 63) / 64 + ranges - 1) / ranges * 64; }      // of n keys or rows
 
 int cross_tiles_fwd(const CrossArgs& a, const CrossPlan& p, int dtype, hipStream_t st);
-int cross_tiles_bwd(const CrossArgs& a, const CrossPlan& p, float* delta, int dtype, hipStream_t st);
+int cross_tiles_bwd(const CrossArgs& a, const CrossPlan& p, float* stat, int dtype, hipStream_t st);
 int cross_combine(const CrossArgs& a, int dtype, hipStream_t st);
 int cross_sum(const float* part, int64_t n, int ranges, void* out, int dtype, hipStream_t st);
 int cross_rows_fwd(const CrossArgs& a, int dtype, hipStream_t st);

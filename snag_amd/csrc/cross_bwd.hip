@@ -6,24 +6,31 @@
 
 namespace snag {
 
-// delta[b, head, l] = sum_d dout o, one 16-lane group per row
+// stat[b, hk, row] = (lse, delta = sum_d dout o) in the kernels' row order, each problem's rows padded to 64 with (+inf, 0): the p of such a row, and
+// of one that sees no key, is 0.  One 16-lane group per row.
 template <class T>
-__global__ __launch_bounds__(256) void cross_delta_kernel(CrossArgs a, float* __restrict__ delta) {
+__global__ __launch_bounds__(256) void cross_stat_kernel(CrossArgs a, float* __restrict__ stat, int padded) {
     constexpr int C = Chunk<T>::n;
-    const int64_t n = (int64_t)a.B * a.Lq * a.H, at = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    const int64_t n = (int64_t)a.B * a.Hkv * padded, at = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
     const int t = threadIdx.x & 15;
+    const int64_t bh = at / padded, b = bh / a.Hkv;
+    const int row = (int)(at - bh * padded), hk = (int)(bh - b * a.Hkv), l = row_l(a, row), head = hk * a.G + row - l * a.G;
+    const bool own = at < n && row < a.rows;
+    const int64_t dense = ((b * a.Lq + l) * a.H + head) * a.d;
     float s = 0.f;
-    if (at < n)
+    if (own)
         for (int col = t * C; col < a.d; col += 16 * C) {
-            const auto x = load_chunk<T>((const T*)a.o + at * a.d, col, a.d, true, a.vec_o);
-            const auto y = load_chunk<T>((const T*)a.dout + at * a.d, col, a.d, true, a.vec_o);
+            const auto x = load_chunk<T>((const T*)a.o + dense, col, a.d, true, a.vec_o);
+            const auto y = load_chunk<T>((const T*)a.dout + dense, col, a.d, true, a.vec_o);
 #pragma unroll
             for (int j = 0; j < C; ++j) s = fmaf((float)x[j], (float)y[j], s);
         }
     s = sum16(s);
     if (at < n && t == 0) {
-        const int64_t head = at % a.H, bl = at / a.H, l = bl % a.Lq, b = bl / a.Lq;
-        delta[(b * a.H + head) * a.Lq + l] = s;
+        float lse = own ? a.lse[(b * a.H + head) * a.Lq + l] : INFINITY;
+        if (lse == -INFINITY) lse = INFINITY;
+        stat[2 * at] = lse;
+        stat[2 * at + 1] = own ? s : 0.f;
     }
 }
 
@@ -45,7 +52,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 128 ? 1 : 2) void 
     const int l = own ? row_l(a, row) : 0, head = hk * a.G + (own ? row - l * a.G : 0);
     const T* kb = (const T*)a.k + b * a.ksb + hk * a.ksh;
     const T* vb = (const T*)a.v + b * a.vsb + hk * a.vsh;
-    const int64_t at = ((int64_t)b * a.H + head) * a.Lq + l, dense = (((int64_t)b * a.Lq + l) * a.H + head) * a.d;
+    const int64_t dense = (((int64_t)b * a.Lq + l) * a.H + head) * a.d;
 
     const int t0 = pr.split * a.per_split / KT, t1 = min((len + KT - 1) / KT, t0 + a.per_split / KT);
     TileFetch<T, DP, KT, NT, DIRECT> fk, fv;
@@ -70,7 +77,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 128 ? 1 : 2) void 
     typename M::Frag q[DP / 16], dout[DP / 16];
     own_row<T, DP>(q, (const T*)a.q + b * a.qsb + l * a.qsl + head * a.qsh, a.d, own, a.vec_q, lane);
     own_row<T, DP>(dout, (const T*)a.dout + dense, a.d, own, a.vec_o, lane);
-    const float lse = own ? usable_lse(a.lse[at]) : INFINITY, delta = own ? a.delta[at] : 0.f;
+    const float* st = a.stat + 2 * (((int64_t)b * a.Hkv + hk) * padded_rows(a.rows) + (own ? row : 0));
+    const float lse = own ? st[0] : INFINITY, delta = own ? st[1] : 0.f;
     if (t0 < t1) store(t0);
     f32x16 acc[DP / 32];
 #pragma unroll
@@ -128,7 +136,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void c
     __shared__ __attribute__((aligned(16))) T lvv[VLDS ? KEYS * DP : 16];
     __shared__ __attribute__((aligned(16))) T lq[2][RT * DP];
     __shared__ __attribute__((aligned(16))) T lo[2][RT * DP];
-    __shared__ __attribute__((aligned(16))) float stat[2][2][RT];
+    __shared__ __attribute__((aligned(16))) float stat[2][2 * RT];
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id_uniform(), h = lane >> 5;
     const int64_t tiles = (a.Lk + NW * 32 - 1) / (NW * 32);
     const Problem pr = problem_of(a, tiles);
@@ -143,7 +151,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void c
     const int t0 = pr.split * a.per_split / RT, t1 = key0 < len ? min((a.rows + RT - 1) / RT, t0 + a.per_split / RT) : t0;
     if (t0 < t1) {
         TileFetch<T, DP, RT, NT, DIRECT> fq, fo;
-        float fs0 = 0.f, fs1 = 0.f;
+        const float* st = a.stat + 2 * ((int64_t)b * a.Hkv + hk) * padded_rows(a.rows);
         // DIRECT: rows behind the last one are read as the last one, their p is 0
         auto fetch = [&](int t) {
             const int r0 = t * RT;
@@ -157,17 +165,15 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void c
                 ok = r0 + i < a.rows;
                 return (const T*)a.dout + (((int64_t)b * a.Lq + l) * a.H + hk * a.G + r - l * a.G) * a.d;
             }, lo[t & 1], a.d, a.vec_o, tid);
-            if (tid < RT) {
-                const int r = min(r0 + tid, a.rows - 1), l = row_l(a, r);
-                const int64_t at = ((int64_t)b * a.H + hk * a.G + r - l * a.G) * a.Lq + l;
-                fs0 = r0 + tid < a.rows ? usable_lse(a.lse[at]) : INFINITY;
-                fs1 = r0 + tid < a.rows ? a.delta[at] : 0.f;
-            }
+#if defined(__HIP_DEVICE_COMPILE__)
+#pragma unroll
+            for (int u = 0; u < 2 * RT / 64; ++u)
+                if (wave == u % NW) __builtin_amdgcn_global_load_lds((SNAG_GLOBAL void*)(st + 2 * r0 + u * 64 + lane), (SNAG_LDS void*)(stat[t & 1] + u * 64), 4, 0, 0);
+#endif
         };
         auto store = [&](int t) {
             fq.store(lq[t & 1], tid);
             fo.store(lo[t & 1], tid);
-            if (tid < RT) stat[t & 1][0][tid] = fs0, stat[t & 1][1][tid] = fs1;
         };
         fetch(t0);
         if constexpr (VLDS) {
@@ -198,13 +204,14 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void c
                 }
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    const int i0 = rt * 32 + g * 8 + h * 4;
-                    const f32x4 ls = *(const f32x4*)(stat[t & 1][0] + i0), de = *(const f32x4*)(stat[t & 1][1] + i0);
+                    // (lse, delta) of four rows.  Keys that are not seen go along: what they gather stays in their own lane and is dropped at the end
+                    const f32x4 s0 = *(const f32x4*)(stat[t & 1] + 2 * (rt * 32 + g * 8 + h * 4)), s1 = *(const f32x4*)(stat[t & 1] + 2 * (rt * 32 + g * 8 + h * 4) + 4);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const int i = 4 * g + j;
-                        s[i] = seen ? __builtin_amdgcn_exp2f(fmaf(s[i], a.c2, -ls[j])) : 0.f;
-                        dp[i] = seen ? s[i] * (dp[i] - de[j]) : 0.f;
+                        const float ls = j < 2 ? s0[2 * j] : s1[2 * j - 4], de = j < 2 ? s0[2 * j + 1] : s1[2 * j - 3];
+                        s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.c2, -ls));
+                        dp[i] = s[i] * (dp[i] - de);
                     }
                 }
 #pragma unroll
@@ -221,6 +228,10 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void c
         }
     }
     if (!own) return;
+    if (!seen) {
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i) dk[i] = dv[i] = f32x16{};
+    }
     const int64_t dense = (((int64_t)b * a.Lk + key) * a.Hkv + hk) * a.d, n = (int64_t)a.B * a.Lk * a.Hkv * a.d;
     if (a.splits > 1) {
         store_row<float, DP>(a.part + pr.split * n + dense, dk, a.scale, a.d, lane);
@@ -253,13 +264,16 @@ int cross_sum(const float* part, int64_t n, int ranges, void* out, int dtype, hi
 }
 
 template <class T, int T4>
-static int bwd(CrossArgs a, const CrossPlan& p, float* delta, int dtype, hipStream_t st) {
+static int bwd(CrossArgs a, const CrossPlan& p, float* stat, hipStream_t st) {
     const int64_t nq = (int64_t)a.B * a.Lq * a.H, nk = (int64_t)a.B * a.Lk * a.Hkv;
     const bool whole = a.d == p.dp && a.vec_q && a.vec_k && a.vec_v && a.vec_o;
-    a.delta = delta;
+    a.stat = stat;
     if (nq > 0) {
-        cross_delta_kernel<T><<<dim3((unsigned)((nq + 15) / 16)), 256, 0, st>>>(a, delta);
-        if (int rc = check_launch("cross_delta")) return rc;
+        const int padded = (int)padded_rows(a.rows);
+        const int64_t ns = ((int64_t)a.B * a.Hkv * padded + 15) / 16;
+        SNAG_REQUIRE(ns < (int64_t)1 << 31, SNAG_ERR_UNSUPPORTED, "cross attention: %lld rows", (long long)nq);
+        cross_stat_kernel<T><<<dim3((unsigned)ns), 256, 0, st>>>(a, stat, padded);
+        if (int rc = check_launch("cross_stat")) return rc;
         a.splits = p.s_dq;
         a.per_split = range_of(a.Lk, a.splits);
         const int64_t tiles = (a.rows + p.nw_q * 32 - 1) / (p.nw_q * 32), n = (int64_t)a.B * a.Hkv * tiles * a.splits;
@@ -297,8 +311,8 @@ static int bwd(CrossArgs a, const CrossPlan& p, float* delta, int dtype, hipStre
     }
     return SNAG_OK;
 }
-int cross_tiles_bwd(const CrossArgs& a, const CrossPlan& p, float* delta, int dtype, hipStream_t st) {
-    return dtype == SNAG_F32 ? bwd<float, 32>(a, p, delta, dtype, st) : dtype == SNAG_BF16 ? bwd<bf16_t, 64>(a, p, delta, dtype, st) : bwd<f16_t, 64>(a, p, delta, dtype, st);
+int cross_tiles_bwd(const CrossArgs& a, const CrossPlan& p, float* stat, int dtype, hipStream_t st) {
+    return dtype == SNAG_F32 ? bwd<float, 32>(a, p, stat, st) : dtype == SNAG_BF16 ? bwd<bf16_t, 64>(a, p, stat, st) : bwd<f16_t, 64>(a, p, stat, st);
 }
 
 }  // namespace snag

@@ -210,10 +210,7 @@ __device__ __forceinline__ Problem problem_of(const CrossArgs& a, int64_t tiles)
 __device__ __forceinline__ bool key_seen(const CrossArgs& a, int b, int key, int len) {
     return key < len && (a.mask == nullptr || a.mask[(int64_t)b * a.mask_ld + key] != 0);
 }
-// row = l G + g without a division where the host found a multiplier that is exact for every row
-__device__ __forceinline__ int row_l(const CrossArgs& a, int row) { return a.G == 1 ? row : a.g_magic != 0 ? (int)__umulhi((uint32_t)row, a.g_magic) : row / a.G; }
-
-// p of a row that sees no key is 0: its lse becomes +inf
-__device__ __forceinline__ float usable_lse(float lse) { return lse == -INFINITY ? INFINITY : lse; }
+// row = l G + g: the host has checked that the multiplier is exact for every row
+__device__ __forceinline__ int row_l(const CrossArgs& a, int row) { return (int)(__umulhi((uint32_t)row, a.g_magic) + ((uint32_t)row & a.g_one)); }
 
 }  // namespace snag
