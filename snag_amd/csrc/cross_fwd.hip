@@ -18,7 +18,6 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 128 ? 1 : 2) void 
     constexpr int NT = NW * 64;
     __shared__ __attribute__((aligned(16))) T lk[2][KT * DP];
     __shared__ __attribute__((aligned(16))) T lv[2][KT * DP];
-    __shared__ __attribute__((aligned(16))) float bias[2][DIRECT ? 4 : KT];
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id_uniform(), h = lane >> 5;
     const int64_t tiles = (a.rows + NW * 32 - 1) / (NW * 32);
     const Problem pr = problem_of(a, tiles);
@@ -32,24 +31,27 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 128 ? 1 : 2) void 
 
     const int t0 = pr.split * a.per_split / KT, t1 = min((len + KT - 1) / KT, t0 + a.per_split / KT);
     TileFetch<T, DP, KT, NT, DIRECT> fk, fv;
-    float fb = 0.f;
-    // DIRECT: rows behind the last key are read as the last key, their scores become -inf below
+    uint64_t now = 0, next = 0;                            // seen keys of the tile that is worked on, and of the one in flight
+    bool byte = false;                                     // this lane's mask byte of the tile behind that
+    // DIRECT: rows behind the last key are read as the last key; what is not seen gets -inf for a score below
     auto fetch = [&](int t) {
         const int key0 = t * KT;
-        auto at = [&](const T* base, int64_t step, int i, bool& ok) {
+        auto row_at = [&](const T* base, int64_t step, int i, bool& ok) {
             const int key = DIRECT ? min(key0 + i, len - 1) : key0 + i;
-            ok = DIRECT || key_seen(a, b, key, len);
+            ok = DIRECT || ((next >> i) & 1);
             return base + key * step;
         };
-        fk.fetch([&](int i, bool& ok) { return at(kb, a.ksl, i, ok); }, lk[t & 1], a.d, a.vec_k, tid);
-        fv.fetch([&](int i, bool& ok) { return at(vb, a.vsl, i, ok); }, lv[t & 1], a.d, a.vec_v, tid);
-        if (!DIRECT && tid < KT) fb = key_seen(a, b, key0 + tid, len) ? 0.f : -INFINITY;
+        fk.fetch([&](int i, bool& ok) { return row_at(kb, a.ksl, i, ok); }, lk[t & 1], a.d, a.vec_k, tid);
+        fv.fetch([&](int i, bool& ok) { return row_at(vb, a.vsl, i, ok); }, lv[t & 1], a.d, a.vec_v, tid);
+        if (!DIRECT && t + 1 < t1) byte = mask_byte(a, b, key0 + KT, len, lane);
     };
     auto store = [&](int t) {
         fk.store(lk[t & 1], tid);
         fv.store(lv[t & 1], tid);
-        if (!DIRECT && tid < KT) bias[t & 1][tid] = fb;
+        now = next;
+        if (!DIRECT) next = seen_bits(byte, (t + 1) * KT, len, lane);
     };
+    if (!DIRECT && t0 < t1) next = seen_bits(mask_byte(a, b, t0 * KT, len, lane), t0 * KT, len, lane);
     if (t0 < t1) fetch(t0);
     typename M::Frag q[DP / 16];
     own_row<T, DP>(q, (const T*)a.q + b * a.qsb + l * a.qsl + head * a.qsh, a.d, own, a.vec_q, lane);
@@ -69,21 +71,10 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 128 ? 1 : 2) void 
 #pragma unroll
             for (int c = 0; c < DP / 16; ++c) s[kt] = M::mma(M::template rows<DP>(ck, kt * 32, c * 16, lane), q[c], s[kt]);
         }
-        if (DIRECT ? (t + 1) * KT > len : a.mask != nullptr || (t + 1) * KT > len) {
+        if ((!DIRECT && a.mask != nullptr) || (t + 1) * KT > len) {
+            if constexpr (DIRECT) now = seen_bits(true, t * KT, len, lane);
 #pragma unroll
-            for (int kt = 0; kt < KT / 32; ++kt)
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int i = kt * 32 + g * 8 + h * 4;
-                    if constexpr (DIRECT) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) s[kt][4 * g + j] = t * KT + i + j < len ? s[kt][4 * g + j] : -INFINITY;
-                    } else {
-                        const f32x4 bb = *(const f32x4*)(bias[t & 1] + i);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) s[kt][4 * g + j] += bb[j];
-                    }
-                }
+            for (int kt = 0; kt < KT / 32; ++kt) hide_keys(s[kt], (uint32_t)(now >> (32 * kt)), lane);
         }
         float top = -INFINITY, lo, hi;
 #pragma unroll

@@ -42,7 +42,7 @@ __device__ __forceinline__ bool rows_key_seen(const CrossArgs& a, int b, int key
 }
 
 template <class T, int DP, int R>
-__global__ __launch_bounds__(512) void cross_rows_fwd_kernel(CrossArgs a, int W) {
+__global__ __launch_bounds__(1024) void cross_rows_fwd_kernel(CrossArgs a, int W) {
     constexpr int C = Chunk<T>::n, LPK = DP / C, NK = 64 / LPK, U = 4;
     extern __shared__ float join[];               // [waves][R][DP + 2]
     const int lane = threadIdx.x & 63, slot = lane / LPK, col = (lane % LPK) * C;
@@ -313,26 +313,26 @@ static int keys_per_step(int d, int dtype) {           // NK * U of the forward
 }
 
 // Waves a problem is given inside one workgroup: enough problems fill the chip with one wave each (4096 waves = 4 per SIMD); fewer are cut
-// over the waves of a workgroup as long as each still has a step of keys.
-static int rows_waves(int64_t problems, int Lk, int step) {
+// over the waves of a workgroup as long as each still has a step of keys.  (The backward needs more than 128 registers: at most eight.)
+static int rows_waves(int64_t problems, int Lk, int step, bool bwd) {
     if (problems >= 4096 || Lk <= step) return 1;
-    if (problems >= 1024 || Lk <= 8 * step) return 4;
-    return 8;
+    if (problems >= 1024 || Lk <= 4 * step) return 4;
+    return bwd || Lk <= 8 * step ? 8 : 16;
 }
 
-// Key ranges on different workgroups (joined by a second launch): only where a problem's eight waves would walk more than 8 steps each while
-// most of the chip idles.
+// Key ranges on different workgroups (joined by a second launch, about 5 us).  A workgroup's four rows x 32 keys a step are some 500 vector
+// instructions, so 32 problems of 1500 keys on 32 of the 256 CUs are bound by those CUs' vector pipes (23 us with 8 waves a problem and with 16).
 int cross_rows_splits(int B, int Hkv, int Lk, int d, int dtype) {
     const int64_t problems = (int64_t)B * Hkv;
     const int step = keys_per_step(d, dtype);
-    if (problems == 0 || problems >= 256 || Lk <= 8 * 8 * step) return 1;
-    const int64_t want = (512 + problems - 1) / problems, most = Lk / (8 * 2 * step);
+    if (problems == 0 || problems >= 256 || Lk <= 16 * step) return 1;
+    const int64_t want = (256 + problems - 1) / problems, most = Lk / (4 * step);
     return (int)(want < most ? want : most);
 }
 
 template <class T, int DP>
 static void rows_launch(const CrossArgs& a, int W, bool bwd, hipStream_t st) {
-    const int threads = W == 8 ? 512 : 256, per_block = threads / 64 / W;
+    const int threads = W <= 4 ? 256 : 64 * W, per_block = threads / 64 / W;
     const int64_t items = (int64_t)a.B * a.Hkv * a.splits;
     const dim3 grid((unsigned)((items + per_block - 1) / per_block));
     const int R = a.rows;
@@ -354,9 +354,9 @@ static void rows_launch(const CrossArgs& a, int W, bool bwd, hipStream_t st) {
 static int rows_go(CrossArgs a, int dtype, bool bwd, hipStream_t st) {
     const int step = keys_per_step(a.d, dtype);
     const int64_t problems = (int64_t)a.B * a.Hkv;
-    const int W = rows_waves(problems * a.splits, a.Lk, step);
+    const int W = rows_waves(problems * a.splits, range_of(a.Lk, a.splits), step, bwd);
     SNAG_REQUIRE(problems * a.splits < (int64_t)1 << 31, SNAG_ERR_UNSUPPORTED, "cross attention: %lld problems", (long long)problems);
-    a.per_split = (a.Lk + a.splits - 1) / a.splits;
+    a.per_split = range_of(a.Lk, a.splits);
 #define GO(T) a.d <= 32 ? rows_launch<T, 32>(a, W, bwd, st) : a.d <= 64 ? rows_launch<T, 64>(a, W, bwd, st) : rows_launch<T, 128>(a, W, bwd, st)
     if (dtype == SNAG_F32) GO(float);
     else if (dtype == SNAG_BF16) GO(bf16_t);

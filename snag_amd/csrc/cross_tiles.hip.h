@@ -210,6 +210,18 @@ __device__ __forceinline__ Problem problem_of(const CrossArgs& a, int64_t tiles)
 __device__ __forceinline__ bool key_seen(const CrossArgs& a, int b, int key, int len) {
     return key < len && (a.mask == nullptr || a.mask[(int64_t)b * a.mask_ld + key] != 0);
 }
+// 64 keys from key0 as bits, one lane's look each.  A tile's bits are collected a tile before its rows are fetched: a mask byte in front of
+// every load would put its latency in front of every load.
+__device__ __forceinline__ bool mask_byte(const CrossArgs& a, int b, int key0, int len, int lane) {
+    return a.mask == nullptr || (key0 + lane < len && a.mask[(int64_t)b * a.mask_ld + key0 + lane] != 0);
+}
+__device__ __forceinline__ uint64_t seen_bits(bool byte, int key0, int len, int lane) { return __ballot(byte && key0 + lane < len); }
+// -inf for the keys of a 32-key block that are not seen; bits: of the block
+__device__ __forceinline__ void hide_keys(f32x16& s, uint32_t bits, int lane) {
+    const uint32_t mine = bits >> (4 * (lane >> 5));
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1 ? s[i] : -INFINITY;
+}
 // row = l G + g: the host has checked that the multiplier is exact for every row
 __device__ __forceinline__ int row_l(const CrossArgs& a, int row) { return (int)(__umulhi((uint32_t)row, a.g_magic) + ((uint32_t)row & a.g_one)); }
 
