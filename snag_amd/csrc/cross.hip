@@ -7,11 +7,11 @@ static int elem_size(int dtype) { return dtype == SNAG_F32 ? 4 : 2; }
 
 // How many ranges a loop over `n` keys or rows is cut into when `groups` workgroups exist without cutting.  Two workgroups fit a CU, so a launch
 // runs in rounds of 512; s ranges take ceil(groups s / 512) / s of the uncut time and each costs its partial result's write and read, taken
-// as 12 % of what is left (measured at 192 groups over 4096 rows of 128: 1 range 270 us, 2 155, 3 200).  At least 256 keys or rows a range.
+// as 12 % of what is left (measured at 192 groups over 4096 rows of 128: 1 range 270 us, 2 155, 3 200).  At least 128 keys or rows a range.
 static int ranges_for(int64_t groups, int64_t n) {
     int best = 1;
     double least = 1e30;
-    for (int s = 1; groups > 0 && groups < 512 && s <= n / 256 && s <= 64; ++s) {
+    for (int s = 1; groups > 0 && groups < 512 && s <= n / 128 && s <= 64; ++s) {
         const double cost = (double)((groups * s + 511) / 512) / s * (1 + (s > 1 ? 0.12 * s : 0));
         if (cost < least) least = cost, best = s;
     }

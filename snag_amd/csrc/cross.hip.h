@@ -65,26 +65,42 @@ template <> struct Chunk<f16_t> {
     typedef vec any __attribute__((aligned(2)));
 };
 
-// Elements col .. col + n of a row of d elements; zero where the row is not valid or ends.  Rows that are not 16-byte aligned take the same wide
-// loads (the hardware splits them where it has to: 63 -> 30 us at 4 heads of 75 fp16 elements against element-wise loads); only the chunk that
-// the row's end cuts is loaded by element.
+// Elements col .. col + n of a row of d elements; zero where the row is not valid or ends: load_raw, then -- where the value is used, so that the
+// load can stay in flight until then -- fix_tail.  vec: d is a multiple of n and every row 16-byte aligned.  Otherwise rows take the same wide
+// loads at any alignment; the chunk that the row's end cuts is loaded as the row's last n elements and shifted into place (element-wise loads
+// made 4 heads of 75 fp16 elements three times slower).  Rows shorter than a chunk are loaded by element.
 template <class T>
-__device__ __forceinline__ typename Chunk<T>::vec load_chunk(const T* __restrict__ row, int col, int d, bool valid, int vec) {
-    typename Chunk<T>::vec r;
-#pragma unroll
-    for (int j = 0; j < Chunk<T>::n; ++j) r[j] = (T)0.f;
+__device__ __forceinline__ typename Chunk<T>::vec load_raw(const T* __restrict__ row, int col, int d, bool valid, int vec) {
+    constexpr int n = Chunk<T>::n;
+    typename Chunk<T>::vec r{};
     if (valid && col < d) {
         if (vec) {
             r = *(const typename Chunk<T>::vec*)(row + col);
-        } else if (col + Chunk<T>::n <= d) {
-            r = *(const typename Chunk<T>::any*)(row + col);
+        } else if (d >= n) {
+            r = *(const typename Chunk<T>::any*)(row + min(col, d - n));
         } else {
 #pragma unroll
-            for (int j = 0; j < Chunk<T>::n; ++j)
-                if (col + j < d) r[j] = row[col + j];
+            for (int j = 0; j < n; ++j)
+                if (j < d) r[j] = row[j];
         }
     }
     return r;
+}
+template <class T>
+__device__ __forceinline__ typename Chunk<T>::vec fix_tail(typename Chunk<T>::vec r, int col, int d, int vec) {
+    constexpr int n = Chunk<T>::n;
+    if (vec || d < n) return r;
+    const int bits = max(col - (d - n), 0) * (int)sizeof(T) * 8;               // shift towards element 0
+    union { typename Chunk<T>::vec v; uint64_t w[2]; } u{r};
+    const uint64_t lo = bits < 64 ? (u.w[0] >> (bits & 63)) | ((u.w[1] << 1) << (63 - (bits & 63))) : u.w[1] >> (bits & 63);
+    const uint64_t hi = u.w[1] >> (bits & 63);
+    u.w[0] = bits < 128 ? lo : 0;
+    u.w[1] = bits < 64 ? hi : 0;
+    return u.v;
+}
+template <class T>
+__device__ __forceinline__ typename Chunk<T>::vec load_chunk(const T* __restrict__ row, int col, int d, bool valid, int vec) {
+    return fix_tail<T>(load_raw<T>(row, col, d, valid, vec), col, d, vec);
 }
 
 static inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }

@@ -36,7 +36,7 @@ __global__ __launch_bounds__(256) void cross_stat_kernel(CrossArgs a, float* __r
 
 // d q: as the forward, 32 rows per wave; splits > 1: part[split][B, Lq, H, d], joined by cross_sum_kernel
 template <class T, int DP, int NW, int KT, bool DIRECT>
-__global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 128 ? 1 : 2) void cross_dq_kernel(CrossArgs a) {
+__global__ __launch_bounds__(NW * 64, NW == 1 || (sizeof(T) == 4 && DP == 128) ? 1 : 2) void cross_dq_kernel(CrossArgs a) {
     using M = Mma<T>;
     constexpr int NT = NW * 64;
     __shared__ __attribute__((aligned(16))) T lk[2][KT * DP];
@@ -55,28 +55,24 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 128 ? 1 : 2) void 
 
     const int t0 = pr.split * a.per_split / KT, t1 = min((len + KT - 1) / KT, t0 + a.per_split / KT);
     TileFetch<T, DP, KT, NT, DIRECT> fk, fv;
-    uint64_t now = 0, next = 0;                            // seen keys of the tile that is worked on, and of the one in flight
-    bool byte = false;                                     // this lane's mask byte of the tile behind that
+    bool byte = true;                                      // this lane's mask byte of the tile in flight
+    uint64_t now = 0;                                      // seen keys of the tile that is worked on
     // DIRECT: rows behind the last key are read as the last key; what is not seen gets -inf for a score below
     auto fetch = [&](int t) {
-        const int key0 = t * KT;
-        auto row_at = [&](const T* base, int64_t step, int i, bool& ok) {
-            const int key = DIRECT ? min(key0 + i, len - 1) : key0 + i;
-            ok = DIRECT || ((next >> i) & 1);
-            return base + key * step;
-        };
-        fk.fetch([&](int i, bool& ok) { return row_at(kb, a.ksl, i, ok); }, lk[t & 1], a.d, a.vec_k, tid);
-        fv.fetch([&](int i, bool& ok) { return row_at(vb, a.vsl, i, ok); }, lv[t & 1], a.d, a.vec_v, tid);
-        if (!DIRECT && t + 1 < t1) byte = mask_byte(a, b, key0 + KT, len, lane);
+        const int key0 = t * KT, end = (DIRECT ? len : a.Lk) - 1;
+        fk.fetch([&](int i) { return kb + min(key0 + i, end) * a.ksl; }, lk[t & 1], a.d, a.vec_k, tid);
+        fv.fetch([&](int i) { return vb + min(key0 + i, end) * a.vsl; }, lv[t & 1], a.d, a.vec_v, tid);
+        if (!DIRECT) byte = mask_byte(a, b, key0, lane);
     };
     auto store = [&](int t) {
-        fk.store(lk[t & 1], tid);
-        fv.store(lv[t & 1], tid);
-        now = next;
-        if (!DIRECT) next = seen_bits(byte, (t + 1) * KT, len, lane);
+        if constexpr (!DIRECT) {
+            now = seen_bits(byte, t * KT, len, lane);
+            auto keep = [&](int i) { return (now >> i) & 1; };
+            fk.store(keep, lk[t & 1], a.d, a.vec_k, tid);
+            fv.store(keep, lv[t & 1], a.d, a.vec_v, tid);
+        }
     };
-    if (!DIRECT && t0 < t1) next = seen_bits(mask_byte(a, b, t0 * KT, len, lane), t0 * KT, len, lane);
-    if (t0 < t1) fetch(t0);
+    if (DIRECT ? t0 < t1 : t0 * KT < a.Lk) fetch(t0);
     typename M::Frag q[DP / 16], dout[DP / 16];
     own_row<T, DP>(q, (const T*)a.q + b * a.qsb + l * a.qsl + head * a.qsh, a.d, own, a.vec_q, lane);
     own_row<T, DP>(dout, (const T*)a.dout + dense, a.d, own, a.vec_o, lane);
@@ -121,7 +117,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 128 ? 1 : 2) void 
 
 // d k, d v: 32 keys per wave, row tiles of RT through LDS; splits > 1: part[2][split][B, Lk, Hkv, d] (d k, then d v)
 template <class T, int DP, int NW, int RT, bool DIRECT>
-__global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void cross_dkv_kernel(CrossArgs a) {
+__global__ __launch_bounds__(NW * 64, NW == 1 || (sizeof(T) == 4 && DP >= 64) ? 1 : 2) void cross_dkv_kernel(CrossArgs a) {
     using M = Mma<T>;
     constexpr int NT = NW * 64, KEYS = NW * 32;
     // 16-bit rows of 128: d k and d v take 128 registers, k another 32; v, the fourth operand, is read from LDS so that two waves fit a SIMD
@@ -145,17 +141,15 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void c
     if (t0 < t1) {
         TileFetch<T, DP, RT, NT, DIRECT> fq, fo;
         const float* st = a.stat + 2 * ((int64_t)b * a.Hkv + hk) * padded_rows(a.rows);
-        // DIRECT: rows behind the last one are read as the last one, their p is 0
+        // rows behind the last one are read as the last one, their p is 0
         auto fetch = [&](int t) {
             const int r0 = t * RT;
-            fq.fetch([&](int i, bool& ok) {
+            fq.fetch([&](int i) {
                 const int r = min(r0 + i, a.rows - 1), l = row_l(a, r);
-                ok = r0 + i < a.rows;
                 return (const T*)a.q + b * a.qsb + l * a.qsl + (hk * a.G + r - l * a.G) * a.qsh;
             }, lq[t & 1], a.d, a.vec_q, tid);
-            fo.fetch([&](int i, bool& ok) {
+            fo.fetch([&](int i) {
                 const int r = min(r0 + i, a.rows - 1), l = row_l(a, r);
-                ok = r0 + i < a.rows;
                 return (const T*)a.dout + (((int64_t)b * a.Lq + l) * a.H + hk * a.G + r - l * a.G) * a.d;
             }, lo[t & 1], a.d, a.vec_o, tid);
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -165,21 +159,21 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void c
 #endif
         };
         auto store = [&](int t) {
-            fq.store(lq[t & 1], tid);
-            fo.store(lo[t & 1], tid);
+            auto all = [](int) { return true; };
+            fq.store(all, lq[t & 1], a.d, a.vec_q, tid);
+            fo.store(all, lo[t & 1], a.d, a.vec_o, tid);
         };
         fetch(t0);
         if constexpr (VLDS) {
             TileFetch<T, DP, KEYS, NT, DIRECT> fv;
-            uint64_t bits[KEYS / 64];
+            const int end = (DIRECT ? len : a.Lk) - 1;
+            fv.fetch([&](int i) { return (const T*)a.v + b * a.vsb + hk * a.vsh + min(key0 + i, end) * a.vsl; }, lvv, a.d, a.vec_v, tid);
+            if constexpr (!DIRECT) {
+                uint64_t bits[KEYS / 64];
 #pragma unroll
-            for (int u = 0; u < KEYS / 64; ++u) bits[u] = DIRECT ? 0 : seen_bits(mask_byte(a, b, key0 + 64 * u, len, lane), key0 + 64 * u, len, lane);
-            fv.fetch([&](int i, bool& ok) {
-                const int at = DIRECT ? min(key0 + i, len - 1) : key0 + i;
-                ok = DIRECT || ((bits[KEYS / 64 - 1] >> (i & 63)) & (i >= 64 * (KEYS / 64 - 1))) || ((bits[0] >> (i & 63)) & (i < 64));
-                return (const T*)a.v + b * a.vsb + hk * a.vsh + at * a.vsl;
-            }, lvv, a.d, a.vec_v, tid);
-            fv.store(lvv, tid);
+                for (int u = 0; u < KEYS / 64; ++u) bits[u] = seen_bits(mask_byte(a, b, key0 + 64 * u, lane), key0 + 64 * u, len, lane);
+                fv.store([&](int i) { return ((i < 64 ? bits[0] : bits[KEYS / 64 - 1]) >> (i & 63)) & 1; }, lvv, a.d, a.vec_v, tid);
+            }
         }
         typename M::Frag k[DP / 16], v[VLDS ? 1 : DP / 16];
         own_row<T, DP>(k, (const T*)a.k + b * a.ksb + hk * a.ksh + key * a.ksl, a.d, seen, a.vec_k, lane);

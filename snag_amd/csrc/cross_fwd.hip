@@ -13,7 +13,7 @@ constexpr float kSlack = 8.f;
 // Workgroup: NW waves x 32 rows; key tiles of KT.  splits > 1: per range part[split][B H Lq][d] = sum exp2(S - m) v (not normalised) and, behind
 // all of those, [split][B H Lq][2] = (m, sum); cross_combine_kernel joins them.
 template <class T, int DP, int NW, int KT, bool DIRECT>
-__global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 128 ? 1 : 2) void cross_fwd_kernel(CrossArgs a) {
+__global__ __launch_bounds__(NW * 64, NW == 1 || (sizeof(T) == 4 && DP == 128) ? 1 : 2) void cross_fwd_kernel(CrossArgs a) {
     using M = Mma<T>;
     constexpr int NT = NW * 64;
     __shared__ __attribute__((aligned(16))) T lk[2][KT * DP];
@@ -31,28 +31,24 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 128 ? 1 : 2) void 
 
     const int t0 = pr.split * a.per_split / KT, t1 = min((len + KT - 1) / KT, t0 + a.per_split / KT);
     TileFetch<T, DP, KT, NT, DIRECT> fk, fv;
-    uint64_t now = 0, next = 0;                            // seen keys of the tile that is worked on, and of the one in flight
-    bool byte = false;                                     // this lane's mask byte of the tile behind that
+    bool byte = true;                                      // this lane's mask byte of the tile in flight
+    uint64_t now = 0;                                      // seen keys of the tile that is worked on
     // DIRECT: rows behind the last key are read as the last key; what is not seen gets -inf for a score below
     auto fetch = [&](int t) {
-        const int key0 = t * KT;
-        auto row_at = [&](const T* base, int64_t step, int i, bool& ok) {
-            const int key = DIRECT ? min(key0 + i, len - 1) : key0 + i;
-            ok = DIRECT || ((next >> i) & 1);
-            return base + key * step;
-        };
-        fk.fetch([&](int i, bool& ok) { return row_at(kb, a.ksl, i, ok); }, lk[t & 1], a.d, a.vec_k, tid);
-        fv.fetch([&](int i, bool& ok) { return row_at(vb, a.vsl, i, ok); }, lv[t & 1], a.d, a.vec_v, tid);
-        if (!DIRECT && t + 1 < t1) byte = mask_byte(a, b, key0 + KT, len, lane);
+        const int key0 = t * KT, end = (DIRECT ? len : a.Lk) - 1;
+        fk.fetch([&](int i) { return kb + min(key0 + i, end) * a.ksl; }, lk[t & 1], a.d, a.vec_k, tid);
+        fv.fetch([&](int i) { return vb + min(key0 + i, end) * a.vsl; }, lv[t & 1], a.d, a.vec_v, tid);
+        if (!DIRECT) byte = mask_byte(a, b, key0, lane);
     };
     auto store = [&](int t) {
-        fk.store(lk[t & 1], tid);
-        fv.store(lv[t & 1], tid);
-        now = next;
-        if (!DIRECT) next = seen_bits(byte, (t + 1) * KT, len, lane);
+        if constexpr (!DIRECT) {
+            now = seen_bits(byte, t * KT, len, lane);
+            auto keep = [&](int i) { return (now >> i) & 1; };
+            fk.store(keep, lk[t & 1], a.d, a.vec_k, tid);
+            fv.store(keep, lv[t & 1], a.d, a.vec_v, tid);
+        }
     };
-    if (!DIRECT && t0 < t1) next = seen_bits(mask_byte(a, b, t0 * KT, len, lane), t0 * KT, len, lane);
-    if (t0 < t1) fetch(t0);
+    if (DIRECT ? t0 < t1 : t0 * KT < a.Lk) fetch(t0);
     typename M::Frag q[DP / 16];
     own_row<T, DP>(q, (const T*)a.q + b * a.qsb + l * a.qsl + head * a.qsh, a.d, own, a.vec_q, lane);
     if (t0 < t1) store(t0);
@@ -130,25 +126,28 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 128 ? 1 : 2) void 
     if (h == 0) a.lse[at] = sum == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(sum);
 }
 
-// Joins the key ranges of the forward: one wave per row (b, head, l).
+// Joins the key ranges of the forward (at most 64): one wave per row (b, head, l), lane s looks at range s.
 template <class T>
 __global__ __launch_bounds__(256) void cross_combine_kernel(CrossArgs a) {
     const int64_t n = (int64_t)a.B * a.H * a.Lq, at = (int64_t)blockIdx.x * 4 + wave_id_uniform();
     const int lane = threadIdx.x & 63;
     if (at >= n) return;
     const float* ml = a.part + (int64_t)a.splits * n * a.d;
-    float m = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ml[(s * n + at) * 2]);
-    const float ref = m == -INFINITY ? 0.f : m;
-    float sum = 0.f, o[2] = {0.f, 0.f};
+    const bool mine = lane < a.splits;
+    const float ms = mine ? ml[(lane * n + at) * 2] : -INFINITY, ts = mine ? ml[(lane * n + at) * 2 + 1] : 0.f;
+    const float m = max64(ms), ref = m == -INFINITY ? 0.f : m;
+    const float w = ts == 0.f ? 0.f : __builtin_amdgcn_exp2f(ms - ref);       // 0: a range none of whose keys is seen
+    const float sum = sum64(w * ts);
+    float o[2] = {0.f, 0.f};
+#pragma unroll 4
     for (int s = 0; s < a.splits; ++s) {
-        const float w = __builtin_amdgcn_exp2f(ml[(s * n + at) * 2] - ref), t = ml[(s * n + at) * 2 + 1];
-        if (t == 0.f) continue;                       // a range none of whose keys is seen
-        sum += w * t;
+        const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), s));
         const float* p = a.part + (s * n + at) * a.d;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-            if (lane + 64 * u < a.d) o[u] = fmaf(w, p[lane + 64 * u], o[u]);
+        for (int u = 0; u < 2; ++u) {
+            const float x = lane + 64 * u < a.d ? p[lane + 64 * u] : 0.f;
+            o[u] = f == 0.f ? o[u] : fmaf(f, x, o[u]);
+        }
     }
     const int64_t l = at % a.Lq, bh = at / a.Lq, head = bh % a.H, b = bh / a.H;
     T* out = (T*)a.out + ((b * a.Lq + l) * a.H + head) * a.d;

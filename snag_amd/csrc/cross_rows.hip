@@ -21,6 +21,42 @@ __device__ __forceinline__ float group_sum(float v) {
     return v;
 }
 
+// The same value of another lane group's, combined: all-reduce over the 64 / LPK groups, every lane ends with the same value.
+__device__ __forceinline__ void swap16(float v, float& a, float& b) {       // the rows of 16 lanes 0, 0, 2, 2 and 1, 1, 3, 3
+#if defined(__HIP_DEVICE_COMPILE__)
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    a = __uint_as_float(r[0]), b = __uint_as_float(r[1]);
+#else
+    a = b = v;
+#endif
+}
+__device__ __forceinline__ void swap32(float v, float& a, float& b) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    a = __uint_as_float(r[0]), b = __uint_as_float(r[1]);
+#else
+    a = b = v;
+#endif
+}
+template <int LPK>
+__device__ __forceinline__ float slots_sum(float v) {
+    float a, b;
+    if constexpr (LPK <= 4) v += dpp_f32<0x124>(v);        // row_ror:4
+    if constexpr (LPK <= 8) v += dpp_f32<0x128>(v);        // row_ror:8
+    if constexpr (LPK <= 16) swap16(v, a, b), v = a + b;
+    swap32(v, a, b);
+    return a + b;
+}
+template <int LPK>
+__device__ __forceinline__ float slots_max(float v) {
+    float a, b;
+    if constexpr (LPK <= 4) v = fmaxf(v, dpp_f32<0x124>(v));
+    if constexpr (LPK <= 8) v = fmaxf(v, dpp_f32<0x128>(v));
+    if constexpr (LPK <= 16) swap16(v, a, b), v = fmaxf(a, b);
+    swap32(v, a, b);
+    return fmaxf(a, b);
+}
+
 struct RowsItem { int b, hk, split, wave; bool live; };
 // waves-per-problem W divides the workgroup's waves; ids of one problem's workgroups are neighbours
 __device__ __forceinline__ RowsItem rows_item(const CrossArgs& a, int W) {
@@ -68,9 +104,11 @@ __global__ __launch_bounds__(1024) void cross_rows_fwd_kernel(CrossArgs a, int W
         for (int u = 0; u < U; ++u) {
             const int key = base + u * NK + slot;
             seen[u] = key < k1 && rows_key_seen(a, it.b, key, len);
-            kc[u] = load_chunk<T>(kb + (int64_t)key * a.ksl, col, a.d, seen[u], a.vec_k);
-            vc[u] = load_chunk<T>(vb + (int64_t)key * a.vsl, col, a.d, seen[u], a.vec_v);
+            kc[u] = load_raw<T>(kb + (int64_t)key * a.ksl, col, a.d, seen[u], a.vec_k);
+            vc[u] = load_raw<T>(vb + (int64_t)key * a.vsl, col, a.d, seen[u], a.vec_v);
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u) kc[u] = fix_tail<T>(kc[u], col, a.d, a.vec_k), vc[u] = fix_tail<T>(vc[u], col, a.d, a.vec_v);
         float s[U][R];
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -103,22 +141,15 @@ __global__ __launch_bounds__(1024) void cross_rows_fwd_kernel(CrossArgs a, int W
     // the lane groups of the wave
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        float mn = m[r];
-#pragma unroll
-        for (int x = LPK; x < 64; x <<= 1) mn = fmaxf(mn, __shfl_xor(mn, x));
+        const float mn = slots_max<LPK>(m[r]);
         const float w = __builtin_amdgcn_exp2f(m[r] - (mn == -INFINITY ? 0.f : mn));
         m[r] = mn;
-        sum[r] *= w;
+        sum[r] = slots_sum<LPK>(sum[r] * w);
 #pragma unroll
-        for (int x = LPK; x < 64; x <<= 1) sum[r] += __shfl_xor(sum[r], x);
-#pragma unroll
-        for (int j = 0; j < C; ++j) {
-            acc[r][j] *= w;
-#pragma unroll
-            for (int x = LPK; x < 64; x <<= 1) acc[r][j] += __shfl_xor(acc[r][j], x);
-        }
+        for (int j = 0; j < C; ++j) acc[r][j] = slots_sum<LPK>(acc[r][j] * w);
     }
-    // the waves of the problem
+    const int64_t n = (int64_t)a.B * a.H * a.Lq;
+    // the waves of the problem (then the workgroup's only one): a thread per row and element
     if (W > 1) {
         constexpr int P = DP + 2;
         float* mine = join + wave_id_uniform() * R * P;
@@ -131,30 +162,36 @@ __global__ __launch_bounds__(1024) void cross_rows_fwd_kernel(CrossArgs a, int W
             }
         }
         __syncthreads();
-        if (it.wave != 0) return;
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            float mn = -INFINITY;
-            for (int w = 0; w < W; ++w) mn = fmaxf(mn, mine[(w * R + r) * P + DP]);
+        for (int i = threadIdx.x; i < R * DP; i += blockDim.x) {
+            const int r = i / DP, c = i % DP;
+            if (r >= a.rows || c >= a.d) continue;
+            float mn = -INFINITY, s = 0.f, o = 0.f;
+            for (int w = 0; w < W; ++w) mn = fmaxf(mn, join[(w * R + r) * P + DP]);
             const float ref = mn == -INFINITY ? 0.f : mn;
-            m[r] = mn;
-            sum[r] = 0.f;
-#pragma unroll
-            for (int j = 0; j < C; ++j) acc[r][j] = 0.f;
             for (int w = 0; w < W; ++w) {
-                const float f = __builtin_amdgcn_exp2f(mine[(w * R + r) * P + DP] - ref);
-                sum[r] = fmaf(f, mine[(w * R + r) * P + DP + 1], sum[r]);
-#pragma unroll
-                for (int j = 0; j < C; ++j) acc[r][j] = fmaf(f, mine[(w * R + r) * P + col + j], acc[r][j]);
+                const float f = __builtin_amdgcn_exp2f(join[(w * R + r) * P + DP] - ref);
+                s = fmaf(f, join[(w * R + r) * P + DP + 1], s);
+                o = fmaf(f, join[(w * R + r) * P + c], o);
+            }
+            const int l = r / a.G, head = it.hk * a.G + r % a.G;
+            const int64_t at = ((int64_t)it.b * a.H + head) * a.Lq + l;
+            if (a.splits > 1) {
+                a.part[(it.split * n + at) * a.d + c] = o;
+                float* ml = a.part + (int64_t)a.splits * n * a.d + (it.split * n + at) * 2;
+                if (c == 0) ml[0] = mn, ml[1] = s;
+            } else {
+                ((T*)a.out)[(((int64_t)it.b * a.Lq + l) * a.H + head) * a.d + c] = (T)(o * (s > 0.f ? 1.f / s : (s == 0.f ? 0.f : s)));
+                if (c == 0) a.lse[at] = s == 0.f ? -INFINITY : mn + __builtin_amdgcn_logf(s);
             }
         }
+        return;
     }
     if (!it.live || slot != 0) return;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         if (r >= a.rows) break;
         const int l = r / a.G, head = it.hk * a.G + r % a.G;
-        const int64_t at = ((int64_t)it.b * a.H + head) * a.Lq + l, n = (int64_t)a.B * a.H * a.Lq;
+        const int64_t at = ((int64_t)it.b * a.H + head) * a.Lq + l;
         if (a.splits > 1) {
             float* o = a.part + (it.split * n + at) * a.d;
 #pragma unroll
@@ -227,9 +264,11 @@ __global__ __launch_bounds__(512) void cross_rows_bwd_kernel(CrossArgs a, int W)
         for (int u = 0; u < U; ++u) {
             const int key = base + u * NK + slot;
             seen[u] = key < k1 && rows_key_seen(a, it.b, key, len);
-            kc[u] = load_chunk<T>(kb + (int64_t)key * a.ksl, col, a.d, seen[u], a.vec_k);
-            vc[u] = load_chunk<T>(vb + (int64_t)key * a.vsl, col, a.d, seen[u], a.vec_v);
+            kc[u] = load_raw<T>(kb + (int64_t)key * a.ksl, col, a.d, seen[u], a.vec_k);
+            vc[u] = load_raw<T>(vb + (int64_t)key * a.vsl, col, a.d, seen[u], a.vec_v);
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u) kc[u] = fix_tail<T>(kc[u], col, a.d, a.vec_k), vc[u] = fix_tail<T>(vc[u], col, a.d, a.vec_v);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int key = base + u * NK + slot;
@@ -265,9 +304,7 @@ __global__ __launch_bounds__(512) void cross_rows_bwd_kernel(CrossArgs a, int W)
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int j = 0; j < C; ++j)
-#pragma unroll
-            for (int x = LPK; x < 64; x <<= 1) dq[r][j] += __shfl_xor(dq[r][j], x);
+        for (int j = 0; j < C; ++j) dq[r][j] = slots_sum<LPK>(dq[r][j]);
     if (W > 1) {
         float* mine = join + wave_id_uniform() * R * DP;
         if (slot == 0) {
@@ -277,14 +314,16 @@ __global__ __launch_bounds__(512) void cross_rows_bwd_kernel(CrossArgs a, int W)
                 for (int j = 0; j < C; ++j) mine[r * DP + col + j] = dq[r][j];
         }
         __syncthreads();
-        if (it.wave != 0) return;
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-            for (int j = 0; j < C; ++j) {
-                dq[r][j] = 0.f;
-                for (int w = 0; w < W; ++w) dq[r][j] += mine[(w * R + r) * DP + col + j];
-            }
+        for (int i = threadIdx.x; i < R * DP; i += blockDim.x) {
+            const int r = i / DP, c = i % DP;
+            if (r >= a.rows || c >= a.d) continue;
+            float s = 0.f;
+            for (int w = 0; w < W; ++w) s += join[w * R * DP + i];
+            const int64_t dense = (((int64_t)it.b * a.Lq + r / a.G) * a.H + it.hk * a.G + r % a.G) * a.d + c;
+            if (a.splits > 1) a.part[(int64_t)it.split * a.B * a.Lq * a.H * a.d + dense] = s;
+            else ((T*)a.dq)[dense] = (T)s;
+        }
+        return;
     }
     if (!it.live || slot != 0) return;
 #pragma unroll
@@ -326,7 +365,7 @@ int cross_rows_splits(int B, int Hkv, int Lk, int d, int dtype) {
     const int64_t problems = (int64_t)B * Hkv;
     const int step = keys_per_step(d, dtype);
     if (problems == 0 || problems >= 256 || Lk <= 16 * step) return 1;
-    const int64_t want = (256 + problems - 1) / problems, most = Lk / (4 * step);
+    const int64_t want = problems < 4 ? 64 : (256 + problems - 1) / problems, most = Lk / (4 * step);      // cross_combine_kernel joins up to 64
     return (int)(want < most ? want : most);
 }
 

@@ -114,50 +114,51 @@ __device__ __forceinline__ void halves(float v, float& lo, float& hi) {
 template <class T, int DP>
 __device__ __forceinline__ void own_row(typename Mma<T>::Frag (&f)[DP / 16], const T* row, int d, bool valid, int vec, int lane) {
     constexpr int C = Chunk<T>::n;
+    typename Chunk<T>::vec r[DP / 16 * 8 / C];
 #pragma unroll
-    for (int kb = 0; kb < DP / 16; ++kb) {
-        const int col = kb * 16 + (lane >> 5) * 8;
+    for (int u = 0; u < DP / 16 * 8 / C; ++u) r[u] = load_raw<T>(row, (u / (8 / C)) * 16 + (lane >> 5) * 8 + u % (8 / C) * C, d, valid, vec);
 #pragma unroll
-        for (int w = 0; w < 8 / C; ++w) {
-            const auto c = load_chunk<T>(row, col + w * C, d, valid, vec);
+    for (int u = 0; u < DP / 16 * 8 / C; ++u) {
+        const auto c = fix_tail<T>(r[u], (u / (8 / C)) * 16 + (lane >> 5) * 8 + u % (8 / C) * C, d, vec);
 #pragma unroll
-            for (int j = 0; j < C; ++j) f[kb][w * C + j] = c[j];
-        }
+        for (int j = 0; j < C; ++j) f[u / (8 / C)][u % (8 / C) * C + j] = c[j];
     }
 }
 
-// A tile of R rows on its way from global memory to LDS, one ahead of the tile that is worked on.
-// DIRECT: straight into LDS, 16 bytes a lane, no registers; every row has to be readable and whole (d == DP, 16-byte aligned).
-// Otherwise through registers: rows that are not valid become zeros, whatever memory holds there, and so do the columns behind d.
+// A tile of R rows on its way from global memory to LDS, one ahead of the tile that is worked on.  Every row pointer has to be readable.
+// DIRECT: straight into LDS, 16 bytes a lane, no registers; rows have to be whole (d == DP, 16-byte aligned).
+// Otherwise through registers: on the way to LDS the columns behind d become zeros, and rows that are not to be kept do, whatever they hold.
+// (Which rows those are is not known yet when the loads go out: nothing waits for a length or a mask.)
 template <class T, int DP, int R, int NT, bool DIRECT>
 struct TileFetch {
     static constexpr int C = Chunk<T>::n, kPerRow = DP / C, kAll = R * kPerRow, kN = (kAll + NT - 1) / NT;
     static_assert(kAll % NT == 0 || (kN == 1 && !DIRECT), "tile does not divide among the threads");
     typename Chunk<T>::vec r[DIRECT ? 1 : kN];
-    // row(i, ok) -> the row's elements; ok: valid
     template <class RowPtr>
     __device__ __forceinline__ void fetch(RowPtr row, T* lds, int d, int vec, int tid) {
 #pragma unroll
         for (int u = 0; u < kN; ++u) {
             const int e = u * NT + tid, i = e / kPerRow;
-            bool ok;
             if constexpr (DIRECT) {
-                const T* p = row(i, ok) + chunk_place<T, DP>(i, e % kPerRow) * C;
+                const T* p = row(i) + chunk_place<T, DP>(i, e % kPerRow) * C;
 #if defined(__HIP_DEVICE_COMPILE__)
                 __builtin_amdgcn_global_load_lds((SNAG_GLOBAL void*)p, (SNAG_LDS void*)(lds + (u * NT + (tid & ~63)) * C), 16, 0, 0);
 #endif
             } else {
-                const T* p = row(i, ok);
-                r[u] = load_chunk<T>(p, (e % kPerRow) * C, d, ok && (kAll % NT == 0 || e < kAll), vec);
+                const bool in = kAll % NT == 0 || e < kAll;
+                r[u] = load_raw<T>(row(in ? i : 0), (e % kPerRow) * C, d, in, vec);
             }
         }
     }
-    __device__ __forceinline__ void store(T* lds, int tid) const {
+    template <class Keep>
+    __device__ __forceinline__ void store(Keep keep, T* lds, int d, int vec, int tid) const {
         if constexpr (!DIRECT) {
 #pragma unroll
             for (int u = 0; u < kN; ++u) {
-                const int e = u * NT + tid;
-                if (kAll % NT == 0 || e < kAll) *(typename Chunk<T>::vec*)(lds + tile_at<T, DP>(e / kPerRow, (e % kPerRow) * C)) = r[u];
+                const int e = u * NT + tid, i = e / kPerRow;
+                auto v = fix_tail<T>(r[u], (e % kPerRow) * C, d, vec);
+                if (!keep(i)) v = typename Chunk<T>::vec{};
+                if (kAll % NT == 0 || e < kAll) *(typename Chunk<T>::vec*)(lds + tile_at<T, DP>(i, (e % kPerRow) * C)) = v;
             }
         }
     }
@@ -210,10 +211,9 @@ __device__ __forceinline__ Problem problem_of(const CrossArgs& a, int64_t tiles)
 __device__ __forceinline__ bool key_seen(const CrossArgs& a, int b, int key, int len) {
     return key < len && (a.mask == nullptr || a.mask[(int64_t)b * a.mask_ld + key] != 0);
 }
-// 64 keys from key0 as bits, one lane's look each.  A tile's bits are collected a tile before its rows are fetched: a mask byte in front of
-// every load would put its latency in front of every load.
-__device__ __forceinline__ bool mask_byte(const CrossArgs& a, int b, int key0, int len, int lane) {
-    return a.mask == nullptr || (key0 + lane < len && a.mask[(int64_t)b * a.mask_ld + key0 + lane] != 0);
+// 64 keys from key0 as bits, one lane's look each
+__device__ __forceinline__ bool mask_byte(const CrossArgs& a, int b, int key0, int lane) {
+    return a.mask == nullptr || (key0 + lane < a.Lk && a.mask[(int64_t)b * a.mask_ld + key0 + lane] != 0);
 }
 __device__ __forceinline__ uint64_t seen_bits(bool byte, int key0, int len, int lane) { return __ballot(byte && key0 + lane < len); }
 // -inf for the keys of a 32-key block that are not seen; bits: of the block

@@ -408,7 +408,7 @@ __device__ __forceinline__ void finish(const MuonTable* __restrict__ L, const Mu
 // last products of the stage before it.
 template <int MODE, int DT, int TILE, int NST>
 __global__ __launch_bounds__(TILE == 128 ? 256 : 512, NST == 2 ? 2 : 1) void muon_product_kernel(const MuonTable* __restrict__ L, int from, int last) {
-    constexpr int PLANES = DT == SNAG_F32 ? 2 : 1;
+    constexpr int PLANES = DT == SNAG_BF16 ? 1 : 2;
     using S = Shape<TILE, PLANES, NST>;
     constexpr int NI = S::kWm / 32, NJ = S::kWn / 32, KB = S::kDepth / 16;
     static_assert(KB % 2 == 0, "fragment sets alternate");
@@ -635,7 +635,7 @@ __device__ __forceinline__ void image_store(_Float16* hi, _Float16* lo, int row,
 // start: only the first A's shares of X copy 0.  One workgroup per 128-column block; slab[block][wave][4][1024] as the product kernel's ranges.
 template <int DT>
 __global__ __launch_bounds__(256) void muon_narrow_kernel(const MuonTable* __restrict__ L, int from, int start, int last) {
-    constexpr int PLANES = DT == SNAG_F32 ? 2 : 1;
+    constexpr int PLANES = DT == SNAG_BF16 ? 1 : 2;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     _Float16 *X = (_Float16*)smem, *S = X + 2 * kImage;                // hi, lo of X's block; hi, lo of A, later of B
     float* block = (float*)(S + 2 * kImage);                           // 4 x 32 x kPitch
@@ -791,7 +791,7 @@ static int grow_lds(K kernel, size_t bytes) {
 }
 template <int MODE, int DT, int TILE, int NST>
 static int product_of(const MuonRun& R, int from, int last, hipStream_t st) {
-    using S = Shape<TILE, DT == SNAG_F32 ? 2 : 1, NST>;
+    using S = Shape<TILE, DT == SNAG_BF16 ? 1 : 2, NST>;
     static const int grown = grow_lds(muon_product_kernel<MODE, DT, TILE, NST>, S::kLds);
     if (grown != SNAG_OK) return grown;
     muon_product_kernel<MODE, DT, TILE, NST><<<dim3(R.blocks_of[MODE]), S::kThreads, S::kLds, st>>>(R.table, from, last);
