@@ -42,7 +42,8 @@ class _CrossAttentionFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, d_out, _):
         q, k, v, kv_lens, key_mask, out, lse = ctx.saved_tensors
-        dq, dk, dv = ops.cross_attention_bwd(q, k, v, out, lse, d_out.contiguous(), kv_lens, key_mask, ctx.scale)
+        shape, args, hold = ops._cross_args(q, k, v, kv_lens, key_mask, ctx.scale)        # (hooks on saved tensors may have moved them)
+        dq, dk, dv = ops._cross_bwd(args, shape, (q, k, v), out, lse, d_out.contiguous())
         need = ctx.needs_input_grad
         return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None
 
@@ -65,9 +66,10 @@ def cross_attention(q, k, v, kv_lens=None, key_mask=None, scale=None, return_lse
 class _SandwichNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, y, post_weight, pre_weight, post_bias, pre_bias, gate, res_scale, kind, eps):
-        h, z, stats = ops.sandwich_norm_fwd(x, y, post_weight, pre_weight, post_bias, pre_bias, gate, res_scale, kind, eps)
+        plan = ops._sandwich_args(x, y, post_weight, post_bias, pre_weight, pre_bias, gate, kind)
+        h, z, stats = ops._sandwich_fwd(plan, x, y, post_weight, pre_weight, post_bias, pre_bias, gate, res_scale, kind, eps, True)
         ctx.save_for_backward(x, y, stats, post_weight, pre_weight, post_bias, pre_bias, gate)
-        ctx.cfg = (res_scale, kind)
+        ctx.cfg = (plan, res_scale, kind)
         ctx.set_materialize_grads(False)
         return h, z
 
@@ -75,8 +77,9 @@ class _SandwichNormFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, d_h, d_z):
         x, y, stats, post_weight, pre_weight, post_bias, pre_bias, gate = ctx.saved_tensors
-        grads = ops.sandwich_norm_bwd(x, y, stats, None if d_h is None else d_h.contiguous(), None if d_z is None else d_z.contiguous(),
-                                      post_weight, pre_weight, post_bias, pre_bias, gate, *ctx.cfg)
+        plan, res_scale, kind = ctx.cfg
+        grads = ops._sandwich_bwd(plan, x, y, stats, None if d_h is None else d_h.contiguous(), None if d_z is None else d_z.contiguous(),
+                                  post_weight, pre_weight, post_bias, pre_bias, gate, res_scale, kind)
         return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None, None)
 
 

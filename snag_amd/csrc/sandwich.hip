@@ -7,7 +7,7 @@
 // put its rounding into d pre_w), from the four statistics per row the forward saved.  All arithmetic and all sums are fp32, each output is
 // rounded once; the variance is taken around the mean (two passes over registers).
 //
-// TPR threads work on one row (32, 64: lane groups, no LDS; 256: a workgroup) with NU x 4 elements per thread in registers.  In the backward
+// TPR threads work on one row (32, 64: lane groups, no LDS; 256, 512: a workgroup) with NU x 4 elements per thread in registers.  In the backward
 // a worker walks a run of rows and keeps the parameter gradients of its columns in registers; its run lies inside one gate row or covers
 // whole gate rows, the partial sums go to a slab [worker][gradient][dim] and are added up in the workers' order (no atomics).
 #include <type_traits>
@@ -37,25 +37,36 @@ template <class T> struct Four { using vec = __attribute__((ext_vector_type(4)))
 // thread t's four elements of step u: neighbours (VEC) or a stride of TPR apart (any dim, any alignment)
 template <int TPR, bool VEC> __device__ __forceinline__ int column(int u, int j, int t) { return VEC ? (u * TPR + t) * 4 + j : (u * 4 + j) * TPR + t; }
 
+// a thread's elements of a row as they lie in memory, and as fp32 (0 behind the row's end)
+template <class T, int NU> struct Raw { typename Four<T>::vec v[NU]; };
 template <class T, int TPR, int NU, bool VEC>
-__device__ __forceinline__ void load_row(float (&r)[NU][4], const T* p, int D, int t) {
+__device__ __forceinline__ Raw<T, NU> raw_row(const T* p, int D, int t) {
+    Raw<T, NU> r;
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
+        r.v[u] = typename Four<T>::vec{};
         if constexpr (VEC) {
             const int c = column<TPR, VEC>(u, 0, t);
-            typename Four<T>::vec v{};
-            if (c < D) v = *(const typename Four<T>::vec*)(p + c);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) r[u][j] = (float)v[j];
+            if (c < D) r.v[u] = *(const typename Four<T>::vec*)(p + c);
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int c = column<TPR, VEC>(u, j, t);
-                r[u][j] = c < D ? (float)p[c] : 0.f;
+                if (c < D) r.v[u][j] = p[c];
             }
         }
     }
+    return r;
 }
+template <class T, int NU>
+__device__ __forceinline__ void widen(float (&r)[NU][4], const Raw<T, NU>& v) {
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[u][j] = (float)v.v[u][j];
+}
+template <class T, int TPR, int NU, bool VEC>
+__device__ __forceinline__ void load_row(float (&r)[NU][4], const T* p, int D, int t) { widen<T, NU>(r, raw_row<T, TPR, NU, VEC>(p, D, t)); }
 template <class T, int TPR, int NU, bool VEC>
 __device__ __forceinline__ void store_row(T* p, const float (&r)[NU][4], int D, int t) {
 #pragma unroll
@@ -91,15 +102,16 @@ __device__ __forceinline__ void load_param(float (&r)[NU][4], const void* p, int
 }
 
 // sums over the TPR threads of a row; every thread gets them
+constexpr int kMaxWaves = 8;
 template <int TPR, int N>
-__device__ __forceinline__ void row_sums(float (&s)[N], float (*red)[4][2], int& turn) {
+__device__ __forceinline__ void row_sums(float (&s)[N], float (*red)[kMaxWaves][2], int& turn) {
     if constexpr (TPR == 32) {
 #pragma unroll
         for (int i = 0; i < N; ++i) s[i] = sum16(s[i]), s[i] += __shfl_xor(s[i], 16);
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) s[i] = sum64(s[i]);
-        if constexpr (TPR == 256) {
+        if constexpr (TPR > 64) {
             // two sets of slots in turn: one barrier per sum
             float (*slot)[2] = red[turn];
             turn ^= 1;
@@ -108,15 +120,22 @@ __device__ __forceinline__ void row_sums(float (&s)[N], float (*red)[4][2], int&
 #pragma unroll
                 for (int i = 0; i < N; ++i) slot[wave][i] = s[i];
             }
-            __syncthreads();
+            // LDS alone has to be visible: global loads may stay in flight across the barrier
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
 #pragma unroll
-            for (int i = 0; i < N; ++i) s[i] = slot[0][i] + slot[1][i] + slot[2][i] + slot[3][i];
+            for (int i = 0; i < N; ++i) {
+                s[i] = slot[0][i];
+#pragma unroll
+                for (int w = 1; w < TPR / 64; ++w) s[i] += slot[w][i];
+            }
         }
     }
 }
 
 template <int TPR, int NU, bool VEC>
-__device__ __forceinline__ void row_stats(const float (&v)[NU][4], int D, int layer, float eps, int t, float (*red)[4][2], int& turn, float& mean, float& rstd) {
+__device__ __forceinline__ void row_stats(const float (&v)[NU][4], int D, int layer, float eps, int t, float (*red)[kMaxWaves][2], int& turn, float& mean, float& rstd) {
     mean = 0.f;
     if (layer) {
         float s[1] = {0.f};
@@ -140,12 +159,12 @@ __device__ __forceinline__ void row_stats(const float (&v)[NU][4], int D, int la
 }
 
 template <class TX, class TY, int TPR, int NU, bool VEC>
-__global__ __launch_bounds__(256) void sandwich_fwd_kernel(SandwichArgs a) {
-    __shared__ float red[2][4][2];
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void sandwich_fwd_kernel(SandwichArgs a) {
+    __shared__ float red[2][kMaxWaves][2];
     int turn = 0;
     const int t = threadIdx.x % TPR;
-    const int64_t row = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
-    if (TPR < 256 && row >= a.rows) return;       // TPR == 256: one row per workgroup
+    const int64_t row = TPR >= 256 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+    if (TPR < 256 && row >= a.rows) return;       // otherwise one row per workgroup
     const int D = a.dim;
     float y[NU][4], x[NU][4], p[NU][4], b[NU][4], g[NU][4];
     load_row<TY, TPR, NU, VEC>(y, (const TY*)a.y + row * D, D, t);
@@ -174,12 +193,15 @@ __global__ __launch_bounds__(256) void sandwich_fwd_kernel(SandwichArgs a) {
     if (t == 0 && a.stats != nullptr) *(f32x4*)(a.stats + row * 4) = f32x4{my, ry, mh, rh};
 }
 
+// With up to eight elements a thread the weights and (while it lasts) the gate stay in registers and the next row is in flight while the present
+// one is worked on (rows of 4096 in bf16 around an fp32 stream: 340 -> 264 us, 4.6 TB/s); with 16 there is no room for either.
 template <class TX, class TY, int TPR, int NU, bool VEC>
-__global__ __launch_bounds__(256) void sandwich_bwd_kernel(SandwichArgs a) {
-    __shared__ float red[2][4][2];
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void sandwich_bwd_kernel(SandwichArgs a) {
+    constexpr bool KEEP = NU <= 2;
+    __shared__ float red[2][kMaxWaves][2];
     int turn = 0;
     const int t = threadIdx.x % TPR;
-    const int64_t worker = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+    const int64_t worker = TPR >= 256 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
     if (TPR < 256 && worker >= a.workers) return;
     const int D = a.dim;
     // rows of this worker: run `worker % chunks` of gate row `worker / chunks`, or `run` rows anywhere (whole gate rows)
@@ -192,7 +214,7 @@ __global__ __launch_bounds__(256) void sandwich_bwd_kernel(SandwichArgs a) {
         r0 = group * a.rows_per_gate + worker % a.chunks * a.run;
         r1 = min((group + 1) * a.rows_per_gate, r0 + a.run);
     }
-    float sum[kGrads][NU][4];
+    float sum[kGrads][NU][4], pw[NU][4], pb[NU][4], qw[NU][4], g[NU][4];
 #pragma unroll
     for (int k = 0; k < kGrads; ++k)
 #pragma unroll
@@ -200,36 +222,44 @@ __global__ __launch_bounds__(256) void sandwich_bwd_kernel(SandwichArgs a) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) sum[k][u][j] = 0.f;
     const float inv_d = 1.0f / (float)D;
+    Raw<TY, NU> ny, ne;
+    Raw<TX, NU> nx, nd;
+    f32x4 nst{};
+    auto fetch = [&](int64_t row) {
+        ny = raw_row<TY, TPR, NU, VEC>((const TY*)a.y + row * D, D, t);
+        nx = raw_row<TX, TPR, NU, VEC>((const TX*)a.x + row * D, D, t);
+        nd = a.dh != nullptr ? raw_row<TX, TPR, NU, VEC>((const TX*)a.dh + row * D, D, t) : Raw<TX, NU>{};
+        ne = a.dz != nullptr ? raw_row<TY, TPR, NU, VEC>((const TY*)a.dz + row * D, D, t) : Raw<TY, NU>{};
+        nst = *(const f32x4*)(a.stats + row * 4);
+    };
+    auto weights = [&]() {
+        load_param<TY, TPR, NU, VEC>(pw, a.post_w, a.w32, 0, 1.f, D, t);
+        load_param<TY, TPR, NU, VEC>(pb, a.post_b, a.w32, 0, 0.f, D, t);
+        load_param<TY, TPR, NU, VEC>(qw, a.pre_w, a.w32, 0, 1.f, D, t);
+    };
+    if (KEEP && r0 < r1) fetch(r0), weights();
+    int64_t grow = r0 < r1 ? r0 / a.rows_per_gate : 0, gate_end = (grow + 1) * a.rows_per_gate;
+    bool fresh = true;                                     // the gate row has not been read yet
     for (int64_t row = r0; row < r1; ++row) {
-        const int64_t grow = row / a.rows_per_gate;
-        float y[NU][4], x[NU][4], d[NU][4], e[NU][4], p[NU][4], b[NU][4], g[NU][4], w[NU][4];
-        load_row<TY, TPR, NU, VEC>(y, (const TY*)a.y + row * D, D, t);
-        load_row<TX, TPR, NU, VEC>(x, (const TX*)a.x + row * D, D, t);
-        if (a.dh != nullptr) {
-            load_row<TX, TPR, NU, VEC>(d, (const TX*)a.dh + row * D, D, t);
-        } else {
-#pragma unroll
-            for (int u = 0; u < NU; ++u)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) d[u][j] = 0.f;
-        }
-        const f32x4 st = *(const f32x4*)(a.stats + row * 4);
-        load_param<TY, TPR, NU, VEC>(p, a.post_w, a.w32, 0, 1.f, D, t);
-        load_param<TY, TPR, NU, VEC>(b, a.post_b, a.w32, 0, 0.f, D, t);
-        load_param<TY, TPR, NU, VEC>(g, a.gate, a.g32, grow, 1.f, D, t);
-        const float my = st[0], ry = st[1], mh = st[2], rh = st[3];
+        if (!KEEP) fetch(row), weights();
+        if (!KEEP || fresh) load_param<TY, TPR, NU, VEC>(g, a.gate, a.g32, grow, 1.f, D, t), fresh = false;
+        float y[NU][4], x[NU][4], d[NU][4], e[NU][4], b[NU][4];
+        widen<TY, NU>(y, ny);
+        widen<TX, NU>(x, nx);
+        widen<TX, NU>(d, nd);
+        widen<TY, NU>(e, ne);
+        const float my = nst[0], ry = nst[1], mh = nst[2], rh = nst[3];
+        if (KEEP && row + 1 < r1) fetch(row + 1);
         // y <- N(y), x <- N(h), b <- post
 #pragma unroll
         for (int u = 0; u < NU; ++u)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 y[u][j] = (y[u][j] - my) * ry;
-                b[u][j] = fmaf(y[u][j], p[u][j], b[u][j]);
+                b[u][j] = fmaf(y[u][j], pw[u][j], pb[u][j]);
                 x[u][j] = (fmaf(g[u][j], b[u][j], a.res_scale * x[u][j]) - mh) * rh;
             }
         if (a.dz != nullptr) {
-            load_row<TY, TPR, NU, VEC>(e, (const TY*)a.dz + row * D, D, t);
-            load_param<TY, TPR, NU, VEC>(w, a.pre_w, a.w32, 0, 1.f, D, t);
             float s[2] = {0.f, 0.f};
 #pragma unroll
             for (int u = 0; u < NU; ++u)
@@ -237,7 +267,7 @@ __global__ __launch_bounds__(256) void sandwich_bwd_kernel(SandwichArgs a) {
                 for (int j = 0; j < 4; ++j) {
                     sum[kPreW][u][j] = fmaf(e[u][j], x[u][j], sum[kPreW][u][j]);
                     sum[kPreB][u][j] += e[u][j];
-                    e[u][j] *= w[u][j];                       // 0 behind the row's end, as dz is
+                    e[u][j] *= qw[u][j];                      // 0 behind the row's end, as dz is
                     s[0] = fmaf(e[u][j], x[u][j], s[0]);
                     s[1] += e[u][j];
                 }
@@ -260,7 +290,7 @@ __global__ __launch_bounds__(256) void sandwich_bwd_kernel(SandwichArgs a) {
                 sum[kPostW][u][j] = fmaf(dp, y[u][j], sum[kPostW][u][j]);
                 sum[kPostB][u][j] += dp;
                 sum[kGate][u][j] += b[u][j];
-                e[u][j] = dp * p[u][j];
+                e[u][j] = dp * pw[u][j];
                 s[0] = fmaf(e[u][j], y[u][j], s[0]);
                 s[1] += e[u][j];
             }
@@ -272,13 +302,18 @@ __global__ __launch_bounds__(256) void sandwich_bwd_kernel(SandwichArgs a) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) e[u][j] = ry * (e[u][j] - fmaf(y[u][j], m1, m2));
         store_row<TY, TPR, NU, VEC>((TY*)a.dy + row * D, e, D, t);
-        if (a.dgate_direct && a.dgate != nullptr && (row + 1) % a.rows_per_gate == 0) {
-            if (a.g32) store_row<float, TPR, NU, VEC>((float*)a.dgate + grow * D, sum[kGate], D, t);
-            else store_row<TY, TPR, NU, VEC>((TY*)a.dgate + grow * D, sum[kGate], D, t);
+        if (row + 1 == gate_end) {
+            if (a.dgate_direct && a.dgate != nullptr) {
+                if (a.g32) store_row<float, TPR, NU, VEC>((float*)a.dgate + grow * D, sum[kGate], D, t);
+                else store_row<TY, TPR, NU, VEC>((TY*)a.dgate + grow * D, sum[kGate], D, t);
 #pragma unroll
-            for (int u = 0; u < NU; ++u)
+                for (int u = 0; u < NU; ++u)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) sum[kGate][u][j] = 0.f;
+                    for (int j = 0; j < 4; ++j) sum[kGate][u][j] = 0.f;
+            }
+            ++grow;
+            gate_end += a.rows_per_gate;
+            fresh = true;
         }
     }
     float* out = a.slab + worker * kGrads * D;
@@ -330,12 +365,14 @@ __global__ __launch_bounds__(1024) void sandwich_sums_kernel(SandwichSums a) {
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
-static int threads_per_row(int dim) { return dim <= 128 ? 32 : dim <= 1024 ? 64 : 256; }
+// the backward holds eight rows' worth of registers per thread (gradients, weights, the next row): wide rows take 512 threads
+static int threads_per_row(int dim) { return dim <= 128 ? 32 : dim <= 512 ? 64 : dim <= 2048 ? 256 : 512; }
 
 struct SandwichPlan { int direct; int64_t workers, run, chunks; };
-// Workers: enough to fill the chip (8 lane-group workers a workgroup: 4096; workgroup-wide ones: 1024), no more than rows.
+// Workers: enough to fill the chip (lane groups: 4096; workgroups of 256: 1024, of 512: 512), no more than rows.
 static SandwichPlan sandwich_plan(int64_t rows, int64_t rows_per_gate, int dim) {
-    const int64_t want = threads_per_row(dim) == 256 ? 1024 : 4096;
+    const int tpr = threads_per_row(dim);
+    const int64_t want = tpr == 512 ? 512 : tpr == 256 ? 1024 : 4096;
     SandwichPlan p{};
     const int64_t share = (rows + want - 1) / want;
     if (rows_per_gate <= share) {
@@ -356,25 +393,26 @@ template <class TX, class TY>
 static void sandwich_launch(const SandwichArgs& a, bool vec, bool bwd, hipStream_t st) {
     const int tpr = threads_per_row(a.dim);
     const int64_t items = bwd ? a.workers : a.rows;
-    const dim3 grid((unsigned)((items + 256 / tpr - 1) / (256 / tpr)));
+    const int threads = tpr > 256 ? tpr : 256, per = threads / tpr;
+    const dim3 grid((unsigned)((items + per - 1) / per));
 #define GO(TPR, NU)                                                                       \
     do {                                                                                  \
         if (bwd) {                                                                        \
-            if (vec) sandwich_bwd_kernel<TX, TY, TPR, NU, true><<<grid, 256, 0, st>>>(a); \
-            else sandwich_bwd_kernel<TX, TY, TPR, NU, false><<<grid, 256, 0, st>>>(a);    \
+            if (vec) sandwich_bwd_kernel<TX, TY, TPR, NU, true><<<grid, threads, 0, st>>>(a); \
+            else sandwich_bwd_kernel<TX, TY, TPR, NU, false><<<grid, threads, 0, st>>>(a);    \
         } else {                                                                          \
-            if (vec) sandwich_fwd_kernel<TX, TY, TPR, NU, true><<<grid, 256, 0, st>>>(a); \
-            else sandwich_fwd_kernel<TX, TY, TPR, NU, false><<<grid, 256, 0, st>>>(a);    \
+            if (vec) sandwich_fwd_kernel<TX, TY, TPR, NU, true><<<grid, threads, 0, st>>>(a); \
+            else sandwich_fwd_kernel<TX, TY, TPR, NU, false><<<grid, threads, 0, st>>>(a);    \
         }                                                                                 \
     } while (0)
     const int D = a.dim;
     if (D <= 128) GO(32, 1);
     else if (D <= 256) GO(64, 1);
     else if (D <= 512) GO(64, 2);
-    else if (D <= 1024) GO(64, 4);
+    else if (D <= 1024) GO(256, 1);
     else if (D <= 2048) GO(256, 2);
-    else if (D <= 4096) GO(256, 4);
-    else GO(256, 8);
+    else if (D <= 4096) GO(512, 2);
+    else GO(512, 4);
 #undef GO
 }
 

@@ -566,14 +566,21 @@ def _any(t, name, ndim=None):
 _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
+@functools.lru_cache(maxsize=None)
+def _entry(name):
+    return getattr(_lib.load(), name)
+
+
 def _call_on(device, name, *args):
     """The entry on the current stream of the operands' device (which need not be the current one)."""
     index = device.index
     if index == _current_device():
-        call(name, *args, _raw_stream(index))
+        rc = _entry(name)(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            call(name, *args, _raw_stream(index))
+            rc = _entry(name)(*args, _raw_stream(index))
+    if rc != 0:
+        raise _lib.SnagHipError(f"{name} failed ({rc}): {_lib.last_error()}")
 
 
 def _one_device(device, **tensors):
@@ -636,12 +643,24 @@ def _cross_work(shape, backward, device):
 def cross_attention_fwd(q, k, v, kv_lens=None, key_mask=None, scale=None):
     """q [B, Lq, H, d], k / v [B, Lk, Hkv, d] (any strides with adjacent head elements) -> out [B, Lq, H, d], lse [B, H, Lq] (log2).
     C ABI: snag_cross_fwd."""
-    shape, args, hold = _cross_args(q, k, v, kv_lens, key_mask, scale)
+    return _cross_fwd(q, *_cross_args(q, k, v, kv_lens, key_mask, scale))
+
+
+def _cross_fwd(q, shape, args, hold):
     out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], device=q.device, dtype=f32)
+    lse = torch.empty((shape[1], shape[4], shape[2]), device=q.device, dtype=f32)
     work, n = _cross_work(shape, False, q.device)
     _call_on(q.device, "snag_cross_fwd", *args, ptr(out), ptr(lse), ptr(work), n)
     return out, lse
+
+
+def _cross_bwd(args, shape, like, out, lse, d_out):
+    """The launch itself, of arguments that have been checked."""
+    q, k, v = like
+    dq, dk, dv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in like)
+    work, n = _cross_work(shape, True, q.device)
+    _call_on(q.device, "snag_cross_bwd", *args, ptr(out), ptr(lse), ptr(d_out), ptr(dq), ptr(dk), ptr(dv), ptr(work), n)
+    return dq, dk, dv
 
 
 def cross_attention_bwd(q, k, v, out, lse, d_out, kv_lens=None, key_mask=None, scale=None):
@@ -655,10 +674,7 @@ def cross_attention_bwd(q, k, v, out, lse, d_out, kv_lens=None, key_mask=None, s
     if tuple(lse.shape) != (q.shape[0], q.shape[2], q.shape[1]):
         raise ValueError(f"lse must be [B, H, Lq], got {tuple(lse.shape)}")
     _one_device(q.device, out=out, lse=lse, d_out=d_out)
-    dq, dk, dv = (torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k, v))
-    work, n = _cross_work(shape, True, q.device)
-    _call_on(q.device, "snag_cross_bwd", *args, ptr(out), ptr(lse), ptr(d_out), ptr(dq), ptr(dk), ptr(dv), ptr(work), n)
-    return dq, dk, dv
+    return _cross_bwd(args, shape, (q, k, v), out, lse, d_out)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -715,9 +731,14 @@ def _sandwich_args(x, y, post_weight, post_bias, pre_weight, pre_bias, gate, kin
 def sandwich_norm_fwd(x, y, post_weight=None, pre_weight=None, post_bias=None, pre_bias=None, gate=None, res_scale=1.0, kind="rms", eps=1e-6, want_stats=True):
     """h = res_scale x + gate (post_weight N(y) + post_bias), z = pre_weight N(h) + pre_bias -> h, z, stats [rows, 4] (or None).
     C ABI: snag_sandwich_fwd."""
-    rows, dim, wt, gt, per_gate = _sandwich_args(x, y, post_weight, post_bias, pre_weight, pre_bias, gate, kind)
+    plan = _sandwich_args(x, y, post_weight, post_bias, pre_weight, pre_bias, gate, kind)
+    return _sandwich_fwd(plan, x, y, post_weight, pre_weight, post_bias, pre_bias, gate, res_scale, kind, eps, want_stats)
+
+
+def _sandwich_fwd(plan, x, y, post_weight, pre_weight, post_bias, pre_bias, gate, res_scale, kind, eps, want_stats):
+    rows, dim, wt, gt, per_gate = plan
     h, z = torch.empty_like(x), torch.empty_like(y)
-    stats = torch.empty(rows, 4, device=x.device, dtype=f32) if want_stats else None
+    stats = torch.empty((rows, 4), device=x.device, dtype=f32) if want_stats else None
     _call_on(x.device, "snag_sandwich_fwd", ptr(x), DTYPES[x.dtype], ptr(y), DTYPES[y.dtype], rows, dim, ptr(post_weight), ptr(post_bias), ptr(pre_weight),
              ptr(pre_bias), wt, ptr(gate), gt, per_gate, float(res_scale), NORMS[kind], float(eps), ptr(h), ptr(z), ptr(stats))
     return h, z, stats
@@ -726,18 +747,23 @@ def sandwich_norm_fwd(x, y, post_weight=None, pre_weight=None, post_bias=None, p
 def sandwich_norm_bwd(x, y, stats, d_h, d_z, post_weight=None, pre_weight=None, post_bias=None, pre_bias=None, gate=None, res_scale=1.0, kind="rms"):
     """-> d_x, d_y, d_post_weight, d_pre_weight, d_post_bias, d_pre_bias, d_gate (None for a parameter that is None).  d_h or d_z may be None (zero).
     C ABI: snag_sandwich_bwd."""
-    rows, dim, wt, gt, per_gate = _sandwich_args(x, y, post_weight, post_bias, pre_weight, pre_bias, gate, kind)
+    plan = _sandwich_args(x, y, post_weight, post_bias, pre_weight, pre_bias, gate, kind)
     for t, like, name in ((d_h, x, "d_h"), (d_z, y, "d_z")):
         if t is not None:
             _chk(t, name, dtype=like.dtype)
             if t.shape != like.shape:
                 raise ValueError(f"{name} must be {tuple(like.shape)}, got {tuple(t.shape)}")
     _chk(stats, "stats", ndim=2)
-    if tuple(stats.shape) != (rows, 4):
-        raise ValueError(f"stats must be [{rows}, 4], got {tuple(stats.shape)}")
+    if tuple(stats.shape) != (plan[0], 4):
+        raise ValueError(f"stats must be [{plan[0]}, 4], got {tuple(stats.shape)}")
     _one_device(x.device, stats=stats, d_h=d_h, d_z=d_z)
-    new = lambda t: None if t is None else torch.empty_like(t) if rows else torch.zeros_like(t)
-    dx, dy, dpw, dqw, dpb, dqb, dg = (new(t) for t in (x, y, post_weight, pre_weight, post_bias, pre_bias, gate))
+    return _sandwich_bwd(plan, x, y, stats, d_h, d_z, post_weight, pre_weight, post_bias, pre_bias, gate, res_scale, kind)
+
+
+def _sandwich_bwd(plan, x, y, stats, d_h, d_z, post_weight, pre_weight, post_bias, pre_bias, gate, res_scale, kind):
+    rows, dim, wt, gt, per_gate = plan
+    new = torch.empty_like if rows else torch.zeros_like
+    dx, dy, dpw, dqw, dpb, dqb, dg = (None if t is None else new(t) for t in (x, y, post_weight, pre_weight, post_bias, pre_bias, gate))
     n = _sandwich_work_floats(rows, per_gate, dim)
     work = torch.empty(n, device=x.device, dtype=f32)
     _call_on(x.device, "snag_sandwich_bwd", ptr(x), DTYPES[x.dtype], ptr(y), DTYPES[y.dtype], rows, dim, ptr(post_weight), ptr(post_bias), ptr(pre_weight), wt,
