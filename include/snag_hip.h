@@ -778,6 +778,8 @@ SNAG_API int snag_spmm_csr(const int32_t* rowptr, const int32_t* col, const floa
  * out [B, Lq, H, d] dense; lse [B, H, Lq] = log2 of the sum of exp2(scale * log2(e) * q . k), kept for the backward.
  * Scores, running maximum, sums and outputs are accumulated in fp32; for 16-bit types the probabilities (and d scores) are rounded to dtype
  * for the product with v (k, q).
+ * out_lo (as out, may be NULL): what the rounding of a 16-bit out dropped, rounded once more.  The backward takes it (NULL: zero) with out for
+ * sum d_out . out, the part of d scores that cancels where a query sees few keys or one key takes nearly all.
  * The backward OVERWRITES d_q (as out), d_k and d_v [B, Lk, Hkv, d] dense (zero at unseen keys); heads that share a key/value head add up
  * in a fixed order: no atomics, bit-reproducible.  out, lse: the forward's; d_out [B, Lq, H, d] dense.
  * work: snag_cross_work_floats(..., backward) floats (may be 0), uninitialised; launches sharing it must be stream-ordered. */
@@ -785,10 +787,10 @@ SNAG_API int snag_spmm_csr(const int32_t* rowptr, const int32_t* col, const floa
 SNAG_API int64_t snag_cross_work_floats(int dtype, int B, int Lq, int Lk, int H, int Hkv, int d, int backward);
 SNAG_API int snag_cross_fwd(const void* q, const void* k, const void* v, int dtype, int B, int Lq, int Lk, int H, int Hkv, int d,
                             const int64_t* strides_host, const void* kv_lens, int lens_bytes, const uint8_t* key_mask, int64_t mask_ld, float scale,
-                            void* out, float* lse, float* work, int64_t work_floats, void* stream);
+                            void* out, void* out_lo, float* lse, float* work, int64_t work_floats, void* stream);
 SNAG_API int snag_cross_bwd(const void* q, const void* k, const void* v, int dtype, int B, int Lq, int Lk, int H, int Hkv, int d,
                             const int64_t* strides_host, const void* kv_lens, int lens_bytes, const uint8_t* key_mask, int64_t mask_ld, float scale,
-                            const void* out, const float* lse, const void* d_out, void* d_q, void* d_k, void* d_v,
+                            const void* out, const void* out_lo, const float* lse, const void* d_out, void* d_q, void* d_k, void* d_v,
                             float* work, int64_t work_floats, void* stream);
 
 /* The norms after and before a block with its gate and the residual, in one pass (the Mformer's own form, model/SNAG_tools.py:218-222,

@@ -164,8 +164,8 @@ SIGNATURES = {
     "snag_rank_summary_pair": [_P, _P, _I, _P, _I, _P, _P],
     "snag_argmin_rows_cols": [_P, _L, _I, _I, _P, _P, _P, _P],
     "snag_entity_token_fwd": [_P, _L, _I, _P, _P, _F, _P, _L, _P],
-    "snag_cross_fwd": [_P, _P, _P] + [_I] * 7 + [_P, _P, _I, _P, _L, _F, _P, _P, _P, _L, _P],
-    "snag_cross_bwd": [_P, _P, _P] + [_I] * 7 + [_P, _P, _I, _P, _L, _F] + [_P] * 7 + [_L, _P],
+    "snag_cross_fwd": [_P, _P, _P] + [_I] * 7 + [_P, _P, _I, _P, _L, _F, _P, _P, _P, _P, _L, _P],
+    "snag_cross_bwd": [_P, _P, _P] + [_I] * 7 + [_P, _P, _I, _P, _L, _F] + [_P] * 8 + [_L, _P],
     "snag_sandwich_fwd": [_P, _I, _P, _I, _L, _I, _P, _P, _P, _P, _I, _P, _I, _L, _F, _I, _F, _P, _P, _P, _P],
     "snag_sandwich_bwd": [_P, _I, _P, _I, _L, _I, _P, _P, _P, _I, _P, _I, _L, _F, _I] + [_P] * 11 + [_L, _P],
     "snag_orthogonalize": [_P, _P, _P, _P, _I, _I, _I, _F, _P, _L, _P],

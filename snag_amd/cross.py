@@ -32,8 +32,8 @@ def _note_stream(out):
 class _CrossAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, kv_lens, key_mask, scale):
-        out, lse = ops.cross_attention_fwd(q, k, v, kv_lens, key_mask, scale)
-        ctx.save_for_backward(q, k, v, kv_lens, key_mask, out, lse)
+        out, lse, lo = ops.cross_attention_fwd(q, k, v, kv_lens, key_mask, scale, want_residual=True)
+        ctx.save_for_backward(q, k, v, kv_lens, key_mask, out, lse, lo)
         ctx.scale = scale
         ctx.mark_non_differentiable(lse)
         return out, lse
@@ -41,9 +41,8 @@ class _CrossAttentionFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, d_out, _):
-        q, k, v, kv_lens, key_mask, out, lse = ctx.saved_tensors
-        shape, args, hold = ops._cross_args(q, k, v, kv_lens, key_mask, ctx.scale)        # (hooks on saved tensors may have moved them)
-        dq, dk, dv = ops._cross_bwd(args, shape, (q, k, v), out, lse, d_out.contiguous())
+        q, k, v, kv_lens, key_mask, out, lse, lo = ctx.saved_tensors
+        dq, dk, dv = ops.cross_attention_bwd(q, k, v, out, lse, d_out.contiguous(), kv_lens, key_mask, ctx.scale, lo)
         need = ctx.needs_input_grad
         return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None
 

@@ -94,7 +94,7 @@ extern "C" SNAG_API int64_t snag_cross_work_floats(int dtype, int B, int Lq, int
 
 extern "C" SNAG_API int snag_cross_fwd(const void* q, const void* k, const void* v, int dtype, int B, int Lq, int Lk, int H, int Hkv, int d,
                                        const int64_t* strides_host, const void* kv_lens, int lens_bytes, const uint8_t* key_mask, int64_t mask_ld, float scale,
-                                       void* out, float* lse, float* work, int64_t work_floats, void* stream) {
+                                       void* out, void* out_lo, float* lse, float* work, int64_t work_floats, void* stream) {
     CrossArgs a{};
     if (int rc = cross_args(a, q, k, v, dtype, B, Lq, Lk, H, Hkv, d, strides_host, kv_lens, lens_bytes, key_mask, mask_ld, scale)) return rc;
     if (B == 0 || Lq == 0) return SNAG_OK;
@@ -103,8 +103,8 @@ extern "C" SNAG_API int snag_cross_fwd(const void* q, const void* k, const void*
     const int64_t need = snag_cross_work_floats(dtype, B, Lq, Lk, H, Hkv, d, 0);
     SNAG_REQUIRE(need == 0 || (work != nullptr && work_floats >= need), SNAG_ERR_ARG, "cross attention: workspace of %lld floats, %lld needed", (long long)work_floats, (long long)need);
     hipStream_t st = (hipStream_t)stream;
-    a.out = out, a.lse = lse, a.part = work, a.splits = p.s_fwd;
-    a.vec_o = d % (16 / elem_size(dtype)) == 0 && aligned16(out);
+    a.out = out, a.out_lo = out_lo, a.lse = lse, a.part = work, a.splits = p.s_fwd;
+    a.vec_o = d % (16 / elem_size(dtype)) == 0 && aligned16(out) && aligned16(out_lo);
     a.per_split = range_of(Lk, a.splits);
     const int rc = p.rows_path ? cross_rows_fwd(a, dtype, st) : cross_tiles_fwd(a, p, dtype, st);
     return rc != SNAG_OK || a.splits == 1 ? rc : cross_combine(a, dtype, st);
@@ -112,7 +112,7 @@ extern "C" SNAG_API int snag_cross_fwd(const void* q, const void* k, const void*
 
 extern "C" SNAG_API int snag_cross_bwd(const void* q, const void* k, const void* v, int dtype, int B, int Lq, int Lk, int H, int Hkv, int d,
                                        const int64_t* strides_host, const void* kv_lens, int lens_bytes, const uint8_t* key_mask, int64_t mask_ld, float scale,
-                                       const void* out, const float* lse, const void* d_out, void* d_q, void* d_k, void* d_v,
+                                       const void* out, const void* out_lo, const float* lse, const void* d_out, void* d_q, void* d_k, void* d_v,
                                        float* work, int64_t work_floats, void* stream) {
     CrossArgs a{};
     if (int rc = cross_args(a, q, k, v, dtype, B, Lq, Lk, H, Hkv, d, strides_host, kv_lens, lens_bytes, key_mask, mask_ld, scale)) return rc;
@@ -123,8 +123,8 @@ extern "C" SNAG_API int snag_cross_bwd(const void* q, const void* k, const void*
     const int64_t need = snag_cross_work_floats(dtype, B, Lq, Lk, H, Hkv, d, 1);
     SNAG_REQUIRE(need == 0 || (work != nullptr && work_floats >= need), SNAG_ERR_ARG, "cross attention backward: workspace of %lld floats, %lld needed", (long long)work_floats, (long long)need);
     hipStream_t st = (hipStream_t)stream;
-    a.o = out, a.lse = (float*)lse, a.dout = d_out, a.dq = d_q, a.dk = d_k, a.dv = d_v;
-    a.vec_o = d % (16 / elem_size(dtype)) == 0 && aligned16(out) && aligned16(d_out) && aligned16(d_q) && aligned16(d_k) && aligned16(d_v);
+    a.o = out, a.o_lo = out_lo, a.lse = (float*)lse, a.dout = d_out, a.dq = d_q, a.dk = d_k, a.dv = d_v;
+    a.vec_o = d % (16 / elem_size(dtype)) == 0 && aligned16(out) && aligned16(out_lo) && aligned16(d_out) && aligned16(d_q) && aligned16(d_k) && aligned16(d_v);
     a.part = work + stat_floats(p, B, Lq, H, Hkv);
     if (p.rows_path && Lq > 0) {
         a.splits = p.s_dq;

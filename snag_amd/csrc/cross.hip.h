@@ -24,13 +24,13 @@ struct CrossArgs {
     int64_t mask_ld;
     float scale, c2;             // c2 = scale * log2(e)
     int vec_q, vec_k, vec_v;     // 16-byte loads legal for this operand
-    void* out;                   // [B, Lq, H, d] dense
+    void *out, *out_lo;          // [B, Lq, H, d] dense; out_lo: what rounding to a 16-bit out dropped, or NULL
     float* lse;                  // [B, H, Lq]: log2 of the row's sum of exp2(c2 q.k); -inf for a row that sees no key
     int splits;                  // key ranges (forward, d q) or row ranges (d k, d v) worked on by different workgroups
     int per_split;               // keys / rows per range, a multiple of 64
     float* part;                 // splits > 1: partial results, see the kernels
     // backward
-    const void *o, *dout;        // [B, Lq, H, d] dense
+    const void *o, *o_lo, *dout; // [B, Lq, H, d] dense; o_lo or NULL
     const float* stat;           // [B, Hkv, padded_rows(rows)][2] = lse (+inf: no key seen), sum_d dout * o
     void *dq, *dk, *dv;          // dense, shapes of q, k, v
     int vec_o;                   // 16-byte access legal for the dense tensors (d a multiple of the chunk, aligned bases)

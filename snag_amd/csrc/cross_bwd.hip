@@ -22,8 +22,10 @@ __global__ __launch_bounds__(256) void cross_stat_kernel(CrossArgs a, float* __r
         for (int col = t * C; col < a.d; col += 16 * C) {
             const auto x = load_chunk<T>((const T*)a.o + dense, col, a.d, true, a.vec_o);
             const auto y = load_chunk<T>((const T*)a.dout + dense, col, a.d, true, a.vec_o);
+            typename Chunk<T>::vec w{};
+            if (a.o_lo != nullptr) w = load_chunk<T>((const T*)a.o_lo + dense, col, a.d, true, a.vec_o);
 #pragma unroll
-            for (int j = 0; j < C; ++j) s = fmaf((float)x[j], (float)y[j], s);
+            for (int j = 0; j < C; ++j) s = fmaf((float)x[j] + (float)w[j], (float)y[j], s);
         }
     s = sum16(s);
     if (at < n && t == 0) {

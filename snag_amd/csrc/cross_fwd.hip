@@ -122,7 +122,8 @@ __global__ __launch_bounds__(NW * 64, NW == 1 || (sizeof(T) == 4 && DP == 128) ?
         }
         return;
     }
-    store_row<T, DP>((T*)a.out + (((int64_t)b * a.Lq + l) * a.H + head) * a.d, acc, sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum), a.d, lane);
+    const int64_t dense = (((int64_t)b * a.Lq + l) * a.H + head) * a.d;
+    store_row<T, DP>((T*)a.out + dense, acc, sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum), a.d, lane, a.out_lo != nullptr ? (T*)a.out_lo + dense : nullptr);
     if (h == 0) a.lse[at] = sum == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(sum);
 }
 
@@ -150,11 +151,16 @@ __global__ __launch_bounds__(256) void cross_combine_kernel(CrossArgs a) {
         }
     }
     const int64_t l = at % a.Lq, bh = at / a.Lq, head = bh % a.H, b = bh / a.H;
-    T* out = (T*)a.out + ((b * a.Lq + l) * a.H + head) * a.d;
+    const int64_t dense = ((b * a.Lq + l) * a.H + head) * a.d;
+    T* out = (T*)a.out + dense;
     const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
 #pragma unroll
     for (int u = 0; u < 2; ++u)
-        if (lane + 64 * u < a.d) out[lane + 64 * u] = (T)(o[u] * inv);
+        if (lane + 64 * u < a.d) {
+            const T v = (T)(o[u] * inv);
+            out[lane + 64 * u] = v;
+            if (a.out_lo != nullptr) ((T*)a.out_lo)[dense + lane + 64 * u] = (T)(o[u] * inv - (float)v);
+        }
     if (lane == 0) a.lse[at] = sum == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(sum);
 }
 

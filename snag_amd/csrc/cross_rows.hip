@@ -77,6 +77,17 @@ __device__ __forceinline__ bool rows_key_seen(const CrossArgs& a, int b, int key
     return key < len && (a.mask == nullptr || a.mask[(int64_t)b * a.mask_ld + key] != 0);
 }
 
+template <class T>
+__device__ __forceinline__ void store_chunk(T* row, int col, int d, int vec, typename Chunk<T>::vec c) {
+    if (vec && col < d) {
+        *(typename Chunk<T>::vec*)(row + col) = c;
+    } else {
+#pragma unroll
+        for (int j = 0; j < Chunk<T>::n; ++j)
+            if (col + j < d) row[col + j] = c[j];
+    }
+}
+
 template <class T, int DP, int R>
 __global__ __launch_bounds__(1024) void cross_rows_fwd_kernel(CrossArgs a, int W) {
     constexpr int C = Chunk<T>::n, LPK = DP / C, NK = 64 / LPK, U = 4;
@@ -180,7 +191,11 @@ __global__ __launch_bounds__(1024) void cross_rows_fwd_kernel(CrossArgs a, int W
                 float* ml = a.part + (int64_t)a.splits * n * a.d + (it.split * n + at) * 2;
                 if (c == 0) ml[0] = mn, ml[1] = s;
             } else {
-                ((T*)a.out)[(((int64_t)it.b * a.Lq + l) * a.H + head) * a.d + c] = (T)(o * (s > 0.f ? 1.f / s : (s == 0.f ? 0.f : s)));
+                const int64_t dense = (((int64_t)it.b * a.Lq + l) * a.H + head) * a.d + c;
+                const float x = o * (s > 0.f ? 1.f / s : (s == 0.f ? 0.f : s));
+                const T v = (T)x;
+                ((T*)a.out)[dense] = v;
+                if (a.out_lo != nullptr) ((T*)a.out_lo)[dense] = (T)(x - (float)v);
                 if (c == 0) a.lse[at] = s == 0.f ? -INFINITY : mn + __builtin_amdgcn_logf(s);
             }
         }
@@ -205,29 +220,13 @@ __global__ __launch_bounds__(1024) void cross_rows_fwd_kernel(CrossArgs a, int W
             continue;
         }
         const float inv = sum[r] > 0.f ? 1.f / sum[r] : (sum[r] == 0.f ? 0.f : sum[r]);
-        T* o = (T*)a.out + (((int64_t)it.b * a.Lq + l) * a.H + head) * a.d;
-        typename Chunk<T>::vec c;
+        const int64_t dense = (((int64_t)it.b * a.Lq + l) * a.H + head) * a.d;
+        typename Chunk<T>::vec c, e;
 #pragma unroll
-        for (int j = 0; j < C; ++j) c[j] = (T)(acc[r][j] * inv);
-        if (a.vec_o && col < a.d) {
-            *(typename Chunk<T>::vec*)(o + col) = c;
-        } else {
-#pragma unroll
-            for (int j = 0; j < C; ++j)
-                if (col + j < a.d) o[col + j] = c[j];
-        }
+        for (int j = 0; j < C; ++j) c[j] = (T)(acc[r][j] * inv), e[j] = (T)(acc[r][j] * inv - (float)c[j]);
+        store_chunk<T>((T*)a.out + dense, col, a.d, a.vec_o, c);
+        if (a.out_lo != nullptr) store_chunk<T>((T*)a.out_lo + dense, col, a.d, a.vec_o, e);
         if (col == 0) a.lse[at] = sum[r] == 0.f ? -INFINITY : m[r] + __builtin_amdgcn_logf(sum[r]);
-    }
-}
-
-template <class T>
-__device__ __forceinline__ void store_chunk(T* row, int col, int d, int vec, typename Chunk<T>::vec c) {
-    if (vec && col < d) {
-        *(typename Chunk<T>::vec*)(row + col) = c;
-    } else {
-#pragma unroll
-        for (int j = 0; j < Chunk<T>::n; ++j)
-            if (col + j < d) row[col + j] = c[j];
     }
 }
 
@@ -247,9 +246,11 @@ __global__ __launch_bounds__(512) void cross_rows_bwd_kernel(CrossArgs a, int W)
         const auto c = load_chunk<T>((const T*)a.q + it.b * a.qsb + l * a.qsl + head * a.qsh, col, a.d, ok, a.vec_q);
         const auto e = load_chunk<T>((const T*)a.dout + dense, col, a.d, ok, a.vec_o);
         const auto f = load_chunk<T>((const T*)a.o + dense, col, a.d, ok, a.vec_o);
+        typename Chunk<T>::vec w{};
+        if (a.o_lo != nullptr) w = load_chunk<T>((const T*)a.o_lo + dense, col, a.d, ok, a.vec_o);
         float t = 0.f;
 #pragma unroll
-        for (int j = 0; j < C; ++j) q[r][j] = (float)c[j], g[r][j] = (float)e[j], t = fmaf((float)e[j], (float)f[j], t), dq[r][j] = 0.f;
+        for (int j = 0; j < C; ++j) q[r][j] = (float)c[j], g[r][j] = (float)e[j], t = fmaf((float)e[j], (float)f[j] + (float)w[j], t), dq[r][j] = 0.f;
         delta[r] = group_sum<LPK>(t);
         const float s = ok ? a.lse[((int64_t)it.b * a.H + head) * a.Lq + l] : INFINITY;
         lse[r] = s == -INFINITY ? INFINITY : s;   // a row that sees no key: every p is 0

@@ -171,8 +171,9 @@ __device__ __forceinline__ void tile_ready() {
 }
 
 // Writes a transposed accumulator (rows = elements, column = the lane's row): 4 neighbouring elements per register quad.
+// lo (or NULL): the same place for what the rounding dropped.
 template <class T, int DP>
-__device__ __forceinline__ void store_row(T* row, const f32x16 (&acc)[DP / 32], float scale, int d, int lane) {
+__device__ __forceinline__ void store_row(T* row, const f32x16 (&acc)[DP / 32], float scale, int d, int lane, T* lo = nullptr) {
     const int h = lane >> 5;
     using V4 = __attribute__((ext_vector_type(4))) T;
     typedef V4 any4 __attribute__((aligned(sizeof(T))));
@@ -181,15 +182,19 @@ __device__ __forceinline__ void store_row(T* row, const f32x16 (&acc)[DP / 32], 
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int col = db * 32 + g * 8 + h * 4;
-            V4 v;
+            V4 v, w;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = (T)(acc[db][4 * g + j] * scale);
+            for (int j = 0; j < 4; ++j) v[j] = (T)(acc[db][4 * g + j] * scale), w[j] = (T)(acc[db][4 * g + j] * scale - (float)v[j]);
             if (col + 4 <= d) {
                 *(any4*)(row + col) = v;
+                if (lo != nullptr) *(any4*)(lo + col) = w;
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (col + j < d) row[col + j] = v[j];
+                    if (col + j < d) {
+                        row[col + j] = v[j];
+                        if (lo != nullptr) lo[col + j] = w[j];
+                    }
             }
         }
 }

@@ -640,41 +640,35 @@ def _cross_work(shape, backward, device):
     return (torch.empty(n, device=device, dtype=f32) if n else None), n
 
 
-def cross_attention_fwd(q, k, v, kv_lens=None, key_mask=None, scale=None):
-    """q [B, Lq, H, d], k / v [B, Lk, Hkv, d] (any strides with adjacent head elements) -> out [B, Lq, H, d], lse [B, H, Lq] (log2).
-    C ABI: snag_cross_fwd."""
-    return _cross_fwd(q, *_cross_args(q, k, v, kv_lens, key_mask, scale))
-
-
-def _cross_fwd(q, shape, args, hold):
+def cross_attention_fwd(q, k, v, kv_lens=None, key_mask=None, scale=None, want_residual=False):
+    """q [B, Lq, H, d], k / v [B, Lk, Hkv, d] (any strides with adjacent head elements) -> out [B, Lq, H, d], lse [B, H, Lq] (log2), and with
+    ``want_residual`` what the rounding of a 16-bit out dropped (None for fp32), for the backward.  C ABI: snag_cross_fwd."""
+    shape, args, hold = _cross_args(q, k, v, kv_lens, key_mask, scale)
     out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    lo = torch.empty_like(out) if want_residual and q.dtype != f32 else None
     lse = torch.empty((shape[1], shape[4], shape[2]), device=q.device, dtype=f32)
     work, n = _cross_work(shape, False, q.device)
-    _call_on(q.device, "snag_cross_fwd", *args, ptr(out), ptr(lse), ptr(work), n)
-    return out, lse
+    _call_on(q.device, "snag_cross_fwd", *args, ptr(out), ptr(lo), ptr(lse), ptr(work), n)
+    return (out, lse, lo) if want_residual else (out, lse)
 
 
-def _cross_bwd(args, shape, like, out, lse, d_out):
-    """The launch itself, of arguments that have been checked."""
-    q, k, v = like
-    dq, dk, dv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in like)
-    work, n = _cross_work(shape, True, q.device)
-    _call_on(q.device, "snag_cross_bwd", *args, ptr(out), ptr(lse), ptr(d_out), ptr(dq), ptr(dk), ptr(dv), ptr(work), n)
-    return dq, dk, dv
-
-
-def cross_attention_bwd(q, k, v, out, lse, d_out, kv_lens=None, key_mask=None, scale=None):
+def cross_attention_bwd(q, k, v, out, lse, d_out, kv_lens=None, key_mask=None, scale=None, out_residual=None):
     """-> d_q, d_k, d_v (dense).  C ABI: snag_cross_bwd."""
     shape, args, hold = _cross_args(q, k, v, kv_lens, key_mask, scale)
-    for t, name in ((out, "out"), (d_out, "d_out")):
+    for t, name in ((out, "out"), (d_out, "d_out"), (out_residual, "out_residual")):
+        if t is None and name == "out_residual":
+            continue
         _chk(t, name, dtype=q.dtype, ndim=4)
         if t.shape != q.shape:
             raise ValueError(f"{name} must be {tuple(q.shape)}, got {tuple(t.shape)}")
     _chk(lse, "lse", ndim=3)
     if tuple(lse.shape) != (q.shape[0], q.shape[2], q.shape[1]):
         raise ValueError(f"lse must be [B, H, Lq], got {tuple(lse.shape)}")
-    _one_device(q.device, out=out, lse=lse, d_out=d_out)
-    return _cross_bwd(args, shape, (q, k, v), out, lse, d_out)
+    _one_device(q.device, out=out, lse=lse, d_out=d_out, out_residual=out_residual)
+    dq, dk, dv = (torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k, v))
+    work, n = _cross_work(shape, True, q.device)
+    _call_on(q.device, "snag_cross_bwd", *args, ptr(out), ptr(out_residual), ptr(lse), ptr(d_out), ptr(dq), ptr(dk), ptr(dv), ptr(work), n)
+    return dq, dk, dv
 
 
 @functools.lru_cache(maxsize=4096)

@@ -18,7 +18,7 @@ def _lib():
 def _fwd(dtype=1, B=2, Lq=3, Lk=5, H=4, Hkv=2, d=64, q=P, k=P, v=P, strides=True, lens=None, lens_bytes=4, mask=None, mask_ld=0, scale=0.125, out=P, lse=P, work=None, floats=0):
     lib, L = _lib()
     s = (ctypes.c_int64 * 9)(*([64] * 9))
-    rc = lib.snag_cross_fwd(q, k, v, dtype, B, Lq, Lk, H, Hkv, d, ctypes.addressof(s) if strides else None, lens, lens_bytes, mask, mask_ld, scale, out, lse, work, floats, None)
+    rc = lib.snag_cross_fwd(q, k, v, dtype, B, Lq, Lk, H, Hkv, d, ctypes.addressof(s) if strides else None, lens, lens_bytes, mask, mask_ld, scale, out, None, lse, work, floats, None)
     return rc, L.last_error()
 
 
@@ -39,7 +39,7 @@ def test_cross_attention_backward_refusals():
     s = (ctypes.c_int64 * 9)(*([64] * 9))
 
     def bwd(out=P, lse=P, do=P, dq=P, dk=P, dv=P, work=None, floats=0):
-        return lib.snag_cross_bwd(P, P, P, 1, 2, 3, 5, 4, 2, 64, ctypes.addressof(s), None, 4, None, 0, 0.1, out, lse, do, dq, dk, dv, work, floats, None), L.last_error()
+        return lib.snag_cross_bwd(P, P, P, 1, 2, 3, 5, 4, 2, 64, ctypes.addressof(s), None, 4, None, 0, 0.1, out, None, lse, do, dq, dk, dv, work, floats, None), L.last_error()
 
     for change in ("out", "lse", "do", "dq", "dk", "dv"):
         rc, text = bwd(**{change: None})

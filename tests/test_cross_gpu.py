@@ -3,7 +3,7 @@ those of cross_reference.attention_bounds: every rounding counted at half a step
 import pytest
 import torch
 
-from cross_reference import attention, attention_bounds
+from cross_reference import attention, attention_bounds, half_step
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -23,8 +23,8 @@ def make(B, Lq, Lk, H, Hkv, d, dtype, seed=0):
 
 def check(q, k, v, do, lens=None, mask=None, scale=None, what=""):
     from snag_amd import ops
-    out, lse = ops.cross_attention_fwd(q, k, v, lens, mask, scale)
-    grads = ops.cross_attention_bwd(q, k, v, out, lse, do, lens, mask, scale)
+    out, lse, lo = ops.cross_attention_fwd(q, k, v, lens, mask, scale, want_residual=True)
+    grads = ops.cross_attention_bwd(q, k, v, out, lse, do, lens, mask, scale, lo)
     r = attention(q, k, v, lens, mask, scale, do)
     b = attention_bounds(q, k, v, lens, mask, scale, do, r)
     for name, t in (("o", out), ("dq", grads[0]), ("dk", grads[1]), ("dv", grads[2])):
@@ -86,8 +86,8 @@ def test_strides_and_alignment(rows, dtype):
     mask = (torch.rand(B, 2 * Lk, generator=g, device=DEV) < 0.7)[:, 3:3 + Lk]
     for k, v in ((kv[:, :, 0], kv[:, :, 1]), (odd, kv[:, :, 1]), (wide, odd), (shared, wide)):
         out, (dq, dk, dv), _ = check(q, k, v, do, None, mask, what="strided")
-        o2, l2 = ops.cross_attention_fwd(q.contiguous(), k.contiguous(), v.contiguous(), None, mask.contiguous())
-        g2 = ops.cross_attention_bwd(q.contiguous(), k.contiguous(), v.contiguous(), o2, l2, do, None, mask.contiguous())
+        o2, l2, lo = ops.cross_attention_fwd(q.contiguous(), k.contiguous(), v.contiguous(), None, mask.contiguous(), want_residual=True)
+        g2 = ops.cross_attention_bwd(q.contiguous(), k.contiguous(), v.contiguous(), o2, l2, do, None, mask.contiguous(), out_residual=lo)
         assert torch.equal(out, o2) and all(torch.equal(a, b) for a, b in zip((dq, dk, dv), g2))
 
 
@@ -99,6 +99,23 @@ def test_large_scores_and_scale(rows, dtype):
     check(q * 8, k * 4, v, do, what="large")
     check(q, k, v, do, scale=0.5, what="scale")
     check(q, k, v, do, scale=1e-4, what="flat")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [2, 40])
+@pytest.mark.parametrize("Lk", [1, 2, 3])
+def test_few_keys_keep_their_gradient(Lk, rows, dtype):
+    """Where p (do v^T - delta) cancels, the output's rounding must not reach delta: with the residual the gradients keep the type's precision.
+    (Every rounding in the chain -- p or ds, q, k, the result -- is half a step; four of them, and the cancellation of fp32 sums.)"""
+    from snag_amd import ops
+    q, k, v, do = make(64, rows, Lk, 2, 2, 64, dtype, seed=8)
+    out, lse, lo = ops.cross_attention_fwd(q, k, v, want_residual=True)
+    got = ops.cross_attention_bwd(q, k, v, out, lse, do, out_residual=lo)
+    r = attention(q, k, v, d_out=do)
+    for name, t in zip(("dq", "dk", "dv"), got):
+        off, size = float((t.double() - r[name]).norm()), float(r[name].norm())
+        floor = 64 * 2.0 ** -24 * float(attention(q.abs(), k.abs(), v.abs(), d_out=do.abs())[name].norm() + do.double().norm() * v.double().norm() / 8)
+        assert off <= 2 * half_step(dtype) * size + floor, (name, off, size, floor)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
