@@ -45,12 +45,11 @@ struct MuonMatrix {
     int r, c, m, n, mp, np;  // shape; m <= n; both rounded up to whole tiles
     int tall, splits;        // A is summed from `splits` ranges of n
     float update;            // lr * s
-    int pad;
+    int vec;                 // rows of g, mom and the result start 16-byte aligned
 };
 // What every launch needs, in device memory: kernel arguments lie in host memory, and a launch of a few workgroups spent most of its time on
 // the chain of reads that finds its matrix (15 us for one tile).  The first launch of an update writes it.
 struct MuonTable {
-    int first[3][kMaxList];  // first workgroup of a matrix in a product launch (A, B, X)
     int count, dtype, step, nesterov;
     float mu, keep, eps;     // keep = 1 - lr * decay
     int pad;
@@ -148,28 +147,59 @@ __global__ __launch_bounds__(256) void muon_start_kernel(const MuonTable* __rest
     __syncthreads();
     const double norm = sqrt(red[0] + red[1] + red[2] + red[3]) + (double)L->eps;
     const double inv = (double)kScaleX / norm;     // beyond fp32's range for tiny gradients
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int u = threadIdx.x >> 4, v = (threadIdx.x & 15) * 4;     // a thread's row (of 16 a turn) and first of its four columns
     _Float16 *xh = x_plane(a, 0, 0), *xl = x_plane(a, 0, 1);
-    auto u_at = [&](int r, int c) {
-        if (r >= a.r || c >= a.c) return 0.f;
+    auto four = [&](int r, int c, float (&x)[4]) {                  // elements (r, c) .. (r, c + 3) of X, or of its transpose
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = 0.f;
+        if (r >= a.r || c >= a.c) return;
         const int64_t at = (int64_t)r * a.c + c;
-        float v = value<T>(a.g, at);
-        if (step) v = update_of(nesterov, mu, v, a.mom[at]);
-        return (float)((double)v * inv);
+        if (a.vec) {                                                // c + 4 <= a.c: both are multiples of four
+            using V = __attribute__((ext_vector_type(4))) T;
+            const V g = *(const V*)((const T*)a.g + at);
+            f32x4 m{};
+            if (step) m = *(const f32x4*)(a.mom + at);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = step ? update_of(nesterov, mu, (float)g[j], m[j]) : (float)g[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (c + j < a.c) x[j] = step ? update_of(nesterov, mu, value<T>(a.g, at + j), a.mom[at + j]) : value<T>(a.g, at + j);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = (float)((double)x[j] * inv);
     };
     for (int blk = blockIdx.x; blk < blocks; blk += gridDim.x) {
         const int i0 = blk / cols * 64, j0 = blk % cols * 64;       // rows and columns of X
+        float x[4];
         if (a.tall) {
             __syncthreads();
-            for (int u = wave; u < 64; u += 4) tile[u][lane] = u_at(j0 + u, i0 + lane);
+#pragma unroll
+            for (int w = 0; w < 64; w += 16) {
+                four(j0 + w + u, i0 + v, x);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) tile[w + u][v + j] = x[j];
+            }
             __syncthreads();
         }
-        for (int u = wave; u < 64; u += 4) {
-            const int64_t at = (int64_t)(i0 + u) * a.np + j0 + lane;
-            _Float16 hi, lo;
-            split16(a.tall ? tile[lane][u] : u_at(i0 + u, j0 + lane), hi, lo);
-            xh[at] = hi;
-            xl[at] = lo;
+#pragma unroll
+        for (int w = 0; w < 64; w += 16) {
+            if (a.tall) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] = tile[v + j][w + u];
+            } else {
+                four(i0 + w + u, j0 + v, x);
+            }
+            f16x4 hi, lo;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                _Float16 p, q;
+                split16(x[j], p, q);
+                hi[j] = p, lo[j] = q;
+            }
+            const int64_t at = (int64_t)(i0 + w + u) * a.np + j0 + v;
+            *(f16x4*)(xh + at) = hi;
+            *(f16x4*)(xl + at) = lo;
         }
     }
 }
@@ -177,11 +207,12 @@ __global__ __launch_bounds__(256) void muon_start_kernel(const MuonTable* __rest
 // ---- products -------------------------------------------------------------------------------------------------------------
 enum { kGram, kPoly, kApply };
 
-// Two workgroup shapes: 4 waves on a 128 x 128 tile (64 x 64 a wave), 8 waves on a 256 x 256 tile (128 x 64 a wave); 64 / PLANES of the contraction
-// per LDS stage, NST stages.
+// Workgroup shapes: a 128 x 128 tile by 4 waves of 64 x 64 (two stages: two workgroups a CU) or by 8 waves of 64 x 32 (four stages: one a CU, two
+// waves a SIMD hide each other's waits), a 256 x 256 tile by 8 waves of 128 x 64.  64 / PLANES of the contraction per LDS stage, NST stages.
+constexpr int threads_of(int tile, int nst) { return tile == 128 && nst == 2 ? 256 : 512; }
 template <int TILE, int PLANES, int NST> struct Shape {
-    static constexpr int kWaves = TILE == 128 ? 4 : 8, kThreads = kWaves * 64;
-    static constexpr int kWm = TILE / 2, kWn = 64;                     // a wave's part
+    static constexpr int kThreads = threads_of(TILE, NST), kWaves = kThreads / 64;
+    static constexpr int kWm = TILE / 2, kWn = TILE * 2 / kWaves;      // a wave's part
     static constexpr int kDepth = 64 / PLANES, kChunks = kDepth / 8;   // 16-byte chunks per row of a stage
     static constexpr int kOperand = TILE * kDepth, kStage = 2 * PLANES * kOperand;     // fp16 values
     static constexpr int kLoads = kStage / 8 / kThreads;               // 16-byte loads of a thread per stage
@@ -221,11 +252,15 @@ __device__ __forceinline__ void rect_at(int k, int t, int u, int& i, int& j) {  
     j = J * kSquare + k / rows;
 }
 
-// the matrix a workgroup belongs to: one parallel look at the table's first[] and a vote
-__device__ __forceinline__ int matrix_of(const int* __restrict__ first, int count, int id) {
-    const int lane = threadIdx.x & 63;
-    const bool before = lane < count && first[lane < kMaxList ? lane : 0] <= id;
-    return __builtin_amdgcn_readfirstlane((int)__popcll(__ballot(before)) - 1);
+// First workgroup of every matrix in a launch (INT_MAX behind the list's end): a kernel argument, so that finding its matrix costs a workgroup no read
+// of its own in front of the read of the matrix.
+struct MuonFirst { int at[kMaxList]; };
+__device__ __forceinline__ int matrix_of(const MuonFirst& first, int id, int& begin) {
+    int which = 0;
+    begin = first.at[0];
+#pragma unroll
+    for (int i = 1; i < kMaxList; ++i) which = id >= first.at[i] ? i : which, begin = id >= first.at[i] ? first.at[i] : begin;
+    return __builtin_amdgcn_readfirstlane(which);
 }
 
 // one 16-byte chunk per lane straight from global memory into LDS: the wave's 64 chunks land at lds, in lane order
@@ -296,9 +331,9 @@ __device__ __forceinline__ void store_pairs(_Float16* hi, _Float16* lo, const Pa
 }
 
 // What a 32 x 32 block of the product becomes.  acc: register i of lane (h, l) = element (row0 + 8 (i / 4) + 4 h + i % 4, col0 + l).  The block goes
-// through this wave's own piece of LDS (32 rows of kPitch floats), so that a lane holds 16 neighbours of one row and everything moves 16 bytes at
+// through this wave's own piece of LDS (32 rows of kPitch floats, whole 16-byte steps), so that a lane holds 16 neighbours of one row and everything moves 16 bytes at
 // a time; a tall result and the mirror image take 16 neighbours of one column instead.
-constexpr int kPitch = 33;
+constexpr int kPitch = 36;
 // LDS keeps a wave's accesses in order; this keeps the compiler from moving one lane's reads in front of another's writes
 __device__ __forceinline__ void lds_turn() { asm volatile("" ::: "memory"); }
 // what a block needs of memory: X (APPLY) or the off-diagonal part of A (POLY) where it lies
@@ -309,14 +344,39 @@ __device__ __forceinline__ Pairs block_pairs(const MuonMatrix& a, int row0, int 
     if (MODE == kPoly) return load_pairs(s_plane(a, 0) + (int64_t)row * a.mp + col, s_plane(a, 1) + (int64_t)row * a.mp + col);
     return Pairs{};
 }
+// the accumulators through LDS: lane (r, c) gets columns c .. c + 15 of row r
+__device__ __forceinline__ void through_block(float* block, const f32x16& acc, float (&v)[16], int lane) {
+    const int h = lane >> 5, r = lane >> 1, c = (lane & 1) * 16;
+    lds_turn();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) block[(8 * (i >> 2) + 4 * h + (i & 3)) * kPitch + (lane & 31)] = acc[i];
+    lds_turn();
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const f32x4 x = *(const f32x4*)(block + r * kPitch + c + 4 * q);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[4 * q + j] = x[j];
+    }
+}
 // values of 16 neighbours of a row become 16 neighbours of a column: lane (r, c) gets rows c .. c + 15 of column r
 __device__ __forceinline__ void turn(float* block, float (&v)[16], int r, int c) {
     lds_turn();
 #pragma unroll
-    for (int j = 0; j < 16; ++j) block[r * kPitch + c + j] = v[j];
+    for (int q = 0; q < 4; ++q) *(f32x4*)(block + r * kPitch + c + 4 * q) = f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
     lds_turn();
 #pragma unroll
     for (int j = 0; j < 16; ++j) v[j] = block[(c + j) * kPitch + r];
+}
+// element `at` (0 .. 15, else nothing) of v: its value; set to 0
+__device__ __forceinline__ void clear(float (&v)[16], int at) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = j == at ? 0.f : v[j];
+}
+__device__ __forceinline__ float pick(const float (&v)[16], int at) {
+    float x = 0.f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) x = j == at ? v[j] : x;
+    return x;
 }
 // the last iteration's 16 values of X (row, col ..; times 2^14) into the user's matrix
 template <class T>
@@ -334,7 +394,7 @@ __device__ __forceinline__ void store_result(const MuonTable* __restrict__ L, co
     constexpr int C = Chunk<T>::n;
     const int step = L->step;
     const float keep = L->keep;
-    if (j0 + 16 <= a.c && a.c % C == 0 && ((uintptr_t)a.w & 15) == 0) {
+    if (j0 + 16 <= a.c && a.vec) {
 #pragma unroll
         for (int q = 0; q < 16 / C; ++q) {
             V o;
@@ -356,49 +416,64 @@ __device__ __forceinline__ void store_result(const MuonTable* __restrict__ L, co
     }
 }
 
+// B from A: v in: A^2's off-diagonal share times 2^26, out: B without its diagonal times 2^13; p: A's off-diagonal part; -> B's diagonal where `at` is on it
+// (on: the block has a piece of the diagonal)
+__device__ __forceinline__ float poly(float (&v)[16], const Pairs& p, float di, const float (&dj)[16], int at, bool on) {
+    const float sq = on ? pick(v, at) * (1.f / (kScaleA * kScaleA)) : 0.f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = fmaf(fmaf(kNsC, di + dj[j], kNsB), sum_of(p, j), v[j] * (kNsC / kScaleA));
+    if (on) clear(v, at);
+    return fmaf(kNsB, di, kNsC * fmaf(di, di, sq));
+}
+__device__ __forceinline__ void load16(float (&v)[16], const float* p) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const f32x4 x = *(const f32x4*)(p + 4 * q);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[4 * q + j] = x[j];
+    }
+}
+
+// the diagonals a block needs: of its row (APPLY: B's, POLY: A's), and of its columns (POLY)
+struct Diagonals { float row, col[16]; };
+template <int MODE>
+__device__ __forceinline__ Diagonals block_diagonals(const MuonMatrix& a, int row0, int col0, int lane) {
+    Diagonals d{};
+    if (MODE != kGram) d.row = diagonal(a, MODE == kApply ? 1 : 0)[row0 + (lane >> 1)];
+    if (MODE == kPoly) load16(d.col, diagonal(a, 0) + col0 + (lane & 1) * 16);
+    return d;
+}
+
 template <int MODE, int DT>
-__device__ __forceinline__ void finish(const MuonTable* __restrict__ L, const MuonMatrix& a, const f32x16& acc, const Pairs& p, int row0, int col0, bool mirror, int from, bool last, float* block, int lane) {
-    const int h = lane >> 5, r = lane >> 1, c = (lane & 1) * 16;           // row r, columns c .. c + 15 of the block
-    lds_turn();
-#pragma unroll
-    for (int i = 0; i < 16; ++i) block[(8 * (i >> 2) + 4 * h + (i & 3)) * kPitch + (lane & 31)] = acc[i];
-    lds_turn();
+__device__ __forceinline__ void finish(const MuonTable* __restrict__ L, const MuonMatrix& a, const f32x16& acc, const Pairs& p, const Diagonals& g, int row0, int col0, bool mirror, int from, bool last,
+                                       float* block, int lane) {
+    const int r = lane >> 1, c = (lane & 1) * 16;                          // row r, columns c .. c + 15 of the block
+    const int row = row0 + r, col = col0 + c, at = row - col;
     float v[16];
-    const int row = row0 + r, col = col0 + c;
+    through_block(block, acc, v, lane);
     if constexpr (MODE == kApply) {
-        const float d = kNsA + diagonal(a, 1)[row];
+        const float d = kNsA + g.row;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = fmaf(d, sum_of(p, j), block[r * kPitch + c + j] * (1.f / kScaleA));            // times 2^14
+        for (int j = 0; j < 16; ++j) v[j] = fmaf(d, sum_of(p, j), v[j] * (1.f / kScaleA));                                 // times 2^14
         if (last) store_result<TypeOf<DT>>(L, a, v, row0, col0, block, lane);
         else store_pairs(x_plane(a, from ^ 1, 0) + (int64_t)row * a.np + col, x_plane(a, from ^ 1, 1) + (int64_t)row * a.np + col, pairs_of(v));
     } else {
         _Float16 *oh = s_plane(a, MODE == kGram ? 0 : 2), *ol = s_plane(a, MODE == kGram ? 1 : 3);
-        float* diag = diagonal(a, MODE == kGram ? 0 : 1);
+        float d;
         if constexpr (MODE == kGram) {
+            d = pick(v, at) * (1.f / (kScaleX * kScaleX));
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                v[j] = block[r * kPitch + c + j] * (1.f / (kScaleX * kScaleX));
-                if (row == col + j) diag[row] = v[j], v[j] = 0.f;
-                v[j] *= kScaleA;
-            }
+            for (int j = 0; j < 16; ++j) v[j] *= kScaleA / (kScaleX * kScaleX);
+            if (row0 == col0) clear(v, at);
         } else {
-            const float* da = diagonal(a, 0);
-            const float di = da[row];
-            float dj[16];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) *(f32x4*)(dj + 4 * q) = *(const f32x4*)(da + col + 4 * q);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const float sq = block[r * kPitch + c + j] * (1.f / kScaleA);                                              // times 2^13
-                v[j] = fmaf(fmaf(kNsC, di + dj[j], kNsB), sum_of(p, j), kNsC * sq);
-                if (row == col + j) diag[row] = fmaf(kNsB, di, kNsC * fmaf(di, di, sq * (1.f / kScaleA))), v[j] = 0.f;
-            }
+            d = poly(v, p, g.row, g.col, at, row0 == col0);
         }
+        if (at >= 0 && at < 16) diagonal(a, MODE == kGram ? 0 : 1)[row] = d;
         store_pairs(oh + (int64_t)row * a.mp + col, ol + (int64_t)row * a.mp + col, pairs_of(v));
         if (mirror) {
             turn(block, v, r, c);
-            const int64_t at = (int64_t)(col0 + r) * a.mp + row0 + c;
-            store_pairs(oh + at, ol + at, pairs_of(v));
+            const int64_t to = (int64_t)(col0 + r) * a.mp + row0 + c;
+            store_pairs(oh + to, ol + to, pairs_of(v));
         }
     }
 }
@@ -407,7 +482,7 @@ __device__ __forceinline__ void finish(const MuonTable* __restrict__ L, const Mu
 // contraction are read while the present ones are multiplied, across the stages too: the barrier that opens a stage stands in front of the
 // last products of the stage before it.
 template <int MODE, int DT, int TILE, int NST>
-__global__ __launch_bounds__(TILE == 128 ? 256 : 512, NST == 2 ? 2 : 1) void muon_product_kernel(const MuonTable* __restrict__ L, int from, int last) {
+__global__ __launch_bounds__(threads_of(TILE, NST), 2) void muon_product_kernel(const MuonTable* __restrict__ L, MuonFirst first, int from, int last) {
     constexpr int PLANES = DT == SNAG_BF16 ? 1 : 2;
     using S = Shape<TILE, PLANES, NST>;
     constexpr int NI = S::kWm / 32, NJ = S::kWn / 32, KB = S::kDepth / 16;
@@ -416,9 +491,9 @@ __global__ __launch_bounds__(TILE == 128 ? 256 : 512, NST == 2 ? 2 : 1) void muo
     _Float16* lds = (_Float16*)smem;
     const int lane = threadIdx.x & 63, wave = wave_id_uniform();
     const int id = (int)xcd_order(blockIdx.x, gridDim.x);
-    const int which = matrix_of(L->first[MODE], L->count, id);
-    const MuonMatrix a = L->a[which];
-    int k = id - L->first[MODE][which], split = 0, ti, tj;
+    int begin;
+    const MuonMatrix a = L->a[matrix_of(first, id, begin)];
+    int k = id - begin, split = 0, ti, tj;
     if (MODE == kApply) {
         rect_at(k, a.mp / TILE, a.np / TILE, ti, tj);
     } else {
@@ -460,8 +535,12 @@ __global__ __launch_bounds__(TILE == 128 ? 256 : 512, NST == 2 ? 2 : 1) void muo
     const int wm = (wave / kWavesN) * S::kWm, wn = (wave % kWavesN) * S::kWn;
     // A launch of one workgroup per CU takes its blocks' own values along with the first stages; otherwise they are fetched one block ahead.
     Pairs own[NI * NJ];
+    Diagonals diag[NI * NJ];
     const int i0 = ti * TILE + wm, j0 = tj * TILE + wn;
-    auto fetch = [&](int q) { own[q] = block_pairs<MODE>(a, i0 + q / NJ * 32, j0 + q % NJ * 32, from, lane); };
+    auto fetch = [&](int q) {
+        own[q] = block_pairs<MODE>(a, i0 + q / NJ * 32, j0 + q % NJ * 32, from, lane);
+        diag[q] = block_diagonals<MODE>(a, i0 + q / NJ * 32, j0 + q % NJ * 32, lane);
+    };
     if (NST > 2) {
 #pragma unroll
         for (int q = 0; q < NI * NJ; ++q) fetch(q);
@@ -520,13 +599,13 @@ __global__ __launch_bounds__(TILE == 128 ? 256 : 512, NST == 2 ? 2 : 1) void muo
         }
     }
     if (MODE == kGram && a.splits > 1) {
-        // the range's partial tile, in register order: muon_gram_sum_kernel adds the ranges up
+        // the range's partial tile, 32 x 32 blocks in register order: muon_gram_sum_kernel adds the ranges up
         const int t = a.mp / TILE, tiles = t * (t + 1) / 2;
-        float* out = slab_of(a) + ((int64_t)(split * tiles + k) * S::kWaves + wave) * NI * NJ * 1024 + lane * 16;
+        float* out = slab_of(a) + (int64_t)(split * tiles + k) * 16 * 1024 + lane * 16;
 #pragma unroll
         for (int i = 0; i < NI; ++i)
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) *(f32x16*)(out + (i * NJ + j) * 1024) = acc[i][j];
+            for (int j = 0; j < NJ; ++j) *(f32x16*)(out + ((wm / 32 + i) * 4 + wn / 32 + j) * 1024) = acc[i][j];
         return;
     }
     __syncthreads();                                           // the stages become the waves' blocks
@@ -535,7 +614,7 @@ __global__ __launch_bounds__(TILE == 128 ? 256 : 512, NST == 2 ? 2 : 1) void muo
 #pragma unroll
     for (int q = 0; q < NI * NJ; ++q) {
         if (NST == 2 && q + 1 < NI * NJ) fetch(q + 1);
-        finish<MODE, DT>(L, a, acc[q / NJ][q % NJ], own[q], i0 + q / NJ * 32, j0 + q % NJ * 32, ti != tj, from, last != 0, block, lane);
+        finish<MODE, DT>(L, a, acc[q / NJ][q % NJ], own[q], diag[q], i0 + q / NJ * 32, j0 + q % NJ * 32, ti != tj, from, last != 0, block, lane);
     }
 }
 
@@ -567,8 +646,7 @@ __global__ __launch_bounds__(256) void muon_gram_sum_kernel(const MuonTable* __r
     for (int u = 0; u < 3; ++u) acc += part[u][lane];
     int i, j;
     tri_at(id, t, i, j);
-    const int wave = sub >> 2, q = sub & 3;
-    finish<kGram, SNAG_F32>(L, a, acc, Pairs{}, i * 128 + (wave >> 1) * 64 + (q >> 1) * 32, j * 128 + (wave & 1) * 64 + (q & 1) * 32, i != j, 0, false, block, lane);
+    finish<kGram, SNAG_F32>(L, a, acc, Pairs{}, Diagonals{}, i * 128 + (sub >> 2) * 32, j * 128 + (sub & 3) * 32, i != j, 0, false, block, lane);
 }
 
 // ---- one side of at most 128 ------------------------------------------------------------------------------------------------
@@ -596,31 +674,39 @@ __device__ __forceinline__ f16x8 image_cols(const _Float16* lds, int col, int kb
 #endif
     return v.f;
 }
-// 64 x 64 part (wm, wn) of a product of two images; RIGHT_COLS: the right operand's contraction runs down its rows
+// 64 x 64 part (wm, wn) of a product of two images, block q at (q / 2, q % 2); RIGHT_COLS: the right operand's contraction runs down its rows.
+// The next 16 of the contraction are read while the present ones are multiplied.
 template <int PLANES, bool RIGHT_COLS>
 __device__ __forceinline__ void image_product(f32x16 (&acc)[4], const _Float16* left, const _Float16* right, int wm, int wn, int lane) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) acc[q] = f32x16{};
-#pragma unroll
-    for (int kb = 0; kb < 8; ++kb) {
-        f16x8 fa[PLANES][2], fb[PLANES][2];
+    f16x8 fa[2][PLANES][2], fb[2][PLANES][2];
+    auto read = [&](int kb) {
 #pragma unroll
         for (int p = 0; p < PLANES; ++p)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                fa[p][i] = image_rows(left + p * kImage, wm + i * 32, kb, lane);
-                fb[p][i] = RIGHT_COLS ? image_cols(right + p * kImage, wn + i * 32, kb, lane) : image_rows(right + p * kImage, wn + i * 32, kb, lane);
+                fa[kb & 1][p][i] = image_rows(left + p * kImage, wm + i * 32, kb, lane);
+                fb[kb & 1][p][i] = RIGHT_COLS ? image_cols(right + p * kImage, wn + i * 32, kb, lane) : image_rows(right + p * kImage, wn + i * 32, kb, lane);
             }
+    };
+    read(0);
+#pragma unroll
+    for (int kb = 0; kb < 8; ++kb) {
+        if (kb < 7) read(kb + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        const int s = kb & 1;
 #if defined(__HIP_DEVICE_COMPILE__)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            acc[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][q >> 1], fb[0][q & 1], acc[q], 0, 0, 0);
+            acc[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[s][0][q >> 1], fb[s][0][q & 1], acc[q], 0, 0, 0);
             if constexpr (PLANES == 2) {
-                acc[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][q >> 1], fb[1][q & 1], acc[q], 0, 0, 0);
-                acc[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[1][q >> 1], fb[0][q & 1], acc[q], 0, 0, 0);
+                acc[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[s][0][q >> 1], fb[s][1][q & 1], acc[q], 0, 0, 0);
+                acc[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[s][1][q >> 1], fb[s][0][q & 1], acc[q], 0, 0, 0);
             }
         }
 #endif
+        __builtin_amdgcn_sched_barrier(0);
     }
 }
 __device__ __forceinline__ Pairs image_pairs(const _Float16* hi, const _Float16* lo, int row, int col) {
@@ -632,62 +718,47 @@ __device__ __forceinline__ void image_store(_Float16* hi, _Float16* lo, int row,
     *(f16x8*)(lo + image_at(row, col)) = p.lo[0], *(f16x8*)(lo + image_at(row, col + 8)) = p.lo[1];
 }
 
-// start: only the first A's shares of X copy 0.  One workgroup per 128-column block; slab[block][wave][4][1024] as the product kernel's ranges.
+// start: only the first A's shares of X copy 0.  One workgroup per 128-column block; slab[block][4][4][1024] as the product kernel's ranges.
 template <int DT>
-__global__ __launch_bounds__(256) void muon_narrow_kernel(const MuonTable* __restrict__ L, int from, int start, int last) {
+__global__ __launch_bounds__(256) void muon_narrow_kernel(const MuonTable* __restrict__ L, MuonFirst first, int from, int start, int last) {
     constexpr int PLANES = DT == SNAG_BF16 ? 1 : 2;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     _Float16 *X = (_Float16*)smem, *S = X + 2 * kImage;                // hi, lo of X's block; hi, lo of A, later of B
-    float* block = (float*)(S + 2 * kImage);                           // 4 x 32 x kPitch
+    float* diag = (float*)(S + 2 * kImage);                            // B's diagonal [128], and behind it the waves' 32 x kPitch blocks
     const int lane = threadIdx.x & 63, wave = wave_id_uniform();
-    const int which = matrix_of(L->first[kApply], L->count, blockIdx.x);
-    const MuonMatrix a = L->a[which];
-    const int col0 = ((int)blockIdx.x - L->first[kApply][which]) * 128;
+    float* block = diag + 128 + wave * 32 * kPitch;
+    int begin;
+    const MuonMatrix a = L->a[matrix_of(first, blockIdx.x, begin)];
+    const int col0 = ((int)blockIdx.x - begin) * 128;
     const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-    block += wave * 32 * kPitch;
     image_load(x_plane(a, from, 0) + col0, a.np, X, wave, lane);
     image_load(x_plane(a, from, 1) + col0, a.np, X + kImage, wave, lane);
     f32x16 acc[4];
-    const int r = lane >> 1, c = (lane & 1) * 16, h = lane >> 5;
-    auto to_block = [&](const f32x16& v) {
-        lds_turn();
-#pragma unroll
-        for (int i = 0; i < 16; ++i) block[(8 * (i >> 2) + 4 * h + (i & 3)) * kPitch + (lane & 31)] = v[i];
-        lds_turn();
-    };
+    const int r = lane >> 1, c = (lane & 1) * 16;
     if (!start) {
         image_load(s_plane(a, 0), 128, S, wave, lane);
         image_load(s_plane(a, 1), 128, S + kImage, wave, lane);
         const float* da = diagonal(a, 0);
         float di[2], dj[2][16];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            di[i] = da[wm + i * 32 + r];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) *(f32x4*)(dj[i] + 4 * q) = *(const f32x4*)(da + wn + i * 32 + c + 4 * q);
-        }
+        for (int i = 0; i < 2; ++i) di[i] = da[wm + i * 32 + r], load16(dj[i], da + wn + i * 32 + c);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         image_product<PLANES, false>(acc, S, S, wm, wn, lane);
-        // B in the place of A; its diagonal stays with the lanes that hold it and goes through LDS below
+        // B in the place of A
         Pairs b[4];
         float db[2] = {0.f, 0.f};
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const int row = wm + (q >> 1) * 32 + r, col = wn + (q & 1) * 32 + c;
             const Pairs p = image_pairs(S, S + kImage, row, col);
-            to_block(acc[q]);
             float v[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const float sq = block[r * kPitch + c + j] * (1.f / kScaleA);
-                v[j] = fmaf(fmaf(kNsC, di[q >> 1] + dj[q & 1][j], kNsB), sum_of(p, j), kNsC * sq);
-                if (row == col + j) db[q >> 1] = fmaf(kNsB, di[q >> 1], kNsC * fmaf(di[q >> 1], di[q >> 1], sq * (1.f / kScaleA))), v[j] = 0.f;
-            }
+            through_block(block, acc[q], v, lane);
+            const float d = poly(v, p, di[q >> 1], dj[q & 1], row - col, wm + (q >> 1) * 32 == wn + (q & 1) * 32);
+            if (row >= col && row < col + 16) db[q >> 1] = d;
             b[q] = pairs_of(v);
         }
         __syncthreads();
-        float* diag = (float*)(S + 2 * kImage) + 4 * 32 * kPitch;      // [128]
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const int row = wm + (q >> 1) * 32 + r, col = wn + (q & 1) * 32 + c;
@@ -701,11 +772,11 @@ __global__ __launch_bounds__(256) void muon_narrow_kernel(const MuonTable* __res
         for (int q = 0; q < 4; ++q) {
             const int row = wm + (q >> 1) * 32 + r, col = wn + (q & 1) * 32 + c;
             const Pairs p = image_pairs(X, X + kImage, row, col);
-            to_block(acc[q]);
-            const float d = kNsA + diag[row];
             float v[16];
+            through_block(block, acc[q], v, lane);
+            const float d = kNsA + diag[row];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = fmaf(d, sum_of(p, j), block[r * kPitch + c + j] * (1.f / kScaleA));
+            for (int j = 0; j < 16; ++j) v[j] = fmaf(d, sum_of(p, j), v[j] * (1.f / kScaleA));
             if (last) {
                 store_result<TypeOf<DT>>(L, a, v, wm + (q >> 1) * 32, col0 + wn + (q & 1) * 32, block, lane);
                 continue;
@@ -725,13 +796,12 @@ __global__ __launch_bounds__(256) void muon_narrow_kernel(const MuonTable* __res
     image_product<PLANES, false>(acc, X, X, wm, wn, lane);
     if (a.splits == 1) {                                               // the only block: A is complete
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-            finish<kGram, DT>(L, a, acc[q], Pairs{}, wm + (q >> 1) * 32, wn + (q & 1) * 32, false, 0, false, block, lane);
+        for (int q = 0; q < 4; ++q) finish<kGram, DT>(L, a, acc[q], Pairs{}, Diagonals{}, wm + (q >> 1) * 32, wn + (q & 1) * 32, false, 0, false, block, lane);
         return;
     }
-    float* out = slab_of(a) + ((int64_t)(col0 / 128) * 4 + wave) * 4096 + lane * 16;
+    float* out = slab_of(a) + (int64_t)(col0 / 128) * 16 * 1024 + lane * 16;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) *(f32x16*)(out + q * 1024) = acc[q];
+    for (int q = 0; q < 4; ++q) *(f32x16*)(out + ((wm / 32 + (q >> 1)) * 4 + wn / 32 + (q & 1)) * 1024) = acc[q];
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
@@ -782,7 +852,7 @@ struct MuonLists {
     }
 };
 
-struct MuonRun { MuonTable L; MuonTable* table; MuonPlan plan; int blocks_of[3], gram_tiles, blocks; bool vec; };
+struct MuonRun { MuonTable L; MuonFirst first[3]; MuonTable* table; MuonPlan plan; int blocks_of[3], gram_tiles, blocks; bool vec; };
 
 template <class K>
 static int grow_lds(K kernel, size_t bytes) {
@@ -794,7 +864,7 @@ static int product_of(const MuonRun& R, int from, int last, hipStream_t st) {
     using S = Shape<TILE, DT == SNAG_BF16 ? 1 : 2, NST>;
     static const int grown = grow_lds(muon_product_kernel<MODE, DT, TILE, NST>, S::kLds);
     if (grown != SNAG_OK) return grown;
-    muon_product_kernel<MODE, DT, TILE, NST><<<dim3(R.blocks_of[MODE]), S::kThreads, S::kLds, st>>>(R.table, from, last);
+    muon_product_kernel<MODE, DT, TILE, NST><<<dim3(R.blocks_of[MODE]), S::kThreads, S::kLds, st>>>(R.table, R.first[MODE], from, last);
     return check_launch("muon_product");
 }
 // A 128 x 128 workgroup takes 64 KB of LDS with two stages, so that two fit a CU and hide each other's waits; a launch with at most one per CU
@@ -824,12 +894,13 @@ static int muon_go(const MuonRun& R, int steps, hipStream_t st) {
     if (int rc = check_launch("muon_start")) return rc;
     if (R.plan.narrow) {
         constexpr size_t lds = 4 * kImage * sizeof(_Float16) + (4 * 32 * kPitch + 128) * sizeof(float);
+        static_assert(lds <= 160 * 1024, "one CU's LDS");
         static const int grown = grow_lds(muon_narrow_kernel<DT>, lds);
         if (grown != SNAG_OK) return grown;
         for (int k = -1; k < steps; ++k) {
             if (k >= 0)
                 if (int rc = gram_sum(R, st)) return rc;
-            muon_narrow_kernel<DT><<<dim3(R.blocks_of[kApply]), 256, lds, st>>>(R.table, k < 0 ? 0 : k & 1, k < 0, k + 1 == steps);
+            muon_narrow_kernel<DT><<<dim3(R.blocks_of[kApply]), 256, lds, st>>>(R.table, R.first[kApply], k < 0 ? 0 : k & 1, k < 0, k + 1 == steps);
             if (int rc = check_launch("muon_narrow")) return rc;
         }
         return SNAG_OK;
@@ -886,6 +957,8 @@ static int muon_run(const char* what, void* const* w, const void* const* g, floa
         L.count = n;
         L.dtype = dtype, L.step = mom != nullptr, L.nesterov = nesterov, L.mu = mu, L.keep = 1.f - lr * decay, L.eps = eps;
         R.table = (MuonTable*)work, R.vec = true;
+        for (auto& f : R.first)
+            for (int& at0 : f.at) at0 = INT32_MAX;
         char* space = (char*)work + kTableBytes;
         for (int i = 0; i < n; ++i) {
             MuonMatrix& a = L.a[i];
@@ -896,9 +969,10 @@ static int muon_run(const char* what, void* const* w, const void* const* g, floa
             a.splits = splits_of(R.plan, a.np);
             const double s = match_rms ? 0.2 * sqrt((double)a.n) : sqrt(r > c ? (double)r / c : 1.0);
             a.update = (float)(lr * s);
+            a.vec = c % 8 == 0 && aligned16(a.g) && aligned16(a.mom) && aligned16(a.w);
             space += matrix_bytes(R.plan, r, c);
             const int t = a.mp / 128, tri = t * (t + 1) / 2, b = (a.mp / 64) * (a.np / 64);
-            for (int q = 0; q < 3; ++q) L.first[q][i] = R.blocks_of[q];
+            for (int q = 0; q < 3; ++q) R.first[q].at[i] = R.blocks_of[q];
             R.blocks_of[kGram] += tri * a.splits;
             R.blocks_of[kPoly] += tri;
             R.blocks_of[kApply] += (a.mp / tile) * (a.np / tile);
