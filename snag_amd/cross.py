@@ -8,6 +8,7 @@ residual fused around it.  All arithmetic is in the HIP library, forward and bac
   sandwich_norm(x, y, ...)        the norm after a block, its gate, the residual and the next block's norm, in one pass
   CrossModalLayer                 the two with fp32 projections and a feed-forward block: one layer of a deeper fusion
 """
+import functools
 import math
 
 import torch
@@ -29,22 +30,38 @@ def _note_stream(out):
             raise _lib.SnagHipError("a backward cannot be captured while an eager graph of the same leaves lives on another stream: drop that graph's outputs first")
 
 
+def _first_order(backward):
+    """once_differentiable without its bookkeeping where no graph of the backward is asked for."""
+    recorded = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
+
+
 class _CrossAttentionFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, kv_lens, key_mask, scale):
+    def forward(ctx, q, k, v, kv_lens, key_mask, scale, want_lse):
         out, lse, lo = ops.cross_attention_fwd(q, k, v, kv_lens, key_mask, scale, want_residual=True)
         ctx.save_for_backward(q, k, v, kv_lens, key_mask, out, lse, lo)
         ctx.scale = scale
+        ctx.set_materialize_grads(False)
+        if not want_lse:
+            return out
         ctx.mark_non_differentiable(lse)
         return out, lse
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, d_out, _):
+    @_first_order
+    def backward(ctx, d_out, *_):
+        if d_out is None:
+            return (None,) * 7
         q, k, v, kv_lens, key_mask, out, lse, lo = ctx.saved_tensors
         dq, dk, dv = ops.cross_attention_bwd(q, k, v, out, lse, d_out.contiguous(), kv_lens, key_mask, ctx.scale, lo)
         need = ctx.needs_input_grad
-        return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None
+        return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None, None
 
 
 def cross_attention(q, k, v, kv_lens=None, key_mask=None, scale=None, return_lse=False):
@@ -55,11 +72,13 @@ def cross_attention(q, k, v, kv_lens=None, key_mask=None, scale=None, return_lse
     False.  Unseen keys may hold anything.  A query that sees no key gets zeros, and gives none of its gradient on.  ``scale`` defaults to d ** -0.5.
     ``return_lse`` adds the natural log-sum-exp of every row's scores [B, H, Lq] (-inf where no key is seen), not differentiable."""
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        out, lse = _CrossAttentionFn.apply(q, k, v, kv_lens, key_mask, scale)
+        got = _CrossAttentionFn.apply(q, k, v, kv_lens, key_mask, scale, return_lse)
+        out = got[0] if return_lse else got
         _note_stream(out)
     else:
-        out, lse = ops.cross_attention_fwd(q, k, v, kv_lens, key_mask, scale)
-    return (out, lse * LN2) if return_lse else out
+        got = ops.cross_attention_fwd(q, k, v, kv_lens, key_mask, scale)
+        out = got[0]
+    return (out, got[1] * LN2) if return_lse else out
 
 
 class _SandwichNormFn(torch.autograd.Function):
@@ -73,13 +92,17 @@ class _SandwichNormFn(torch.autograd.Function):
         return h, z
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, d_h, d_z):
         x, y, stats, post_weight, pre_weight, post_bias, pre_bias, gate = ctx.saved_tensors
         plan, res_scale, kind = ctx.cfg
         grads = ops._sandwich_bwd(plan, x, y, stats, None if d_h is None else d_h.contiguous(), None if d_z is None else d_z.contiguous(),
                                   post_weight, pre_weight, post_bias, pre_bias, gate, res_scale, kind)
         return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None, None)
+
+
+def _wants_grad(*ts):
+    return any(t is not None and t.requires_grad for t in ts)
 
 
 def sandwich_norm(x, y, post_weight=None, pre_weight=None, post_bias=None, pre_bias=None, gate=None, res_scale=1.0, kind="rms", eps=1e-6):
@@ -89,14 +112,13 @@ def sandwich_norm(x, y, post_weight=None, pre_weight=None, post_bias=None, pre_b
     (v / sqrt(mean v^2 + eps)) or "layer" (around the mean, biased variance).  ``gate`` [dim], or [G, dim] whose rows serve rows / G
     neighbouring rows each (one gate per sequence, or per row).  x may stay fp32 while y is 16-bit; h has x's type, z y's.  Weights and biases
     share one type, fp32 or y's; so does the gate.  Differentiable in every tensor."""
-    x, y = x.contiguous(), y.contiguous()
-    params = (post_weight, pre_weight, post_bias, pre_bias, gate)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, y, *params)):
-        h, z = _SandwichNormFn.apply(x, y, *params, res_scale, kind, eps)
+    if not (x.is_contiguous() and y.is_contiguous()):
+        x, y = x.contiguous(), y.contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or y.requires_grad or _wants_grad(post_weight, pre_weight, post_bias, pre_bias, gate)):
+        h, z = _SandwichNormFn.apply(x, y, post_weight, pre_weight, post_bias, pre_bias, gate, res_scale, kind, eps)
         _note_stream(h)
         return h, z
-    h, z, _ = ops.sandwich_norm_fwd(x, y, *params, res_scale, kind, eps, want_stats=False)
-    return h, z
+    return ops.sandwich_norm_fwd(x, y, post_weight, pre_weight, post_bias, pre_bias, gate, res_scale, kind, eps, want_stats=False)[:2]
 
 
 class _SandwichNorm(nn.Module):

@@ -596,8 +596,8 @@ def _cross_work_floats(shape, backward):
 
 def _cross_args(q, k, v, kv_lens, key_mask, scale):
     _any(q, "q", 4), _any(k, "k", 4), _any(v, "v", 4)
-    (B, Lq, H, d), ks = q.shape, k.shape
-    if k.dtype != q.dtype or v.dtype != q.dtype:
+    (B, Lq, H, d), ks, dtype, dev = q.shape, k.shape, q.dtype, q.device
+    if k.dtype != dtype or v.dtype != dtype:
         raise TypeError(f"q, k and v must share one type, got {q.dtype}, {k.dtype}, {v.dtype}")
     if ks != v.shape or ks[0] != B or ks[3] != d:
         raise ValueError(f"k and v must be [{B}, Lk, Hkv, {d}], got {tuple(k.shape)} and {tuple(v.shape)}")
@@ -606,16 +606,22 @@ def _cross_args(q, k, v, kv_lens, key_mask, scale):
         raise ValueError(f"{H} heads are not a multiple of {Hkv} key/value heads")
     if not 1 <= d <= CROSS_MAX_HEAD_DIM:
         raise ValueError(f"head dimension {d} is not in 1..{CROSS_MAX_HEAD_DIM}")
+    if k.device != dev or v.device != dev:
+        raise ValueError(f"k and v are on {k.device} and {v.device}, q on {dev}")
     qs, kt, vt = q.stride(), k.stride(), v.stride()
-    for t, st, name in ((q, qs, "q"), (k, kt, "k"), (v, vt, "v")):
-        if st[3] != 1 and d > 1 and t.numel():
-            raise ValueError(f"{name}: the elements of a head must be adjacent (strides {st})")
+    if d > 1 and (qs[3] != 1 or kt[3] != 1 or vt[3] != 1):
+        for t, st, name in ((q, qs, "q"), (k, kt, "k"), (v, vt, "v")):
+            if st[3] != 1 and t.numel():
+                raise ValueError(f"{name}: the elements of a head must be adjacent (strides {st})")
     lens_bytes = mask_ld = 0
+    lens_at = mask_at = None
     if kv_lens is not None:
         _idx(kv_lens, "kv_lens", 1)
         if kv_lens.shape[0] != B:
             raise ValueError(f"kv_lens must be [{B}], got {tuple(kv_lens.shape)}")
-        lens_bytes = kv_lens.element_size()
+        if kv_lens.device != dev:
+            raise ValueError(f"kv_lens is on {kv_lens.device}, q on {dev}")
+        lens_bytes, lens_at = kv_lens.element_size(), kv_lens.data_ptr()
     if key_mask is not None:
         if not isinstance(key_mask, torch.Tensor) or key_mask.dtype not in (torch.bool, torch.uint8):
             raise TypeError("key_mask: expected a bool (or uint8) tensor, true where a key is seen")
@@ -623,16 +629,17 @@ def _cross_args(q, k, v, kv_lens, key_mask, scale):
             raise ValueError(f"key_mask must be [{B}, {Lk}], got {tuple(key_mask.shape)}")
         if not key_mask.is_cuda:
             raise _lib.SnagHipError(f"key_mask: tensor is on {key_mask.device}; snag_amd kernels run on the GPU only (no CPU fallback)")
+        if key_mask.device != dev:
+            raise ValueError(f"key_mask is on {key_mask.device}, q on {dev}")
         if Lk > 1 and key_mask.stride(1) != 1:
             raise ValueError("key_mask: a row's elements must be adjacent")
-        mask_ld = key_mask.stride(0) if B > 1 else Lk
-    _one_device(q.device, k=k, v=v, kv_lens=kv_lens, key_mask=key_mask)
+        mask_ld, mask_at = key_mask.stride(0) if B > 1 else Lk, key_mask.data_ptr()
     scale = d ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < float("inf"):
         raise ValueError(f"scale must be positive and finite, got {scale}")
-    strides = _Strides(*qs[:3], *kt[:3], *vt[:3])
-    shape = (DTYPES[q.dtype], B, Lq, Lk, H, Hkv, d)
-    return shape, (ptr(q), ptr(k), ptr(v), *shape, ctypes.addressof(strides), ptr(kv_lens), lens_bytes, ptr(key_mask), mask_ld, scale), strides
+    strides = _Strides(qs[0], qs[1], qs[2], kt[0], kt[1], kt[2], vt[0], vt[1], vt[2])
+    shape = (DTYPES[dtype], B, Lq, Lk, H, Hkv, d)
+    return shape, (q.data_ptr(), k.data_ptr(), v.data_ptr(), *shape, ctypes.addressof(strides), lens_at, lens_bytes, mask_at, mask_ld, scale), strides
 
 
 def _cross_work(shape, backward, device):
@@ -655,16 +662,16 @@ def cross_attention_fwd(q, k, v, kv_lens=None, key_mask=None, scale=None, want_r
 def cross_attention_bwd(q, k, v, out, lse, d_out, kv_lens=None, key_mask=None, scale=None, out_residual=None):
     """-> d_q, d_k, d_v (dense).  C ABI: snag_cross_bwd."""
     shape, args, hold = _cross_args(q, k, v, kv_lens, key_mask, scale)
+    dev, qs = q.device, q.shape
     for t, name in ((out, "out"), (d_out, "d_out"), (out_residual, "out_residual")):
         if t is None and name == "out_residual":
             continue
         _chk(t, name, dtype=q.dtype, ndim=4)
-        if t.shape != q.shape:
-            raise ValueError(f"{name} must be {tuple(q.shape)}, got {tuple(t.shape)}")
+        if t.shape != qs or t.device != dev:
+            raise ValueError(f"{name} must be {tuple(qs)} on {dev}, got {tuple(t.shape)} on {t.device}")
     _chk(lse, "lse", ndim=3)
-    if tuple(lse.shape) != (q.shape[0], q.shape[2], q.shape[1]):
-        raise ValueError(f"lse must be [B, H, Lq], got {tuple(lse.shape)}")
-    _one_device(q.device, out=out, lse=lse, d_out=d_out, out_residual=out_residual)
+    if tuple(lse.shape) != (qs[0], qs[2], qs[1]) or lse.device != dev:
+        raise ValueError(f"lse must be [B, H, Lq] on {dev}, got {tuple(lse.shape)} on {lse.device}")
     dq, dk, dv = (torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k, v))
     work, n = _cross_work(shape, True, q.device)
     _call_on(q.device, "snag_cross_bwd", *args, ptr(out), ptr(out_residual), ptr(lse), ptr(d_out), ptr(dq), ptr(dk), ptr(dv), ptr(work), n)
