@@ -822,7 +822,8 @@ SNAG_API int snag_sandwich_bwd(const void* x, int x_dtype, const void* y, int y_
  *                   (a, b, c) = (3.4445, -4.7750, 2.0315);  out = X.   out[i] may be g[i].
  *   muon step:      M <- mu M + (1 - mu) g;  U = nesterov ? (1 - mu) g + mu M : M;  X = orthogonalize(U);
  *                   w <- (1 - lr decay) w - lr s X,  s = sqrt(max(1, rows / cols)), or 0.2 sqrt(max(rows, cols)) with match_rms.
- * Products accumulate in fp32; fp32 matrices carry 22 bits through them, 16-bit matrices 11 (csrc/muon.hip states the error of each).
+ * Products accumulate in fp32; fp32 and fp16 matrices carry 22 bits through them, bf16 matrices 11 (csrc/muon.hip states the error of each).
+ * Nothing that is written may share memory with another matrix of the call.
  * work: snag_muon_work_bytes(...) bytes, 256-byte aligned, uninitialised; launches sharing it must be stream-ordered. */
 #define SNAG_MUON_MAX_SIDE 16384
 SNAG_API int64_t snag_muon_work_bytes(const int32_t* rows_host, const int32_t* cols_host, int count);

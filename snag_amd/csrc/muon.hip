@@ -8,13 +8,14 @@
 // The products run on the matrix pipe in fp16 with fp32 accumulation.  fp16 keeps 11 bits, so every operand is stored as a pair (hi, lo) of
 // fp16 values of ONE power-of-two scaling (X 2^14, A and B 2^13: |X| <= 1.21 and |A|, |B| <= 2.9 stay below fp16's 65504, and the small
 // entries of a large matrix stay normal), 22 bits together:
-//   * fp32 matrices: three products hi hi + hi lo + lo hi (the dropped lo lo is 2^-22 of the product);
-//   * 16-bit matrices: one product hi hi, with the DIAGONALS of A and B kept out of it, in fp32:  with A = D + R,
+//   * fp32 and fp16 matrices: three products hi hi + hi lo + lo hi (the dropped lo lo is 2^-22 of the product);
+//   * bf16 matrices: one product hi hi, with the DIAGONALS of A and B kept out of it, in fp32:  with A = D + R,
 //     A^2 = D^2 + D R + R D + R^2  and  a X + B X = (a + diag B) X + offdiag(B) X.  Near orthogonality A is almost its diagonal, and rounding
 //     that diagonal to 11 bits is what dominates a plain fp16 iteration (2e-3 relative; 5e-4 this way, against 1.7e-3 for the rounding of
 //     the bf16 result); the linear terms take R and X at 22 bits.
 // A and B are symmetric: only tiles on and below the diagonal are computed, and both halves written.
 // All matrices of the list share each launch.
+#include <atomic>
 #include <type_traits>
 #include "cross.hip.h"
 
@@ -854,16 +855,22 @@ struct MuonLists {
 
 struct MuonRun { MuonTable L; MuonFirst first[3]; MuonTable* table; MuonPlan plan; int blocks_of[3], gram_tiles, blocks; bool vec; };
 
+// more than 64 KB of LDS for `kernel`, once per device (done: a bit each; devices from 64 on are set every time)
 template <class K>
-static int grow_lds(K kernel, size_t bytes) {
-    const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    return e == hipSuccess ? SNAG_OK : fail(SNAG_ERR_LAUNCH, "muon: %s", hipGetErrorString(e));
+static int grow_lds(K kernel, size_t bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e == hipSuccess && dev < 64 && (done.load() >> dev & 1)) return SNAG_OK;
+    if (e == hipSuccess) e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e != hipSuccess) return fail(SNAG_ERR_LAUNCH, "muon: %s", hipGetErrorString(e));
+    if (dev < 64) done.fetch_or((uint64_t)1 << dev);
+    return SNAG_OK;
 }
 template <int MODE, int DT, int TILE, int NST>
 static int product_of(const MuonRun& R, int from, int last, hipStream_t st) {
     using S = Shape<TILE, DT == SNAG_BF16 ? 1 : 2, NST>;
-    static const int grown = grow_lds(muon_product_kernel<MODE, DT, TILE, NST>, S::kLds);
-    if (grown != SNAG_OK) return grown;
+    static std::atomic<uint64_t> done{0};
+    if (int rc = grow_lds(muon_product_kernel<MODE, DT, TILE, NST>, S::kLds, done)) return rc;
     muon_product_kernel<MODE, DT, TILE, NST><<<dim3(R.blocks_of[MODE]), S::kThreads, S::kLds, st>>>(R.table, R.first[MODE], from, last);
     return check_launch("muon_product");
 }
@@ -895,8 +902,8 @@ static int muon_go(const MuonRun& R, int steps, hipStream_t st) {
     if (R.plan.narrow) {
         constexpr size_t lds = 4 * kImage * sizeof(_Float16) + (4 * 32 * kPitch + 128) * sizeof(float);
         static_assert(lds <= 160 * 1024, "one CU's LDS");
-        static const int grown = grow_lds(muon_narrow_kernel<DT>, lds);
-        if (grown != SNAG_OK) return grown;
+        static std::atomic<uint64_t> done{0};
+        if (int rc = grow_lds(muon_narrow_kernel<DT>, lds, done)) return rc;
         for (int k = -1; k < steps; ++k) {
             if (k >= 0)
                 if (int rc = gram_sum(R, st)) return rc;

@@ -796,6 +796,19 @@ def _matrices(ts, name, dtype=None, shapes=None, device=None):
     return ts, got
 
 
+def _disjoint(written, read):
+    """Nothing that is written shares memory with anything else in the call."""
+    spans = sorted([(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), True) for t in written] +
+                   [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), False) for t in read])
+    any_end = written_end = 0
+    for start, end, writes in spans:
+        if start < written_end or (writes and start < any_end):
+            raise ValueError("a matrix is listed twice, or shares memory with another one of the call")
+        any_end = max(any_end, end)
+        if writes:
+            written_end = max(written_end, end)
+
+
 def _muon_lists(*lists):
     return [(ctypes.c_void_p * len(ts))(*[t.data_ptr() for t in ts]) for ts in lists]
 
@@ -822,11 +835,8 @@ def orthogonalize(gs, outs=None, steps=5, eps=1e-7):
             raise ValueError(f"{len(gs)} matrices, {len(outs)} outputs")
         if gs:
             _matrices(outs, "outs", gs[0].dtype, shapes, gs[0].device)
-            if len({t.data_ptr() for t in outs}) != len(outs):
-                raise ValueError("a matrix is listed twice")
-            at = {g.data_ptr(): i for i, g in enumerate(gs)}
-            if any(at.get(t.data_ptr(), i) != i for i, t in enumerate(outs)):
-                raise ValueError("an output may be its own input, not another one's")
+            _disjoint(outs, [g for g, o in zip(gs, outs) if g.data_ptr() != o.data_ptr()])
+            torch.autograd.graph.increment_version(outs)
     if not gs:
         return outs
     rows, cols, n = _muon_shapes(tuple(shapes))
@@ -851,8 +861,8 @@ def muon_step(weights, grads, momenta, lr, momentum=0.95, nesterov=True, weight_
         return
     dev = weights[0].device
     _matrices(grads, "grads", weights[0].dtype, shapes, dev), _matrices(momenta, "momenta", f32, shapes, dev)
-    if len({t.data_ptr() for t in weights}) != len(weights) or len({t.data_ptr() for t in momenta}) != len(momenta):
-        raise ValueError("a matrix is listed twice")
+    _disjoint(weights + momenta, grads)
+    torch.autograd.graph.increment_version(weights + momenta)      # a graph that saved one of them must not run on the new values
     rows, cols, n = _muon_shapes(tuple(shapes))
     work = torch.empty(n, device=dev, dtype=torch.uint8)
     pw, pg, pm = _muon_lists(weights, grads, momenta)

@@ -46,6 +46,15 @@ class Muon(optim.Optimizer):
             self.param_groups.pop()
             raise ValueError("Muon: a parameter that is not a matrix (put it into a group with muon=False)")
 
+    def load_state_dict(self, state_dict):
+        """torch casts the state to its parameter's type: the momentum of a 16-bit matrix is put back as it was saved, in fp32."""
+        super().load_state_dict(state_dict)
+        saved = (i for g in state_dict["param_groups"] for i in g["params"])
+        for i, p in zip(saved, (p for g in self.param_groups for p in g["params"])):
+            m = state_dict["state"].get(i, {}).get("momentum_buffer")
+            if m is not None:
+                self.state[p]["momentum_buffer"] = m.to(device=p.device, dtype=torch.float32).contiguous()
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
@@ -83,7 +92,7 @@ class Muon(optim.Optimizer):
 
 def _is_matrix(name, p):
     """What Muon updates: matrices that are multiplied by; tables that rows are looked up in and weights of other ranks stay with AdamW."""
-    return p.dim() == 2 and min(p.shape) > 1 and "emb" not in name
+    return p.dim() == 2 and min(p.shape) > 1 and max(p.shape) <= ops.MUON_MAX_SIDE and "emb" not in name
 
 
 def set_optim(opt, model_list, freeze_part=(), no_freeze_part=(), accumulation_step=None):

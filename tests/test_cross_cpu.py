@@ -176,3 +176,27 @@ def test_plain_gradients_agree_with_differences():
             up, dn = (sandwich(**{**p, name: t + s * e}, res_scale=0.7, kind=kind, eps=1e-6) for s in (1, -1))
             diff = (((up["h"] - dn["h"]) * dh).sum() + ((up["z"] - dn["z"]) * dz).sum()) / 2e-5
             assert abs(float(diff - (ref["d_" + name] * e).sum() / 1e-5)) < 1e-7, (kind, name)
+
+
+def test_muon_optimizer_keeps_the_momentum_of_16_bit_matrices_in_fp32():
+    from snag_amd.optim import Muon, _is_matrix
+    w = [torch.nn.Parameter(torch.zeros(4, 6, dtype=t)) for t in (torch.bfloat16, torch.float16, torch.float32)]
+    opt, again = Muon(w), Muon(w)
+    for p in w:
+        opt.state[p]["momentum_buffer"] = torch.rand(4, 6)
+    again.load_state_dict(opt.state_dict())
+    for p in w:
+        m = again.state[p]["momentum_buffer"]
+        assert m.dtype == torch.float32 and torch.equal(m, opt.state[p]["momentum_buffer"])
+    wide = torch.empty(2, 16385, device="meta")
+    assert not _is_matrix("fc.weight", wide) and _is_matrix("fc.weight", wide[:, :16384])
+
+
+def test_muon_lists_that_share_memory():
+    from snag_amd import ops
+    a, b = torch.zeros(10, 4), torch.zeros(10, 4)
+    ops._disjoint([a[:5], a[5:]], [b, b])
+    ops._disjoint([], [a, a[2:]])
+    for written, read in (([a, a], []), ([a[:5], a[4:]], []), ([a], [a]), ([a[3:5]], [a]), ([a, b], [b[9:]])):
+        with pytest.raises(ValueError, match="twice"):
+            ops._disjoint(written, read)

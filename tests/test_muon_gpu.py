@@ -162,9 +162,35 @@ def test_refusals_in_python():
         ops.orthogonalize([a], steps=0)
     b = a.clone()
     for args, err in ((([a], [a, a], [b]), ValueError), (([a], [a], [b.bfloat16()]), TypeError), (([a], [a.bfloat16()], [b]), TypeError), (([a], [a[:3]], [b]), ValueError),
-                      (([a, a], [a, a], [b, b.clone()]), ValueError)):
+                      (([a, a], [a, a], [b, b.clone()]), ValueError), (([a], [b], [a]), ValueError), (([a], [a], [b]), ValueError), (([a[:2], a[1:3]], [b[:2], b[:2]], [b[2:], b.clone()[:2]]), ValueError)):
         with pytest.raises(err):
             ops.muon_step(*args, lr=0.1)
+    # written in place: a graph that saved the old values refuses to run on the new ones
+    w = a.clone().requires_grad_(True)
+    y = (w * w).sum()
+    ops.muon_step([w.detach()], [torch.ones_like(a)], [b], lr=0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_resumed_optimizer_goes_on_bit_for_bit(dtype):
+    from snag_amd.optim import Muon
+    g = torch.Generator(device=DEV).manual_seed(15)
+    grads = [torch.randn(40, 70, generator=g, device=DEV).to(dtype) for _ in range(4)]
+    w = torch.nn.Parameter(torch.randn(40, 70, generator=g, device=DEV).to(dtype))
+    opt = Muon([w], lr=0.1)
+    for d in grads[:2]:
+        w.grad = d
+        opt.step()
+    copy = torch.nn.Parameter(w.detach().clone())
+    again = Muon([copy], lr=0.1)
+    again.load_state_dict({"state": {i: {k: t.clone() for k, t in s.items()} for i, s in opt.state_dict()["state"].items()}, "param_groups": opt.state_dict()["param_groups"]})
+    for p, o in ((w, opt), (copy, again)):
+        for d in grads[2:]:
+            p.grad = d
+            o.step()
+    assert torch.equal(w, copy)
 
 
 def test_a_block_trained_by_the_optimizer():
