@@ -11,28 +11,30 @@ namespace snag {
 template <class T>
 __global__ __launch_bounds__(256) void cross_stat_kernel(CrossArgs a, float* __restrict__ stat, int padded) {
     constexpr int C = Chunk<T>::n;
-    const int64_t n = (int64_t)a.B * a.Hkv * padded, at = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    const int64_t n = (int64_t)a.B * a.Hkv * padded;
     const int t = threadIdx.x & 15;
-    const int64_t bh = at / padded, b = bh / a.Hkv;
-    const int row = (int)(at - bh * padded), hk = (int)(bh - b * a.Hkv), l = row_l(a, row), head = hk * a.G + row - l * a.G;
-    const bool own = at < n && row < a.rows;
-    const int64_t dense = ((b * a.Lq + l) * a.H + head) * a.d;
-    float s = 0.f;
-    if (own)
-        for (int col = t * C; col < a.d; col += 16 * C) {
-            const auto x = load_chunk<T>((const T*)a.o + dense, col, a.d, true, a.vec_o);
-            const auto y = load_chunk<T>((const T*)a.dout + dense, col, a.d, true, a.vec_o);
-            typename Chunk<T>::vec w{};
-            if (a.o_lo != nullptr) w = load_chunk<T>((const T*)a.o_lo + dense, col, a.d, true, a.vec_o);
+    for (int64_t at = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); at < n; at += (int64_t)gridDim.x * 16) {
+        const int64_t bh = at / padded, b = bh / a.Hkv;
+        const int row = (int)(at - bh * padded), hk = (int)(bh - b * a.Hkv), l = row_l(a, row), head = hk * a.G + row - l * a.G;
+        const bool own = row < a.rows;
+        const int64_t dense = ((b * a.Lq + l) * a.H + head) * a.d;
+        float s = 0.f;
+        if (own)
+            for (int col = t * C; col < a.d; col += 16 * C) {
+                const auto x = load_chunk<T>((const T*)a.o + dense, col, a.d, true, a.vec_o);
+                const auto y = load_chunk<T>((const T*)a.dout + dense, col, a.d, true, a.vec_o);
+                typename Chunk<T>::vec w{};
+                if (a.o_lo != nullptr) w = load_chunk<T>((const T*)a.o_lo + dense, col, a.d, true, a.vec_o);
 #pragma unroll
-            for (int j = 0; j < C; ++j) s = fmaf((float)x[j] + (float)w[j], (float)y[j], s);
+                for (int j = 0; j < C; ++j) s = fmaf((float)x[j] + (float)w[j], (float)y[j], s);
+            }
+        s = sum16(s);
+        if (t == 0) {
+            float lse = own ? a.lse[(b * a.H + head) * a.Lq + l] : INFINITY;
+            if (lse == -INFINITY) lse = INFINITY;
+            stat[2 * at] = lse;
+            stat[2 * at + 1] = own ? s : 0.f;
         }
-    s = sum16(s);
-    if (at < n && t == 0) {
-        float lse = own ? a.lse[(b * a.H + head) * a.Lq + l] : INFINITY;
-        if (lse == -INFINITY) lse = INFINITY;
-        stat[2 * at] = lse;
-        stat[2 * at + 1] = own ? s : 0.f;
     }
 }
 
@@ -113,6 +115,10 @@ __global__ __launch_bounds__(NW * 64, NW == 1 || (sizeof(T) == 4 && DP == 128) ?
         if (t + 1 < t1) store(t + 1);
     }
     if (!own) return;
+    if (lse == INFINITY) {                                 // no key seen: zero, whatever d_out holds
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i) acc[i] = f32x16{};
+    }
     if (a.splits > 1) store_row<float, DP>(a.part + (int64_t)pr.split * a.B * a.Lq * a.H * a.d + dense, acc, a.scale, a.d, lane);
     else store_row<T, DP>((T*)a.dq + dense, acc, a.scale, a.d, lane);
 }
@@ -263,13 +269,12 @@ static int bwd(CrossArgs a, const CrossPlan& p, float* stat, hipStream_t st) {
     if (nq > 0) {
         const int padded = (int)padded_rows(a.rows);
         const int64_t ns = ((int64_t)a.B * a.Hkv * padded + 15) / 16;
-        SNAG_REQUIRE(ns < (int64_t)1 << 31, SNAG_ERR_UNSUPPORTED, "cross attention: %lld rows", (long long)nq);
-        cross_stat_kernel<T><<<dim3((unsigned)ns), 256, 0, st>>>(a, stat, padded);
+        cross_stat_kernel<T><<<dim3((unsigned)(ns < kMaxBlocks ? ns : kMaxBlocks)), 256, 0, st>>>(a, stat, padded);
         if (int rc = check_launch("cross_stat")) return rc;
         a.splits = p.s_dq;
         a.per_split = range_of(a.Lk, a.splits);
         const int64_t tiles = (a.rows + p.nw_q * 32 - 1) / (p.nw_q * 32), n = (int64_t)a.B * a.Hkv * tiles * a.splits;
-        SNAG_REQUIRE(n < (int64_t)1 << 31, SNAG_ERR_UNSUPPORTED, "cross attention: %lld workgroups", (long long)n);
+        SNAG_REQUIRE(n < kMaxBlocks, SNAG_ERR_UNSUPPORTED, "cross attention: %lld workgroups, at most 2^24 in a launch", (long long)n);
         const dim3 grid((unsigned)n);
         const bool direct = p.nw_q == 4 && whole && a.mask == nullptr;
 #define CALL(DP)                                                                                  \
@@ -286,7 +291,7 @@ static int bwd(CrossArgs a, const CrossPlan& p, float* stat, hipStream_t st) {
         a.splits = p.s_dkv;
         a.per_split = range_of(a.rows, a.splits);
         const int64_t tiles = (a.Lk + p.nw_k * 32 - 1) / (p.nw_k * 32), n = (int64_t)a.B * a.Hkv * tiles * a.splits;
-        SNAG_REQUIRE(n < (int64_t)1 << 31, SNAG_ERR_UNSUPPORTED, "cross attention: %lld workgroups", (long long)n);
+        SNAG_REQUIRE(n < kMaxBlocks, SNAG_ERR_UNSUPPORTED, "cross attention: %lld workgroups, at most 2^24 in a launch", (long long)n);
         const dim3 grid((unsigned)n);
         const bool direct = p.nw_k == 4 && whole && a.rows > 0;
 #define CALL(DP)                                                                                  \

@@ -18,7 +18,7 @@ namespace snag {
 struct SandwichArgs {
     const void *x, *y, *post_w, *post_b, *pre_w, *pre_b, *gate;
     int w32, g32;                  // parameters / gate in fp32 (else y's type)
-    int64_t rows, rows_per_gate;
+    int64_t row0, rows, rows_per_gate;      // row0: the launch's first row (forward; a launch stays below 2^32 threads)
     int dim, layer;
     float res_scale, eps;
     void *h, *z;
@@ -163,7 +163,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void sandwich_fwd_kernel(San
     __shared__ float red[2][kMaxWaves][2];
     int turn = 0;
     const int t = threadIdx.x % TPR;
-    const int64_t row = TPR >= 256 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+    const int64_t row = a.row0 + (TPR >= 256 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR);
     if (TPR < 256 && row >= a.rows) return;       // otherwise one row per workgroup
     const int D = a.dim;
     float y[NU][4], x[NU][4], p[NU][4], b[NU][4], g[NU][4];
@@ -390,9 +390,8 @@ static SandwichPlan sandwich_plan(int64_t rows, int64_t rows_per_gate, int dim) 
 }
 
 template <class TX, class TY>
-static void sandwich_launch(const SandwichArgs& a, bool vec, bool bwd, hipStream_t st) {
+static void sandwich_launch(const SandwichArgs& a, int64_t items, bool vec, bool bwd, hipStream_t st) {
     const int tpr = threads_per_row(a.dim);
-    const int64_t items = bwd ? a.workers : a.rows;
     const int threads = tpr > 256 ? tpr : 256, per = threads / tpr;
     const dim3 grid((unsigned)((items + per - 1) / per));
 #define GO(TPR, NU)                                                                       \
@@ -433,10 +432,11 @@ static int sandwich_check(const void* x, int x_dtype, const void* y, int y_dtype
 static size_t bytes_of(int dtype) { return dtype == SNAG_F32 ? 4 : 2; }
 static bool aligned4(const void* p, int dtype) { return ((uintptr_t)p & (4 * bytes_of(dtype) - 1)) == 0; }
 
-static void sandwich_go(const SandwichArgs& a, int x_dtype, int y_dtype, bool vec, bool bwd, hipStream_t st) {
-    if (y_dtype == SNAG_F32) sandwich_launch<float, float>(a, vec, bwd, st);
-    else if (y_dtype == SNAG_BF16) x_dtype == SNAG_F32 ? sandwich_launch<float, bf16_t>(a, vec, bwd, st) : sandwich_launch<bf16_t, bf16_t>(a, vec, bwd, st);
-    else x_dtype == SNAG_F32 ? sandwich_launch<float, f16_t>(a, vec, bwd, st) : sandwich_launch<f16_t, f16_t>(a, vec, bwd, st);
+// items: rows of this launch (forward) or workers
+static void sandwich_go(const SandwichArgs& a, int64_t items, int x_dtype, int y_dtype, bool vec, bool bwd, hipStream_t st) {
+    if (y_dtype == SNAG_F32) sandwich_launch<float, float>(a, items, vec, bwd, st);
+    else if (y_dtype == SNAG_BF16) x_dtype == SNAG_F32 ? sandwich_launch<float, bf16_t>(a, items, vec, bwd, st) : sandwich_launch<bf16_t, bf16_t>(a, items, vec, bwd, st);
+    else x_dtype == SNAG_F32 ? sandwich_launch<float, f16_t>(a, items, vec, bwd, st) : sandwich_launch<f16_t, f16_t>(a, items, vec, bwd, st);
 }
 
 }  // namespace snag
@@ -457,8 +457,12 @@ extern "C" SNAG_API int snag_sandwich_fwd(const void* x, int x_dtype, const void
     a.h = h, a.z = z, a.stats = stats;
     const bool vec = dim % 4 == 0 && aligned4(x, x_dtype) && aligned4(y, y_dtype) && aligned4(h, x_dtype) && aligned4(z, y_dtype) && aligned4(post_w, w_dtype) &&
                      aligned4(post_b, w_dtype) && aligned4(pre_w, w_dtype) && aligned4(pre_b, w_dtype) && aligned4(gate, gate_dtype);
-    sandwich_go(a, x_dtype, y_dtype, vec, false, (hipStream_t)stream);
-    return check_launch("sandwich_fwd");
+    constexpr int64_t kRows = (int64_t)1 << 22;                // of up to 512 threads
+    for (; a.row0 < rows; a.row0 += kRows) {
+        sandwich_go(a, rows - a.row0 < kRows ? rows - a.row0 : kRows, x_dtype, y_dtype, vec, false, (hipStream_t)stream);
+        if (int rc = check_launch("sandwich_fwd")) return rc;
+    }
+    return SNAG_OK;
 }
 
 extern "C" SNAG_API int64_t snag_sandwich_work_floats(int64_t rows, int64_t rows_per_gate, int dim) {
@@ -490,7 +494,7 @@ extern "C" SNAG_API int snag_sandwich_bwd(const void* x, int x_dtype, const void
         const bool vec = dim % 4 == 0 && aligned4(x, x_dtype) && aligned4(y, y_dtype) && aligned4(post_w, w_dtype) && aligned4(post_b, w_dtype) &&
                          aligned4(pre_w, w_dtype) && aligned4(gate, gate_dtype) && aligned4(d_h, x_dtype) && aligned4(d_z, y_dtype) && aligned4(d_x, x_dtype) &&
                          aligned4(d_y, y_dtype) && aligned4(d_gate, gate_dtype) && aligned16(work);
-        sandwich_go(a, x_dtype, y_dtype, vec, true, st);
+        sandwich_go(a, a.workers, x_dtype, y_dtype, vec, true, st);
         if (int rc = check_launch("sandwich_bwd")) return rc;
     }
     if (d_post_w == nullptr && d_post_b == nullptr && d_pre_w == nullptr && d_pre_b == nullptr && d_gate == nullptr) return SNAG_OK;

@@ -165,6 +165,43 @@ def test_long_cache_offsets_pass_32_bits():
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [(3, 2, 70, 2, 2, 64), (3, 40, 70, 2, 1, 64), (3, 130, 200, 2, 2, 128)])
+def test_gradients_of_rows_that_see_nothing_may_hold_anything(size, dtype):
+    from snag_amd import ops
+    q, k, v, do = make(*size, dtype, seed=12)
+    lens = torch.tensor([size[2], 0, size[2] - 3], device=DEV, dtype=torch.int32)
+    mask = torch.ones(3, size[2], dtype=torch.bool, device=DEV)
+    mask[2] = False
+    for m, rows in ((None, slice(1, 2)), (mask, slice(1, 3))):
+        d = do.clone()
+        d[rows] = float("nan")
+        out, lse, lo = ops.cross_attention_fwd(q, k, v, lens, m, want_residual=True)
+        got = ops.cross_attention_bwd(q, k, v, out, lse, d, lens, m, out_residual=lo)
+        d[rows] = 0
+        ref = ops.cross_attention_bwd(q, k, v, out, lse, d, lens, m, out_residual=lo)
+        assert all(torch.equal(a, b) and bool((a[rows] == 0).all()) for a, b in zip(got, ref))
+
+
+def test_more_rows_than_threads_of_a_launch():
+    """2^28 rows of one problem: 16 lanes a row are more than 2^32 threads.  Only the last rows have a gradient: everything equals the small problem's."""
+    from snag_amd import ops
+    n, last, Lk, d = (1 << 28) + 70, 50, 3, 4
+    g = torch.Generator(device=DEV).manual_seed(13)
+    q = torch.empty(1, n, 1, d, device=DEV, dtype=torch.bfloat16).normal_(generator=g)
+    k, v = (torch.randn(1, Lk, 1, d, generator=g, device=DEV).bfloat16() for _ in range(2))
+    do = torch.zeros_like(q)
+    do[:, -last:] = torch.randn(1, last, 1, d, generator=g, device=DEV).bfloat16()
+    out, lse, lo = ops.cross_attention_fwd(q, k, v, want_residual=True)
+    dq, dk, dv = ops.cross_attention_bwd(q, k, v, out, lse, do, out_residual=lo)
+    small = q[:, -last:]
+    r = attention(small, k, v, None, None, None, do[:, -last:])
+    b = attention_bounds(small, k, v, None, None, None, do[:, -last:], r)
+    for name, t in (("o", out[:, -last:]), ("dq", dq[:, -last:]), ("dk", dk), ("dv", dv)):
+        assert bool(((t.double() - r[name]).abs() <= b[name]).all()), name
+    assert bool((dq[:, :-last] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_two_streams_graph_replays_and_repeats(dtype):
     """The same bits on another stream, twice in a row, and in every replay of a captured graph with other work between; a capture while an
     eager graph of the same leaves lives is refused."""

@@ -189,3 +189,16 @@ def test_empty_and_refusals():
                           ((b, b, torch.ones(64, device=DEV), torch.ones(64, device=DEV).bfloat16()), {}, TypeError)):
         with pytest.raises(err):
             ops.sandwich_norm_fwd(*args, **kw)
+
+
+def test_more_rows_than_threads_of_a_launch():
+    """2^27 rows, 32 threads each: the forward takes several launches.  Rows are independent: any part alone gives the same bits."""
+    from snag_amd import ops
+    rows, dim, per = (1 << 27) + 8, 4, 8
+    g = torch.Generator(device=DEV).manual_seed(14)
+    x, y = (torch.empty(rows, dim, device=DEV, dtype=torch.bfloat16).normal_(generator=g) for _ in range(2))
+    gate = torch.randn(rows // per, dim, generator=g, device=DEV)
+    h, z, _ = ops.sandwich_norm_fwd(x, y, gate=gate, res_scale=0.5, want_stats=False)
+    for a, b in ((0, 64), ((1 << 22) - 16, (1 << 22) + 16), (1 << 26, (1 << 26) + 4096), (rows - 4096, rows)):
+        hp, zp, _ = ops.sandwich_norm_fwd(x[a:b], y[a:b], gate=gate[a // per:b // per], res_scale=0.5, want_stats=False)
+        assert torch.equal(h[a:b], hp) and torch.equal(z[a:b], zp), (a, b)
