@@ -5,36 +5,48 @@ namespace snag {
 
 static int elem_size(int dtype) { return dtype == SNAG_F32 ? 4 : 2; }
 
-// How many ranges a loop over `n` keys or rows is cut into when `groups` workgroups exist without cutting.  Two workgroups fit a CU, so a launch
-// runs in rounds of 512; s ranges take ceil(groups s / 512) / s of the uncut time and each costs its partial result's write and read, taken
-// as 12 % of what is left (measured at 192 groups over 4096 rows of 128: 1 range 270 us, 2 155, 3 200).  At least 128 keys or rows a range.
-static int ranges_for(int64_t groups, int64_t n) {
+// Workgroups that run at a time: two of four waves on a CU, or four waves on their own, one per SIMD -- two per SIMD where their registers allow
+// (the kernels' launch bounds): 16-bit forward, and backward up to 64 elements a head.  64 sequences x 8 heads of 64 in bf16 with 8 rows over
+// 4096 keys, ranges for 512 / 1024 / 2048 workgroups: 250 / 162 / 128 us; with 16 rows in fp32 512 / 271 / 275.
+static int slots(int waves, int dtype, int dp, bool backward) {
+    if (waves > 1) return 2 * 256;
+    return dtype != SNAG_F32 && (!backward || dp <= 64) ? 8 * 256 : 4 * 256;
+}
+// How many ranges a loop over `n` keys or rows is cut into when `groups` workgroups exist without cutting.  s ranges take ceil(groups s / slots) / s
+// of the uncut time and each costs its partial result's write and read, taken as 12 % of what is left (192 groups over 4096 rows of 128:
+// the rule's 2 ranges 154 us, 3 ranges 181).  At least 128 keys or rows a range.
+static int ranges_for(int64_t groups, int64_t n, int64_t slots) {
     int best = 1;
     double least = 1e30;
-    for (int s = 1; groups > 0 && groups < 512 && s <= n / 128 && s <= 64; ++s) {
-        const double cost = (double)((groups * s + 511) / 512) / s * (1 + (s > 1 ? 0.12 * s : 0));
+    for (int s = 1; groups > 0 && groups < slots && s <= n / 128 && s <= 64; ++s) {
+        const double cost = (double)((groups * s + slots - 1) / slots) / s * (1 + (s > 1 ? 0.12 * s : 0));
         if (cost < least) least = cost, best = s;
     }
     return best;
 }
 
-// rows_path: a few rows per key/value head (csrc/cross_rows.hip) -- a 32-row product would multiply mostly padding.  One wave a workgroup where
-// 32 rows (keys) are all there is; four otherwise, and for fp32 rows over 64, whose tiles do not fit one wave's registers.
+// rows_path: a few rows per key/value head (csrc/cross_rows.hip) -- a 32-row product would multiply mostly padding.  Up to 4 rows; up to 8 in fp32,
+// whose matrix instructions are 16 times slower (heads of 128, 512 problems over 4096 keys, here / in tiles: 5 rows 438 / 590 us, 8 rows 632 / 580;
+// 64 problems backward: 5 rows 125 / 470, 8 rows 138 / 470).  16 bit, 8 rows in tiles: 234 us, 4.6 TB/s of keys.
+// One wave a workgroup where 32 rows (keys) are all there is; four otherwise, and for the backward of fp32 rows over 64, whose tiles do not fit
+// one wave's registers.
 static CrossPlan cross_plan(int dtype, int B, int Lq, int Lk, int H, int Hkv, int d) {
     CrossPlan p{};
     const int64_t rows = (int64_t)Lq * (H / Hkv), bh = (int64_t)B * Hkv;
     p.dp = d <= 32 ? 32 : d <= 64 ? 64 : 128;
     const bool wide = dtype == SNAG_F32 && p.dp == 128;
-    p.nw_q = rows > 32 || wide ? 4 : 1;
+    p.nw_fwd = rows > 32 ? 4 : 1;
+    p.nw_dq = rows > 32 || wide ? 4 : 1;
     p.nw_k = Lk > 32 || wide ? 4 : 1;
-    p.rows_path = rows <= 4;
+    p.rows_path = rows <= (dtype == SNAG_F32 ? 8 : 4);
     if (p.rows_path) {
         p.s_fwd = p.s_dq = cross_rows_splits(B, Hkv, Lk, d, dtype);
         p.s_dkv = 1;
         return p;
     }
-    p.s_fwd = p.s_dq = ranges_for(bh * ((rows + p.nw_q * 32 - 1) / (p.nw_q * 32)), Lk);
-    p.s_dkv = ranges_for(bh * ((Lk + p.nw_k * 32 - 1) / (p.nw_k * 32)), rows);
+    p.s_fwd = ranges_for(bh * ((rows + p.nw_fwd * 32 - 1) / (p.nw_fwd * 32)), Lk, slots(p.nw_fwd, dtype, p.dp, false));
+    p.s_dq = ranges_for(bh * ((rows + p.nw_dq * 32 - 1) / (p.nw_dq * 32)), Lk, slots(p.nw_dq, dtype, p.dp, true));
+    p.s_dkv = ranges_for(bh * ((Lk + p.nw_k * 32 - 1) / (p.nw_k * 32)), rows, slots(p.nw_k, dtype, p.dp, true));
     return p;
 }
 

@@ -31,7 +31,7 @@ struct CrossArgs {
     float* part;                 // splits > 1: partial results, see the kernels
     // backward
     const void *o, *o_lo, *dout; // [B, Lq, H, d] dense; o_lo or NULL
-    const float* stat;           // [B, Hkv, padded_rows(rows)][2] = lse (+inf: no key seen), sum_d dout * o
+    float* stat;                 // [B, Hkv, padded_rows(rows)][2] = lse (+inf: no key seen), sum_d dout * o: d q writes it, d k / d v read it
     void *dq, *dk, *dv;          // dense, shapes of q, k, v
     int vec_o;                   // 16-byte access legal for the dense tensors (d a multiple of the chunk, aligned bases)
 };
@@ -110,7 +110,7 @@ static inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 // How a call is worked on (csrc/cross.hip chooses)
 struct CrossPlan {
     int rows_path;               // a few rows per key/value head: csrc/cross_rows.hip
-    int nw_q, nw_k;              // waves of a workgroup that owns rows / keys
+    int nw_fwd, nw_dq, nw_k;     // waves of a workgroup that owns rows (forward, d q) / keys
     int dp;                      // d rounded up to what the kernels are built for
     int s_fwd, s_dq, s_dkv;      // ranges
 };

@@ -13,11 +13,12 @@ constexpr float kSlack = 8.f;
 // Workgroup: NW waves x 32 rows; key tiles of KT.  splits > 1: per range part[split][B H Lq][d] = sum exp2(S - m) v (not normalised) and, behind
 // all of those, [split][B H Lq][2] = (m, sum); cross_combine_kernel joins them.
 template <class T, int DP, int NW, int KT, bool DIRECT>
-__global__ __launch_bounds__(NW * 64, NW == 1 || (sizeof(T) == 4 && DP == 128) ? 1 : 2) void cross_fwd_kernel(CrossArgs a) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && (NW == 1 || DP == 128) ? 1 : 2) void cross_fwd_kernel(CrossArgs a) {
     using M = Mma<T>;
     constexpr int NT = NW * 64;
-    __shared__ __attribute__((aligned(16))) T lk[2][KT * DP];
-    __shared__ __attribute__((aligned(16))) T lv[2][KT * DP];
+    constexpr int NB = NW == 1 ? 1 : 2;                    // one wave holds its next tile in registers until it is done with this one
+    __shared__ __attribute__((aligned(16))) T lk[NB][KT * DP];
+    __shared__ __attribute__((aligned(16))) T lv[NB][KT * DP];
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id_uniform(), h = lane >> 5;
     const int64_t tiles = (a.rows + NW * 32 - 1) / (NW * 32);
     const Problem pr = problem_of(a, tiles);
@@ -36,16 +37,16 @@ __global__ __launch_bounds__(NW * 64, NW == 1 || (sizeof(T) == 4 && DP == 128) ?
     // DIRECT: rows behind the last key are read as the last key; what is not seen gets -inf for a score below
     auto fetch = [&](int t) {
         const int key0 = t * KT, end = (DIRECT ? len : a.Lk) - 1;
-        fk.fetch([&](int i) { return kb + min(key0 + i, end) * a.ksl; }, lk[t & 1], a.d, a.vec_k, tid);
-        fv.fetch([&](int i) { return vb + min(key0 + i, end) * a.vsl; }, lv[t & 1], a.d, a.vec_v, tid);
+        fk.fetch([&](int i) { return kb + min(key0 + i, end) * a.ksl; }, lk[t % NB], a.d, a.vec_k, tid);
+        fv.fetch([&](int i) { return vb + min(key0 + i, end) * a.vsl; }, lv[t % NB], a.d, a.vec_v, tid);
         if (!DIRECT) byte = mask_byte(a, b, key0, lane);
     };
     auto store = [&](int t) {
         if constexpr (!DIRECT) {
             now = seen_bits(byte, t * KT, len, lane);
             auto keep = [&](int i) { return (now >> i) & 1; };
-            fk.store(keep, lk[t & 1], a.d, a.vec_k, tid);
-            fv.store(keep, lv[t & 1], a.d, a.vec_v, tid);
+            fk.store(keep, lk[t % NB], a.d, a.vec_k, tid);
+            fv.store(keep, lv[t % NB], a.d, a.vec_v, tid);
         }
     };
     if (DIRECT ? t0 < t1 : t0 * KT < a.Lk) fetch(t0);
@@ -59,7 +60,7 @@ __global__ __launch_bounds__(NW * 64, NW == 1 || (sizeof(T) == 4 && DP == 128) ?
     for (int t = t0; t < t1; ++t) {
         tile_ready();
         if (t + 1 < t1) fetch(t + 1);
-        const T *ck = lk[t & 1], *cv = lv[t & 1];
+        const T *ck = lk[t % NB], *cv = lv[t % NB];
         f32x16 s[KT / 32];
 #pragma unroll
         for (int kt = 0; kt < KT / 32; ++kt) {
@@ -167,17 +168,17 @@ __global__ __launch_bounds__(256) void cross_combine_kernel(CrossArgs a) {
 // ---- host ---------------------------------------------------------------------------------------------------------------
 template <class T, int KT4>
 static void go(const CrossArgs& a, const CrossPlan& p, dim3 grid, hipStream_t st) {
-    const bool direct = p.nw_q == 4 && a.mask == nullptr && a.d == p.dp && a.vec_k && a.vec_v;
+    const bool direct = p.nw_fwd == 4 && a.mask == nullptr && a.d == p.dp && a.vec_k && a.vec_v;
 #define CALL(DP)                                                                                   \
     if (direct) cross_fwd_kernel<T, DP, 4, KT4, true><<<grid, 256, 0, st>>>(a);                    \
-    else if (p.nw_q == 4) cross_fwd_kernel<T, DP, 4, KT4, false><<<grid, 256, 0, st>>>(a);         \
-    else if constexpr (sizeof(T) == 2 || DP < 128) cross_fwd_kernel<T, DP, 1, 32, false><<<grid, 64, 0, st>>>(a)
+    else if (p.nw_fwd == 4) cross_fwd_kernel<T, DP, 4, KT4, false><<<grid, 256, 0, st>>>(a);         \
+    else cross_fwd_kernel<T, DP, 1, 32, false><<<grid, 64, 0, st>>>(a)
     SNAG_CROSS_DP(CALL)
 #undef CALL
 }
 
 int cross_tiles_fwd(const CrossArgs& a, const CrossPlan& p, int dtype, hipStream_t st) {
-    const int64_t tiles = (a.rows + p.nw_q * 32 - 1) / (p.nw_q * 32), n = (int64_t)a.B * a.Hkv * tiles * a.splits;
+    const int64_t tiles = (a.rows + p.nw_fwd * 32 - 1) / (p.nw_fwd * 32), n = (int64_t)a.B * a.Hkv * tiles * a.splits;
     SNAG_REQUIRE(n < kMaxBlocks, SNAG_ERR_UNSUPPORTED, "cross attention: %lld workgroups, at most 2^24 in a launch", (long long)n);
     const dim3 grid((unsigned)n);
     if (dtype == SNAG_F32) go<float, 32>(a, p, grid, st);

@@ -1,4 +1,4 @@
-// Cross attention for at most four rows per key/value head: a single new token, an entity's few modality tokens.
+// Cross attention for at most four rows (fp32: eight) per key/value head: a single new token, an entity's few modality tokens.
 //
 // A 32 x 32 matrix product would multiply mostly padding, and the keys and values are read once whatever is done with them: the work is
 // the stream of K and V from memory, so it runs on the vector pipe.  DP / (16 bytes) lanes hold one key (16 bytes a lane), 64 / that
@@ -89,7 +89,7 @@ __device__ __forceinline__ void store_chunk(T* row, int col, int d, int vec, typ
 }
 
 template <class T, int DP, int R>
-__global__ __launch_bounds__(1024) void cross_rows_fwd_kernel(CrossArgs a, int W) {
+__global__ __launch_bounds__(R > 4 ? 512 : 1024) void cross_rows_fwd_kernel(CrossArgs a, int W) {
     constexpr int C = Chunk<T>::n, LPK = DP / C, NK = 64 / LPK, U = 4;
     extern __shared__ float join[];               // [waves][R][DP + 2]
     const int lane = threadIdx.x & 63, slot = lane / LPK, col = (lane % LPK) * C;
@@ -353,11 +353,11 @@ static int keys_per_step(int d, int dtype) {           // NK * U of the forward
 }
 
 // Waves a problem is given inside one workgroup: enough problems fill the chip with one wave each (4096 waves = 4 per SIMD); fewer are cut
-// over the waves of a workgroup as long as each still has a step of keys.  (The backward needs more than 128 registers: at most eight.)
-static int rows_waves(int64_t problems, int Lk, int step, bool bwd) {
+// over the waves of a workgroup as long as each still has a step of keys.  (The backward, and more than four rows, need more registers than sixteen waves leave: at most eight.)
+static int rows_waves(int64_t problems, int Lk, int step, bool at_most_8) {
     if (problems >= 4096 || Lk <= step) return 1;
     if (problems >= 1024 || Lk <= 4 * step) return 4;
-    return bwd || Lk <= 8 * step ? 8 : 16;
+    return at_most_8 || Lk <= 8 * step ? 8 : 16;
 }
 
 // Key ranges on different workgroups (joined by a second launch, about 5 us).  A workgroup's four rows x 32 keys a step are some 500 vector
@@ -386,7 +386,12 @@ static void rows_launch(const CrossArgs& a, int W, bool bwd, hipStream_t st) {
         case 1: GO(1); break;
         case 2: GO(2); break;
         case 3: GO(3); break;
-        default: GO(4); break;
+        case 4: GO(4); break;
+        default:                                       // fp32 only
+            if constexpr (sizeof(T) == 4) {
+                if (R <= 6) GO(6);
+                else GO(8);
+            }
     }
 #undef GO
 }
@@ -394,7 +399,7 @@ static void rows_launch(const CrossArgs& a, int W, bool bwd, hipStream_t st) {
 static int rows_go(CrossArgs a, int dtype, bool bwd, hipStream_t st) {
     const int step = keys_per_step(a.d, dtype);
     const int64_t problems = (int64_t)a.B * a.Hkv;
-    const int W = rows_waves(problems * a.splits, range_of(a.Lk, a.splits), step, bwd);
+    const int W = rows_waves(problems * a.splits, range_of(a.Lk, a.splits), step, bwd || a.rows > 4);
     // four problems a workgroup of 256 threads where there are that many
     SNAG_REQUIRE(problems * a.splits < 4 * kMaxBlocks, SNAG_ERR_UNSUPPORTED, "cross attention: %lld problems, fewer than 2^26 in a launch", (long long)problems);
     a.per_split = range_of(a.Lk, a.splits);

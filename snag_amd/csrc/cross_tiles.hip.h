@@ -58,7 +58,7 @@ template <class T> struct Mma {
     // A operand whose contraction index runs over the LDS rows: columns col0 .. col0 + 31, LDS rows row0 + 8 (j / 4) + 4 h + j % 4 (row0: of 16).
     // The transposing read hands a group of 16 lanes a 4 x 16 block: lane t addresses row t / 4, columns 4 (t % 4), and receives column t.
     template <int DP> static __device__ __forceinline__ Frag cols(const T* base, int row0, int col0, int lane) {
-        const int r = 4 * (lane >> 5) + ((lane & 15) >> 2), c = col0 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+        [[maybe_unused]] const int r = 4 * (lane >> 5) + ((lane & 15) >> 2), c = col0 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
         union { Frag f; s16x4 h[2]; } u;
 #if defined(__HIP_DEVICE_COMPILE__)
         u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SNAG_LDS s16x4*)(base + row0 * DP + tile_at<T, DP>(r, c) + (c & 7)));
@@ -140,7 +140,7 @@ struct TileFetch {
         for (int u = 0; u < kN; ++u) {
             const int e = u * NT + tid, i = e / kPerRow;
             if constexpr (DIRECT) {
-                const T* p = row(i) + chunk_place<T, DP>(i, e % kPerRow) * C;
+                [[maybe_unused]] const T* p = row(i) + chunk_place<T, DP>(i, e % kPerRow) * C;
 #if defined(__HIP_DEVICE_COMPILE__)
                 __builtin_amdgcn_global_load_lds((SNAG_GLOBAL void*)p, (SNAG_LDS void*)(lds + (u * NT + (tid & ~63)) * C), 16, 0, 0);
 #endif
