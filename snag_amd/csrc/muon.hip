@@ -620,7 +620,7 @@ __global__ __launch_bounds__(threads_of(TILE, NST), 2) void muon_product_kernel(
 }
 
 // A from its ranges: a workgroup per 32 x 32 block of the 128 x 128 tiles, each of its four waves adds up a quarter of the ranges, in order; the
-// quarters are joined through LDS.  Grid (16 x the largest number of tiles, matrices)
+// quarters are joined through LDS (eight waves: 10 us instead of 6 for six matrices around 1024 x 1024).  Grid (16 x the largest number of tiles, matrices)
 __global__ __launch_bounds__(256) void muon_gram_sum_kernel(const MuonTable* __restrict__ L) {
     __shared__ float block[32 * kPitch];
     __shared__ __attribute__((aligned(16))) f32x16 part[3][64];
@@ -651,158 +651,164 @@ __global__ __launch_bounds__(256) void muon_gram_sum_kernel(const MuonTable* __r
 }
 
 // ---- one side of at most 128 ------------------------------------------------------------------------------------------------
-// A is one 128 x 128 tile: every workgroup of a 128-column block of X computes B for itself, in LDS, and goes on to its block of the new X and
+// A is one 128 x 128 tile: every workgroup of a 64-column block of X computes B for itself, in LDS, and goes on to its block of the new X and
 // that block's share of the next A.  An iteration is two launches (this one and muon_gram_sum_kernel, which adds the shares up) in place of
-// four, and these matrices are all launch latency: 128 x 128 .. 128 x 4096, 22 launches of 6-14 us before, 13 now.
-// LDS images are [128 rows][128] fp16, chunk c (16 bytes) of row r at place c ^ (4 (r % 4) + r / 4 % 4): without bank conflicts both for
-// fragments along the rows and for transposing reads across them.
-constexpr int kImage = 128 * 128;
-__device__ __forceinline__ int image_at(int row, int col) { return row * 128 + (((col >> 3) ^ (((row & 3) << 2) | ((row >> 2) & 3))) << 3) + (col & 7); }
-__device__ __forceinline__ void image_load(const _Float16* src, int ld, _Float16* lds, int wave, int lane) {
+// four, and these matrices are all latency: 128 x 128 .. 128 x 4096, 22 launches of 6-14 us before, 13 now.  Eight waves, two a SIMD, of 64 x 32 (A^2,
+// the shares) and 32 x 32 (B X) hide each other's waits (128 x 128 .. 128 x 4096 in fp32: 14.7 us a launch; 17.9 with 128 columns and four waves).
+// LDS images: [128 rows][128] fp16 with chunk c (16 bytes) of row r at place c ^ (4 (r % 4) + r / 4 % 4), and X's block [128 rows][64] with chunk c at
+// c ^ (4 (r / 2 % 2) + r / 4 % 4): without bank conflicts both for fragments along the rows and for transposing reads across them.
+constexpr int kBlock = 64;                                             // columns of X per workgroup
+template <int COLS> struct Image {
+    static constexpr int kSize = 128 * COLS, kChunks = COLS / 8;
+    static __device__ __forceinline__ int turn(int row) { return COLS == 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : (((row >> 1) & 1) << 2) | ((row >> 2) & 3); }
+    static __device__ __forceinline__ int at(int row, int col) { return row * COLS + (((col >> 3) ^ turn(row)) << 3) + (col & 7); }
+    static __device__ __forceinline__ void load(const _Float16* src, int ld, _Float16* lds, int wave, int lane) {
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-        const int e = (u * 4 + wave) * 64 + lane, r = e >> 4, c = (e & 15) ^ (((r & 3) << 2) | ((r >> 2) & 3));
-        to_lds(src + (int64_t)r * ld + c * 8, lds + (u * 4 + wave) * 512);
+        for (int u = 0; u < kSize / 8 / 512; ++u) {
+            const int e = (u * 8 + wave) * 64 + lane, r = e / kChunks, c = e % kChunks ^ turn(r);
+            to_lds(src + (int64_t)r * ld + c * 8, lds + (u * 8 + wave) * 512);
+        }
     }
-}
-__device__ __forceinline__ f16x8 image_rows(const _Float16* lds, int row, int kb, int lane) { return *(const f16x8*)(lds + image_at(row + (lane & 31), kb * 16 + (lane >> 5) * 8)); }
-__device__ __forceinline__ f16x8 image_cols(const _Float16* lds, int col, int kb, int lane) {
-    union { f16x8 f; s16x4 h[2]; } v;
-    const int r = kb * 16 + (lane >> 5) * 8 + ((lane & 15) >> 2), n = col + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+    static __device__ __forceinline__ f16x8 rows(const _Float16* lds, int row, int kb, int lane) { return *(const f16x8*)(lds + at(row + (lane & 31), kb * 16 + (lane >> 5) * 8)); }
+    static __device__ __forceinline__ f16x8 cols(const _Float16* lds, int col, int kb, int lane) {
+        union { f16x8 f; s16x4 h[2]; } v;
+        [[maybe_unused]] const int r = kb * 16 + (lane >> 5) * 8 + ((lane & 15) >> 2), n = col + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
 #if defined(__HIP_DEVICE_COMPILE__)
 #pragma unroll
-    for (int w = 0; w < 2; ++w) v.h[w] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SNAG_LDS s16x4*)(lds + image_at(r + 4 * w, n)));
+        for (int w = 0; w < 2; ++w) v.h[w] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SNAG_LDS s16x4*)(lds + at(r + 4 * w, n)));
 #endif
-    return v.f;
-}
-// 64 x 64 part (wm, wn) of a product of two images, block q at (q / 2, q % 2); RIGHT_COLS: the right operand's contraction runs down its rows.
-// The next 16 of the contraction are read while the present ones are multiplied.
-template <int PLANES, bool RIGHT_COLS>
-__device__ __forceinline__ void image_product(f32x16 (&acc)[4], const _Float16* left, const _Float16* right, int wm, int wn, int lane) {
+        return v.f;
+    }
+    static __device__ __forceinline__ Pairs pairs(const _Float16* lds, int row, int col) {
+        const _Float16* lo = lds + kSize;
+        return Pairs{{*(const f16x8*)(lds + at(row, col)), *(const f16x8*)(lds + at(row, col + 8))}, {*(const f16x8*)(lo + at(row, col)), *(const f16x8*)(lo + at(row, col + 8))}};
+    }
+    static __device__ __forceinline__ void store(_Float16* lds, int row, int col, const Pairs& p) {
+        _Float16* lo = lds + kSize;
+        *(f16x8*)(lds + at(row, col)) = p.hi[0], *(f16x8*)(lds + at(row, col + 8)) = p.hi[1];
+        *(f16x8*)(lo + at(row, col)) = p.lo[0], *(f16x8*)(lo + at(row, col + 8)) = p.lo[1];
+    }
+};
+// NB blocks of 32 x 32 below each other over 16 KB of the contraction: left(plane, block, kb) and right(plane, kb) are the fragments.  The next 16 of the
+// contraction are read while the present ones are multiplied.
+template <int PLANES, int NB, int KB, class Left, class Right>
+__device__ __forceinline__ void image_product(f32x16 (&acc)[NB], Left left, Right right) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) acc[q] = f32x16{};
-    f16x8 fa[2][PLANES][2], fb[2][PLANES][2];
+    for (int i = 0; i < NB; ++i) acc[i] = f32x16{};
+    f16x8 fa[2][PLANES][NB], fb[2][PLANES];
     auto read = [&](int kb) {
 #pragma unroll
-        for (int p = 0; p < PLANES; ++p)
+        for (int p = 0; p < PLANES; ++p) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                fa[kb & 1][p][i] = image_rows(left + p * kImage, wm + i * 32, kb, lane);
-                fb[kb & 1][p][i] = RIGHT_COLS ? image_cols(right + p * kImage, wn + i * 32, kb, lane) : image_rows(right + p * kImage, wn + i * 32, kb, lane);
-            }
+            for (int i = 0; i < NB; ++i) fa[kb & 1][p][i] = left(p, i, kb);
+            fb[kb & 1][p] = right(p, kb);
+        }
     };
     read(0);
 #pragma unroll
-    for (int kb = 0; kb < 8; ++kb) {
-        if (kb < 7) read(kb + 1);
+    for (int kb = 0; kb < KB; ++kb) {
+        if (kb + 1 < KB) read(kb + 1);
         __builtin_amdgcn_sched_barrier(0);
-        const int s = kb & 1;
+        [[maybe_unused]] const int s = kb & 1;
 #if defined(__HIP_DEVICE_COMPILE__)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            acc[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[s][0][q >> 1], fb[s][0][q & 1], acc[q], 0, 0, 0);
+        for (int i = 0; i < NB; ++i) {
+            acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[s][0][i], fb[s][0], acc[i], 0, 0, 0);
             if constexpr (PLANES == 2) {
-                acc[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[s][0][q >> 1], fb[s][1][q & 1], acc[q], 0, 0, 0);
-                acc[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[s][1][q >> 1], fb[s][0][q & 1], acc[q], 0, 0, 0);
+                acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[s][0][i], fb[s][1], acc[i], 0, 0, 0);
+                acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[s][1][i], fb[s][0], acc[i], 0, 0, 0);
             }
         }
 #endif
         __builtin_amdgcn_sched_barrier(0);
     }
 }
-__device__ __forceinline__ Pairs image_pairs(const _Float16* hi, const _Float16* lo, int row, int col) {
-    return Pairs{{*(const f16x8*)(hi + image_at(row, col)), *(const f16x8*)(hi + image_at(row, col + 8))},
-                 {*(const f16x8*)(lo + image_at(row, col)), *(const f16x8*)(lo + image_at(row, col + 8))}};
-}
-__device__ __forceinline__ void image_store(_Float16* hi, _Float16* lo, int row, int col, const Pairs& p) {
-    *(f16x8*)(hi + image_at(row, col)) = p.hi[0], *(f16x8*)(hi + image_at(row, col + 8)) = p.hi[1];
-    *(f16x8*)(lo + image_at(row, col)) = p.lo[0], *(f16x8*)(lo + image_at(row, col + 8)) = p.lo[1];
-}
 
-// start: only the first A's shares of X copy 0.  One workgroup per 128-column block; slab[block][4][4][1024] as the product kernel's ranges.
+// start: only the first A's shares of X copy 0.  One workgroup per 64-column block; slab[block][4][4][1024] as the product kernel's ranges.
 template <int DT>
-__global__ __launch_bounds__(256) void muon_narrow_kernel(const MuonTable* __restrict__ L, MuonFirst first, int from, int start, int last) {
+__global__ __launch_bounds__(512) void muon_narrow_kernel(const MuonTable* __restrict__ L, MuonFirst first, int from, int start, int last) {
     constexpr int PLANES = DT == SNAG_BF16 ? 1 : 2;
+    using IX = Image<kBlock>;
+    using IS = Image<128>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    _Float16 *X = (_Float16*)smem, *S = X + 2 * kImage;                // hi, lo of X's block; hi, lo of A, later of B
-    float* diag = (float*)(S + 2 * kImage);                            // B's diagonal [128], and behind it the waves' 32 x kPitch blocks
+    _Float16 *X = (_Float16*)smem, *S = X + 2 * IX::kSize;             // hi, lo of X's block; hi, lo of A, later of B
+    float* diag = (float*)(S + 2 * IS::kSize);                         // B's diagonal [128], and behind it the waves' 32 x kPitch blocks
     const int lane = threadIdx.x & 63, wave = wave_id_uniform();
     float* block = diag + 128 + wave * 32 * kPitch;
     int begin;
     const MuonMatrix a = L->a[matrix_of(first, blockIdx.x, begin)];
-    const int col0 = ((int)blockIdx.x - begin) * 128;
-    const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-    image_load(x_plane(a, from, 0) + col0, a.np, X, wave, lane);
-    image_load(x_plane(a, from, 1) + col0, a.np, X + kImage, wave, lane);
-    f32x16 acc[4];
+    const int col0 = ((int)blockIdx.x - begin) * kBlock;
+    const int wm = (wave >> 2) * 64, wn = (wave & 3) * 32;             // 64 x 32 of A, B
+    const int xm = (wave >> 1) * 32, xn = (wave & 1) * 32;             // 32 x 32 of X's block
+    IX::load(x_plane(a, from, 0) + col0, a.np, X, wave, lane);
+    IX::load(x_plane(a, from, 1) + col0, a.np, X + IX::kSize, wave, lane);
+    f32x16 acc[2];
     const int r = lane >> 1, c = (lane & 1) * 16;
     if (!start) {
-        image_load(s_plane(a, 0), 128, S, wave, lane);
-        image_load(s_plane(a, 1), 128, S + kImage, wave, lane);
+        IS::load(s_plane(a, 0), 128, S, wave, lane);
+        IS::load(s_plane(a, 1), 128, S + IS::kSize, wave, lane);
         const float* da = diagonal(a, 0);
-        float di[2], dj[2][16];
+        float di[2], dj[16];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) di[i] = da[wm + i * 32 + r], load16(dj[i], da + wn + i * 32 + c);
+        for (int i = 0; i < 2; ++i) di[i] = da[wm + i * 32 + r];
+        load16(dj, da + wn + c);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        image_product<PLANES, false>(acc, S, S, wm, wn, lane);
+        image_product<PLANES, 2, 8>(acc, [&](int p, int i, int kb) { return IS::rows(S + p * IS::kSize, wm + i * 32, kb, lane); },
+                                    [&](int p, int kb) { return IS::rows(S + p * IS::kSize, wn, kb, lane); });
         // B in the place of A
-        Pairs b[4];
+        Pairs b[2];
         float db[2] = {0.f, 0.f};
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int row = wm + (q >> 1) * 32 + r, col = wn + (q & 1) * 32 + c;
-            const Pairs p = image_pairs(S, S + kImage, row, col);
+        for (int i = 0; i < 2; ++i) {
+            const int row = wm + i * 32 + r, col = wn + c;
+            const Pairs p = IS::pairs(S, row, col);
             float v[16];
-            through_block(block, acc[q], v, lane);
-            const float d = poly(v, p, di[q >> 1], dj[q & 1], row - col, wm + (q >> 1) * 32 == wn + (q & 1) * 32);
-            if (row >= col && row < col + 16) db[q >> 1] = d;
-            b[q] = pairs_of(v);
+            through_block(block, acc[i], v, lane);
+            db[i] = poly(v, p, di[i], dj, row - col, wm + i * 32 == wn);
+            b[i] = pairs_of(v);
         }
         __syncthreads();
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int row = wm + (q >> 1) * 32 + r, col = wn + (q & 1) * 32 + c;
-            image_store(S, S + kImage, row, col, b[q]);
-            if (row >= col && row < col + 16) diag[row] = db[q >> 1];
+        for (int i = 0; i < 2; ++i) {
+            const int row = wm + i * 32 + r, col = wn + c;
+            IS::store(S, row, col, b[i]);
+            if (row >= col && row < col + 16) diag[row] = db[i];
         }
         __syncthreads();
-        image_product<PLANES, true>(acc, S, X, wm, wn, lane);
-        Pairs y[4];
+        f32x16 bx[1];
+        image_product<PLANES, 1, 8>(bx, [&](int p, int, int kb) { return IS::rows(S + p * IS::kSize, xm, kb, lane); },
+                                    [&](int p, int kb) { return IX::cols(X + p * IX::kSize, xn, kb, lane); });
+        const int row = xm + r, col = xn + c;
+        const Pairs p = IX::pairs(X, row, col);
+        float v[16];
+        through_block(block, bx[0], v, lane);
+        const float d = kNsA + diag[row];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int row = wm + (q >> 1) * 32 + r, col = wn + (q & 1) * 32 + c;
-            const Pairs p = image_pairs(X, X + kImage, row, col);
-            float v[16];
-            through_block(block, acc[q], v, lane);
-            const float d = kNsA + diag[row];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = fmaf(d, sum_of(p, j), v[j] * (1.f / kScaleA));
-            if (last) {
-                store_result<TypeOf<DT>>(L, a, v, wm + (q >> 1) * 32, col0 + wn + (q & 1) * 32, block, lane);
-                continue;
-            }
-            y[q] = pairs_of(v);
-            const int64_t at = (int64_t)row * a.np + col0 + col;
-            store_pairs(x_plane(a, from ^ 1, 0) + at, x_plane(a, from ^ 1, 1) + at, y[q]);
+        for (int j = 0; j < 16; ++j) v[j] = fmaf(d, sum_of(p, j), v[j] * (1.f / kScaleA));
+        if (last) {
+            store_result<TypeOf<DT>>(L, a, v, xm, col0 + xn, block, lane);
+            return;
         }
-        if (last) return;
+        const Pairs y = pairs_of(v);
+        const int64_t at = (int64_t)row * a.np + col0 + col;
+        store_pairs(x_plane(a, from ^ 1, 0) + at, x_plane(a, from ^ 1, 1) + at, y);
         __syncthreads();
-#pragma unroll
-        for (int q = 0; q < 4; ++q) image_store(X, X + kImage, wm + (q >> 1) * 32 + r, wn + (q & 1) * 32 + c, y[q]);
+        IX::store(X, row, col, y);
     } else {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
     __syncthreads();
-    image_product<PLANES, false>(acc, X, X, wm, wn, lane);
+    image_product<PLANES, 2, kBlock / 16>(acc, [&](int p, int i, int kb) { return IX::rows(X + p * IX::kSize, wm + i * 32, kb, lane); },
+                                          [&](int p, int kb) { return IX::rows(X + p * IX::kSize, wn, kb, lane); });
     if (a.splits == 1) {                                               // the only block: A is complete
 #pragma unroll
-        for (int q = 0; q < 4; ++q) finish<kGram, DT>(L, a, acc[q], Pairs{}, Diagonals{}, wm + (q >> 1) * 32, wn + (q & 1) * 32, false, 0, false, block, lane);
+        for (int i = 0; i < 2; ++i) finish<kGram, DT>(L, a, acc[i], Pairs{}, Diagonals{}, wm + i * 32, wn, false, 0, false, block, lane);
         return;
     }
-    float* out = slab_of(a) + (int64_t)(col0 / 128) * 16 * 1024 + lane * 16;
+    float* out = slab_of(a) + (int64_t)(col0 / kBlock) * 16 * 1024 + lane * 16;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) *(f32x16*)(out + ((wm / 32 + (q >> 1)) * 4 + wn / 32 + (q & 1)) * 1024) = acc[q];
+    for (int i = 0; i < 2; ++i) *(f32x16*)(out + ((wm / 32 + i) * 4 + wn / 32) * 1024) = acc[i];
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
@@ -829,10 +835,11 @@ static MuonPlan plan_of(const int32_t* rows, const int32_t* cols, const int* at,
     p.stages = (int)(per < 4 ? 4 : per);
     return p;
 }
-static int splits_of(const MuonPlan& p, int np) { return p.narrow ? np / 128 : (np / 64 + p.stages - 1) / p.stages; }
+static int splits_of(const MuonPlan& p, int np) { return p.narrow ? np / kBlock : (np / 64 + p.stages - 1) / p.stages; }
+static int pad_n(const MuonPlan& p, int n) { return pad_to(n, p.narrow ? kBlock : p.tile); }
 
 static int64_t matrix_bytes(const MuonPlan& p, int r, int c) {
-    const int m = r < c ? r : c, n = r < c ? c : r, mp = pad_to(m, p.tile), np = pad_to(n, p.tile), s = splits_of(p, np);
+    const int m = r < c ? r : c, n = r < c ? c : r, mp = pad_to(m, p.tile), np = pad_n(p, n), s = splits_of(p, np);
     const int64_t x = (int64_t)mp * np, q = (int64_t)mp * mp, t = mp / 128;
     const int64_t bytes = 8 * x + 8 * q + 8 * kNormParts + 8 * (int64_t)mp + (s > 1 ? 4 * s * (t * (t + 1) / 2) * 128 * 128 : 0);
     return (bytes + 255) / 256 * 256;
@@ -900,14 +907,14 @@ static int muon_go(const MuonRun& R, int steps, hipStream_t st) {
     muon_start_kernel<DT><<<gs, 256, 0, st>>>(R.table);
     if (int rc = check_launch("muon_start")) return rc;
     if (R.plan.narrow) {
-        constexpr size_t lds = 4 * kImage * sizeof(_Float16) + (4 * 32 * kPitch + 128) * sizeof(float);
+        constexpr size_t lds = 2 * (Image<kBlock>::kSize + Image<128>::kSize) * sizeof(_Float16) + (8 * 32 * kPitch + 128) * sizeof(float);
         static_assert(lds <= 160 * 1024, "one CU's LDS");
         static std::atomic<uint64_t> done{0};
         if (int rc = grow_lds(muon_narrow_kernel<DT>, lds, done)) return rc;
         for (int k = -1; k < steps; ++k) {
             if (k >= 0)
                 if (int rc = gram_sum(R, st)) return rc;
-            muon_narrow_kernel<DT><<<dim3(R.blocks_of[kApply]), 256, lds, st>>>(R.table, R.first[kApply], k < 0 ? 0 : k & 1, k < 0, k + 1 == steps);
+            muon_narrow_kernel<DT><<<dim3(R.blocks_of[kApply]), 512, lds, st>>>(R.table, R.first[kApply], k < 0 ? 0 : k & 1, k < 0, k + 1 == steps);
             if (int rc = check_launch("muon_narrow")) return rc;
         }
         return SNAG_OK;
@@ -972,7 +979,7 @@ static int muon_run(const char* what, void* const* w, const void* const* g, floa
             const int r = rows[at[i]], c = cols[at[i]];
             a.g = g[at[i]], a.w = w[at[i]], a.mom = mom != nullptr ? mom[at[i]] : nullptr, a.work = space;
             a.r = r, a.c = c, a.tall = r > c, a.m = r < c ? r : c, a.n = r < c ? c : r;
-            a.mp = pad_to(a.m, tile), a.np = pad_to(a.n, tile);
+            a.mp = pad_to(a.m, tile), a.np = pad_n(R.plan, a.n);
             a.splits = splits_of(R.plan, a.np);
             const double s = match_rms ? 0.2 * sqrt((double)a.n) : sqrt(r > c ? (double)r / c : 1.0);
             a.update = (float)(lr * s);
@@ -982,7 +989,7 @@ static int muon_run(const char* what, void* const* w, const void* const* g, floa
             for (int q = 0; q < 3; ++q) R.first[q].at[i] = R.blocks_of[q];
             R.blocks_of[kGram] += tri * a.splits;
             R.blocks_of[kPoly] += tri;
-            R.blocks_of[kApply] += (a.mp / tile) * (a.np / tile);
+            R.blocks_of[kApply] += R.plan.narrow ? a.np / kBlock : (a.mp / tile) * (a.np / tile);
             R.blocks = b > R.blocks ? b : R.blocks;
             if (a.splits > 1 && tri > R.gram_tiles) R.gram_tiles = tri;
             R.vec = R.vec && (int64_t)r * c % 4 == 0 && aligned16(a.g) && aligned16(a.mom);
