@@ -12,14 +12,15 @@ static int slots(int waves, int dtype, int dp, bool backward) {
     if (waves > 1) return 2 * 256;
     return dtype != SNAG_F32 && (!backward || dp <= 64) ? 8 * 256 : 4 * 256;
 }
-// How many ranges a loop over `n` keys or rows is cut into when `groups` workgroups exist without cutting.  s ranges take ceil(groups s / slots) / s
-// of the uncut time and each costs its partial result's write and read, taken as 12 % of what is left (192 groups over 4096 rows of 128:
-// the rule's 2 ranges 154 us, 3 ranges 181).  At least 128 keys or rows a range.
+// How many ranges a loop over `n` keys or rows is cut into when `groups` workgroups exist without cutting.  In units of 64 keys' or rows' time (1 - 3
+// us): a round of workgroups takes 5 to start and end besides its loop, joining ranges 4 and 0.5 for each (a launch, the partial results).  Both
+// sides: 192 groups over 4096 rows of 128: 2 ranges 154 us, 3 181; 92 groups over 316 keys: 1 range 17, 2 24; 72 groups over 777 keys: 1 range
+// 46, 5 32, 12 40.  At least 128 keys or rows a range.
 static int ranges_for(int64_t groups, int64_t n, int64_t slots) {
     int best = 1;
     double least = 1e30;
-    for (int s = 1; groups > 0 && groups < slots && s <= n / 128 && s <= 64; ++s) {
-        const double cost = (double)((groups * s + slots - 1) / slots) / s * (1 + (s > 1 ? 0.12 * s : 0));
+    for (int s = 1; groups > 0 && groups < slots && s <= 64 && (s == 1 || s <= n / 128); ++s) {
+        const double cost = (double)((groups * s + slots - 1) / slots) * (5 + (double)n / 64 / s) + (s > 1 ? 4 + 0.5 * s : 0);
         if (cost < least) least = cost, best = s;
     }
     return best;
