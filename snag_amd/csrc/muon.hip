@@ -15,8 +15,10 @@
 //     the bf16 result); the linear terms take R and X at 22 bits.
 // A and B are symmetric: only tiles on and below the diagonal are computed, and both halves written.
 // All matrices of the list share each launch.
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
+#include <utility>
 #include "cross.hip.h"
 
 namespace snag {
@@ -44,7 +46,8 @@ struct MuonMatrix {
     void* w;                 // step: the weight; otherwise the output
     char* work;              // this matrix's workspace
     int r, c, m, n, mp, np;  // shape; m <= n; both rounded up to whole tiles
-    int tall, splits;        // A is summed from `splits` ranges of n
+    int tall;
+    int cut[2], ranges[2];   // A (0) and A^2 (1): tiles from `cut` on are summed from `ranges` ranges of the contraction
     float update;            // lr * s
     int vec;                 // rows of g, mom and the result start 16-byte aligned
 };
@@ -483,7 +486,7 @@ __device__ __forceinline__ void finish(const MuonTable* __restrict__ L, const Mu
 // contraction are read while the present ones are multiplied, across the stages too: the barrier that opens a stage stands in front of the
 // last products of the stage before it.
 template <int MODE, int DT, int TILE, int NST>
-__global__ __launch_bounds__(threads_of(TILE, NST), 2) void muon_product_kernel(const MuonTable* __restrict__ L, MuonFirst first, int from, int last) {
+__global__ __launch_bounds__(threads_of(TILE, NST), 2) void muon_product_kernel(const MuonTable* __restrict__ L, MuonFirst first, int whole, int from, int last) {
     constexpr int PLANES = DT == SNAG_BF16 ? 1 : 2;
     using S = Shape<TILE, PLANES, NST>;
     constexpr int NI = S::kWm / 32, NJ = S::kWn / 32, KB = S::kDepth / 16;
@@ -491,27 +494,30 @@ __global__ __launch_bounds__(threads_of(TILE, NST), 2) void muon_product_kernel(
     extern __shared__ __attribute__((aligned(16))) char smem[];
     _Float16* lds = (_Float16*)smem;
     const int lane = threadIdx.x & 63, wave = wave_id_uniform();
-    const int id = (int)xcd_order(blockIdx.x, gridDim.x);
+    // ranges of cut tiles have a launch's last ids, and are dealt over the XCDs as they come
+    const int id = (int)blockIdx.x < whole ? (int)xcd_order(blockIdx.x, whole) : (int)blockIdx.x;
     int begin;
     const MuonMatrix a = L->a[matrix_of(first, id, begin)];
     int k = id - begin, split = 0, ti, tj;
+    bool cut = false;
     if (MODE == kApply) {
         rect_at(k, a.mp / TILE, a.np / TILE, ti, tj);
     } else {
-        const int t = a.mp / TILE;
-        if (MODE == kGram) {
-            const int tiles = t * (t + 1) / 2;
-            split = k / tiles;
-            k -= split * tiles;
+        const int t = a.mp / TILE, c0 = a.cut[MODE];
+        cut = k >= c0;
+        if (cut) {
+            const int n = t * (t + 1) / 2 - c0;
+            split = (k - c0) / n;
+            k = c0 + (k - c0) % n;
         }
         tri_at(k, t, ti, tj);
     }
     const int lda = MODE == kGram ? a.np : a.mp;
     int k0 = 0, k1 = lda;
-    if (MODE == kGram && a.splits > 1) {
-        const int per = (a.np / 64 + a.splits - 1) / a.splits * 64;
+    if (MODE != kApply && cut) {
+        const int per = (lda / 64 + a.ranges[MODE] - 1) / a.ranges[MODE] * 64;
         k0 = split * per;
-        k1 = min(a.np, k0 + per);
+        k1 = min(lda, k0 + per);
     }
     const int n = k1 > k0 ? (k1 - k0) / S::kDepth : 0;                 // stages
     const _Float16* left = MODE == kGram ? x_plane(a, from, 0) : s_plane(a, MODE == kPoly ? 0 : 2);
@@ -599,10 +605,10 @@ __global__ __launch_bounds__(threads_of(TILE, NST), 2) void muon_product_kernel(
             __builtin_amdgcn_sched_barrier(0);
         }
     }
-    if (MODE == kGram && a.splits > 1) {
-        // the range's partial tile, 32 x 32 blocks in register order: muon_gram_sum_kernel adds the ranges up
-        const int t = a.mp / TILE, tiles = t * (t + 1) / 2;
-        float* out = slab_of(a) + (int64_t)(split * tiles + k) * 16 * 1024 + lane * 16;
+    if (MODE != kApply && cut) {
+        // the range's partial tile, 32 x 32 blocks in register order: muon_sum_kernel adds the ranges up
+        const int t = a.mp / TILE, c0 = a.cut[MODE], n = t * (t + 1) / 2 - c0;
+        float* out = slab_of(a) + (int64_t)(split * n + k - c0) * 16 * 1024 + lane * 16;
 #pragma unroll
         for (int i = 0; i < NI; ++i)
 #pragma unroll
@@ -619,15 +625,16 @@ __global__ __launch_bounds__(threads_of(TILE, NST), 2) void muon_product_kernel(
     }
 }
 
-// A from its ranges: a workgroup per 32 x 32 block of the 128 x 128 tiles, each of its four waves adds up a quarter of the ranges, in order; the
-// quarters are joined through LDS (eight waves: 10 us instead of 6 for six matrices around 1024 x 1024).  Grid (16 x the largest number of tiles, matrices)
-__global__ __launch_bounds__(256) void muon_gram_sum_kernel(const MuonTable* __restrict__ L) {
+// The cut tiles of A or A^2 from their ranges: a workgroup per 32 x 32 block of the 128 x 128 tiles, each of its four waves adds up a quarter of the ranges, in order; the
+// quarters are joined through LDS (eight waves: 10 us instead of 6 for six matrices around 1024 x 1024).  Grid (16 x the largest number of cut tiles, matrices)
+template <int MODE>
+__global__ __launch_bounds__(256) void muon_sum_kernel(const MuonTable* __restrict__ L) {
     __shared__ float block[32 * kPitch];
     __shared__ __attribute__((aligned(16))) f32x16 part[3][64];
     const MuonMatrix a = L->a[blockIdx.y];
-    const int t = a.mp / 128, tiles = t * (t + 1) / 2, id = blockIdx.x >> 4, sub = blockIdx.x & 15, lane = threadIdx.x & 63, quarter = wave_id_uniform();
-    if (a.splits == 1 || id >= tiles) return;     // the whole workgroup
-    const int per = (a.splits + 3) / 4, s1 = min(a.splits, (quarter + 1) * per);
+    const int t = a.mp / 128, tiles = t * (t + 1) / 2 - a.cut[MODE], id = blockIdx.x >> 4, sub = blockIdx.x & 15, lane = threadIdx.x & 63, quarter = wave_id_uniform();
+    if (id >= tiles) return;     // the whole workgroup
+    const int per = (a.ranges[MODE] + 3) / 4, s1 = min(a.ranges[MODE], (quarter + 1) * per);
     int s = quarter * per;
     f32x16 acc{};
     const int64_t step = (int64_t)tiles * 16 * 1024;
@@ -646,13 +653,14 @@ __global__ __launch_bounds__(256) void muon_gram_sum_kernel(const MuonTable* __r
 #pragma unroll
     for (int u = 0; u < 3; ++u) acc += part[u][lane];
     int i, j;
-    tri_at(id, t, i, j);
-    finish<kGram, SNAG_F32>(L, a, acc, Pairs{}, Diagonals{}, i * 128 + (sub >> 2) * 32, j * 128 + (sub & 3) * 32, i != j, 0, false, block, lane);
+    tri_at(a.cut[MODE] + id, t, i, j);
+    const int row0 = i * 128 + (sub >> 2) * 32, col0 = j * 128 + (sub & 3) * 32;
+    finish<MODE, SNAG_F32>(L, a, acc, block_pairs<MODE>(a, row0, col0, 0, lane), block_diagonals<MODE>(a, row0, col0, lane), row0, col0, i != j, 0, false, block, lane);
 }
 
 // ---- one side of at most 128 ------------------------------------------------------------------------------------------------
 // A is one 128 x 128 tile: every workgroup of a 64-column block of X computes B for itself, in LDS, and goes on to its block of the new X and
-// that block's share of the next A.  An iteration is two launches (this one and muon_gram_sum_kernel, which adds the shares up) in place of
+// that block's share of the next A.  An iteration is two launches (this one and muon_sum_kernel, which adds the shares up) in place of
 // four, and these matrices are all latency: 128 x 128 .. 128 x 4096, 22 launches of 6-14 us before, 13 now.  Eight waves, two a SIMD, of 64 x 32 (A^2,
 // the shares) and 32 x 32 (B X) hide each other's waits (128 x 128 .. 128 x 4096 in fp32: 14.7 us a launch; 17.9 with 128 columns and four waves).
 // LDS images: [128 rows][128] fp16 with chunk c (16 bytes) of row r at place c ^ (4 (r % 4) + r / 4 % 4), and X's block [128 rows][64] with chunk c at
@@ -801,7 +809,7 @@ __global__ __launch_bounds__(512) void muon_narrow_kernel(const MuonTable* __res
     __syncthreads();
     image_product<PLANES, 2, kBlock / 16>(acc, [&](int p, int i, int kb) { return IX::rows(X + p * IX::kSize, wm + i * 32, kb, lane); },
                                           [&](int p, int kb) { return IX::rows(X + p * IX::kSize, wn, kb, lane); });
-    if (a.splits == 1) {                                               // the only block: A is complete
+    if (a.ranges[kGram] == 1) {                                        // the only block: A is complete
 #pragma unroll
         for (int i = 0; i < 2; ++i) finish<kGram, DT>(L, a, acc[i], Pairs{}, Diagonals{}, wm + i * 32, wn, false, 0, false, block, lane);
         return;
@@ -818,9 +826,12 @@ constexpr int kCus = 256;
 // How one list of matrices is worked on.  narrow: every m <= 128 (muon_narrow_kernel).  Otherwise 256 x 256 tiles for the product with X when the
 // list has enough of them to occupy most CUs (they read half as much per multiplication; 128 x 128 ones fill the chip earlier).  The symmetric
 // products, half as many tiles, always run on 128 x 128 ones.
-struct MuonPlan { bool narrow; int tile, stages; };
+struct MuonPlan { bool narrow; int tile, stages, over, over_ranges[2]; };
+static int pad_n(const MuonPlan& p, int n) { return pad_to(n, p.narrow ? kBlock : p.tile); }
+static int splits_of(const MuonPlan& p, int np) { return p.narrow ? np / kBlock : (np / 64 + p.stages - 1) / p.stages; }
 static MuonPlan plan_of(const int32_t* rows, const int32_t* cols, const int* at, int count) {
-    MuonPlan p{true, 128, 4};
+    MuonPlan p{};
+    p.narrow = true, p.tile = 128;
     int64_t big = 0, total = 0;
     for (int k = 0; k < count; ++k) {
         const int r = rows[at[k]], c = cols[at[k]], m = r < c ? r : c, n = r < c ? c : r;
@@ -833,15 +844,43 @@ static MuonPlan plan_of(const int32_t* rows, const int32_t* cols, const int* at,
     // LDS stages in a range of A's contraction: the list's stages over all CUs, at least four
     const int64_t per = (total + kCus - 1) / kCus;
     p.stages = (int)(per < 4 ? 4 : per);
+    // The symmetric products run 512 tiles at a time.  A few tiles more (up to 128) would be a round of their own on an empty chip: the last tiles of the
+    // last matrix, the list's largest, are cut into ranges of at least eight stages that fill it (4096 x 4096 in bf16, 16 tiles over: 116 -> 91 us and 5 for muon_sum_kernel).
+    if (p.narrow) return p;
+    int64_t tiles = 0;
+    bool split = false;
+    for (int k = 0; k < count; ++k) {
+        const int r = rows[at[k]], c = cols[at[k]], t = pad_to(r < c ? r : c, p.tile) / 128;
+        tiles += t * (t + 1) / 2;
+        split = split || splits_of(p, pad_n(p, r < c ? c : r)) > 1;
+    }
+    const int r = rows[at[count - 1]], c = cols[at[count - 1]], mp = pad_to(r < c ? r : c, p.tile), np = pad_n(p, r < c ? c : r), t = mp / 128;
+    const int over = (int)(tiles % (2 * kCus));
+    if (split || tiles < 2 * kCus || over == 0 || over > kCus / 2 || over > t * (t + 1) / 2 || mp < 64 * 16) return p;
+    p.over = over;
+    for (int q = 0; q < 2; ++q) {
+        const int most = (q ? mp : np) / 64 / 8, want = 2 * kCus / over;
+        p.over_ranges[q] = most < want ? most : want;
+    }
     return p;
 }
-static int splits_of(const MuonPlan& p, int np) { return p.narrow ? np / kBlock : (np / 64 + p.stages - 1) / p.stages; }
-static int pad_n(const MuonPlan& p, int n) { return pad_to(n, p.narrow ? kBlock : p.tile); }
 
-static int64_t matrix_bytes(const MuonPlan& p, int r, int c) {
-    const int m = r < c ? r : c, n = r < c ? c : r, mp = pad_to(m, p.tile), np = pad_n(p, n), s = splits_of(p, np);
-    const int64_t x = (int64_t)mp * np, q = (int64_t)mp * mp, t = mp / 128;
-    const int64_t bytes = 8 * x + 8 * q + 8 * kNormParts + 8 * (int64_t)mp + (s > 1 ? 4 * s * (t * (t + 1) / 2) * 128 * 128 : 0);
+// where the cut tiles of matrix `r` x `c` begin and how many ranges each has, for A and A^2
+static void cuts_of(const MuonPlan& p, int mp, int np, bool last, int (&cut)[2], int (&ranges)[2]) {
+    const int t = mp / 128, tiles = t * (t + 1) / 2, s = splits_of(p, np);
+    for (int q = 0; q < 2; ++q) {
+        ranges[q] = last && p.over > 0 ? p.over_ranges[q] : q == 0 ? s : 1;
+        cut[q] = last && p.over > 0 ? tiles - p.over : ranges[q] > 1 ? 0 : tiles;
+    }
+}
+static int64_t matrix_bytes(const MuonPlan& p, int r, int c, bool last) {
+    const int m = r < c ? r : c, n = r < c ? c : r, mp = pad_to(m, p.tile), np = pad_n(p, n), t = mp / 128;
+    int cut[2], ranges[2];
+    cuts_of(p, mp, np, last, cut, ranges);
+    int64_t slab = 0;                                              // 128 x 128 partial tiles: A's, then A^2's
+    for (int q = 0; q < 2; ++q) slab = std::max(slab, (int64_t)ranges[q] * (t * (t + 1) / 2 - cut[q]));
+    const int64_t x = (int64_t)mp * np, q = (int64_t)mp * mp;
+    const int64_t bytes = 8 * x + 8 * q + 8 * kNormParts + 8 * (int64_t)mp + 4 * slab * 128 * 128;
     return (bytes + 255) / 256 * 256;
 }
 
@@ -854,13 +893,19 @@ struct MuonLists {
         for (n = 0; pass < 2; ++pass, i = 0) {
             for (; i < count && n < kMaxList; ++i)
                 if (((rows[i] < cols[i] ? rows[i] : cols[i]) <= 128) == (pass == 0)) at[n++] = i;
-            if (n > 0) return true;
+            if (n > 0) {
+                int big = 0;                                   // the largest goes last
+                auto side = [&](int k) { return rows[at[k]] < cols[at[k]] ? rows[at[k]] : cols[at[k]]; };
+                for (int k = 1; k < n; ++k) big = side(k) > side(big) ? k : big;
+                std::swap(at[big], at[n - 1]);
+                return true;
+            }
         }
         return false;
     }
 };
 
-struct MuonRun { MuonTable L; MuonFirst first[3]; MuonTable* table; MuonPlan plan; int blocks_of[3], gram_tiles, blocks; bool vec; };
+struct MuonRun { MuonTable L; MuonFirst first[3]; MuonTable* table; MuonPlan plan; int blocks_of[3], cut_tiles[2], blocks; bool vec; };
 
 // more than 64 KB of LDS for `kernel`, once per device (done: a bit each; devices from 64 on are set every time)
 template <class K>
@@ -878,7 +923,9 @@ static int product_of(const MuonRun& R, int from, int last, hipStream_t st) {
     using S = Shape<TILE, DT == SNAG_BF16 ? 1 : 2, NST>;
     static std::atomic<uint64_t> done{0};
     if (int rc = grow_lds(muon_product_kernel<MODE, DT, TILE, NST>, S::kLds, done)) return rc;
-    muon_product_kernel<MODE, DT, TILE, NST><<<dim3(R.blocks_of[MODE]), S::kThreads, S::kLds, st>>>(R.table, R.first[MODE], from, last);
+    int whole = R.blocks_of[MODE];                             // tiles before the ranges of cut ones (a list all of whose matrices are cut: in any order)
+    if (MODE != kApply && R.plan.over > 0) whole -= R.plan.over * R.plan.over_ranges[MODE];
+    muon_product_kernel<MODE, DT, TILE, NST><<<dim3(R.blocks_of[MODE]), S::kThreads, S::kLds, st>>>(R.table, R.first[MODE], whole, from, last);
     return check_launch("muon_product");
 }
 // A 128 x 128 workgroup takes 64 KB of LDS with two stages, so that two fit a CU and hide each other's waits; a launch with at most one per CU
@@ -892,10 +939,11 @@ static int product(const MuonRun& R, int from, int last, hipStream_t st) {
     return product_of<MODE, DT, 128, 2>(R, from, last, st);
 }
 
-static int gram_sum(const MuonRun& R, hipStream_t st) {
-    if (R.gram_tiles == 0) return SNAG_OK;
-    muon_gram_sum_kernel<<<dim3(16 * R.gram_tiles, R.L.count), 256, 0, st>>>(R.table);
-    return check_launch("muon_gram_sum");
+template <int MODE>
+static int sum(const MuonRun& R, hipStream_t st) {
+    if (R.cut_tiles[MODE] == 0) return SNAG_OK;
+    muon_sum_kernel<MODE><<<dim3(16 * R.cut_tiles[MODE], R.L.count), 256, 0, st>>>(R.table);
+    return check_launch("muon_sum");
 }
 
 template <int DT>
@@ -913,7 +961,7 @@ static int muon_go(const MuonRun& R, int steps, hipStream_t st) {
         if (int rc = grow_lds(muon_narrow_kernel<DT>, lds, done)) return rc;
         for (int k = -1; k < steps; ++k) {
             if (k >= 0)
-                if (int rc = gram_sum(R, st)) return rc;
+                if (int rc = sum<kGram>(R, st)) return rc;
             muon_narrow_kernel<DT><<<dim3(R.blocks_of[kApply]), 512, lds, st>>>(R.table, R.first[kApply], k < 0 ? 0 : k & 1, k < 0, k + 1 == steps);
             if (int rc = check_launch("muon_narrow")) return rc;
         }
@@ -921,8 +969,9 @@ static int muon_go(const MuonRun& R, int steps, hipStream_t st) {
     }
     for (int k = 0; k < steps; ++k) {
         if (int rc = product<kGram, DT>(R, k & 1, 0, st)) return rc;
-        if (int rc = gram_sum(R, st)) return rc;
+        if (int rc = sum<kGram>(R, st)) return rc;
         if (int rc = product<kPoly, DT>(R, k & 1, 0, st)) return rc;
+        if (int rc = sum<kPoly>(R, st)) return rc;
         if (int rc = product<kApply, DT>(R, k & 1, k + 1 == steps, st)) return rc;
     }
     return SNAG_OK;
@@ -944,7 +993,7 @@ static int64_t work_bytes_of(const int32_t* rows, const int32_t* cols, int count
     for (MuonLists o(rows, cols, count); o.next();) {
         const MuonPlan p = plan_of(rows, cols, o.at, o.n);
         int64_t bytes = kTableBytes;
-        for (int i = 0; i < o.n; ++i) bytes += matrix_bytes(p, rows[o.at[i]], cols[o.at[i]]);
+        for (int i = 0; i < o.n; ++i) bytes += matrix_bytes(p, rows[o.at[i]], cols[o.at[i]], i + 1 == o.n);
         most = bytes > most ? bytes : most;
     }
     return most;
@@ -980,18 +1029,19 @@ static int muon_run(const char* what, void* const* w, const void* const* g, floa
             a.g = g[at[i]], a.w = w[at[i]], a.mom = mom != nullptr ? mom[at[i]] : nullptr, a.work = space;
             a.r = r, a.c = c, a.tall = r > c, a.m = r < c ? r : c, a.n = r < c ? c : r;
             a.mp = pad_to(a.m, tile), a.np = pad_n(R.plan, a.n);
-            a.splits = splits_of(R.plan, a.np);
+            cuts_of(R.plan, a.mp, a.np, i + 1 == n, a.cut, a.ranges);
             const double s = match_rms ? 0.2 * sqrt((double)a.n) : sqrt(r > c ? (double)r / c : 1.0);
             a.update = (float)(lr * s);
             a.vec = c % 8 == 0 && aligned16(a.g) && aligned16(a.mom) && aligned16(a.w);
-            space += matrix_bytes(R.plan, r, c);
+            space += matrix_bytes(R.plan, r, c, i + 1 == n);
             const int t = a.mp / 128, tri = t * (t + 1) / 2, b = (a.mp / 64) * (a.np / 64);
             for (int q = 0; q < 3; ++q) R.first[q].at[i] = R.blocks_of[q];
-            R.blocks_of[kGram] += tri * a.splits;
-            R.blocks_of[kPoly] += tri;
+            for (int q = 0; q < 2; ++q) {
+                R.blocks_of[q] += a.cut[q] + (tri - a.cut[q]) * a.ranges[q];
+                R.cut_tiles[q] = std::max(R.cut_tiles[q], tri - a.cut[q]);
+            }
             R.blocks_of[kApply] += R.plan.narrow ? a.np / kBlock : (a.mp / tile) * (a.np / tile);
             R.blocks = b > R.blocks ? b : R.blocks;
-            if (a.splits > 1 && tri > R.gram_tiles) R.gram_tiles = tri;
             R.vec = R.vec && (int64_t)r * c % 4 == 0 && aligned16(a.g) && aligned16(a.mom);
         }
         hipStream_t st = (hipStream_t)stream;
