@@ -103,7 +103,7 @@ __device__ __forceinline__ typename Chunk<T>::vec load_chunk(const T* __restrict
     return fix_tail<T>(load_raw<T>(row, col, d, valid, vec), col, d, vec);
 }
 
-constexpr int64_t kMaxBlocks = ((int64_t)1 << 24) - 1;          // of 256 threads: a launch has to stay below 2^32 threads
+constexpr int64_t kLaunchWaves = ((int64_t)1 << 26) - 64;           // a launch has to stay below 2^32 threads
 
 static inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 

@@ -272,7 +272,7 @@ static int bwd(CrossArgs a, const CrossPlan& p, float* stat, hipStream_t st) {
         a.splits = p.s_dq;
         a.per_split = range_of(a.Lk, a.splits);
         const int64_t tiles = (a.rows + p.nw_dq * 32 - 1) / (p.nw_dq * 32), n = (int64_t)a.B * a.Hkv * tiles * a.splits;
-        SNAG_REQUIRE(n < kMaxBlocks, SNAG_ERR_UNSUPPORTED, "cross attention: %lld workgroups, at most 2^24 in a launch", (long long)n);
+        SNAG_REQUIRE(n * p.nw_dq < kLaunchWaves, SNAG_ERR_UNSUPPORTED, "cross attention: %lld workgroups, more than 2^32 threads in a launch", (long long)n);
         const dim3 grid((unsigned)n);
         const bool direct = p.nw_dq == 4 && whole && a.mask == nullptr;
 #define CALL(DP)                                                                                  \
@@ -289,7 +289,7 @@ static int bwd(CrossArgs a, const CrossPlan& p, float* stat, hipStream_t st) {
         a.splits = p.s_dkv;
         a.per_split = range_of(a.rows, a.splits);
         const int64_t tiles = (a.Lk + p.nw_k * 32 - 1) / (p.nw_k * 32), n = (int64_t)a.B * a.Hkv * tiles * a.splits;
-        SNAG_REQUIRE(n < kMaxBlocks, SNAG_ERR_UNSUPPORTED, "cross attention: %lld workgroups, at most 2^24 in a launch", (long long)n);
+        SNAG_REQUIRE(n * p.nw_k < kLaunchWaves, SNAG_ERR_UNSUPPORTED, "cross attention: %lld workgroups, more than 2^32 threads in a launch", (long long)n);
         const dim3 grid((unsigned)n);
         const bool direct = p.nw_k == 4 && whole && a.rows > 0;
 #define CALL(DP)                                                                                  \

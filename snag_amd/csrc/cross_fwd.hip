@@ -181,7 +181,7 @@ static void go(const CrossArgs& a, const CrossPlan& p, dim3 grid, hipStream_t st
 
 int cross_tiles_fwd(const CrossArgs& a, const CrossPlan& p, int dtype, hipStream_t st) {
     const int64_t tiles = (a.rows + p.nw_fwd * 32 - 1) / (p.nw_fwd * 32), n = (int64_t)a.B * a.Hkv * tiles * a.splits;
-    SNAG_REQUIRE(n < kMaxBlocks, SNAG_ERR_UNSUPPORTED, "cross attention: %lld workgroups, at most 2^24 in a launch", (long long)n);
+    SNAG_REQUIRE(n * p.nw_fwd < kLaunchWaves, SNAG_ERR_UNSUPPORTED, "cross attention: %lld workgroups, more than 2^32 threads in a launch", (long long)n);
     const dim3 grid((unsigned)n);
     if (dtype == SNAG_F32) go<float, 32>(a, p, grid, st);
     else if (dtype == SNAG_BF16) go<bf16_t, 64>(a, p, grid, st);

@@ -402,8 +402,8 @@ static int rows_go(CrossArgs a, int dtype, bool bwd, hipStream_t st) {
     const int step = keys_per_step(a.d, dtype);
     const int64_t problems = (int64_t)a.B * a.Hkv;
     const int W = rows_waves(problems * a.splits, range_of(a.Lk, a.splits), step, bwd || a.rows > 4);
-    // four problems a workgroup of 256 threads where there are that many
-    SNAG_REQUIRE(problems * a.splits < 4 * kMaxBlocks, SNAG_ERR_UNSUPPORTED, "cross attention: %lld problems, fewer than 2^26 in a launch", (long long)problems);
+    // a wave each where there are that many
+    SNAG_REQUIRE(problems * a.splits < kLaunchWaves, SNAG_ERR_UNSUPPORTED, "cross attention: %lld problems, more than 2^32 threads in a launch", (long long)problems);
     a.per_split = range_of(a.Lk, a.splits);
 #define GO(T) a.d <= 32 ? rows_launch<T, 32>(a, W, bwd, st) : a.d <= 64 ? rows_launch<T, 64>(a, W, bwd, st) : rows_launch<T, 128>(a, W, bwd, st)
     if (dtype == SNAG_F32) GO(float);

@@ -202,7 +202,7 @@ __device__ __forceinline__ void store_row(T* row, const f32x16 (&acc)[DP / 32], 
 struct Problem { int b, hk, split; int64_t tile; };
 // workgroup -> (problem, split, tile): the tiles of one problem are neighbours, so that one XCD's L2 serves its keys
 __device__ __forceinline__ Problem problem_of(const CrossArgs& a, int64_t tiles) {
-    const uint32_t id = (uint32_t)xcd_order(blockIdx.x, gridDim.x), t = (uint32_t)tiles;      // at most 2^24 workgroups
+    const uint32_t id = (uint32_t)xcd_order(blockIdx.x, gridDim.x), t = (uint32_t)tiles;      // fewer than 2^26 workgroups
     Problem p;
     p.tile = id % t;
     const uint32_t rest = id / t;

@@ -28,6 +28,7 @@ def _fwd(dtype=1, B=2, Lq=3, Lk=5, H=4, Hkv=2, d=64, q=P, k=P, v=P, strides=True
     (dict(lens=P, lens_bytes=2), -1, "lens_bytes"), (dict(scale=0.0), -1, "scale"), (dict(scale=float("nan")), -1, "scale"), (dict(scale=float("inf")), -1, "scale"),
     (dict(scale=-1.0), -1, "scale"), (dict(out=None), -1, "null out"), (dict(lse=None), -1, "null out"), (dict(mask=P, mask_ld=-1), -1, "mask"),
     (dict(Lq=1 << 29, H=8, Hkv=2), -2, "2^30"), (dict(Lq=1, Lk=100000, B=1), -1, "workspace"),
+    (dict(B=1 << 26, Lq=1, Lk=1), -2, "threads"), (dict(B=1 << 25, Lq=10, Lk=1), -2, "threads"), (dict(B=1 << 23, Lq=40, Lk=1), -2, "threads"),
 ])
 def test_cross_attention_refusals(change, code, word):
     rc, text = _fwd(**change)
