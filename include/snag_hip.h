@@ -777,7 +777,7 @@ SNAG_API int snag_spmm_csr(const int32_t* rowptr, const int32_t* col, const floa
  * What memory holds at an unseen key, NaN included, does not reach any result.  A query that sees no key gets out = 0 and lse = -inf.
  * out [B, Lq, H, d] dense; lse [B, H, Lq] = log2 of the sum of exp2(scale * log2(e) * q . k), kept for the backward.
  * Scores, running maximum, sums and outputs are accumulated in fp32; for 16-bit types the probabilities (and d scores) are rounded to dtype
- * for the product with v (k, q).
+ * for the product with v (k, q); fp16 ones behind a power of two that follows their size, so that small gradients keep their bits.
  * out_lo (as out, may be NULL): what the rounding of a 16-bit out dropped, rounded once more.  The backward takes it (NULL: zero) with out for
  * sum d_out . out, the part of d scores that cancels where a query sees few keys or one key takes nearly all.
  * The backward OVERWRITES d_q (as out), d_k and d_v [B, Lk, Hkv, d] dense (zero at unseen keys); heads that share a key/value head add up

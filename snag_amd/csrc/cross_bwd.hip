@@ -80,13 +80,15 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 && (sizeof(T) == 4 || DP == 128))
         const int padded = (int)padded_rows(a.rows);
         float* st = a.stat + 2 * ((int64_t)b * a.Hkv + hk) * padded;
         const int64_t at = row, behind = at + NW * 32;
-        if (h == 0 && at < padded) st[2 * at] = lse, st[2 * at + 1] = delta;
+        if (h == 0 && at < padded) st[2 * at] = kIsHalf<T> ? lse - kHalfP : lse, st[2 * at + 1] = delta;
         if (h == 1 && behind < padded && pr.tile == tiles - 1) st[2 * behind] = INFINITY, st[2 * behind + 1] = 0.f;
     }
     if (t0 < t1) store(t0);
     f32x16 acc[DP / 32];
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) acc[i] = f32x16{};
+    [[maybe_unused]] float power = kHalfStart;             // fp16: ds and acc are times 2^power
+    float ref = kIsHalf<T> ? lse - power : lse;
     for (int t = t0; t < t1; ++t) {
         tile_ready();
         if (t + 1 < t1) fetch(t + 1);
@@ -105,7 +107,21 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 && (sizeof(T) == 4 || DP == 128))
             }
             if (hide) hide_keys(s, (uint32_t)(now >> (32 * kt)), lane);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.c2, -lse)) * (dp[i] - delta);
+            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.c2, -ref)) * (dp[i] - delta);
+            if constexpr (kIsHalf<T>) {
+                const int down = half_shift(largest(s));
+                if (__any(down != 0)) {
+                    power += (float)down;
+                    ref = lse - power;
+                    const float f = __builtin_amdgcn_exp2f((float)down);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[i] *= f;
+#pragma unroll
+                    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) acc[db][i] *= f;
+                }
+            }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const typename M::Frag ds = pack<T>(s, u);
@@ -120,8 +136,9 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 && (sizeof(T) == 4 || DP == 128))
 #pragma unroll
         for (int i = 0; i < DP / 32; ++i) acc[i] = f32x16{};
     }
-    if (a.splits > 1) store_row<float, DP>(a.part + (int64_t)pr.split * a.B * a.Lq * a.H * a.d + dense, acc, a.scale, a.d, lane);
-    else store_row<T, DP>((T*)a.dq + dense, acc, a.scale, a.d, lane);
+    const float scale = kIsHalf<T> ? a.scale * __builtin_amdgcn_exp2f(-power) : a.scale;
+    if (a.splits > 1) store_row<float, DP>(a.part + (int64_t)pr.split * a.B * a.Lq * a.H * a.d + dense, acc, scale, a.d, lane);
+    else store_row<T, DP>((T*)a.dq + dense, acc, scale, a.d, lane);
 }
 
 // d k, d v: 32 keys per wave, row tiles of RT through LDS; splits > 1: part[2][split][B, Lk, Hkv, d] (d k, then d v)
@@ -147,6 +164,7 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 && (sizeof(T) == 4 || DP == 128))
     f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) dk[i] = dv[i] = f32x16{};
+    [[maybe_unused]] float power = kHalfStart;             // fp16: ds and dk are times 2^power, p and dv times 2^kHalfP
     const int t0 = pr.split * a.per_split / RT, t1 = key0 < len ? min((a.rows + RT - 1) / RT, t0 + a.per_split / RT) : t0;
     if (t0 < t1) {
         TileFetch<T, DP, RT, NT, DIRECT> fq, fo;
@@ -204,7 +222,7 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 && (sizeof(T) == 4 || DP == 128))
                 }
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    // (lse, delta) of four rows.  Keys that are not seen go along: what they gather stays in their own lane and is dropped at the end
+                    // (lse, delta) of four rows; fp16: lse - kHalfP.  Keys that are not seen go along: what they gather stays in their own lane and is dropped at the end
                     const f32x4 s0 = *(const f32x4*)(stat[t & 1] + 2 * (rt * 32 + g * 8 + h * 4)), s1 = *(const f32x4*)(stat[t & 1] + 2 * (rt * 32 + g * 8 + h * 4) + 4);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
@@ -212,6 +230,22 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 && (sizeof(T) == 4 || DP == 128))
                         const float ls = j < 2 ? s0[2 * j] : s1[2 * j - 4], de = j < 2 ? s0[2 * j + 1] : s1[2 * j - 3];
                         s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.c2, -ls));
                         dp[i] = s[i] * (dp[i] - de);
+                    }
+                }
+                if constexpr (kIsHalf<T>) {
+                    const float to = __builtin_amdgcn_exp2f(power - kHalfP);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) dp[i] *= to;
+                    const int down = half_shift(largest(dp));
+                    if (__any(down != 0)) {
+                        power += (float)down;
+                        const float f = __builtin_amdgcn_exp2f((float)down);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) dp[i] *= f;
+#pragma unroll
+                        for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) dk[db][i] *= f;
                     }
                 }
 #pragma unroll
@@ -233,12 +267,13 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 && (sizeof(T) == 4 || DP == 128))
         for (int i = 0; i < DP / 32; ++i) dk[i] = dv[i] = f32x16{};
     }
     const int64_t dense = (((int64_t)b * a.Lk + key) * a.Hkv + hk) * a.d, n = (int64_t)a.B * a.Lk * a.Hkv * a.d;
+    const float k_scale = kIsHalf<T> ? a.scale * __builtin_amdgcn_exp2f(-power) : a.scale, v_scale = kIsHalf<T> ? 1.f / kHalfTop : 1.f;
     if (a.splits > 1) {
-        store_row<float, DP>(a.part + pr.split * n + dense, dk, a.scale, a.d, lane);
-        store_row<float, DP>(a.part + (a.splits + pr.split) * n + dense, dv, 1.f, a.d, lane);
+        store_row<float, DP>(a.part + pr.split * n + dense, dk, k_scale, a.d, lane);
+        store_row<float, DP>(a.part + (a.splits + pr.split) * n + dense, dv, v_scale, a.d, lane);
     } else {
-        store_row<T, DP>((T*)a.dk + dense, dk, a.scale, a.d, lane);
-        store_row<T, DP>((T*)a.dv + dense, dv, 1.f, a.d, lane);
+        store_row<T, DP>((T*)a.dk + dense, dk, k_scale, a.d, lane);
+        store_row<T, DP>((T*)a.dv + dense, dv, v_scale, a.d, lane);
     }
 }
 

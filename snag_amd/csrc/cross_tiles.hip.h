@@ -9,6 +9,10 @@
 // (keys 8 (i / 4) + 4 h + i % 4 for register i of lane half h); the A operand is read from LDS in that order (16 bit: transposing LDS reads).
 // fp32 runs on the fp32 matrix instruction (32 x 32 x 2), so its sums and products are fp32 throughout; 16-bit inputs round p and ds to the
 // inputs' type for the second products (what the matrix pipe takes); their sums, the running maximum and the row sums stay in fp32.
+// fp16 keeps nothing below 2^-24, and the backward's operands are small: p is 1 / keys, ds about p |do| |v|.  They are rounded as 2^15 p and 2^e ds, e
+// following the largest |ds| met so far (kHalfStart below); without that d q of 8192 keys
+// was 7.5e-3 off for a d_out of 1e-3 and 7e-2 for 1e-4; now 9.6e-4 and 9.3e-3, which is the rounding of the fp16 result alone.  fp16 backwards take
+// 2-7 % longer for it (2048 x 8192 x 128: 1061 -> 1089 us; heads of 100, whose d k / d v spills: 370 -> 427).
 #pragma once
 #include <type_traits>
 #include "cross.hip.h"
@@ -99,6 +103,12 @@ __device__ __forceinline__ typename Mma<T>::Frag pack(const f32x16& s, int u) {
     return f;
 }
 
+// The power of two that fp16 operands ds carry.  It belongs to an output column, the lane pair's own row or key, so the accumulators carry it too and it
+// is taken off when they are stored.  It starts at 2^60 (|ds| < 2^40: no overflow in fp32) and is lowered -- with the accumulators -- whenever a value passes 2^15,
+// so that the largest lies in [2^8, 2^9): what is 2^-22 of it is still a normal number, and it takes a 64 times larger one to move the scale again.
+constexpr float kHalfTop = 32768.f, kHalfStart = 60.f, kHalfP = 15.f;      // p <= 1 travels as 2^15 p
+template <class T> constexpr bool kIsHalf = std::is_same_v<T, f16_t>;
+
 // v of the other half of the wave (lane ^ 32), combined by the caller's operation
 __device__ __forceinline__ void halves(float v, float& lo, float& hi) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -108,6 +118,16 @@ __device__ __forceinline__ void halves(float v, float& lo, float& hi) {
 #else
     lo = hi = v;
 #endif
+}
+
+// exponent by which the lane pair's power has to move (0 or less; infinities move nothing) for values whose largest magnitude is top
+__device__ __forceinline__ int half_shift(float top) { return top > kHalfTop ? min(9 - __builtin_amdgcn_frexp_expf(top), 0) : 0; }
+__device__ __forceinline__ float largest(const f32x16& s) {
+    float a = 0.f, b = 0.f, lo, hi;
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) a = fmaxf(a, fabsf(s[i])), b = fmaxf(b, fabsf(s[i + 1]));
+    halves(fmaxf(a, b), lo, hi);
+    return fmaxf(lo, hi);
 }
 
 // B operands of one row of d elements (the lane's own row), DP / 16 fragments of 8 elements

@@ -1,0 +1,88 @@
+"""GPU: cross attention, the sandwich norm and the orthogonalisation at the calls where precision, infinities or a derivative can get lost."""
+import math
+
+import pytest
+import torch
+
+from cross_reference import attention, attention_bounds, half_step, orthogonalized, orthogonalized_in_fp16, tiny_step
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+E32 = 2.0 ** -24
+
+
+def make(B, Lq, Lk, H, Hkv, d, dtype, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g, device=DEV).to(dtype)
+    return r(B, Lq, H, d), r(B, Lk, Hkv, d), r(B, Lk, Hkv, d), r(B, Lq, H, d)
+
+
+def _row_tolerances(q, k, v, do, scale, r):
+    """Norms that the errors of one gradient row (d elements) stay below, in fp16.  Each of the second products' operands (p, d scores) is rounded once, by
+    at most half a step u of its value, independently of the others: squares add up, u sqrt(sum ds^2 k^2) -- doubled, for the spread of a norm over d
+    elements.  fp32 sums of d terms of either sign: sqrt(d) 2^-24 of the terms' magnitudes, doubled, taken at their worst over keys or rows.  The result is
+    rounded once: u, and half a subnormal step.  None of it grows when d_out gets small."""
+    u, f = half_step(q.dtype), torch.float64
+    B, Lq, H, d = q.shape
+    Lk, Hkv = k.shape[1], k.shape[2]
+    G, e = H // Hkv, 2 * math.sqrt(d) * E32
+    heads = lambda t: t.to(f).abs().repeat_interleave(H // t.shape[2], dim=2).permute(0, 2, 1, 3).contiguous()
+    share = lambda t: t.view(B, Hkv, G, Lk, d).sum(2).permute(0, 2, 1, 3)
+    qa, ka, va, da = (heads(t) for t in (q, k, v, do))
+    p, ds = r["p"], r["ds"].abs()
+    dpa = da @ va.transpose(2, 3).contiguous() + (da * r["o"].permute(0, 2, 1, 3).abs()).sum(-1, keepdim=True)
+    norm = lambda t: t.square().sum(-1).sqrt()
+    pt, dt, pd = (t.transpose(2, 3).contiguous() for t in (p, ds, p * dpa))
+    es = e * (qa @ ka.transpose(2, 3).contiguous() * scale).amax() + 32 * E32
+    last = tiny_step(q.dtype) * math.sqrt(d)
+    return {"dq": (2 * u * scale * norm(((ds * ds) @ (ka * ka)).sqrt()) + (e + es) * scale * norm((p * dpa) @ ka)).permute(0, 2, 1) + u * norm(r["dq"]) + last,
+            "dk": 2 * u * scale * norm(share((dt * dt) @ (qa * qa)).sqrt()) + (e + es) * scale * norm(share(pd @ qa)) + u * norm(r["dk"]) + last,
+            "dv": 2 * u * norm(share((pt * pt) @ (da * da)).sqrt()) + (e + es) * norm(share(pt @ da)) + u * norm(r["dv"]) + last}
+
+
+@pytest.mark.parametrize("size", [(2, 40, 2100, 2, 1, 64), (1, 20, 2100, 1, 1, 64), (1, 200, 2100, 2, 2, 128), (2, 5, 4096, 1, 1, 75), (1, 700, 30, 1, 1, 64), (3, 70, 500, 4, 2, 32)])
+@pytest.mark.parametrize("magnitude", [1e-5, 1e-4, 1e-3, 1.0, 1e3])
+def test_fp16_gradients_of_any_magnitude(size, magnitude):
+    """d scores are about p |d_out| sqrt(d): over a few thousand keys they lie below fp16's smallest step for ordinary gradients."""
+    from snag_amd import ops
+    q, k, v, do = make(*size, torch.float16, seed=21)
+    do = (do.float() * magnitude).half()
+    q, scale = q * 0.25, 0.5
+    if magnitude > 1:
+        q, scale = q * 50, 0.01                          # d scores above 65504 whose gradients are not
+    out, lse, lo = ops.cross_attention_fwd(q, k, v, scale=scale, want_residual=True)
+    got = ops.cross_attention_bwd(q, k, v, out, lse, do, scale=scale, out_residual=lo)
+    r = attention(q, k, v, scale=scale, d_out=do)
+    tol = _row_tolerances(q, k, v, do, scale, r)
+    for name, t in zip(("dq", "dk", "dv"), got):
+        off = (t.double() - r[name]).square().sum(-1).sqrt()
+        assert bool((off <= tol[name]).all()), (name, float((off / tol[name]).max()), float(off.norm() / r[name].norm()))
+
+
+def test_fp16_gradients_of_large_scores():
+    """Values and gradients whose d scores pass 65504 although no gradient does."""
+    from snag_amd import ops
+    q, k, v, do = make(2, 40, 6, 2, 1, 64, torch.float16, seed=30)
+    v, do, scale = v * 30, do * 1000, 1e-3
+    out, lse, lo = ops.cross_attention_fwd(q, k, v, scale=scale, want_residual=True)
+    got = ops.cross_attention_bwd(q, k, v, out, lse, do, scale=scale, out_residual=lo)
+    r = attention(q, k, v, scale=scale, d_out=do)
+    assert float(r["ds"].abs().max()) > 65504 and all(float(r[n].abs().max()) < 65504 for n in ("dq", "dk", "dv"))
+    tol = _row_tolerances(q, k, v, do, scale, r)
+    for name, t in zip(("dq", "dk", "dv"), got):
+        off = (t.double() - r[name]).square().sum(-1).sqrt()
+        assert bool((off <= tol[name]).all()), (name, float((off / tol[name]).max()))
+
+
+def test_fp16_probabilities_of_many_keys():
+    """Probabilities of 300000 keys lie below fp16's smallest normal number, d v -- under a gradient scaled up as in 16-bit training -- does not."""
+    from snag_amd import ops
+    q, k, v, do = make(1, 6, 300000, 1, 1, 64, torch.float16, seed=22)
+    q, do = q * 0.1, do * 200
+    out, lse, lo = ops.cross_attention_fwd(q, k, v, want_residual=True)
+    _, _, dv = ops.cross_attention_bwd(q, k, v, out, lse, do, out_residual=lo)
+    r = attention(q, k, v, d_out=do)
+    tol = _row_tolerances(q, k, v, do, 0.125, r)["dv"]
+    off = (dv.double() - r["dv"]).square().sum(-1).sqrt()
+    assert bool((off <= tol).all()), float((off / tol).max())
