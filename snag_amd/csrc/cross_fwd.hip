@@ -36,11 +36,11 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && (NW == 1 || DP == 128) ?
     TileFetch<T, DP, KT, NT, DIRECT> fk, fv;
     bool byte = true;                                      // this lane's mask byte of the tile in flight
     uint64_t now = 0;                                      // seen keys of the tile that is worked on
-    // DIRECT: rows behind the last key are read as the last key; what is not seen gets -inf for a score below
+    // keys that are not seen are zeros in LDS and get -inf for a score below
     auto fetch = [&](int t) {
-        const int key0 = t * KT, end = (DIRECT ? len : a.Lk) - 1;
-        fk.fetch([&](int i) { return kb + min(key0 + i, end) * a.ksl; }, lk[t % NB], a.d, a.vec_k, tid);
-        fv.fetch([&](int i) { return vb + min(key0 + i, end) * a.vsl; }, lv[t % NB], a.d, a.vec_v, tid);
+        const int key0 = t * KT, end = DIRECT ? INT32_MAX : a.Lk - 1;
+        fk.fetch([&](int i) { return kb + min(key0 + i, end) * a.ksl; }, len - key0, lk[t % NB], a.d, a.vec_k, tid);
+        fv.fetch([&](int i) { return vb + min(key0 + i, end) * a.vsl; }, len - key0, lv[t % NB], a.d, a.vec_v, tid);
         if (!DIRECT) byte = mask_byte(a, b, key0, lane);
     };
     auto store = [&](int t) {

@@ -145,22 +145,24 @@ __device__ __forceinline__ void own_row(typename Mma<T>::Frag (&f)[DP / 16], con
     }
 }
 
-// A tile of R rows on its way from global memory to LDS, one ahead of the tile that is worked on.  Every row pointer has to be readable.
-// DIRECT: straight into LDS, 16 bytes a lane, no registers; rows have to be whole (d == DP, 16-byte aligned).
-// Otherwise through registers: on the way to LDS the columns behind d become zeros, and rows that are not to be kept do, whatever they hold.
-// (Which rows those are is not known yet when the loads go out: nothing waits for a length or a mask.)
+// A tile of R rows on its way from global memory to LDS, one ahead of the tile that is worked on.  What pads a tile has to be zeros: p is 0 there, but
+// 0 x inf is NaN.
+// DIRECT: straight into LDS, 16 bytes a lane, no registers; rows have to be whole (d == DP, 16-byte aligned).  Rows from `count` on are read from kZeros.
+// Otherwise through registers, every row pointer has to be readable: on the way to LDS the columns behind d become zeros, and rows that are not to be
+// kept do, whatever they hold.  (Which rows those are is not known yet when the loads go out: nothing waits for a length or a mask.)
+static __device__ const float4 kZeros = {0.f, 0.f, 0.f, 0.f};
 template <class T, int DP, int R, int NT, bool DIRECT>
 struct TileFetch {
     static constexpr int C = Chunk<T>::n, kPerRow = DP / C, kAll = R * kPerRow, kN = (kAll + NT - 1) / NT;
     static_assert(kAll % NT == 0 || (kN == 1 && !DIRECT), "tile does not divide among the threads");
     typename Chunk<T>::vec r[DIRECT ? 1 : kN];
     template <class RowPtr>
-    __device__ __forceinline__ void fetch(RowPtr row, T* lds, int d, int vec, int tid) {
+    __device__ __forceinline__ void fetch(RowPtr row, [[maybe_unused]] int count, T* lds, int d, int vec, int tid) {
 #pragma unroll
         for (int u = 0; u < kN; ++u) {
             const int e = u * NT + tid, i = e / kPerRow;
             if constexpr (DIRECT) {
-                [[maybe_unused]] const T* p = row(i) + chunk_place<T, DP>(i, e % kPerRow) * C;
+                [[maybe_unused]] const T* p = i < count ? row(i) + chunk_place<T, DP>(i, e % kPerRow) * C : (const T*)&kZeros;
 #if defined(__HIP_DEVICE_COMPILE__)
                 __builtin_amdgcn_global_load_lds((SNAG_GLOBAL void*)p, (SNAG_LDS void*)(lds + (u * NT + (tid & ~63)) * C), 16, 0, 0);
 #endif

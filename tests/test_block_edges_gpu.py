@@ -86,3 +86,31 @@ def test_fp16_probabilities_of_many_keys():
     tol = _row_tolerances(q, k, v, do, 0.125, r)["dv"]
     off = (dv.double() - r["dv"]).square().sum(-1).sqrt()
     assert bool((off <= tol).all()), float((off / tol).max())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [(2, 40, 70, 2, 1, 64), (2, 130, 70, 2, 2, 128), (2, 50, 100, 1, 1, 32), (2, 3, 70, 2, 2, 64), (2, 20, 45, 1, 1, 64), (2, 40, 70, 2, 1, 75)])
+def test_infinity_at_the_last_key_and_row(size, dtype):
+    """What pads a tile must not be a copy of a key or row that holds an infinity: 0 x inf is NaN where the sum is infinite."""
+    from snag_amd import ops
+    q, k, v, do = make(*size, dtype, seed=23)
+    B, Lk = size[0], size[2]
+    lens = torch.tensor([Lk, Lk - 7], device=DEV, dtype=torch.int32)
+    for ln in (None, lens):
+        ends = [Lk - 1, Lk - 1 if ln is None else Lk - 8]
+        clean, lse, lo = ops.cross_attention_fwd(q, k, v, ln, want_residual=True)
+        bad = v.clone()
+        for b in range(B):
+            bad[b, ends[b], :, 5] = float("inf")
+        out, _ = ops.cross_attention_fwd(q, k, bad, ln)
+        assert bool((out[..., 5] == float("inf")).all())
+        others = [c for c in range(size[5]) if c != 5]
+        assert torch.equal(out[..., others], clean[..., others])
+        # the last row of each problem, its element 5: d v[.., 5] is infinite at every seen key and nothing else of d v changes
+        ref = ops.cross_attention_bwd(q, k, v, clean, lse, do, ln, out_residual=lo)[2]
+        worse = do.clone()
+        worse[:, -1, :, 5] = float("inf")
+        dv = ops.cross_attention_bwd(q, k, v, clean, lse, worse, ln, out_residual=lo)[2]
+        for b in range(B):
+            assert bool((dv[b, :ends[b] + 1, :, 5] == float("inf")).all()) and bool((dv[b, ends[b] + 1:] == 0).all())
+        assert torch.equal(dv[..., others], ref[..., others])
