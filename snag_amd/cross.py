@@ -13,6 +13,7 @@ import math
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
@@ -41,6 +42,12 @@ def _first_order(backward):
     return run
 
 
+def _no_tangents(name, *ts):
+    """Forward-mode derivatives have no formula here, and a call past the autograd function would drop them without a word."""
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise _lib.SnagHipError(f"{name}: forward-mode derivatives are not implemented")
+
+
 class _CrossAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, kv_lens, key_mask, scale, want_lse):
@@ -65,12 +72,14 @@ class _CrossAttentionFn(torch.autograd.Function):
 
 
 def cross_attention(q, k, v, kv_lens=None, key_mask=None, scale=None, return_lse=False):
-    """Attention of q [B, Lq, H, d] over k, v [B, Lk, Hkv, d] -> [B, Lq, H, d], differentiable in q, k and v.
+    """Attention of q [B, Lq, H, d] over k, v [B, Lk, Hkv, d] -> [B, Lq, H, d], differentiable (backward, once) in q, k and v.
 
     H is a multiple of Hkv (heads h (H / Hkv) .. share a key/value head), d <= 128.  Any strides whose last one is 1; fp32, bf16 or fp16.
     ``kv_lens`` [B] (int32 / int64, on the device): keys at and behind it are not seen; ``key_mask`` [B, Lk] (bool): nor are those that are
     False.  Unseen keys may hold anything.  A query that sees no key gets zeros, and gives none of its gradient on.  ``scale`` defaults to d ** -0.5.
     ``return_lse`` adds the natural log-sum-exp of every row's scores [B, H, Lq] (-inf where no key is seen), not differentiable."""
+    if forward_ad._current_level >= 0:
+        _no_tangents("cross_attention", q, k, v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         got = _CrossAttentionFn.apply(q, k, v, kv_lens, key_mask, scale, return_lse)
         out = got[0] if return_lse else got
@@ -111,7 +120,9 @@ def sandwich_norm(x, y, post_weight=None, pre_weight=None, post_bias=None, pre_b
     x: the residual stream, y: the block's output, [..., dim] (dim <= 8192); h continues the stream, z enters the next block.  ``kind`` "rms"
     (v / sqrt(mean v^2 + eps)) or "layer" (around the mean, biased variance).  ``gate`` [dim], or [G, dim] whose rows serve rows / G
     neighbouring rows each (one gate per sequence, or per row).  x may stay fp32 while y is 16-bit; h has x's type, z y's.  Weights and biases
-    share one type, fp32 or y's; so does the gate.  Differentiable in every tensor."""
+    share one type, fp32 or y's; so does the gate.  Differentiable (backward, once) in every tensor."""
+    if forward_ad._current_level >= 0:
+        _no_tangents("sandwich_norm", x, y, post_weight, pre_weight, post_bias, pre_bias, gate)
     if not (x.is_contiguous() and y.is_contiguous()):
         x, y = x.contiguous(), y.contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or y.requires_grad or _wants_grad(post_weight, pre_weight, post_bias, pre_bias, gate)):

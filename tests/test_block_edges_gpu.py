@@ -114,3 +114,27 @@ def test_infinity_at_the_last_key_and_row(size, dtype):
         for b in range(B):
             assert bool((dv[b, :ends[b] + 1, :, 5] == float("inf")).all()) and bool((dv[b, ends[b] + 1:] == 0).all())
         assert torch.equal(dv[..., others], ref[..., others])
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A tangent has no formula here: it must not be dropped (a missing tangent reads as zero)."""
+    import torch.autograd.forward_ad as forward_ad
+    from snag_amd._lib import SnagHipError
+    from snag_amd.cross import cross_attention, sandwich_norm
+    q, k, v, t = make(1, 3, 3, 2, 2, 32, torch.float32, seed=24)
+    x, w = torch.randn(5, 64, device=DEV), torch.ones(64, device=DEV)
+    plain, norm = cross_attention(q, k, v), sandwich_norm(x, x, w, w, gate=w)
+    with forward_ad.dual_level():
+        for i in range(3):
+            args = [forward_ad.make_dual(a, t) if i == j else a for j, a in enumerate((q, k, v))]
+            with pytest.raises(SnagHipError, match="forward"):
+                cross_attention(*args)
+        for names in (("x",), ("y",), ("post_weight",), ("pre_weight",), ("gate",)):
+            args = dict(x=x, y=x, post_weight=w, pre_weight=w, gate=w)
+            args.update({n: forward_ad.make_dual(args[n], torch.ones_like(args[n])) for n in names})
+            with pytest.raises(SnagHipError, match="forward"):
+                sandwich_norm(**args)
+        assert torch.equal(cross_attention(q, k, v), plain)
+        assert all(torch.equal(a, b) for a, b in zip(sandwich_norm(x, x, w, w, gate=w), norm))
+        with pytest.raises(RuntimeError):
+            cross_attention(forward_ad.make_dual(q.clone().requires_grad_(True), t), k, v)
