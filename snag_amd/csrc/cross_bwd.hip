@@ -302,13 +302,16 @@ template <class T, int T4>
 static int bwd(CrossArgs a, const CrossPlan& p, float* stat, hipStream_t st) {
     const int64_t nq = (int64_t)a.B * a.Lq * a.H, nk = (int64_t)a.B * a.Lk * a.Hkv;
     const bool whole = a.d == p.dp && a.vec_q && a.vec_k && a.vec_v && a.vec_o;
+    // both launches are checked before the first one writes anything
+    auto groups = [&](int64_t n, int waves, int ranges) { return (int64_t)a.B * a.Hkv * ((n + waves * 32 - 1) / (waves * 32)) * ranges; };
+    const int64_t n_dq = groups(a.rows, p.nw_dq, p.s_dq), n_dkv = groups(a.Lk, p.nw_k, p.s_dkv);
+    for (const int64_t waves : {n_dq * p.nw_dq, n_dkv * p.nw_k})
+        SNAG_REQUIRE(waves < kLaunchWaves, SNAG_ERR_UNSUPPORTED, "cross attention backward: %lld waves, more than 2^32 threads in a launch", (long long)waves);
     a.stat = stat;
     if (nq > 0) {
         a.splits = p.s_dq;
         a.per_split = range_of(a.Lk, a.splits);
-        const int64_t tiles = (a.rows + p.nw_dq * 32 - 1) / (p.nw_dq * 32), n = (int64_t)a.B * a.Hkv * tiles * a.splits;
-        SNAG_REQUIRE(n * p.nw_dq < kLaunchWaves, SNAG_ERR_UNSUPPORTED, "cross attention: %lld workgroups, more than 2^32 threads in a launch", (long long)n);
-        const dim3 grid((unsigned)n);
+        const dim3 grid((unsigned)n_dq);
         const bool direct = p.nw_dq == 4 && whole && a.mask == nullptr;
 #define CALL(DP)                                                                                  \
     if (direct) cross_dq_kernel<T, DP, 4, T4, true><<<grid, 256, 0, st>>>(a);                     \
@@ -323,9 +326,7 @@ static int bwd(CrossArgs a, const CrossPlan& p, float* stat, hipStream_t st) {
     if (nk > 0) {
         a.splits = p.s_dkv;
         a.per_split = range_of(a.rows, a.splits);
-        const int64_t tiles = (a.Lk + p.nw_k * 32 - 1) / (p.nw_k * 32), n = (int64_t)a.B * a.Hkv * tiles * a.splits;
-        SNAG_REQUIRE(n * p.nw_k < kLaunchWaves, SNAG_ERR_UNSUPPORTED, "cross attention: %lld workgroups, more than 2^32 threads in a launch", (long long)n);
-        const dim3 grid((unsigned)n);
+        const dim3 grid((unsigned)n_dkv);
         const bool direct = p.nw_k == 4 && whole && a.rows > 0;
 #define CALL(DP)                                                                                  \
     if (direct) cross_dkv_kernel<T, DP, 4, DP == 128 ? 32 : T4, true><<<grid, 256, 0, st>>>(a);           \

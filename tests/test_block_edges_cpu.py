@@ -23,3 +23,14 @@ def test_forward_mode_tangents_are_not_dropped(monkeypatch):
                 cross.sandwich_norm(*args)
         assert torch.equal(cross.cross_attention(t, t, t), t)
     assert torch.equal(cross.cross_attention(t, t, t), t) and torch.equal(cross.sandwich_norm(t, t)[0], t)
+
+
+@pytest.mark.parametrize("B, Lq, Lk, dtype, d", [(1 << 20, 5, 2048, 1, 64), (1 << 24, 9, 129, 0, 128), (1 << 22, 2048, 5, 2, 64), (1 << 26, 5, 1, 1, 32), (1 << 26, 0, 5, 1, 32)])
+def test_a_backward_past_the_launch_limit_is_refused_before_anything_is_launched(B, Lq, Lk, dtype, d):
+    """Too many waves on the keys' or on the rows' side, whichever the other one needs: nothing may be written first (without a device a launch
+    answers with another error)."""
+    from snag_amd import _lib
+    lib, P = _lib.load(), ctypes.c_void_p(4096)
+    strides = (ctypes.c_int64 * 9)(*([64] * 9))
+    rc = lib.snag_cross_bwd(P, P, P, dtype, B, Lq, Lk, 1, 1, d, ctypes.addressof(strides), None, 4, None, 0, 0.1, P, None, P, P, P, P, P, P, 1 << 62, None)
+    assert rc == -2 and "threads" in _lib.last_error(), (rc, _lib.last_error())
