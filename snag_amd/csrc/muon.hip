@@ -1057,8 +1057,8 @@ using namespace snag;
 
 extern "C" SNAG_API int64_t snag_muon_work_bytes(const int32_t* rows_host, const int32_t* cols_host, int count) {
     if (rows_host == nullptr || cols_host == nullptr) return 0;
-    for (int i = 0; i < count; ++i)
-        if (rows_host[i] < 1 || cols_host[i] < 1) return 0;
+    for (int i = 0; i < count; ++i)                        // refused by the call itself
+        if (rows_host[i] < 1 || cols_host[i] < 1 || rows_host[i] > SNAG_MUON_MAX_SIDE || cols_host[i] > SNAG_MUON_MAX_SIDE) return 0;
     return work_bytes_of(rows_host, cols_host, count);
 }
 

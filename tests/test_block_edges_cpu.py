@@ -34,3 +34,12 @@ def test_a_backward_past_the_launch_limit_is_refused_before_anything_is_launched
     strides = (ctypes.c_int64 * 9)(*([64] * 9))
     rc = lib.snag_cross_bwd(P, P, P, dtype, B, Lq, Lk, 1, 1, d, ctypes.addressof(strides), None, 4, None, 0, 0.1, P, None, P, P, P, P, P, P, 1 << 62, None)
     assert rc == -2 and "threads" in _lib.last_error(), (rc, _lib.last_error())
+
+
+@pytest.mark.parametrize("r, c", [(2 ** 31 - 1, 2 ** 31 - 1), (16385, 8), (8, 2 ** 31 - 1), (0, 8), (8, -1)])
+def test_no_workspace_is_computed_for_a_refused_matrix(r, c):
+    """Sides past the limit are refused by the call; sizing their workspace would overflow 32-bit tile counts."""
+    from snag_amd import _lib
+    rows, cols = (ctypes.c_int32 * 2)(8, r), (ctypes.c_int32 * 2)(8, c)
+    size = lambda n: _lib.load().snag_muon_work_bytes(ctypes.addressof(rows), ctypes.addressof(cols), n)
+    assert size(2) == 0 and size(1) > 0
