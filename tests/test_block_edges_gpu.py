@@ -138,3 +138,20 @@ def test_forward_mode_derivatives_are_refused():
         assert all(torch.equal(a, b) for a, b in zip(sandwich_norm(x, x, w, w, gate=w), norm))
         with pytest.raises(RuntimeError):
             cross_attention(forward_ad.make_dual(q.clone().requires_grad_(True), t), k, v)
+
+
+@pytest.mark.parametrize("rows, dim", [(45000, 128), (100003, 96), (30000, 600)])
+def test_parameter_gradients_of_many_rows(rows, dim):
+    """d pre_bias = sum of d_z over the rows: nothing but the order of the sum.  Serial fp32 sums of n terms of either sign lose up to 2^-24 sqrt(n / 2)
+    of the result, each rounding at its largest; the kernel's chain (a worker's run of at most 30 rows, 16 workers' partials, a tree of 16, a tree of
+    16 runs): sqrt(15 + 8 + 4 + 4) 2^-24 at most."""
+    from snag_amd import ops
+    g = torch.Generator(device=DEV).manual_seed(25)
+    x, y, dz = (torch.randn(rows, dim, generator=g, device=DEV) for _ in range(3))
+    w = torch.ones(dim, device=DEV)
+    _, _, stats = ops.sandwich_norm_fwd(x, y, pre_bias=w)
+    got = ops.sandwich_norm_bwd(x, y, stats, None, dz, pre_bias=w)[5]
+    ref = dz.double().sum(0)
+    off = float((got.double() - ref).norm() / ref.norm())
+    run = {128: 11, 96: 25, 600: 30}[dim]
+    assert off <= E32 * math.sqrt(run / 2 + 8 + 4 + 4), (off, E32 * math.sqrt(run / 2 + 16))
