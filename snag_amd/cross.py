@@ -24,11 +24,31 @@ LN2 = math.log(2.0)
 
 def _note_stream(out):
     """A gradient node belongs to the stream it was made on, a leaf's to that of the first live graph that reaches it.  A backward captured on
-    another stream would pull that stream into the capture, and torch then ends the process: refuse the capture while such a graph is alive."""
-    st = ops._raw_stream(out.device.index)
-    for node, _ in out.grad_fn.next_functions:
-        if node is not None and node.metadata.setdefault("snag_stream", st) != st and torch.cuda.is_current_stream_capturing():
+    another stream would pull that stream into the capture, and torch then ends the process.  torch does not tell a node's stream, so each call
+    leaves its own on the nodes it reads from, and a call inside a capture looks through the whole graph below it: one that reaches a node left by
+    an eager call on another stream is refused.  Graphs that other operations alone built of the same leaves are not seen."""
+    st, capturing = ops._raw_stream(out.device.index), torch.cuda.is_current_stream_capturing()
+    below = [node for node, _ in out.grad_fn.next_functions if node is not None]
+    for node in below:
+        node.metadata.setdefault("snag_stream", st)
+    if not capturing:
+        return
+    seen = set(below)
+    while below:
+        node = below.pop()
+        if node.metadata.get("snag_stream", st) != st:
             raise _lib.SnagHipError("a backward cannot be captured while an eager graph of the same leaves lives on another stream: drop that graph's outputs first")
+        for n, _ in node.next_functions:
+            if n is not None and n not in seen:
+                seen.add(n)
+                below.append(n)
+
+
+def _noted(out):
+    """A projection's output, its leaves' nodes noted as those of the operators beside it."""
+    if out.grad_fn is not None:
+        _note_stream(out)
+    return out
 
 
 def _first_order(backward):
@@ -175,10 +195,10 @@ class CrossModalLayer(nn.Module):
         L = states.shape[1]
         z = x if z is None else z
         flat = lambda t: t.reshape(-1, t.shape[-1])
-        q = self.query(flat(z)).view(N, M, self.num_heads, self.head)
-        k = self.key(flat(states)).view(N, L, self.kv_heads, self.head)
-        v = self.value(flat(states)).view(N, L, self.kv_heads, self.head)
+        q = _noted(self.query(flat(z))).view(N, M, self.num_heads, self.head)
+        k = _noted(self.key(flat(states))).view(N, L, self.kv_heads, self.head)
+        v = _noted(self.value(flat(states))).view(N, L, self.kv_heads, self.head)
         a = cross_attention(q, k, v, kv_lens, key_mask)
-        x, z = self.attention_norm(x, self.output(a.reshape(N * M, D)).view(N, M, D))
-        f = self.feed_forward(flat(z))
+        x, z = self.attention_norm(x, _noted(self.output(a.reshape(N * M, D))).view(N, M, D))
+        f = _noted(self.feed_forward(flat(z)))
         return self.feed_forward_norm(x, f.view(N, M, D))

@@ -43,3 +43,59 @@ def test_no_workspace_is_computed_for_a_refused_matrix(r, c):
     rows, cols = (ctypes.c_int32 * 2)(8, r), (ctypes.c_int32 * 2)(8, c)
     size = lambda n: _lib.load().snag_muon_work_bytes(ctypes.addressof(rows), ctypes.addressof(cols), n)
     assert size(2) == 0 and size(1) > 0
+
+
+@pytest.fixture
+def streams(monkeypatch):
+    """The stream and whether it is capturing, as the test says."""
+    from snag_amd import ops
+    now = {"stream": 1, "capturing": False}
+    monkeypatch.setattr(ops, "_raw_stream", lambda index: now["stream"])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now["capturing"])
+    return now
+
+
+def test_a_capture_over_leaves_of_a_live_eager_graph_is_refused_at_any_depth(streams):
+    from snag_amd import cross
+    from snag_amd._lib import SnagHipError
+    w, other = torch.ones(3, requires_grad=True), torch.ones(3, requires_grad=True)
+    alive = w * 2
+    cross._note_stream(alive)
+    streams.update(stream=2, capturing=True)
+    for depth in range(4):
+        t = w
+        for _ in range(depth):
+            t = t.view(3).clone()
+        with pytest.raises(SnagHipError, match="eager graph"):
+            cross._note_stream((t + other) * other if depth else t * other)
+        cross._note_stream((other.view(3).clone() + 1) * other)
+    del alive, t
+    cross._note_stream(w.view(3).clone() * 2)                       # the eager graph is gone, and its nodes with it
+    streams.update(stream=1, capturing=False)
+    cross._note_stream(w * other)
+
+
+def test_a_layer_notes_the_leaves_of_its_projections(streams, monkeypatch):
+    """With its norms frozen the projections' weights are all that an eager graph and a captured one share."""
+    from snag_amd import cross, ops, projection
+    from snag_amd._lib import SnagHipError
+
+    def gemm(a, b, bias=None, act=None, **_):
+        r = a @ b.T if bias is None else a @ b.T + bias
+        return r.relu() if act == "relu" else r
+
+    monkeypatch.setattr(ops, "gemm", gemm)
+    monkeypatch.setattr(cross, "cross_attention", lambda q, k, v, *_: q + k.mean() + v.mean())
+    monkeypatch.setattr(cross, "sandwich_norm", lambda x, y, *_, **__: (x + y, x - y))
+    for frozen in ([], ["query", "key", "value"], ["query", "key", "output", "feed_forward"], ["query", "key", "value", "output"]):
+        layer = cross.CrossModalLayer(8, 2)
+        for n, p in layer.named_parameters():
+            p.requires_grad = n.split(".")[0] not in frozen and "norm" not in n
+        x = torch.randn(2, 3, 8)
+        streams.update(stream=1, capturing=False)
+        alive = layer(x, x)
+        streams.update(stream=2, capturing=True)
+        with pytest.raises(SnagHipError, match="eager graph"):
+            layer(x, x)
+        del alive
+        layer(x, x)

@@ -155,3 +155,19 @@ def test_parameter_gradients_of_many_rows(rows, dim):
     off = float((got.double() - ref).norm() / ref.norm())
     run = {128: 11, 96: 25, 600: 30}[dim]
     assert off <= E32 * math.sqrt(run / 2 + 8 + 4 + 4), (off, E32 * math.sqrt(run / 2 + 16))
+
+
+def test_a_layer_with_frozen_norms_is_not_captured_over_a_live_graph():
+    """Only the check runs: the forward inside the capture is refused before any backward is."""
+    from snag_amd._lib import SnagHipError
+    from snag_amd.cross import CrossModalLayer
+    layer = CrossModalLayer(64, 4).to(DEV)
+    for n, p in layer.named_parameters():
+        p.requires_grad = "norm" not in n
+    x = torch.randn(5, 3, 64, device=DEV)
+    h, _ = layer(x, x)
+    with pytest.raises(SnagHipError, match="eager graph"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            layer(x, x)
+    h.sum().backward()
+    assert all(bool(torch.isfinite(p.grad).all()) for p in layer.parameters() if p.grad is not None)
