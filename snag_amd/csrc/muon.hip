@@ -824,24 +824,27 @@ __global__ __launch_bounds__(512) void muon_narrow_kernel(const MuonTable* __res
 static int pad_to(int n, int tile) { return (n + tile - 1) / tile * tile; }
 constexpr int kCus = 256;
 
-// How one list of matrices is worked on.  narrow: every m <= 128 (muon_narrow_kernel).  Otherwise 256 x 256 tiles for the product with X when the
-// list has enough of them to occupy most CUs (they read half as much per multiplication; 128 x 128 ones fill the chip earlier).  The symmetric
-// products, half as many tiles, always run on 128 x 128 ones.
+// How one list of matrices is worked on.  narrow: every m <= 128 (muon_narrow_kernel).  Otherwise the product with X takes the tiles whose rounds are done
+// first: 512 tiles of 128 x 128 run at a time (two a CU), or 256 of 256 x 256, four times the work, which read half as much per multiplication and take 3-6 % less
+// than two rounds of small ones.  bf16, large / small tiles: 8 matrices of 1024 x 1024 (one round / one) 541 / 477 us, 9 of them (one / two) 539 / 546, 2816 x 2816
+// (one / one) 861 / 702, 3584 x 3584 (one / two) 1321 / 1393, 4352 x 4352 (two / three) 2814 / 2509.  The symmetric products, half as many tiles, always run on
+// 128 x 128 ones.
 struct MuonPlan { bool narrow; int tile, stages, over, over_ranges[2]; };
 static int pad_n(const MuonPlan& p, int n) { return pad_to(n, p.narrow ? kBlock : p.tile); }
 static int splits_of(const MuonPlan& p, int np) { return p.narrow ? np / kBlock : (np / 64 + p.stages - 1) / p.stages; }
 static MuonPlan plan_of(const int32_t* rows, const int32_t* cols, const int* at, int count) {
     MuonPlan p{};
     p.narrow = true, p.tile = 128;
-    int64_t big = 0, total = 0;
+    int64_t big = 0, small = 0, total = 0;
     for (int k = 0; k < count; ++k) {
         const int r = rows[at[k]], c = cols[at[k]], m = r < c ? r : c, n = r < c ? c : r;
         p.narrow = p.narrow && m <= 128;
         big += (int64_t)(pad_to(m, 256) / 256) * (pad_to(n, 256) / 256);
         const int64_t t = pad_to(m, 128) / 128;
+        small += t * (pad_to(n, 128) / 128);
         total += t * (t + 1) / 2 * (pad_to(n, 128) / 64);
     }
-    if (!p.narrow && big >= kCus * 3 / 8) p.tile = 256;
+    if (!p.narrow && 2 * ((big + kCus - 1) / kCus) <= (small + 2 * kCus - 1) / (2 * kCus)) p.tile = 256;
     // LDS stages in a range of A's contraction: the list's stages over all CUs, at least four
     const int64_t per = (total + kCus - 1) / kCus;
     p.stages = (int)(per < 4 ? 4 : per);

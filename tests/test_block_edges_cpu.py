@@ -99,3 +99,14 @@ def test_a_layer_notes_the_leaves_of_its_projections(streams, monkeypatch):
             layer(x, x)
         del alive
         layer(x, x)
+
+
+@pytest.mark.parametrize("side, padded, ranges", [(2600, 2688, 2 * 231), (4360, 4480, 4 * 118), (3400, 3584, 0), (3700, 3840, 0)])
+def test_the_large_tile_is_taken_where_its_rounds_are_done_first(side, padded, ranges):
+    """Seen from outside by the workspace (X, A and B: 16 bytes an element of the padded square; partial tiles of 64 KB): 2600 x 2600 are 121 tiles of 256,
+    a whole round of the chip for less than half of it, or 441 of 128, one round of 512; 4360 x 4360 two rounds or three half as long; 3400 x 3400 and
+    3700 x 3700 one or two half as long."""
+    from snag_amd import _lib
+    n = (ctypes.c_int32 * 1)(side)
+    got = _lib.load().snag_muon_work_bytes(ctypes.addressof(n), ctypes.addressof(n), 1)
+    assert 0 <= got - 16 * padded ** 2 - 65536 * ranges < 65536, got
