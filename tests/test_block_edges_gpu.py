@@ -171,3 +171,92 @@ def test_a_layer_with_frozen_norms_is_not_captured_over_a_live_graph():
             layer(x, x)
     h.sum().backward()
     assert all(bool(torch.isfinite(p.grad).all()) for p in layer.parameters() if p.grad is not None)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("size", [(1, 40, 3000, 2, 1, 64), (1, 2, 300, 2, 2, 64), (1, 2, 3000, 2, 1, 100), (4100, 1, 300, 1, 1, 32), (2, 40, 400, 2, 2, 75), (2, 200, 400, 1, 1, 128), (1, 3, 3000, 1, 1, 33)])
+def test_the_residual_holds_what_rounding_dropped(size, dtype):
+    """Values around 3: out's own rounding is what is off, and out + residual is much nearer.  (p's rounding, independent from key to key, reaches the
+    output as u |v| sqrt(sum p^2), below a sixteenth of u |o| over these hundreds of keys; the residual's own is u^2.)  One wave, several waves and
+    several ranges a problem, whole and odd widths."""
+    from snag_amd import ops
+    q, k, v, _ = make(*size, dtype, seed=26)
+    q, v = q * 0.5, (v.float() * 0.2 + 3).to(dtype)
+    out, _, lo = ops.cross_attention_fwd(q, k, v, want_residual=True)
+    ref = attention(q, k, v)["o"]
+    alone, both = float((out.double() - ref).norm()), float((out.double() + lo.double() - ref).norm())
+    assert both <= alone / 4, (alone, both)
+    assert bool((lo.double().abs() <= half_step(dtype) * 1.001 * out.double().abs()).all())
+    assert bool((lo != 0).any(-1).float().mean() > 0.9)
+
+
+def test_long_cache_gradients_pass_32_bits():
+    """Element offsets behind 2^31 in both directions, keys and values apart: the last sequence's 100 seen keys at the end of 2.3 G elements."""
+    from snag_amd import ops
+    B, Lk, H, d = 72, 250000, 1, 128
+    k, v = (torch.zeros(B, Lk, H, d, device=DEV, dtype=torch.bfloat16) for _ in range(2))
+    g = torch.Generator(device=DEV).manual_seed(27)
+    k[-1, -100:], v[-1, -100:] = (torch.randn(100, H, d, generator=g, device=DEV).bfloat16() for _ in range(2))
+    lens = torch.full((B,), 3, device=DEV, dtype=torch.int32)
+    lens[-1] = Lk
+    mask = torch.zeros(B, Lk, dtype=torch.bool, device=DEV)
+    mask[:, :3] = True
+    mask[-1] = False
+    mask[-1, -100:] = True
+    for rows in (1, 40):
+        q, do = (torch.randn(B, rows, H, d, generator=g, device=DEV).bfloat16() for _ in range(2))
+        out, lse, lo = ops.cross_attention_fwd(q, k, v, lens, mask, want_residual=True)
+        dq, dk, dv = ops.cross_attention_bwd(q, k, v, out, lse, do, lens, mask, out_residual=lo)
+        small = (q[-1:], k[-1:, -100:], v[-1:, -100:])
+        r = attention(*small, d_out=do[-1:])
+        b = attention_bounds(*small, None, None, None, do[-1:], r)
+        for name, t in (("o", out[-1:]), ("dq", dq[-1:]), ("dk", dk[-1:, -100:]), ("dv", dv[-1:, -100:])):
+            assert bool(((t.double() - r[name]).abs() <= b[name]).all()), (rows, name)
+        assert bool((dk[-1, :-100] == 0).all()) and bool((dv[-1, :-100] == 0).all())
+        assert bool((dk[:-1, 3:] == 0).all()) and bool((out[:-1] == 0).all())
+        del out, lse, lo, dq, dk, dv
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(16384, 300), (90, 16384)])
+def test_the_longest_side(shape, dtype):
+    from snag_amd.optim import orthogonalize
+    g = torch.randn(*shape, generator=torch.Generator(device=DEV).manual_seed(28), device=DEV).to(dtype)
+    x = orthogonalized(g)
+    cost = float((orthogonalized_in_fp16(g, 1 if dtype == torch.bfloat16 else 2).double() - x).norm() / x.norm())
+    assert float((orthogonalize(g).double() - x).norm() / x.norm()) <= 2 * cost + 2e-6 + half_step(dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_the_step_keeps_its_types_bits(dtype):
+    """A weight of zero, so that the update is all there is of the new one: fp32 and fp16 matrices carry 22 bits through the products, bf16 ones 11."""
+    from snag_amd.optim import muon_step
+    shapes = [(128, 700), (700, 128), (300, 200), (64, 129)]
+    g = torch.Generator(device=DEV).manual_seed(29)
+    gs = [(torch.randn(r, c, generator=g, device=DEV) * 1e-3).to(dtype) for r, c in shapes]
+    ws, ms = [torch.zeros_like(t) for t in gs], [torch.randn(r, c, generator=g, device=DEV) * 1e-3 for r, c in shapes]
+    m64 = [m.double() for m in ms]
+    muon_step(ws, gs, ms, 1.0, 0.9)
+    for (r, c), w, d, m in zip(shapes, ws, gs, m64):
+        u = 0.1 * d.double() + 0.9 * (0.9 * m + 0.1 * d.double())
+        x = orthogonalized(u)
+        cost = float((orthogonalized_in_fp16(u, 1 if dtype == torch.bfloat16 else 2).double() - x).norm() / x.norm())
+        off = float((w.double() + math.sqrt(max(1, r / c)) * x).norm() / (math.sqrt(max(1, r / c)) * x.norm()))
+        assert off <= 2 * cost + 2e-6 + half_step(dtype), ((r, c), off, cost)
+
+
+def test_a_layer_without_states_or_tokens():
+    from snag_amd.cross import CrossModalLayer
+    torch.manual_seed(0)
+    layer = CrossModalLayer(64, 4, state_dim=48, kv_heads=2, intermediate_size=96).to(DEV)
+    for N, M, L in ((5, 3, 0), (0, 3, 7), (5, 0, 7)):
+        x, states = torch.randn(N, M, 64, device=DEV, requires_grad=True), torch.randn(N, L, 48, device=DEV, requires_grad=True)
+        h, z = layer(x, states)
+        assert h.shape == z.shape == (N, M, 64) and bool(torch.isfinite(h).all())
+        (h.sum() + z.square().sum()).backward()
+        assert x.grad.shape == x.shape and states.grad.shape == states.shape
+        for n, p in layer.named_parameters():
+            assert bool(torch.isfinite(p.grad).all()), n
+            if n.split(".")[0] in ("key", "value") or N * M == 0:
+                assert bool((p.grad == 0).all()), n
+        layer.zero_grad(set_to_none=True)
