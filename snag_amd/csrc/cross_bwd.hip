@@ -34,11 +34,11 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 && (sizeof(T) == 4 || DP == 128))
     TileFetch<T, DP, KT, NT, DIRECT> fk, fv;
     bool byte = true;                                      // this lane's mask byte of the tile in flight
     uint64_t now = 0;                                      // seen keys of the tile that is worked on
-    // keys that are not seen are zeros in LDS and get -inf for a score below
+    // DIRECT: rows behind the last key are read as the last key; keys that are not seen are zeros in LDS before they are used, and get -inf for a score
     auto fetch = [&](int t) {
-        const int key0 = t * KT, end = DIRECT ? INT32_MAX : a.Lk - 1;
-        fk.fetch([&](int i) { return kb + min(key0 + i, end) * a.ksl; }, len - key0, lk[t % NB], a.d, a.vec_k, tid);
-        fv.fetch([&](int i) { return vb + min(key0 + i, end) * a.vsl; }, len - key0, lv[t % NB], a.d, a.vec_v, tid);
+        const int key0 = t * KT, end = (DIRECT ? len : a.Lk) - 1;
+        fk.fetch([&](int i) { return kb + min(key0 + i, end) * a.ksl; }, lk[t % NB], a.d, a.vec_k, tid);
+        fv.fetch([&](int i) { return vb + min(key0 + i, end) * a.vsl; }, lv[t % NB], a.d, a.vec_v, tid);
         if (!DIRECT) byte = mask_byte(a, b, key0, lane);
     };
     auto store = [&](int t) {
@@ -91,6 +91,11 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 && (sizeof(T) == 4 || DP == 128))
     float ref = kIsHalf<T> ? lse - power : lse;
     for (int t = t0; t < t1; ++t) {
         tile_ready();
+        if (DIRECT && (t + 1) * KT > len) {
+            fk.pad(len - t * KT, lk[t % NB], tid);
+            fv.pad(len - t * KT, lv[t % NB], tid);
+            pad_ready();
+        }
         if (t + 1 < t1) fetch(t + 1);
         const T *ck = lk[t % NB], *cv = lv[t % NB];
         const bool hide = (!DIRECT && a.mask != nullptr) || (t + 1) * KT > len;
@@ -169,17 +174,17 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 && (sizeof(T) == 4 || DP == 128))
     if (t0 < t1) {
         TileFetch<T, DP, RT, NT, DIRECT> fq, fo;
         [[maybe_unused]] const float* st = a.stat + 2 * ((int64_t)b * a.Hkv + hk) * padded_rows(a.rows);
-        // rows behind the last one are zeros in LDS, their p is 0
+        // rows behind the last one are read as the last one and cleared in LDS, their p is 0
         auto fetch = [&](int t) {
             const int r0 = t * RT;
             fq.fetch([&](int i) {
                 const int r = min(r0 + i, a.rows - 1), l = row_l(a, r);
                 return (const T*)a.q + b * a.qsb + l * a.qsl + (hk * a.G + r - l * a.G) * a.qsh;
-            }, a.rows - r0, lq[t % NB], a.d, a.vec_q, tid);
+            }, lq[t % NB], a.d, a.vec_q, tid);
             fo.fetch([&](int i) {
                 const int r = min(r0 + i, a.rows - 1), l = row_l(a, r);
                 return (const T*)a.dout + (((int64_t)b * a.Lq + l) * a.H + hk * a.G + r - l * a.G) * a.d;
-            }, a.rows - r0, lo[t % NB], a.d, a.vec_o, tid);
+            }, lo[t % NB], a.d, a.vec_o, tid);
 #if defined(__HIP_DEVICE_COMPILE__)
 #pragma unroll
             for (int u = 0; u < 2 * RT / 64; ++u)
@@ -194,8 +199,8 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 && (sizeof(T) == 4 || DP == 128))
         fetch(t0);
         if constexpr (VLDS) {
             TileFetch<T, DP, KEYS, NT, DIRECT> fv;
-            const int end = DIRECT ? INT32_MAX : a.Lk - 1;
-            fv.fetch([&](int i) { return (const T*)a.v + b * a.vsb + hk * a.vsh + min(key0 + i, end) * a.vsl; }, len - key0, lvv, a.d, a.vec_v, tid);
+            const int end = (DIRECT ? len : a.Lk) - 1;
+            fv.fetch([&](int i) { return (const T*)a.v + b * a.vsb + hk * a.vsh + min(key0 + i, end) * a.vsl; }, lvv, a.d, a.vec_v, tid);
             if constexpr (!DIRECT) {
                 uint64_t bits[KEYS / 64];
 #pragma unroll
@@ -209,6 +214,11 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 && (sizeof(T) == 4 || DP == 128))
         store(t0);
         for (int t = t0; t < t1; ++t) {
             tile_ready();
+            if (DIRECT && (t + 1) * RT > a.rows) {
+                fq.pad(a.rows - t * RT, lq[t % NB], tid);
+                fo.pad(a.rows - t * RT, lo[t % NB], tid);
+                pad_ready();
+            }
             if (t + 1 < t1) fetch(t + 1);
             const T *cq = lq[t % NB], *co = lo[t % NB];
 #pragma unroll

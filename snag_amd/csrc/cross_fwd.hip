@@ -36,11 +36,11 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && (NW == 1 || DP == 128) ?
     TileFetch<T, DP, KT, NT, DIRECT> fk, fv;
     bool byte = true;                                      // this lane's mask byte of the tile in flight
     uint64_t now = 0;                                      // seen keys of the tile that is worked on
-    // keys that are not seen are zeros in LDS and get -inf for a score below
+    // DIRECT: rows behind the last key are read as the last key; keys that are not seen are zeros in LDS before they are used, and get -inf for a score
     auto fetch = [&](int t) {
-        const int key0 = t * KT, end = DIRECT ? INT32_MAX : a.Lk - 1;
-        fk.fetch([&](int i) { return kb + min(key0 + i, end) * a.ksl; }, len - key0, lk[t % NB], a.d, a.vec_k, tid);
-        fv.fetch([&](int i) { return vb + min(key0 + i, end) * a.vsl; }, len - key0, lv[t % NB], a.d, a.vec_v, tid);
+        const int key0 = t * KT, end = (DIRECT ? len : a.Lk) - 1;
+        fk.fetch([&](int i) { return kb + min(key0 + i, end) * a.ksl; }, lk[t % NB], a.d, a.vec_k, tid);
+        fv.fetch([&](int i) { return vb + min(key0 + i, end) * a.vsl; }, lv[t % NB], a.d, a.vec_v, tid);
         if (!DIRECT) byte = mask_byte(a, b, key0, lane);
     };
     auto store = [&](int t) {
@@ -61,6 +61,11 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && (NW == 1 || DP == 128) ?
     float m = -INFINITY, sum = 0.f;                        // m: what the exponentials are relative to, within kSlack of the maximum
     for (int t = t0; t < t1; ++t) {
         tile_ready();
+        if (DIRECT && (t + 1) * KT > len) {
+            fk.pad(len - t * KT, lk[t % NB], tid);
+            fv.pad(len - t * KT, lv[t % NB], tid);
+            pad_ready();
+        }
         if (t + 1 < t1) fetch(t + 1);
         const T *ck = lk[t % NB], *cv = lv[t % NB];
         f32x16 s[KT / 32];

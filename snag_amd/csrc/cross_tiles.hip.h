@@ -145,24 +145,24 @@ __device__ __forceinline__ void own_row(typename Mma<T>::Frag (&f)[DP / 16], con
     }
 }
 
-// A tile of R rows on its way from global memory to LDS, one ahead of the tile that is worked on.  What pads a tile has to be zeros: p is 0 there, but
-// 0 x inf is NaN.
-// DIRECT: straight into LDS, 16 bytes a lane, no registers; rows have to be whole (d == DP, 16-byte aligned).  Rows from `count` on are read from kZeros.
-// Otherwise through registers, every row pointer has to be readable: on the way to LDS the columns behind d become zeros, and rows that are not to be
-// kept do, whatever they hold.  (Which rows those are is not known yet when the loads go out: nothing waits for a length or a mask.)
-static __device__ const float4 kZeros = {0.f, 0.f, 0.f, 0.f};
+// A tile of R rows on its way from global memory to LDS, one ahead of the tile that is worked on.  Every row pointer has to be readable.  What pads a
+// tile has to be zeros when it is worked on: p is 0 there, but 0 x inf is NaN.
+// DIRECT: straight into LDS, 16 bytes a lane, no registers; rows have to be whole (d == DP, 16-byte aligned).  pad() clears the rows from `count` on once the
+// tile has landed (reading zeros in their place cost every tile 1-2 %).
+// Otherwise through registers: on the way to LDS the columns behind d become zeros, and rows that are not to be kept do, whatever they hold.
+// (Which rows those are is not known yet when the loads go out: nothing waits for a length or a mask.)
 template <class T, int DP, int R, int NT, bool DIRECT>
 struct TileFetch {
     static constexpr int C = Chunk<T>::n, kPerRow = DP / C, kAll = R * kPerRow, kN = (kAll + NT - 1) / NT;
     static_assert(kAll % NT == 0 || (kN == 1 && !DIRECT), "tile does not divide among the threads");
     typename Chunk<T>::vec r[DIRECT ? 1 : kN];
     template <class RowPtr>
-    __device__ __forceinline__ void fetch(RowPtr row, [[maybe_unused]] int count, T* lds, int d, int vec, int tid) {
+    __device__ __forceinline__ void fetch(RowPtr row, T* lds, int d, int vec, int tid) {
 #pragma unroll
         for (int u = 0; u < kN; ++u) {
             const int e = u * NT + tid, i = e / kPerRow;
             if constexpr (DIRECT) {
-                [[maybe_unused]] const T* p = i < count ? row(i) + chunk_place<T, DP>(i, e % kPerRow) * C : (const T*)&kZeros;
+                [[maybe_unused]] const T* p = row(i) + chunk_place<T, DP>(i, e % kPerRow) * C;
 #if defined(__HIP_DEVICE_COMPILE__)
                 __builtin_amdgcn_global_load_lds((SNAG_GLOBAL void*)p, (SNAG_LDS void*)(lds + (u * NT + (tid & ~63)) * C), 16, 0, 0);
 #endif
@@ -171,6 +171,10 @@ struct TileFetch {
                 r[u] = load_raw<T>(row(in ? i : 0), (e % kPerRow) * C, d, in, vec);
             }
         }
+    }
+    static __device__ __forceinline__ void pad(int count, T* lds, int tid) {
+        if constexpr (DIRECT)
+            for (int e = max(count, 0) * kPerRow + tid; e < kAll; e += NT) *(typename Chunk<T>::vec*)(lds + e * C) = typename Chunk<T>::vec{};
     }
     template <class Keep>
     __device__ __forceinline__ void store(Keep keep, T* lds, int d, int vec, int tid) const {
@@ -188,6 +192,13 @@ struct TileFetch {
 // The tile in flight has landed, everybody's part of it, and everybody is done with the one before.
 __device__ __forceinline__ void tile_ready() {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// What this workgroup has written to LDS since is there for everybody.
+__device__ __forceinline__ void pad_ready() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
