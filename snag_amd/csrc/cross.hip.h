@@ -1,4 +1,5 @@
-// Cross attention: what its kernels share (csrc/cross.hip: tiles on the matrix pipe; csrc/cross_rows.hip: a few rows per key/value head).
+// Cross attention: what its kernels share (csrc/cross_fwd.hip, csrc/cross_bwd.hip: tiles on the matrix pipe; csrc/cross_rows.hip: a few rows per key/value head;
+// csrc/cross.hip: the choice between them).
 //
 // The rows of one problem (b, hk) are the Lq * G queries of the G = H / Hkv heads that share key/value head hk, row = l * G + g: a key/value
 // tile is read once for all of them, and d K, d V of a shared head are sums inside one workgroup (no atomics).

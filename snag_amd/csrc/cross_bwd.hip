@@ -2,7 +2,8 @@
 //
 // Two passes, each recomputing the scores: d q with 32 rows per wave (three products per key tile), d k / d v with 32 keys per wave (four).  One
 // pass that did both would save two of the seven products and need atomics for one of the sides.  Bound by the matrix pipe.
-// 2 x 16 heads of 128, 2048 rows, 8192 keys in bf16: d q 400 us (1.03 PFLOP/s), d k / d v 655 us (0.84).
+// 2 x 16 heads of 128, 2048 rows, 8192 keys in bf16: d q 400 - 435 us by the card (0.95 - 1.03 PFLOP/s), d k / d v 620 - 690 (0.80 - 0.89); fp16, with the power of
+// two that d scores carry, 448 and 658 (432 and 646 without).
 #include "cross_tiles.hip.h"
 
 namespace snag {

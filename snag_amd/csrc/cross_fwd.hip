@@ -4,8 +4,8 @@
 // about 900 of softmax per wave, which two waves per SIMD overlap (hence at most 256 registers).  The running maximum is only moved -- and the
 // 64 accumulators rescaled -- when a score passes it by more than 8 (in log2): until then p stays below 2^8, which costs nothing in fp32 sums or
 // in the 8 / 11 significant bits of the rounded p.
-// 2 x 16 heads of 128, 2048 rows, 8192 keys in bf16: 304 us, 0.90 PFLOP/s (a 4096^3 library product on the same card: 1.24); 4 x 16 x 1024 x 2048
-// in fp32: 642 us, 107 TFLOP/s (library: 134 - 154).
+// 2 x 16 heads of 128, 2048 rows, 8192 keys in bf16: 300 - 340 us by the card, 0.81 - 0.92 PFLOP/s (a 4096^3 library product: 1.24); 4 x 16 x 1024 x 2048
+// in fp32: 672 us, 102 TFLOP/s (library: 134 - 154).
 #include "cross_tiles.hip.h"
 
 namespace snag {

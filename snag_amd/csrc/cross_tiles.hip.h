@@ -12,7 +12,7 @@
 // fp16 keeps nothing below 2^-24, and the backward's operands are small: p is 1 / keys, ds about p |do| |v|.  They are rounded as 2^15 p and 2^e ds, e
 // following the largest |ds| met so far (kHalfStart below); without that d q of 8192 keys
 // was 7.5e-3 off for a d_out of 1e-3 and 7e-2 for 1e-4; now 9.6e-4 and 9.3e-3, which is the rounding of the fp16 result alone.  fp16 backwards take
-// 2-7 % longer for it (2048 x 8192 x 128: 1061 -> 1089 us; heads of 100, whose d k / d v spills: 370 -> 427).
+// 2-7 % longer for it (2048 x 8192 x 128: 1066 -> 1106 us; heads of 100, whose d k / d v spills: 370 -> 427).
 #pragma once
 #include <type_traits>
 #include "cross.hip.h"

@@ -485,7 +485,7 @@ __device__ __forceinline__ void finish(const MuonTable* __restrict__ L, const Mu
 // PLANES 1: hi hi, 2: hi hi + hi lo + lo hi.  The LDS stages are filled straight from memory, NST - 1 ahead; the fragments of the next 16 of the
 // contraction are read while the present ones are multiplied, across the stages too: the barrier that opens a stage stands in front of the
 // last products of the stage before it.
-// 4096 x 4096 in bf16: A 91 us (0.78 PFLOP/s), A^2 93, B X 155 - 168 (0.82 - 0.89); a library product of that size: 110 (1.24).
+// 4096 x 4096 in bf16: A 91 - 94 us (0.75 - 0.78 PFLOP/s), A^2 93 - 95, B X 155 - 177 (0.78 - 0.89); a library product of that size: 110 (1.24).
 template <int MODE, int DT, int TILE, int NST>
 __global__ __launch_bounds__(threads_of(TILE, NST), 2) void muon_product_kernel(const MuonTable* __restrict__ L, MuonFirst first, int whole, int from, int last) {
     constexpr int PLANES = DT == SNAG_BF16 ? 1 : 2;

@@ -5,7 +5,8 @@ cosine schedules with warm-up.  Plain host code on torch.optim: the drop-in ``sn
 names, so the groups come out identical (golden G14).
 
 Not in the reference: ``orthogonalize`` / ``muon_step`` (HIP, csrc/muon.hip) and the ``Muon`` optimiser, which ``set_optim`` builds for
-``opt.optim == "muon"`` -- each group above is then cut into its matrices (Muon, at ``opt.muon_lr`` if given) and the rest (AdamW)."""
+``opt.optim == "muon"`` -- each group above is then cut into its matrices (Muon, at ``opt.muon_lr``, without it at the group's own AdamW rate) and the
+rest (AdamW); Muon's momentum, steps and scaling keep their defaults there."""
 import torch
 from torch import optim
 from torch.optim.adamw import adamw
@@ -16,7 +17,8 @@ from . import ops
 def orthogonalize(matrices, steps=5, eps=1e-7):
     """Newton-Schulz orthogonalisation on the matrix pipe: X = G / (|G|_F + eps), then ``steps`` times X <- a X + (b A + c A^2) X with
     A = X X^T and (a, b, c) = (3.4445, -4.7750, 2.0315), which takes every singular value that is not tiny into about 0.7 .. 1.2.
-    One matrix or a list of matrices of one type (fp32, bf16, fp16) -> the same, new tensors.  All matrices of a list share the launches."""
+    One matrix or a list of matrices of one type (fp32, bf16, fp16) -> the same, new tensors, detached: not differentiable.  All matrices of a list share the
+    launches.  Products take operands of 22 bits for fp32 and fp16 matrices, of 11 off the diagonal for bf16 (5e-4 where the result's rounding is 1.7e-3)."""
     if torch.is_tensor(matrices):
         return ops.orthogonalize([matrices.detach()], steps=steps, eps=eps)[0]
     return ops.orthogonalize([m.detach() for m in matrices], steps=steps, eps=eps)
@@ -25,7 +27,7 @@ def orthogonalize(matrices, steps=5, eps=1e-7):
 def muon_step(weights, grads, momenta, lr, momentum=0.95, nesterov=True, weight_decay=0.0, match_rms=False, steps=5, eps=1e-7):
     """One Muon update of a list of matrices, in place: M <- mu M + (1 - mu) G; U = (1 - mu) G + mu M (``nesterov``) or M;
     W <- (1 - lr weight_decay) W - lr s orthogonalize(U), s = sqrt(max(1, rows / cols)) or, with ``match_rms``, 0.2 sqrt(max(rows, cols)).
-    ``momenta`` are fp32, ``grads`` of the weights' type."""
+    ``momenta`` are fp32, ``grads`` of the weights' type; U enters the products as orthogonalize's matrices of that type do."""
     ops.muon_step([w.detach() for w in weights], [g.detach() for g in grads], momenta, lr, momentum, nesterov, weight_decay, match_rms, steps, eps)
 
 
